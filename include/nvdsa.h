@@ -52,7 +52,8 @@ typedef enum nvdsa_dtype {
   NVDSA_INT32 = 0,
   NVDSA_FLOAT16 = 1,
   NVDSA_BFLOAT16 = 2,
-  NVDSA_FLOAT32 = 3
+  NVDSA_FLOAT32 = 3,
+  NVDSA_FLOAT8_E4M3 = 4 /* the 8-bit latent cache (nvdsa_ext.h) */
 } nvdsa_dtype;
 
 /* Device ordinal value for pinned host memory that is mapped into the GPU

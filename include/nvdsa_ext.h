@@ -65,6 +65,94 @@ typedef struct nvdsa_stage_item {
  * item may read what another one writes. */
 int nvdsa_stage_inputs(const nvdsa_stage_item* items, int64_t count, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* The 8-bit latent cache: latent_cache [blocks, 128, G, 576] e4m3 (512
+ * latent ++ 64 rope values of a token and latent head), cache_scale
+ * [blocks, G] fp32 (positive, finite): value = code * scale.  Requests own
+ * their pages through block_table [B, cols] (entries that name no block are
+ * skipped); token records (positions int32, accumulated attention weights
+ * fp32) are pool rows [pool_rows, cols * 128], request b's at
+ * req_pool_entries[b], one value per cache slot of the request.  Two requests
+ * of a call that write must share neither a written page nor a pool row.
+ *
+ * Query / new rows are packed: request b's are
+ * [actual_seq_lengths_query[b-1], actual_seq_lengths_query[b]), and
+ * actual_seq_lengths_kv[b] counts its cached tokens with the new ones.  Rows
+ * behind the last request are neither read nor written.  No counterpart in
+ * the reference, whose caches are 16-bit. */
+
+/* New row i of n goes to slot actual_seq_lengths_kv[b] - n + i.  A page's
+ * scale is the least power of two (2^-126 to 2^120) under which its rows'
+ * largest finite magnitude is at most 448; a page that holds older rows keeps
+ * its scale where that suffices, and otherwise its older codes are rounded to
+ * the larger one.  Codes are rounded to nearest even; infinities and NaN
+ * become NaN.  kv [T, G, 512], k_rope [T, G, 64] (16-bit).  positions [T] and
+ * token_positions go together, either of them or token_weights (set to 0 at
+ * new slots) needs req_pool_entries; all four may be NULL.  No workspace. */
+int nvdsa_latent8_append(const nvdsa_tensor* kv,
+                         const nvdsa_tensor* k_rope,
+                         const nvdsa_tensor* actual_seq_lengths_query,
+                         const nvdsa_tensor* actual_seq_lengths_kv,
+                         const nvdsa_tensor* block_table,
+                         const nvdsa_tensor* latent_cache,
+                         const nvdsa_tensor* cache_scale,
+                         const nvdsa_tensor* positions,
+                         const nvdsa_tensor* req_pool_entries,
+                         const nvdsa_tensor* token_positions,
+                         const nvdsa_tensor* token_weights,
+                         void* stream);
+
+/* attention_out[r] = softmax(scale_value * q[r] . k) . k[:512] over the slots
+ * that row r sees: row i of a request's n sees the first
+ * actual_seq_lengths_kv - (n - 1 - i), or, with topk_ids [T, K], those of its
+ * list (entries outside that range are skipped, a slot listed twice counts
+ * twice).  A row that sees nothing is zero.  query [T, N, 512], query_rope
+ * [T, N, 64], N a multiple of G: head h attends latent head h / (N / G).
+ * With token_weights (not with topk_ids), every slot's attention weight,
+ * summed over the request's rows and heads, is added to its record. */
+size_t nvdsa_latent8_attention_workspace_size(int64_t query_rows, int64_t heads, int32_t with_weights);
+int nvdsa_latent8_attention(const nvdsa_tensor* query_rope,
+                            const nvdsa_tensor* query,
+                            const nvdsa_tensor* actual_seq_lengths_query,
+                            const nvdsa_tensor* actual_seq_lengths_kv,
+                            const nvdsa_tensor* block_table,
+                            const nvdsa_tensor* latent_cache,
+                            const nvdsa_tensor* cache_scale,
+                            const nvdsa_tensor* topk_ids,
+                            const nvdsa_tensor* req_pool_entries,
+                            const nvdsa_tensor* token_weights,
+                            double scale_value,
+                            const nvdsa_tensor* attention_out,
+                            void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Brings every request with more than budgets[b] cached tokens down to that
+ * many.  Kept are tokens at a position below protect_first or among the
+ * protect_last latest positions, then those of the largest weight (NaN above
+ * all), ties to the lower slot.  The kept tokens at slots >= budget move, in
+ * order, into the slots below it that were given up: their rows (to the
+ * larger of the pages' scales), positions and weights.  move_src_slots /
+ * move_dst_slots [B, cols * 128] list the moves (entries past move_counts[b]
+ * are left as they were), kept_lengths[b] is the new length.  A request whose
+ * pool entry names no row is left alone. */
+size_t nvdsa_latent8_evict_workspace_size(int64_t batch, int64_t table_cols, int64_t latent_heads);
+int nvdsa_latent8_evict(const nvdsa_tensor* actual_seq_lengths_kv,
+                        const nvdsa_tensor* budgets,
+                        const nvdsa_tensor* block_table,
+                        const nvdsa_tensor* req_pool_entries,
+                        const nvdsa_tensor* latent_cache,
+                        const nvdsa_tensor* cache_scale,
+                        const nvdsa_tensor* token_positions,
+                        const nvdsa_tensor* token_weights,
+                        int64_t protect_first,
+                        int64_t protect_last,
+                        const nvdsa_tensor* move_src_slots,
+                        const nvdsa_tensor* move_dst_slots,
+                        const nvdsa_tensor* move_counts,
+                        const nvdsa_tensor* kept_lengths,
+                        void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,1279 @@
+// The 8-bit latent cache: append, attention and eviction.
+//
+// A token's row is 576 e4m3 values per latent head (512 latent, 64 rope) in
+// pages of 128 tokens, [blocks, 128, G, 576], with one fp32 scale per page and
+// latent head: value = code * scale.  The codes are exact in bf16 and fp16, so
+// products run on the 16-bit MFMAs with the scale taken outside the sum.
+//
+//   append    scale = least power of two >= amax / 448 over a page's rows; a
+//             page that grows its scale shifts its older rows.
+//   attention s = scale * c_page * (q . k), p = softmax(s), o = sum p c_page v
+//   weights   token_weights[slot] += sum over rows and heads of p
+//   evict     keeps a request's most attended tokens and moves the kept ones
+//             beyond the budget into the holes below it.
+#include <algorithm>
+#include <cfloat>
+
+#include "nvdsa_common.h"
+#include "nvdsa_kernels.h"
+
+namespace nvdsa {
+namespace {
+
+constexpr int kRow = kQkDim;              // bytes of a token's row and latent head
+constexpr int kRowChunks = kRow / 16;     // 36 chunks of 16 bytes
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// ------------------------------------------------------------- e4m3 helpers
+__device__ inline uint32_t cvt2(Bf16, uint32_t v, std::integral_constant<bool, false>) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, false));
+}
+__device__ inline uint32_t cvt2(Bf16, uint32_t v, std::integral_constant<bool, true>) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, true));
+}
+__device__ inline uint32_t cvt2(F16, uint32_t v, std::integral_constant<bool, false>) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false));
+}
+__device__ inline uint32_t cvt2(F16, uint32_t v, std::integral_constant<bool, true>) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true));
+}
+// Eight codes to eight 16-bit values (exact).
+template <typename T>
+__device__ inline typename T::vec8 widen8(uint32_t lo, uint32_t hi) {
+  u32x4_t r;
+  r[0] = cvt2(T{}, lo, std::integral_constant<bool, false>{});
+  r[1] = cvt2(T{}, lo, std::integral_constant<bool, true>{});
+  r[2] = cvt2(T{}, hi, std::integral_constant<bool, false>{});
+  r[3] = cvt2(T{}, hi, std::integral_constant<bool, true>{});
+  return __builtin_bit_cast(typename T::vec8, r);
+}
+// Four fp32 values (at most 448, or NaN) to four codes, round to nearest even.
+__device__ inline uint32_t encode4(float a, float b, float c, float d) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true));
+}
+__device__ inline uint32_t rescale4(uint32_t v, float ratio) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v), true);
+  return encode4(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
+}
+__device__ inline uint4 rescale16(uint4 v, float ratio) {
+  return make_uint4(rescale4(v.x, ratio), rescale4(v.y, ratio), rescale4(v.z, ratio), rescale4(v.w, ratio));
+}
+// Zero in the place of NaN codes (0x7f, 0xff): the byte's low seven bits all
+// set carry into bit 7 when one is added.
+__device__ inline uint32_t nan_to_zero4(uint32_t v) {
+  const uint32_t bad = (((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return v & ~(bad * 0xffu);
+}
+
+// Least power of two s in [2^-126, 2^120] with amax / s <= 448 = 1.75 * 2^8.
+__device__ inline float least_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int k = static_cast<int>(u >> 23) - 126 - ((u & 0x7fffffu) > 0x600000u ? 8 : 9);
+  k = k < -126 ? -126 : (k > 120 ? 120 : k);
+  return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+}
+
+// -------------------------------------------------------------------- append
+// One workgroup per (page that receives rows, latent head).  It reads the
+// page's new rows once into registers (at most 128 * 72 chunks of 8 values
+// over 512 threads), takes their largest magnitude, and writes the codes.
+// Bound by the rows' bytes (3 per value); a decode step's by latency.
+constexpr int kAppendThreads = 512;
+constexpr int kAppendChunks = kBlock * (kRow / 8) / kAppendThreads;  // 18 a thread
+
+struct Span {  // a request's new rows: row0 + i goes to slot first + i, i < count
+  int64_t row0;
+  int first;
+  int count;
+};
+__device__ inline Span append_span(const Latent8AppendArgs& a, int64_t b) {
+  int64_t lo = b > 0 ? a.seq_q[b - 1] : 0, hi = a.seq_q[b];
+  lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
+  hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
+  const int64_t cap = a.cols * kBlock;
+  int64_t s0 = static_cast<int64_t>(a.seq_kv[b]) - (hi - lo), s1 = a.seq_kv[b];
+  if (s1 > cap) s1 = cap;
+  int64_t skip = 0;
+  if (s0 < 0) {
+    skip = -s0;
+    s0 = 0;
+  }
+  return {lo + skip, static_cast<int>(s0), static_cast<int>(s1 > s0 ? s1 - s0 : 0)};
+}
+__device__ inline int pages_of(const Span& s) {
+  return s.count > 0 ? ((s.first + s.count - 1) >> kBlockShift) - (s.first >> kBlockShift) + 1 : 0;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kAppendThreads) void latent8_append_kernel(Latent8AppendArgs a) {
+  __shared__ int scratch[kAppendThreads / 64 + 1];
+  __shared__ int found_page;
+  __shared__ int64_t found_b;
+  __shared__ uint32_t wave_max[kAppendThreads / 64];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int g = blockIdx.y;
+  // The workgroup's request and page, counted over the requests in order.
+  if (tid == 0) found_b = -1;
+  int before = 0;
+  for (int64_t b0 = 0; b0 < a.batch; b0 += kAppendThreads) {
+    const int64_t b = b0 + tid;
+    const int n = b < a.batch ? pages_of(append_span(a, b)) : 0;
+    int total;
+    const int at = before + block_exclusive_scan(n, scratch, &total);
+    const int64_t want = blockIdx.x;
+    if (want >= at && want < at + n) {
+      found_b = b;
+      found_page = static_cast<int>(want) - at;
+    }
+    before += total;
+    if (want < before) break;
+  }
+  __syncthreads();
+  const int64_t b = found_b;
+  if (b < 0) return;
+  const Span span = append_span(a, b);
+  const int page = (span.first >> kBlockShift) + found_page;
+  const int32_t block = a.block_table[b * a.cols + page];
+  const int lo = span.first > page * kBlock ? span.first - page * kBlock : 0;  // first new row of the page
+  const int end = span.first + span.count - page * kBlock;
+  const int n = (end < kBlock ? end : kBlock) - lo;
+  const int64_t row0 = span.row0 + (page * kBlock + lo - span.first);
+  if (g == 0 && a.entries != nullptr) {
+    const int64_t e = a.entries[b];
+    if (e >= 0 && e < a.pool_rows && tid < n) {
+      const int64_t at = e * a.cols * kBlock + page * kBlock + lo + tid;
+      if (a.token_positions != nullptr) a.token_positions[at] = a.positions[row0 + tid];
+      if (a.token_weights != nullptr) a.token_weights[at] = 0.f;
+    }
+  }
+  if (block < 0 || block >= a.blocks) return;
+
+  const int chunks = n * (kRow / 8);
+  u32x4_t v[kAppendChunks];
+  uint32_t most = 0;
+  constexpr uint32_t kInf = std::is_same<T, Bf16>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; ++i) {
+    const int q = i * kAppendThreads + tid;
+    v[i] = u32x4_t{0, 0, 0, 0};
+    if (q < chunks) {
+      const int r = q / (kRow / 8), c = q - r * (kRow / 8);
+      const int64_t at = (row0 + r) * a.latent_heads + g;
+      v[i] = *(c < kCkvDim / 8 ? static_cast<const u32x4_t*>(a.kv) + at * (kCkvDim / 8) + c
+                               : static_cast<const u32x4_t*>(a.k_rope) + at * (kKpeDim / 8) + c - kCkvDim / 8);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; ++i) {
+    if (i * kAppendThreads < chunks) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t x = v[i][k] & 0x7fffu, y = (v[i][k] >> 16) & 0x7fffu;
+        if (x < kInf && x > most) most = x;
+        if (y < kInf && y > most) most = y;
+      }
+    }
+  }
+  most = wave_reduce_to_lane63(most, MaxU32Op{});
+  if (lane == 63) wave_max[wave] = most;
+  float* scale_at = a.cache_scale + static_cast<int64_t>(block) * a.latent_heads + g;
+  const float old = *scale_at;  // (before the barrier: thread 0 writes it at the end)
+  __syncthreads();
+  most = wave_max[0];
+#pragma unroll
+  for (int w = 1; w < kAppendThreads / 64; ++w) most = most < wave_max[w] ? wave_max[w] : most;
+  const float need = least_scale(T::to_float(static_cast<uint16_t>(most)));
+  const bool keeps = lo > 0 && old >= need;
+  const float now = keeps ? old : need;
+  uint8_t* base = static_cast<uint8_t*>(a.latent_cache) + static_cast<int64_t>(block) * kBlock * a.latent_heads * kRow +
+                  static_cast<int64_t>(g) * kRow;
+  const int64_t stride = a.latent_heads * kRow;
+  if (lo > 0 && !keeps) {  // the older rows under the larger scale
+    const float ratio = old / now;
+    for (int q = tid; q < lo * kRowChunks; q += kAppendThreads) {
+      const int r = q / kRowChunks, c = q - r * kRowChunks;
+      uint4* p = reinterpret_cast<uint4*>(base + r * stride) + c;
+      *p = rescale16(*p, ratio);
+    }
+  }
+  // Division by a power of two is the product with its reciprocal, exactly.
+  const uint32_t bits = __float_as_uint(now);
+  const bool pow2 = (bits & 0x807fffffu) == 0 && (bits >> 23) >= 1 && (bits >> 23) <= 253;
+  const float inverse = pow2 ? __uint_as_float((254u - (bits >> 23)) << 23) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; ++i) {
+    const int q = i * kAppendThreads + tid;
+    if (q < chunks) {
+      const int r = q / (kRow / 8), c = q - r * (kRow / 8);
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint16_t h = static_cast<uint16_t>(v[i][k >> 1] >> (16 * (k & 1)));
+        const float x = T::to_float(h);
+        const float y = pow2 ? x * inverse : x / now;
+        f[k] = (h & 0x7fffu) < kInf ? y : __uint_as_float(0x7fc00000u);  // infinities have no code: NaN
+      }
+      *(reinterpret_cast<uint2*>(base + (lo + r) * stride) + c) =
+          make_uint2(encode4(f[0], f[1], f[2], f[3]), encode4(f[4], f[5], f[6], f[7]));
+    }
+  }
+  if (tid == 0 && !keeps) *scale_at = now;
+}
+
+// ----------------------------------------------------------------- attention
+// Split attention over a list of units.  A unit is one tile of 64 keys of one
+// item; an item is up to 64 (query row, head) pairs of one request and latent
+// head (with a list: heads of one query row).  The units of all items lie in a
+// row, and workgroup w takes the w-th of equal parts, so a ragged batch loads
+// every CU alike; an item that lies across parts leaves fp32 partials that a
+// second kernel joins.
+constexpr int kAttnThreads = 512;
+constexpr int kRows = 64;       // (query row, head) pairs of an item
+constexpr int kKeys = 64;       // keys of a tile
+constexpr int kWindow = 512;    // resolved pages (or list entries) held at a time
+constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
+constexpr float kNoMax = -3.0e38f;
+constexpr float kSlack = 8.f;   // headroom of the running maximum (base 2): P <= 2^8 in fp16
+constexpr int kMinUnits = 2;    // least tiles of a workgroup
+constexpr int kPartFloats = kRows * kCkvDim;
+
+struct Plan {
+  int64_t total;  // units
+  int64_t parts;  // workgroups that share them
+};
+__host__ __device__ inline int64_t part_start(const Plan& p, int64_t w) { return p.total * w / p.parts; }
+__device__ inline int64_t part_of(const Plan& p, int64_t unit) { return ((unit + 1) * p.parts + p.total - 1) / p.total - 1; }
+
+struct Request {
+  int64_t row0;   // first query row
+  int n;          // query rows
+  int len;        // cached tokens, clipped to the table
+  int items_g;    // items of one latent head
+  int64_t items;
+  int64_t tiles;  // units of an item
+};
+__device__ inline Request request_of(const Latent8Args& a, int64_t b) {
+  int64_t lo = b > 0 ? a.seq_q[b - 1] : 0, hi = a.seq_q[b];
+  lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
+  hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
+  Request r;
+  r.row0 = lo;
+  r.n = static_cast<int>(hi - lo);
+  const int64_t cap = a.cols * kBlock;
+  int64_t len = a.seq_kv[b];
+  r.len = static_cast<int>(len < 0 ? 0 : (len > cap ? cap : len));
+  const int64_t per = a.heads / a.latent_heads;
+  r.items_g = static_cast<int>(a.topk != nullptr ? r.n * ceil_div(per, kRows) : ceil_div(r.n * per, kRows));
+  r.items = static_cast<int64_t>(r.items_g) * a.latent_heads;
+  r.tiles = a.topk != nullptr ? ceil_div(a.list_len, kKeys) : ceil_div(r.len, kKeys);
+  if (r.tiles < 1) r.tiles = 1;
+  return r;
+}
+
+// Exclusive prefix of a 64-bit count over the workgroup's threads.
+template <int THREADS>
+__device__ inline int64_t scan64(int64_t v, int64_t* scratch, int64_t* total) {
+  const int wid = threadIdx.x >> 6;
+  const int64_t x = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(v)));
+  if ((threadIdx.x & 63) == 63) scratch[wid] = x;
+  __syncthreads();
+  int64_t before = 0, tot = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int64_t t = scratch[w];
+    before += w < wid ? t : 0;
+    tot += t;
+  }
+  *total = tot;
+  __syncthreads();
+  return before + x - v;
+}
+
+// Where a workgroup's part begins: the request and the unit within it.
+struct Start {
+  Plan plan;
+  int64_t b;
+  int64_t unit;  // of the request
+  int64_t base;  // first unit of the request
+};
+template <int THREADS, typename COST>
+__device__ inline Start find_start(int64_t batch, int64_t part, int64_t parts, int64_t least, COST cost,
+                                   int64_t* scratch, int64_t* found) {
+  Start s;
+  const int tid = threadIdx.x;
+  int64_t sum = 0;
+  const int64_t first = tid < batch ? cost(static_cast<int64_t>(tid)) : 0;
+  for (int64_t b = tid + THREADS; b < batch; b += THREADS) sum += cost(b);
+  int64_t total;
+  if (tid == 0) found[0] = -1;
+  if (batch <= THREADS) {
+    const int64_t at = scan64<THREADS>(first, scratch, &total);
+    s.plan.total = total;
+    s.plan.parts = total / least < 1 ? 1 : (total / least < parts ? total / least : parts);
+    if (part < s.plan.parts && total > 0) {
+      const int64_t u = part_start(s.plan, part);
+      if (u >= at && u < at + first) {
+        found[0] = tid;
+        found[1] = u - at;
+        found[2] = at;
+      }
+    }
+  } else {
+    scan64<THREADS>(first + sum, scratch, &total);
+    s.plan.total = total;
+    s.plan.parts = total / least < 1 ? 1 : (total / least < parts ? total / least : parts);
+    if (part < s.plan.parts && total > 0) {
+      const int64_t u = part_start(s.plan, part);
+      int64_t before = 0;
+      for (int64_t b0 = 0; b0 < batch; b0 += THREADS) {
+        const int64_t b = b0 + tid;
+        const int64_t c = b < batch ? cost(b) : 0;
+        int64_t chunk;
+        const int64_t at = before + scan64<THREADS>(c, scratch, &chunk);
+        if (u >= at && u < at + c) {
+          found[0] = b;
+          found[1] = u - at;
+          found[2] = at;
+        }
+        before += chunk;
+        if (u < before) break;
+      }
+    }
+  }
+  __syncthreads();
+  s.b = found[0];
+  s.unit = found[1];
+  s.base = found[2];
+  return s;
+}
+
+// The item's rows: pair f = first + m (m < count) is query row f / per, head
+// f % per of the latent head's; it sees `vis` keys.
+struct Item {
+  int g;
+  int first;
+  int count;
+  int lead;  // list: the item's query row
+};
+__device__ inline Item item_of(const Latent8Args& a, const Request& r, int64_t it) {
+  Item x;
+  const int per = static_cast<int>(a.heads / a.latent_heads);
+  x.g = static_cast<int>(it / r.items_g);
+  int j = static_cast<int>(it - static_cast<int64_t>(x.g) * r.items_g);
+  if (a.topk != nullptr) {
+    const int groups = static_cast<int>(ceil_div(per, kRows));
+    x.lead = j / groups;
+    j -= x.lead * groups;
+    x.first = x.lead * per + j * kRows;
+    const int left = per - j * kRows;
+    x.count = left < kRows ? left : kRows;
+  } else {
+    // Early and late rows in turn: under the causal bound they cost little and
+    // much, and neighbours share a workgroup's part.
+    j = (j & 1) ? r.items_g - 1 - (j >> 1) : (j >> 1);
+    x.lead = 0;
+    x.first = j * kRows;
+    const int left = r.n * per - j * kRows;
+    x.count = left < kRows ? left : kRows;
+  }
+  return x;
+}
+__device__ inline int visible(const Request& r, int i) {
+  const int64_t v = static_cast<int64_t>(r.len) - (r.n - 1 - i);
+  return v > 0 ? static_cast<int>(v) : 0;
+}
+
+// What the joining kernel needs of an item that lies across parts.
+struct JoinEntry {
+  int64_t row0;
+  int32_t first, count, g;
+  int32_t slot0;   // slot of the first part's partial
+  int32_t w0, w1;  // parts w0 .. w1 (w0's partial in slot0, w's in 2 w)
+};
+
+struct Work {
+  float* part;      // [2 parts][64 * 512], in the accumulators' order
+  float* ml;        // [2 parts][64][2]
+  JoinEntry* join;  // [parts], row0 < 0: nothing
+  float* lse;       // [rows, heads], base 2 (with weights)
+};
+constexpr size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+__host__ __device__ inline Work carve_work(void* ws, int64_t parts) {
+  Work w;
+  char* p = static_cast<char*>(ws);
+  w.part = reinterpret_cast<float*>(p);
+  p += sizeof(float) * 2 * parts * kPartFloats;
+  w.ml = reinterpret_cast<float*>(p);
+  p += sizeof(float) * 2 * parts * kRows * 2;
+  w.join = reinterpret_cast<JoinEntry*>(p);
+  p += round256(sizeof(JoinEntry) * parts);
+  w.lse = reinterpret_cast<float*>(p);
+  return w;
+}
+
+__device__ inline uint2 read_tr8(const uint8_t* p) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) v2i lds_v2i;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(const_cast<uint8_t*>(p))));
+}
+
+// A page's (or list entry's) scale c = fraction * 2^exponent, fraction in
+// [1, 2): scores take c, P enters the product with V as p * 2^exponent *
+// fraction against the codes, and the sum of p divides 2^exponent out again.
+struct Window {
+  int32_t row;    // first cache row of the page, or the entry's row; -1: none
+  float score;    // softmax scale * log2(e) * c
+  float exponent;
+  float fraction;
+};
+__device__ inline Window resolve(const Latent8Args& a, int64_t b, int g, int64_t slot, bool ok) {
+  Window w{-1, 0.f, 0.f, 0.f};
+  if (!ok) return w;
+  const int32_t block = a.block_table[b * a.cols + (slot >> kBlockShift)];
+  if (block < 0 || block >= a.blocks) return w;
+  float c = a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g];
+  c = fminf(fmaxf(c, kMinScale), FLT_MAX);
+  const uint32_t u = __float_as_uint(c);
+  w.row = block * kBlock + static_cast<int32_t>(slot & (kBlock - 1));
+  w.score = a.scale * kLog2e * c;
+  w.exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
+  w.fraction = __uint_as_float((u & 0x7fffffu) | 0x3f800000u);
+  return w;
+}
+
+// Eight waves.  Scores: wave = (32 keys, 32 rows, half of the 576 dims), so
+// the halves meet through LDS; then every lane holds 8 keys of one row.
+// Output: wave = 64 latent dims of all 64 rows, transposed: O^T = V^T P^T, V^T
+// by transposing 8-bit LDS reads.  P is fp16 of values up to 2^8.
+template <typename T, bool LIST>
+__global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Latent8Args a) {
+  __shared__ __align__(16) uint8_t keys[2][kKeys * kRow];
+  __shared__ __align__(16) float4 half_s[8 * 2 * 64];
+  __shared__ __align__(16) uint16_t p_tile[kRows * kPStride];
+  __shared__ __align__(16) float row_max[kRows][4];
+  __shared__ Window windows[LIST ? 2 : 1][kWindow];
+  __shared__ int64_t scratch[kAttnThreads / 64];
+  __shared__ int64_t found[3];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int l32 = lane & 31;
+  const int hh = lane >> 5;
+  const int kg = wave & 1, mg = (wave >> 1) & 1, dh = wave >> 2;
+  const int64_t part = blockIdx.x;
+  const Start start = find_start<kAttnThreads>(
+      a.batch, part, a.parts, kMinUnits,
+      [&](int64_t b) {
+        const Request r = request_of(a, b);
+        return r.items * r.tiles;
+      },
+      scratch, found);
+  const Work work = carve_work(a.workspace, a.parts);
+  if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
+  if (part >= start.plan.parts || start.b < 0) return;
+  const int64_t stop = part_start(start.plan, part + 1);
+  int64_t at = part_start(start.plan, part);
+  int64_t b = start.b;
+  int64_t base = start.base;
+  const int per = static_cast<int>(a.heads / a.latent_heads);
+  const int64_t row_bytes = a.latent_heads * kRow;
+
+  // This thread's 16-byte chunks of a tile: chunk c of key k at row k, chunk
+  // c ^ ((k >> 2) & 3) within its group of four (16 keys of one chunk then lie
+  // in 64 different banks).
+  int key_of[5], src_of[5], dst_of[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const int q = i * kAttnThreads + tid;
+    const int k = q / kRowChunks, c = q - k * kRowChunks;
+    key_of[i] = k;
+    src_of[i] = c * 16;
+    dst_of[i] = k * kRow + ((c & ~3) | ((c ^ (k >> 2)) & 3)) * 16;
+  }
+  // LDS addresses of the score operand (chunks 18 dh + 2 j + hh) and of V.
+  int k_at[2];
+  {
+    // The second half's waves take their 32 keys with the halves swapped, so
+    // that accumulators 0-7 are the keys that a wave finishes itself.
+    const int k = kg * 32 + (l32 ^ (dh * 16));
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const int c = 18 * dh + hh + 2 * odd;
+      k_at[odd] = k * kRow + ((c & ~3) | ((c ^ (k >> 2)) & 3)) * 16;
+    }
+  }
+  int v_at[2];
+  {
+    const int i = lane & 15, grp = (lane >> 4) & 1;
+    const int k = 8 * hh + (i >> 1);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+      v_at[dt] = k * kRow + (wave * 4 + ((2 * dt + grp) ^ ((k >> 2) & 3))) * 16 + 8 * (i & 1);
+  }
+
+  while (at < stop) {
+    // The next segment: units [u0, u1) of one item.
+    Request r = request_of(a, b);
+    while (at >= base + r.items * r.tiles) {
+      base += r.items * r.tiles;
+      ++b;
+      r = request_of(a, b);
+    }
+    const int64_t it = (at - base) / r.tiles;
+    const int64_t item_start = base + it * r.tiles;
+    const int64_t item_end = item_start + r.tiles;
+    const int64_t seg_end = item_end < stop ? item_end : stop;
+    const Item x = item_of(a, r, it);
+    const int i_last = LIST ? x.lead : (x.first + x.count - 1) / per;
+    const int i_first = LIST ? x.lead : x.first / per;
+    const int vis_most = visible(r, i_last), vis_least = visible(r, i_first);
+    const int list_len = LIST ? static_cast<int>(a.list_len) : vis_most;
+    int t0 = static_cast<int>(at - item_start), t1 = static_cast<int>(seg_end - item_start);
+    const int tiles_seen = (list_len + kKeys - 1) / kKeys;
+    if (t1 > tiles_seen) t1 = tiles_seen;
+    if (t0 > t1) t0 = t1;
+
+    // Rows of this lane: m = mg * 32 + l32 for the scores, both halves for the output.
+    int vis_row;
+    uint4 q[9][2];
+    {
+      const int m = mg * 32 + l32;
+      const int f = x.first + (m < x.count ? m : 0);
+      const int i = f / per, h = f - i * per;
+      vis_row = m < x.count ? visible(r, i) : 0;
+      const int64_t row = (r.row0 + i) * a.heads + x.g * per + h;
+      const uint4* qn = static_cast<const uint4*>(a.query) + row * (kCkvDim / 8);
+      const uint4* qr = static_cast<const uint4*>(a.query_rope) + row * (kKpeDim / 8);
+#pragma unroll
+      for (int j = 0; j < 9; ++j) {
+        const int c = dh * 36 + 4 * j + 2 * hh;  // chunk of 8 values
+        const uint4* p = (dh == 1 && j >= 7) ? qr + (c - kCkvDim / 8) : qn + c;
+        q[j][0] = p[0];
+        q[j][1] = p[1];
+      }
+    }
+    f32x16_t o[2][2];
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][mt][e] = 0.f;
+    float m_run[2] = {kNoMax, kNoMax};
+    float l_run = 0.f;
+
+    const int32_t* list = LIST ? a.topk + (r.row0 + x.lead) * a.list_len : nullptr;
+    int win0 = 0;  // first page (list: entry) of the window
+    int win_buf = 0;
+    auto fill_window = [&](int tile) {
+      if (LIST) {
+        win0 = tile * kKeys;
+        win_buf ^= 1;
+        const int e = win0 + tid;
+        const int id = e < list_len ? list[e] : -1;
+        windows[win_buf][tid] = resolve(a, b, x.g, id, id >= 0 && id < vis_most);
+      } else {
+        win0 = tile >> 1;
+        const int64_t slot = static_cast<int64_t>(win0 + tid) * kBlock;
+        windows[0][tid] = resolve(a, b, x.g, slot, slot < vis_most);
+      }
+    };
+    constexpr int kWindowTiles = LIST ? kWindow / kKeys : 2 * kWindow;
+    u32x4_t ahead[5];
+    auto load_tile = [&](int tile) {
+      if (LIST) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+          if (i < 4 || tid < 256) {
+            const int32_t row = windows[win_buf][tile * kKeys - win0 + key_of[i]].row;
+            ahead[i] = u32x4_t{0, 0, 0, 0};  // (an entry that is not attended: P is zero, so must not meet NaN)
+            if (row >= 0)
+              ahead[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.latent_cache) +
+                                                             static_cast<int64_t>(row) * row_bytes + x.g * kRow + src_of[i]);
+          }
+      } else {
+        const int32_t page = __builtin_amdgcn_readfirstlane(windows[0][(tile >> 1) - win0].row);
+        const uint8_t* p = static_cast<const uint8_t*>(a.latent_cache) +
+                           (static_cast<int64_t>(page < 0 ? 0 : page) + (tile & 1) * kKeys) * row_bytes + x.g * kRow;
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+          if (i < 4 || tid < 256)
+            ahead[i] = *reinterpret_cast<const u32x4_t*>(p + static_cast<int64_t>(key_of[i]) * row_bytes + src_of[i]);
+      }
+    };
+    auto store_tile = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i)
+        if (i < 4 || tid < 256) *reinterpret_cast<u32x4_t*>(&keys[buf][dst_of[i]]) = ahead[i];
+    };
+
+    __syncthreads();  // the previous segment is done with LDS
+    if (t0 < t1) {
+      fill_window(t0);
+      __syncthreads();
+      load_tile(t0);
+      store_tile(0);
+      __syncthreads();
+    }
+    int buf = 0;
+    int win_end = t0 + kWindowTiles;  // dense: tiles of the window's pages (t0 may be a page's second tile)
+    if (!LIST) win_end = 2 * win0 + kWindowTiles;
+    for (int t = t0; t < t1; ++t) {
+      Window tile_w{};
+      if (!LIST) tile_w = windows[0][(t >> 1) - win0];
+      // (list) this lane's entries of the tile: key_w[8 (e >> 2) + (e & 3)]
+      const Window* key_w = &windows[LIST ? win_buf : 0][LIST ? t * kKeys - win0 + kg * 32 + dh * 16 + 4 * hh : 0];
+      if (t + 1 < t1) {
+        if (t + 1 >= win_end) {
+          if (!LIST) __syncthreads();  // (the last reads of the one window)
+          fill_window(t + 1);
+          win_end = LIST ? t + 1 + kWindowTiles : 2 * win0 + kWindowTiles;
+          __syncthreads();
+        }
+        load_tile(t + 1);
+      }
+      // S^T = K Q^T over this wave's half of the dims.
+      f32x16_t s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 9; ++j) {
+        const uint4 k = *reinterpret_cast<const uint4*>(&keys[buf][k_at[j & 1] + (j >> 1) * 64]);
+        s = T::mfma32(widen8<T>(k.x, k.y), __builtin_bit_cast(typename T::vec8, q[j][0]), s);
+        s = T::mfma32(widen8<T>(k.z, k.w), __builtin_bit_cast(typename T::vec8, q[j][1]), s);
+      }
+      // Keys 0-15 of a wave's 32 are finished by the first half of the
+      // waves, 16-31 by the second: each hands the other eight over.
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        half_s[(wave * 2 + e) * 64 + lane] = make_float4(s[8 + 4 * e], s[9 + 4 * e], s[10 + 4 * e], s[11 + 4 * e]);
+      lds_barrier();
+      if (t + 1 < t1) store_tile(buf ^ 1);
+      float sc[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 other = half_s[((wave ^ 4) * 2 + e) * 64 + lane];
+        sc[4 * e + 0] = s[4 * e] + other.x;
+        sc[4 * e + 1] = s[4 * e + 1] + other.y;
+        sc[4 * e + 2] = s[4 * e + 2] + other.z;
+        sc[4 * e + 3] = s[4 * e + 3] + other.w;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = kg * 32 + dh * 16 + 8 * (e >> 2) + 4 * hh + (e & 3);
+        const Window& w = LIST ? key_w[8 * (e >> 2) + (e & 3)] : tile_w;
+        const bool ok = w.row >= 0 && (LIST || t * kKeys + key < vis_row);
+        sc[e] = ok ? fmaf(sc[e], w.score, w.exponent) : -INFINITY;
+        top = fmaxf(top, sc[e]);
+      }
+      top = xor32_op(top, MaxOp{});
+      if (hh == 0) row_max[mg * 32 + l32][kg * 2 + dh] = top;
+      lds_barrier();
+      // A key that some row must not see may hold NaN; its P is zero there,
+      // and zero times NaN must not reach the sum.  (Rows that do see it have
+      // NaN scores, hence NaN sums.)
+      const bool ragged = !LIST && ((t + 1) * kKeys > vis_least || tile_w.row < 0);
+      float grow[2];
+      bool moved = false;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const float4 v = *reinterpret_cast<const float4*>(row_max[mt * 32 + l32]);
+        const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+        grow[mt] = 1.f;
+        if (most > m_run[mt] + kSlack) {
+          grow[mt] = __builtin_amdgcn_exp2f(m_run[mt] - most);
+          m_run[mt] = most;
+          moved = true;
+        }
+      }
+      if (__any(moved)) {
+        l_run *= mg ? grow[1] : grow[0];
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][mt][e] *= grow[mt];
+      }
+      const float m_mine = mg ? m_run[1] : m_run[0];
+      float l_tile = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float pw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const Window& w = LIST ? key_w[8 * e + k] : tile_w;
+          const float v = __builtin_amdgcn_exp2f(sc[4 * e + k] - m_mine);
+          l_tile += LIST ? ldexpf(v, -static_cast<int>(w.exponent)) : v;
+          pw[k] = v * w.fraction;
+        }
+        const uint2 packed = make_uint2(F16::pack2(pw[0], pw[1]), F16::pack2(pw[2], pw[3]));
+        *reinterpret_cast<uint2*>(&p_tile[(mg * 32 + l32) * kPStride + kg * 32 + dh * 16 + 8 * e + 4 * hh]) = packed;
+      }
+      l_run += LIST ? l_tile : ldexpf(l_tile, -static_cast<int>(tile_w.exponent));
+      if (ragged) {
+        for (int c = tid; c < kKeys * kRowChunks; c += kAttnThreads) {
+          uint4* v = reinterpret_cast<uint4*>(&keys[buf][c * 16]);
+          const uint4 u = *v;
+          *v = make_uint4(nan_to_zero4(u.x), nan_to_zero4(u.y), nan_to_zero4(u.z), nan_to_zero4(u.w));
+        }
+      }
+      lds_barrier();
+      // O^T += V^T P^T.
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        f16x8_t v[2], p[2];
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+          const uint2 u = read_tr8(&keys[buf][v_at[dt] + ks * 16 * kRow]);
+          v[dt] = widen8<F16>(u.x, u.y);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+          p[mt] = *reinterpret_cast<const f16x8_t*>(&p_tile[(mt * 32 + l32) * kPStride + ks * 16 + 8 * hh]);
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) o[dt][mt] = F16::mfma32(v[dt], p[mt], o[dt][mt]);
+      }
+      buf ^= 1;
+    }
+
+    // Sum of p of every row: over the lane halves and the four waves of its 32 rows.
+    float l_all[2];
+    l_run = xor32_op(l_run, AddOp{});
+    lds_barrier();
+    if (hh == 0) row_max[mg * 32 + l32][kg * 2 + dh] = l_run;
+    lds_barrier();
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const float4 v = *reinterpret_cast<const float4*>(row_max[mt * 32 + l32]);
+      l_all[mt] = (v.x + v.y) + (v.z + v.w);
+    }
+    const bool whole = at == item_start && seg_end == item_end;
+    if (whole) {
+      uint16_t* out = static_cast<uint16_t*>(a.out);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const int m = mt * 32 + l32;
+        if (m < x.count) {
+          const int f = x.first + m, i = f / per, h = f - i * per;
+          const int64_t row = (r.row0 + i) * a.heads + x.g * per + h;
+          const float inv = l_all[mt] == 0.f ? 0.f : 1.f / l_all[mt];
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = wave * 64 + dt * 32 + 8 * e + 4 * hh;
+              const uint2 u = make_uint2(T::pack2(o[dt][mt][4 * e] * inv, o[dt][mt][4 * e + 1] * inv),
+                                         T::pack2(o[dt][mt][4 * e + 2] * inv, o[dt][mt][4 * e + 3] * inv));
+              *reinterpret_cast<uint2*>(&out[row * kCkvDim + d]) = u;
+            }
+          if (a.token_weights != nullptr && wave == 0 && hh == 0)
+            work.lse[row] = m_run[mt] + __builtin_amdgcn_logf(l_all[mt]);
+        }
+      }
+    } else {
+      const bool first_seg = at == part_start(start.plan, part);
+      const int64_t slot = 2 * part + (first_seg ? 0 : 1);
+      float4* p = reinterpret_cast<float4*>(work.part) + slot * (kPartFloats / 4);
+      const bool empty = t0 >= t1;
+      if (!empty) {
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              p[(((wave * 2 + dt) * 2 + mt) * 4 + e) * 64 + lane] =
+                  make_float4(o[dt][mt][4 * e], o[dt][mt][4 * e + 1], o[dt][mt][4 * e + 2], o[dt][mt][4 * e + 3]);
+      }
+      if (wave == 0 && hh == 0) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          work.ml[(slot * kRows + mt * 32 + l32) * 2] = empty ? -INFINITY : m_run[mt];
+          work.ml[(slot * kRows + mt * 32 + l32) * 2 + 1] = l_all[mt];
+        }
+      }
+      // The first border of parts inside an item names it to the joining kernel.
+      if (first_seg && at > item_start && tid == 0 && part_start(start.plan, part - 1) <= item_start) {
+        JoinEntry j;
+        j.row0 = r.row0;
+        j.first = x.first;
+        j.count = x.count;
+        j.g = x.g;
+        j.w0 = static_cast<int32_t>(part - 1);
+        j.slot0 = static_cast<int32_t>(2 * (part - 1) + (part_start(start.plan, part - 1) == item_start ? 0 : 1));
+        j.w1 = static_cast<int32_t>(part_of(start.plan, item_end - 1));
+        work.join[part] = j;
+      }
+    }
+    at = seg_end;
+  }
+}
+
+// Joins the partials of items that lie across parts: block (w, y) takes what
+// part w names; waves take the accumulators' order, 64 lanes a quad of dims.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinBlocks = 16;  // 128 groups of 64 float4 over 16 x 4 waves: 2 a wave
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args a) {
+  const Work work = carve_work(a.workspace, a.parts);
+  const JoinEntry j = work.join[blockIdx.x];
+  if (j.row0 < 0) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int per = static_cast<int>(a.heads / a.latent_heads);
+  for (int grp = blockIdx.y * 4 + wave; grp < 128; grp += 4 * kJoinBlocks) {
+    const int e = grp & 3, mt = (grp >> 2) & 1, dt = (grp >> 3) & 1, dw = grp >> 4;
+    const int m = mt * 32 + (lane & 31);
+    float most = -INFINITY;
+    for (int w = j.w0; w <= j.w1; ++w) {
+      const int64_t slot = w == j.w0 ? j.slot0 : 2 * w;
+      most = fmaxf(most, work.ml[(slot * kRows + m) * 2]);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (most > -INFINITY) {
+      for (int w = j.w0; w <= j.w1; ++w) {
+        const int64_t slot = w == j.w0 ? j.slot0 : 2 * w;
+        const float mw = work.ml[(slot * kRows + m) * 2];
+        if (mw == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(mw - most);
+        l = fmaf(work.ml[(slot * kRows + m) * 2 + 1], f, l);
+        const float4 v = reinterpret_cast<const float4*>(work.part)[slot * (kPartFloats / 4) + grp * 64 + lane];
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+      }
+    }
+    if (m >= j.count) continue;
+    const int f = j.first + m, i = f / per, h = f - i * per;
+    const int64_t row = (j.row0 + i) * a.heads + j.g * per + h;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int d = dw * 64 + dt * 32 + 8 * e + 4 * (lane >> 5);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * kCkvDim + d) =
+        make_uint2(T::pack2(acc.x * inv, acc.y * inv), T::pack2(acc.z * inv, acc.w * inv));
+    if (a.token_weights != nullptr && e == 0 && dt == 0 && dw == 0 && lane < 32)
+      work.lse[row] = most + __builtin_amdgcn_logf(l);
+  }
+}
+
+// -------------------------------------------------------- attention weights
+// token_weights[slot] += sum over the request's (row, head) pairs of p, from
+// the scores once more and the rows' known log-sums.  A unit is one page of
+// one request; a wave holds 32 keys, S^T = K Q^T has keys in registers and
+// pairs in lanes, so the sum over pairs stays in registers until the end.  One
+// workgroup owns a page's weights: no atomics, one order of summation.
+constexpr int kSumThreads = 256;
+constexpr int kQStride = kRow + 8;  // 16-bit row of Q in LDS: 1168 bytes
+template <typename T>
+__global__ __launch_bounds__(kSumThreads, 1) void latent8_weights_kernel(Latent8Args a) {
+  __shared__ __align__(16) uint8_t keys[4][32 * kRow];
+  __shared__ __align__(16) uint16_t q_tile[32 * kQStride];
+  __shared__ float sums[4][32];
+  __shared__ int64_t scratch[kSumThreads / 64];
+  __shared__ int64_t found[3];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int l32 = lane & 31;
+  const int hh = lane >> 5;
+  const Work work = carve_work(a.workspace, a.parts);
+  const int per = static_cast<int>(a.heads / a.latent_heads);
+  auto pages = [&](int64_t b) -> int64_t {
+    const Request r = request_of(a, b);
+    return r.n > 0 ? ceil_div(r.len, kBlock) : 0;
+  };
+  const Start start = find_start<kSumThreads>(a.batch, blockIdx.x, gridDim.x, 1, pages, scratch, found);
+  if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
+  const int64_t stop = part_start(start.plan, blockIdx.x + 1);
+  int64_t b = start.b, base = start.base;
+  for (int64_t at = part_start(start.plan, blockIdx.x); at < stop; ++at) {
+    while (at >= base + pages(b)) {
+      base += pages(b);
+      ++b;
+    }
+    const Request r = request_of(a, b);
+    const int page = static_cast<int>(at - base);
+    const int64_t entry = a.entries[b];
+    const int32_t block = a.block_table[b * a.cols + page];
+    if (entry < 0 || entry >= a.pool_rows || block < 0 || block >= a.blocks) continue;
+    float sum[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+    const int pairs = r.n * per;
+    for (int g = 0; g < a.latent_heads; ++g) {
+      const float c = fminf(fmaxf(a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g], kMinScale), FLT_MAX);
+      const float score = a.scale * kLog2e * c;
+      const uint8_t* src = static_cast<const uint8_t*>(a.latent_cache) +
+                           ((static_cast<int64_t>(block) * kBlock + wave * 32) * a.latent_heads + g) * kRow;
+#pragma unroll
+      for (int i = 0; i < 18; ++i) {  // the wave's own 32 rows
+        const int q = i * 64 + lane;
+        const int k = q / kRowChunks, ch = q - k * kRowChunks;
+        *reinterpret_cast<uint4*>(&keys[wave][k * kRow + ((ch & ~3) | ((ch ^ (k >> 2)) & 3)) * 16]) =
+            *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(k) * a.latent_heads * kRow + ch * 16);
+      }
+      for (int f0 = 0; f0 < pairs; f0 += 32) {
+        __syncthreads();
+        for (int q = tid; q < 32 * 72; q += kSumThreads) {
+          const int m = q / 72, ch = q - m * 72;
+          const int f = f0 + m < pairs ? f0 + m : f0;
+          const int i = f / per, h = f - i * per;
+          const int64_t row = (r.row0 + i) * a.heads + g * per + h;
+          *reinterpret_cast<uint4*>(&q_tile[m * kQStride + ch * 8]) =
+              ch < 64 ? static_cast<const uint4*>(a.query)[row * 64 + ch]
+                      : static_cast<const uint4*>(a.query_rope)[row * 8 + ch - 64];
+        }
+        const int f = f0 + l32;
+        int vis = 0;
+        float lse = 0.f;
+        if (f < pairs) {
+          const int i = f / per, h = f - i * per;
+          vis = visible(r, i);
+          lse = work.lse[(r.row0 + i) * a.heads + g * per + h];
+        }
+        __syncthreads();
+        f32x16_t s;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 18; ++j) {
+          const int ch = 2 * j + hh;
+          const uint4 k = *reinterpret_cast<const uint4*>(
+              &keys[wave][l32 * kRow + ((ch & ~3) | ((ch ^ (l32 >> 2)) & 3)) * 16]);
+          const typename T::vec8 q0 = *reinterpret_cast<const typename T::vec8*>(&q_tile[l32 * kQStride + ch * 16]);
+          const typename T::vec8 q1 = *reinterpret_cast<const typename T::vec8*>(&q_tile[l32 * kQStride + ch * 16 + 8]);
+          s = T::mfma32(widen8<T>(k.x, k.y), q0, s);
+          s = T::mfma32(widen8<T>(k.z, k.w), q1, s);
+        }
+        const int key0 = page * kBlock + wave * 32 + 4 * hh;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = key0 + 8 * (e >> 2) + (e & 3);
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[e], score, -lse));
+          sum[e] += key < vis ? p : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) sum[e] += __shfl_xor(sum[e], x, 64);
+      if (l32 == e) sums[wave][8 * (e >> 2) + 4 * hh + (e & 3)] = sum[e];
+    }
+    __syncthreads();
+    if (tid < kBlock && page * kBlock + tid < r.len)
+      a.token_weights[entry * a.cols * kBlock + page * kBlock + tid] += sums[tid >> 5][tid & 31];
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ eviction
+// Selection: one workgroup per request finds the K-th largest key by three
+// digit counts, then lists holes and sources in slot order.
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr int kDigitBins = 2048;
+
+__device__ inline uint32_t evict_key(const Latent8EvictArgs& a, float w, int32_t pos, int64_t latest) {
+  if (pos < a.protect_first || pos > latest - a.protect_last) return 0xffffffffu;
+  const uint32_t k = float_key(w + 0.f);  // (-0 counts as 0)
+  return k < 0xfffffffeu ? k : 0xfffffffeu;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8EvictArgs a) {
+  __shared__ uint32_t bins[kDigitBins];
+  __shared__ int scratch[kEvictWaves + 1];
+  __shared__ int wave_latest[kEvictWaves];
+  __shared__ int s_bin, s_above;
+  __shared__ int wave_a[kEvictWaves], wave_b[kEvictWaves];
+  const int64_t b = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t cap = a.cols * kBlock;
+  int64_t len64 = a.seq_kv[b];
+  const int len = static_cast<int>(len64 < 0 ? 0 : (len64 > cap ? cap : len64));
+  const int budget = a.budgets[b] < 0 ? 0 : a.budgets[b];
+  const int64_t entry = a.entries[b];
+  const bool known = entry >= 0 && entry < a.pool_rows;
+  const int keep = known && budget < len ? budget : len;
+  if (keep == len || keep == 0) {
+    if (tid == 0) {
+      a.move_counts[b] = 0;
+      a.kept_lengths[b] = keep;
+    }
+    return;
+  }
+  const float* weights = a.token_weights + entry * cap;
+  const int32_t* positions = a.token_positions + entry * cap;
+  // Wave w's slots: [w seg, w seg + seg), 64 a round.
+  const int seg = static_cast<int>(ceil_div(ceil_div(len, kEvictWaves), 64)) * 64;
+  const int s0 = wave * seg, s1 = s0 + seg < len ? s0 + seg : len;
+  int latest = INT32_MIN;
+  for (int s = s0 + lane; s < s1; s += 64) latest = positions[s] > latest ? positions[s] : latest;
+  latest = static_cast<int>(wave_reduce_to_lane63(static_cast<uint32_t>(latest) ^ 0x80000000u, MaxU32Op{}) ^ 0x80000000u);
+  if (lane == 63) wave_latest[wave] = latest;
+  __syncthreads();
+  latest = wave_latest[0];
+  for (int w = 1; w < kEvictWaves; ++w) latest = wave_latest[w] > latest ? wave_latest[w] : latest;
+  auto key_at = [&](int s) { return evict_key(a, weights[s], positions[s], latest); };
+
+  // The keep-th largest key: digits of 11, 11 and 10 bits from the top.
+  uint32_t prefix = 0;
+  int want = keep;  // rank among the keys that share the prefix
+  int shift = 32;
+  for (int round = 0; round < 3; ++round) {
+    const int bits = round < 2 ? 11 : 10;
+    shift -= bits;
+    for (int i = tid; i < kDigitBins; i += kEvictThreads) bins[i] = 0;
+    __syncthreads();
+    for (int s = s0 + lane; s < s1; s += 64) {
+      const uint32_t k = key_at(s);
+      if (round == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << bits) - 1)], 1u);
+    }
+    __syncthreads();
+    // Thread t owns bins top - 2t and top - 2t - 1 (from the largest digit down).
+    const int top = (1 << bits) - 1;
+    const int hi = top - 2 * tid, lo = hi - 1;
+    const int c_hi = hi >= 0 ? static_cast<int>(bins[hi]) : 0, c_lo = lo >= 0 ? static_cast<int>(bins[lo]) : 0;
+    int total;
+    const int before = block_exclusive_scan(c_hi + c_lo, scratch, &total);
+    if (before < want && want <= before + c_hi) {
+      s_bin = hi;
+      s_above = before;
+    } else if (before + c_hi < want && want <= before + c_hi + c_lo) {
+      s_bin = lo;
+      s_above = before + c_hi;
+    }
+    __syncthreads();
+    prefix = (prefix << bits) | static_cast<uint32_t>(s_bin);
+    want -= s_above;
+    __syncthreads();
+  }
+  const uint32_t threshold = prefix;  // `want` of the keys equal to it are kept, the lower slots first
+
+  int equal = 0;
+  for (int r0 = s0; r0 < s1; r0 += 64) {
+    const int s = r0 + lane;
+    equal += __popcll(__ballot(s < s1 && key_at(s) == threshold));
+  }
+  if (lane == 0) wave_a[wave] = equal;
+  __syncthreads();
+  int equal_before = 0;
+  for (int w = 0; w < wave; ++w) equal_before += wave_a[w];
+  __syncthreads();
+  auto walk = [&](auto each) {
+    int eq = equal_before;
+    for (int r0 = s0; r0 < s1; r0 += 64) {
+      const int s = r0 + lane;
+      const uint32_t k = s < s1 ? key_at(s) : 0u;
+      const bool tie = s < s1 && k == threshold;
+      uint64_t ties;
+      const int rank = eq + wave_flag_prefix(tie, &ties);
+      eq += __popcll(ties);
+      const bool kept = s < s1 && (k > threshold || (tie && rank < want));
+      each(r0, s, s < s1 && !kept && s < keep, kept && s >= keep);
+    }
+  };
+  int holes = 0, sources = 0;
+  walk([&](int, int, bool hole, bool source) {
+    holes += __popcll(__ballot(hole));
+    sources += __popcll(__ballot(source));
+  });
+  if (lane == 0) {
+    wave_a[wave] = holes;
+    wave_b[wave] = sources;
+  }
+  __syncthreads();
+  int hole_at = 0, source_at = 0, count = 0;
+  for (int w = 0; w < kEvictWaves; ++w) {
+    if (w < wave) {
+      hole_at += wave_a[w];
+      source_at += wave_b[w];
+    }
+    count += wave_a[w];
+  }
+  int32_t* hole_start = a.hole_start + b * (a.cols + 1);
+  int32_t* dst = a.move_dst + b * cap;
+  int32_t* src = a.move_src + b * cap;
+  walk([&](int r0, int s, bool hole, bool source) {
+    if ((r0 & (kBlock - 1)) == 0 && lane == 0) hole_start[r0 >> kBlockShift] = hole_at;
+    uint64_t hs, ss;
+    const int ha = hole_at + wave_flag_prefix(hole, &hs), sa = source_at + wave_flag_prefix(source, &ss);
+    if (hole) dst[ha] = s;
+    if (source) src[sa] = s;
+    hole_at += __popcll(hs);
+    source_at += __popcll(ss);
+  });
+  if (tid == 0) {
+    a.move_counts[b] = count;
+    a.kept_lengths[b] = keep;
+  }
+  // The page that holds both kept slots and slots beyond the budget may grow
+  // its scale while other pages still read rows from it: its scale as it was.
+  if ((keep & (kBlock - 1)) != 0 && tid < a.latent_heads) {
+    const int32_t block = a.block_table[b * a.cols + (keep >> kBlockShift)];
+    a.border_scale[b * a.latent_heads + tid] =
+        block >= 0 && block < a.blocks ? a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + tid] : 0.f;
+  }
+}
+
+// Moves: one workgroup per (request, page that has holes).
+constexpr int kMoveThreads = 256;
+__global__ __launch_bounds__(kMoveThreads) void latent8_move_kernel(Latent8EvictArgs a) {
+  __shared__ int32_t from[kBlock];  // slot that moves into the page's row, -1: the row stays
+  __shared__ float from_scale[kBlock];
+  __shared__ float wave_top[kMoveThreads / 64];
+  const int64_t b = blockIdx.y;
+  const int tid = threadIdx.x;
+  const int64_t cap = a.cols * kBlock;
+  const int keep = a.kept_lengths[b], count = a.move_counts[b];
+  if (count <= 0) return;
+  const int64_t entry = a.entries[b];
+  const int32_t* table = a.block_table + b * a.cols;
+  const int32_t* hole_start = a.hole_start + b * (a.cols + 1);
+  const int border = (keep & (kBlock - 1)) != 0 ? keep >> kBlockShift : -1;
+  const int pages = static_cast<int>(ceil_div(keep, kBlock));
+  for (int page = blockIdx.x; page < pages; page += gridDim.x) {
+    const int h0 = hole_start[page], h1 = page + 1 < pages ? hole_start[page + 1] : count;
+    const int n = h1 - h0;
+    const int32_t block = table[page];
+    if (n <= 0) continue;
+    const int rows = keep - page * kBlock < kBlock ? keep - page * kBlock : kBlock;
+    __syncthreads();
+    if (tid < kBlock) from[tid] = -1;
+    __syncthreads();
+    int64_t src = 0;
+    int dst = 0;
+    if (tid < n) {
+      src = a.move_src[b * cap + h0 + tid];
+      dst = a.move_dst[b * cap + h0 + tid] - page * kBlock;
+      from[dst] = static_cast<int32_t>(src);
+      float* w = a.token_weights + entry * cap;
+      int32_t* p = a.token_positions + entry * cap;
+      w[page * kBlock + dst] = w[src];
+      p[page * kBlock + dst] = p[src];
+    }
+    if (block < 0 || block >= a.blocks) continue;
+    for (int g = 0; g < a.latent_heads; ++g) {
+      float* scale_at = a.cache_scale + static_cast<int64_t>(block) * a.latent_heads + g;
+      const float old = *scale_at;
+      float mine = 0.f;
+      if (tid < n) {
+        const int sp = static_cast<int>(src >> kBlockShift);
+        const int32_t sb = table[sp];
+        if (sp == border)
+          mine = a.border_scale[b * a.latent_heads + g];
+        else if (sb >= 0 && sb < a.blocks)
+          mine = a.cache_scale[static_cast<int64_t>(sb) * a.latent_heads + g];
+      }
+      __syncthreads();  // (every thread has read the old scale and is done with the last head's)
+      if (tid < n) from_scale[dst] = mine;
+      const float top = wave_all_op(mine, MaxOp{});
+      if ((tid & 63) == 0) wave_top[tid >> 6] = top;
+      __syncthreads();
+      float now = old;
+      for (int w = 0; w < kMoveThreads / 64; ++w) now = fmaxf(now, wave_top[w]);
+      const float stay = old / now;
+      const int64_t stride = a.latent_heads * kRow;
+      uint8_t* cache = static_cast<uint8_t*>(a.latent_cache);
+      uint8_t* base = cache + (static_cast<int64_t>(block) * kBlock * a.latent_heads + g) * kRow;
+      for (int q = tid; q < rows * kRowChunks; q += kMoveThreads) {
+        const int r = q / kRowChunks, c = q - r * kRowChunks;
+        const int s = from[r];
+        if (s < 0 && now == old) continue;
+        uint4* to = reinterpret_cast<uint4*>(base + r * stride) + c;
+        if (s < 0) {
+          *to = rescale16(*to, stay);
+        } else {
+          const int32_t sb = table[s >> kBlockShift];
+          if (sb < 0 || sb >= a.blocks) continue;
+          const uint4 v = *(reinterpret_cast<const uint4*>(
+                                cache + ((static_cast<int64_t>(sb) * kBlock + (s & (kBlock - 1))) * a.latent_heads + g) *
+                                            kRow) +
+                            c);
+          *to = rescale16(v, from_scale[r] / now);
+        }
+      }
+      if (tid == 0 && now != old) *scale_at = now;
+    }
+  }
+}
+
+// Items of a launch are at most this many (for the check of 64-bit products).
+constexpr int64_t kParts = 256;  // one workgroup per CU (LDS)
+
+}  // namespace
+
+// ------------------------------------------------------------------- launches
+hipError_t launch_latent8_append(const Latent8AppendArgs& a, hipStream_t stream) {
+  if (a.rows == 0 || a.batch == 0) return hipSuccess;
+  // A request of n rows touches at most n pages and at most n / 128 + 2.
+  const int64_t pages = std::min(a.rows, a.rows / kBlock + 2 * std::min(a.batch, a.rows));
+  const dim3 grid(static_cast<unsigned>(pages), static_cast<unsigned>(a.latent_heads));
+  if (a.elem == Elem::kBf16)
+    launch_kernel(kKernLatent8Append, latent8_append_kernel<Bf16>, grid, dim3(kAppendThreads), stream, a);
+  else
+    launch_kernel(kKernLatent8Append, latent8_append_kernel<F16>, grid, dim3(kAppendThreads), stream, a);
+  return hipGetLastError();
+}
+
+size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights) {
+  return sizeof(float) * 2 * kParts * (kPartFloats + kRows * 2) + round256(sizeof(JoinEntry) * kParts) +
+         (weights ? sizeof(float) * rows * heads : 0);
+}
+
+template <typename T>
+static void attend(const Latent8Args& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.parts));
+  if (a.topk != nullptr)
+    launch_kernel(kKernLatent8Attention, latent8_attention_kernel<T, true>, grid, dim3(kAttnThreads), stream, a);
+  else
+    launch_kernel(kKernLatent8Attention, latent8_attention_kernel<T, false>, grid, dim3(kAttnThreads), stream, a);
+  launch_kernel(kKernLatent8Join, latent8_join_kernel<T>, dim3(static_cast<unsigned>(a.parts), kJoinBlocks),
+                dim3(kJoinThreads), stream, a);
+  if (a.token_weights != nullptr)
+    launch_kernel(kKernLatent8Weights, latent8_weights_kernel<T>, dim3(512), dim3(kSumThreads), stream, a);
+}
+
+hipError_t launch_latent8_attention(const Latent8Args& args, hipStream_t stream) {
+  if (args.rows == 0 || args.batch == 0) return hipSuccess;
+  Latent8Args a = args;
+  a.parts = kParts;
+  if (a.elem == Elem::kBf16)
+    attend<Bf16>(a, stream);
+  else
+    attend<F16>(a, stream);
+  return hipGetLastError();
+}
+
+size_t latent8_evict_workspace_bytes(int64_t batch, int64_t cols, int64_t latent_heads) {
+  return round256(sizeof(int32_t) * batch * (cols + 1)) + sizeof(float) * batch * latent_heads;
+}
+
+hipError_t launch_latent8_evict(const Latent8EvictArgs& args, hipStream_t stream) {
+  if (args.batch == 0) return hipSuccess;
+  Latent8EvictArgs a = args;
+  a.hole_start = static_cast<int32_t*>(a.workspace);
+  a.border_scale = reinterpret_cast<float*>(static_cast<char*>(a.workspace) +
+                                            round256(sizeof(int32_t) * a.batch * (a.cols + 1)));
+  launch_kernel(kKernLatent8Select, latent8_select_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(kEvictThreads),
+                stream, a);
+  launch_kernel(kKernLatent8Move, latent8_move_kernel,
+                dim3(static_cast<unsigned>(std::min<int64_t>(a.cols, 64)), static_cast<unsigned>(a.batch)),
+                dim3(kMoveThreads), stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace nvdsa

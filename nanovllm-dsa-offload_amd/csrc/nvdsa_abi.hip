@@ -186,7 +186,9 @@ const char* nvdsa_kernel_name(int32_t kernel_id) {
                                 "indexer_rope_kernel", "persist_blocks_kernel", "lim_classify_kernel",
                                 "lim_chunks_kernel",   "lim_resolve_kernel",
                                 "indexer_kw_kernel",   "indexer_kw_finish_kernel",
-                                "stage_inputs_kernel"};
+                                "stage_inputs_kernel",  "latent8_append_kernel",
+                                "latent8_attention_kernel", "latent8_join_kernel",
+                                "latent8_weights_kernel", "latent8_select_kernel", "latent8_move_kernel"};
   static_assert(sizeof(names) / sizeof(names[0]) == nvdsa::kKernCount, "one name per kernel id");
   if (kernel_id < 0 || kernel_id >= nvdsa::kKernCount) return "unknown";
   return names[kernel_id];
@@ -1267,6 +1269,268 @@ int nvdsa_stage_inputs(const nvdsa_stage_item* items, int64_t count, void* strea
          reads ? it.src_stride : 0, static_cast<int32_t>(f), 0};
   }
   return launch_status(nvdsa::launch_stage_inputs(a, static_cast<hipStream_t>(stream)), "stage_inputs");
+}
+
+// ------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+// The cache, its scales and the page tables that the three entry points share.
+void check_latent_cache(Check& c, const nvdsa_tensor* latent_cache, const nvdsa_tensor* cache_scale,
+                        const nvdsa_tensor* block_table, int64_t batch) {
+  c.need(dims_are(latent_cache, 4) && sz(latent_cache, 0) > 0 && sz(latent_cache, 1) == 128 &&
+             sz(latent_cache, 2) > 0 && sz(latent_cache, 3) == nvdsa::kQkDim,
+         NVDSA_ERR_SHAPE, "latent_cache must be [blocks, 128, latent heads, 576]")
+      .need(sz(latent_cache, 0) < (int64_t{1} << 24), NVDSA_ERR_SHAPE, "latent_cache holds too many blocks")
+      .need(sz(latent_cache, 2) <= 1024, NVDSA_ERR_SHAPE, "at most 1024 latent heads")
+      .need(latent_cache->dtype == NVDSA_FLOAT8_E4M3, NVDSA_ERR_DTYPE, "latent_cache must be float8_e4m3fn")
+      .need(dims_are(cache_scale, 2) && sz(cache_scale, 0) == sz(latent_cache, 0) &&
+                sz(cache_scale, 1) == sz(latent_cache, 2),
+            NVDSA_ERR_SHAPE, "cache_scale must be [blocks, latent heads]")
+      .need(cache_scale->dtype == NVDSA_FLOAT32, NVDSA_ERR_DTYPE, "cache_scale must be float32")
+      .need(dims_are(block_table, 2) && sz(block_table, 0) == batch && sz(block_table, 1) > 0, NVDSA_ERR_SHAPE,
+            "block_table must be [B, columns]")
+      .need(sz(block_table, 1) <= (1 << 14), NVDSA_ERR_SHAPE, "block-table capacity must be <= 16384 blocks")
+      .need(batch < (1 << 16), NVDSA_ERR_SHAPE, "batch must be < 65536")
+      .need(block_table->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE, "block_table must be int32");
+}
+
+void check_lengths(Check& c, const nvdsa_tensor* t, int64_t batch, const char* msg) {
+  c.need(dims_are(t, 1) && sz(t, 0) == batch, NVDSA_ERR_SHAPE, msg)
+      .need(t->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE, "lengths, counts and pool entries must be int32");
+}
+
+// A pool row record [pool_rows, columns * 128].
+void check_records(Check& c, const nvdsa_tensor* t, const nvdsa_tensor* block_table, int dtype, const char* msg) {
+  c.need(dims_are(t, 2) && sz(t, 0) > 0 && sz(t, 1) == sz(block_table, 1) * 128, NVDSA_ERR_SHAPE, msg)
+      .need(t->dtype == dtype, NVDSA_ERR_DTYPE, "token positions must be int32, token weights float32");
+}
+
+void check_optional(Check& c, const nvdsa_tensor* t, int device) {
+  if (t == nullptr) return;
+  const nvdsa_tensor* const one[] = {t};
+  check_common(c, one, device);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nvdsa_latent8_append(const nvdsa_tensor* kv, const nvdsa_tensor* k_rope,
+                         const nvdsa_tensor* actual_seq_lengths_query, const nvdsa_tensor* actual_seq_lengths_kv,
+                         const nvdsa_tensor* block_table, const nvdsa_tensor* latent_cache,
+                         const nvdsa_tensor* cache_scale, const nvdsa_tensor* positions,
+                         const nvdsa_tensor* req_pool_entries, const nvdsa_tensor* token_positions,
+                         const nvdsa_tensor* token_weights, void* stream) {
+  const nvdsa_tensor* const all[] = {kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
+                                     latent_cache, cache_scale};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "latent8_append: null tensor argument");
+  Check c("latent8_append");
+  c.need((positions != nullptr) == (token_positions != nullptr), NVDSA_ERR_ARG,
+         "positions and token_positions go together")
+      .need((req_pool_entries != nullptr) == (token_positions != nullptr || token_weights != nullptr), NVDSA_ERR_ARG,
+            "req_pool_entries goes with token_positions or token_weights")
+      .need(dims_are(actual_seq_lengths_query, 1), NVDSA_ERR_SHAPE, "actual_seq_lengths_query must be rank one");
+  const int64_t B = sz(actual_seq_lengths_query, 0);
+  if (c.ok()) check_latent_cache(c, latent_cache, cache_scale, block_table, B);
+  if (c.ok()) {
+    const int64_t T = sz(kv, 0), G = sz(latent_cache, 2);
+    c.need(dims_are(kv, 3) && sz(kv, 1) == G && sz(kv, 2) == nvdsa::kCkvDim, NVDSA_ERR_SHAPE,
+           "kv must be [T, latent heads, 512]")
+        .need(dims_are(k_rope, 3) && sz(k_rope, 0) == T && sz(k_rope, 1) == G && sz(k_rope, 2) == nvdsa::kKpeDim,
+              NVDSA_ERR_SHAPE, "k_rope must be [T, latent heads, 64]")
+        .need(T < (int64_t{1} << 30), NVDSA_ERR_SHAPE, "too many rows")
+        .need(is_half(kv) && kv->dtype == k_rope->dtype, NVDSA_ERR_DTYPE, "kv and k_rope must share one 16-bit dtype");
+    check_lengths(c, actual_seq_lengths_query, B, "actual_seq_lengths_query must be [B]");
+    check_lengths(c, actual_seq_lengths_kv, B, "actual_seq_lengths_kv must be [B]");
+    if (req_pool_entries) check_lengths(c, req_pool_entries, B, "req_pool_entries must be [B]");
+    if (positions) check_lengths(c, positions, T, "positions must be [T]");
+    if (token_positions)
+      check_records(c, token_positions, block_table, NVDSA_INT32, "token_positions must be [pool rows, columns * 128]");
+    if (token_weights)
+      check_records(c, token_weights, block_table, NVDSA_FLOAT32, "token_weights must be [pool rows, columns * 128]");
+    if (token_positions && token_weights)
+      c.need(same_shape(token_positions, token_weights), NVDSA_ERR_SHAPE, "token records must have one shape");
+    check_common(c, all, latent_cache->device);
+    for (const auto* t : {positions, req_pool_entries, token_positions, token_weights})
+      check_optional(c, t, latent_cache->device);
+    c.need(latent_cache->device >= 0, NVDSA_ERR_DEVICE, "latent_cache must be on a GPU")
+        .need(aligned16(kv) && aligned16(k_rope) && aligned16(latent_cache), NVDSA_ERR_LAYOUT,
+              "kv, k_rope and latent_cache must be 16-byte aligned");
+  }
+  if (!c.ok()) return c.finish();
+  nvdsa::Latent8AppendArgs a{};
+  a.kv = kv->data;
+  a.k_rope = k_rope->data;
+  a.positions = positions ? static_cast<const int32_t*>(positions->data) : nullptr;
+  a.seq_q = static_cast<const int32_t*>(actual_seq_lengths_query->data);
+  a.seq_kv = static_cast<const int32_t*>(actual_seq_lengths_kv->data);
+  a.block_table = static_cast<const int32_t*>(block_table->data);
+  a.entries = req_pool_entries ? static_cast<const int32_t*>(req_pool_entries->data) : nullptr;
+  a.latent_cache = latent_cache->data;
+  a.cache_scale = static_cast<float*>(cache_scale->data);
+  a.token_positions = token_positions ? static_cast<int32_t*>(token_positions->data) : nullptr;
+  a.token_weights = token_weights ? static_cast<float*>(token_weights->data) : nullptr;
+  a.rows = sz(kv, 0);
+  a.batch = B;
+  a.cols = sz(block_table, 1);
+  a.blocks = sz(latent_cache, 0);
+  a.latent_heads = sz(latent_cache, 2);
+  a.pool_rows = token_positions ? sz(token_positions, 0) : (token_weights ? sz(token_weights, 0) : 0);
+  a.elem = elem_of(kv);
+  return launch_status(nvdsa::launch_latent8_append(a, static_cast<hipStream_t>(stream)), "latent8_append");
+}
+
+size_t nvdsa_latent8_attention_workspace_size(int64_t query_rows, int64_t heads, int32_t with_weights) {
+  if (query_rows < 0 || heads < 0) return 0;
+  return nvdsa::latent8_attention_workspace_bytes(query_rows, heads, with_weights != 0);
+}
+
+int nvdsa_latent8_attention(const nvdsa_tensor* query_rope, const nvdsa_tensor* query,
+                            const nvdsa_tensor* actual_seq_lengths_query, const nvdsa_tensor* actual_seq_lengths_kv,
+                            const nvdsa_tensor* block_table, const nvdsa_tensor* latent_cache,
+                            const nvdsa_tensor* cache_scale, const nvdsa_tensor* topk_ids,
+                            const nvdsa_tensor* req_pool_entries, const nvdsa_tensor* token_weights,
+                            double scale_value, const nvdsa_tensor* attention_out, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const nvdsa_tensor* const all[] = {query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
+                                     latent_cache, cache_scale, attention_out};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "latent8_attention: null tensor argument");
+  Check c("latent8_attention");
+  c.need((req_pool_entries != nullptr) == (token_weights != nullptr), NVDSA_ERR_ARG,
+         "req_pool_entries and token_weights go together")
+      .need(topk_ids == nullptr || token_weights == nullptr, NVDSA_ERR_ARG,
+            "token_weights are accumulated over every cached token: not with topk_ids")
+      .need(dims_are(actual_seq_lengths_query, 1), NVDSA_ERR_SHAPE, "actual_seq_lengths_query must be rank one");
+  const int64_t B = sz(actual_seq_lengths_query, 0);
+  if (c.ok()) check_latent_cache(c, latent_cache, cache_scale, block_table, B);
+  if (c.ok()) {
+    const int64_t T = sz(query, 0), N = sz(query, 1), G = sz(latent_cache, 2);
+    c.need(dims_are(query, 3) && sz(query, 2) == nvdsa::kCkvDim, NVDSA_ERR_SHAPE, "query must be [T, heads, 512]")
+        .need(dims_are(query_rope, 3) && sz(query_rope, 0) == T && sz(query_rope, 1) == N &&
+                  sz(query_rope, 2) == nvdsa::kKpeDim,
+              NVDSA_ERR_SHAPE, "query_rope must be [T, heads, 64]")
+        .need(N > 0 && N <= 1024 && N % G == 0, NVDSA_ERR_SHAPE,
+              "heads must be a multiple of the latent heads, at most 1024")
+        .need(T < (int64_t{1} << 20), NVDSA_ERR_SHAPE, "too many query rows")
+        .need(same_shape(attention_out, query), NVDSA_ERR_SHAPE, "attention_out must match query")
+        .need(is_half(query) && query->dtype == query_rope->dtype && query->dtype == attention_out->dtype,
+              NVDSA_ERR_DTYPE, "query, query_rope and attention_out must share one 16-bit dtype");
+    check_lengths(c, actual_seq_lengths_query, B, "actual_seq_lengths_query must be [B]");
+    check_lengths(c, actual_seq_lengths_kv, B, "actual_seq_lengths_kv must be [B]");
+    if (topk_ids)
+      c.need(dims_are(topk_ids, 2) && sz(topk_ids, 0) == T && sz(topk_ids, 1) > 0 && sz(topk_ids, 1) <= (1 << 21),
+             NVDSA_ERR_SHAPE, "topk_ids must be [T, list length]")
+          .need(topk_ids->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE, "topk_ids must be int32");
+    if (req_pool_entries) check_lengths(c, req_pool_entries, B, "req_pool_entries must be [B]");
+    if (token_weights)
+      check_records(c, token_weights, block_table, NVDSA_FLOAT32, "token_weights must be [pool rows, columns * 128]");
+    check_common(c, all, latent_cache->device);
+    for (const auto* t : {topk_ids, req_pool_entries, token_weights}) check_optional(c, t, latent_cache->device);
+    c.need(latent_cache->device >= 0, NVDSA_ERR_DEVICE, "latent_cache must be on a GPU")
+        .need(aligned16(query) && aligned16(query_rope) && aligned16(latent_cache) && aligned16(attention_out),
+              NVDSA_ERR_LAYOUT, "query, query_rope, latent_cache and attention_out must be 16-byte aligned");
+  }
+  if (!c.ok()) return c.finish();
+  const int64_t T = sz(query, 0), N = sz(query, 1);
+  if (T == 0 || B == 0) return NVDSA_OK;
+  if (workspace == nullptr ||
+      workspace_bytes < nvdsa::latent8_attention_workspace_bytes(T, N, token_weights != nullptr))
+    return fail(NVDSA_ERR_WORKSPACE, "latent8_attention: workspace too small");
+  nvdsa::Latent8Args a{};
+  a.query = query->data;
+  a.query_rope = query_rope->data;
+  a.seq_q = static_cast<const int32_t*>(actual_seq_lengths_query->data);
+  a.seq_kv = static_cast<const int32_t*>(actual_seq_lengths_kv->data);
+  a.block_table = static_cast<const int32_t*>(block_table->data);
+  a.latent_cache = latent_cache->data;
+  a.cache_scale = static_cast<const float*>(cache_scale->data);
+  a.topk = topk_ids ? static_cast<const int32_t*>(topk_ids->data) : nullptr;
+  a.entries = req_pool_entries ? static_cast<const int32_t*>(req_pool_entries->data) : nullptr;
+  a.token_weights = token_weights ? static_cast<float*>(token_weights->data) : nullptr;
+  a.out = attention_out->data;
+  a.rows = T;
+  a.heads = N;
+  a.latent_heads = sz(latent_cache, 2);
+  a.batch = B;
+  a.cols = sz(block_table, 1);
+  a.blocks = sz(latent_cache, 0);
+  a.list_len = topk_ids ? sz(topk_ids, 1) : 0;
+  a.pool_rows = token_weights ? sz(token_weights, 0) : 0;
+  a.scale = static_cast<float>(scale_value);
+  a.elem = elem_of(query);
+  a.workspace = workspace;
+  return launch_status(nvdsa::launch_latent8_attention(a, static_cast<hipStream_t>(stream)), "latent8_attention");
+}
+
+size_t nvdsa_latent8_evict_workspace_size(int64_t batch, int64_t table_cols, int64_t latent_heads) {
+  if (batch < 0 || table_cols < 0 || latent_heads < 0) return 0;
+  return nvdsa::latent8_evict_workspace_bytes(batch, table_cols, latent_heads);
+}
+
+int nvdsa_latent8_evict(const nvdsa_tensor* actual_seq_lengths_kv, const nvdsa_tensor* budgets,
+                        const nvdsa_tensor* block_table, const nvdsa_tensor* req_pool_entries,
+                        const nvdsa_tensor* latent_cache, const nvdsa_tensor* cache_scale,
+                        const nvdsa_tensor* token_positions, const nvdsa_tensor* token_weights, int64_t protect_first,
+                        int64_t protect_last, const nvdsa_tensor* move_src_slots, const nvdsa_tensor* move_dst_slots,
+                        const nvdsa_tensor* move_counts, const nvdsa_tensor* kept_lengths, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  const nvdsa_tensor* const all[] = {actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache,
+                                     cache_scale, token_positions, token_weights, move_src_slots, move_dst_slots,
+                                     move_counts, kept_lengths};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "latent8_evict: null tensor argument");
+  Check c("latent8_evict");
+  c.need(protect_first >= 0 && protect_last >= 0 && protect_first <= INT32_MAX && protect_last <= INT32_MAX,
+         NVDSA_ERR_ARG, "protect_first and protect_last must not be negative")
+      .need(dims_are(actual_seq_lengths_kv, 1), NVDSA_ERR_SHAPE, "actual_seq_lengths_kv must be rank one");
+  const int64_t B = sz(actual_seq_lengths_kv, 0);
+  if (c.ok()) check_latent_cache(c, latent_cache, cache_scale, block_table, B);
+  if (c.ok()) {
+    check_lengths(c, actual_seq_lengths_kv, B, "actual_seq_lengths_kv must be [B]");
+    check_lengths(c, budgets, B, "budgets must be [B]");
+    check_lengths(c, req_pool_entries, B, "req_pool_entries must be [B]");
+    check_lengths(c, move_counts, B, "move_counts must be [B]");
+    check_lengths(c, kept_lengths, B, "kept_lengths must be [B]");
+    check_records(c, token_positions, block_table, NVDSA_INT32, "token_positions must be [pool rows, columns * 128]");
+    check_records(c, token_weights, block_table, NVDSA_FLOAT32, "token_weights must be [pool rows, columns * 128]");
+    c.need(same_shape(token_positions, token_weights), NVDSA_ERR_SHAPE, "token records must have one shape")
+        .need(dims_are(move_src_slots, 2) && sz(move_src_slots, 0) == B &&
+                  sz(move_src_slots, 1) == sz(block_table, 1) * 128 && same_shape(move_src_slots, move_dst_slots),
+              NVDSA_ERR_SHAPE, "move_src_slots and move_dst_slots must be [B, columns * 128]")
+        .need(move_src_slots->dtype == NVDSA_INT32 && move_dst_slots->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE,
+              "move lists must be int32");
+    check_common(c, all, latent_cache->device);
+    c.need(latent_cache->device >= 0, NVDSA_ERR_DEVICE, "latent_cache must be on a GPU")
+        .need(aligned16(latent_cache), NVDSA_ERR_LAYOUT, "latent_cache must be 16-byte aligned");
+  }
+  if (!c.ok()) return c.finish();
+  if (B == 0) return NVDSA_OK;
+  const int64_t cols = sz(block_table, 1), G = sz(latent_cache, 2);
+  if (workspace == nullptr || workspace_bytes < nvdsa::latent8_evict_workspace_bytes(B, cols, G))
+    return fail(NVDSA_ERR_WORKSPACE, "latent8_evict: workspace too small");
+  nvdsa::Latent8EvictArgs a{};
+  a.seq_kv = static_cast<const int32_t*>(actual_seq_lengths_kv->data);
+  a.budgets = static_cast<const int32_t*>(budgets->data);
+  a.block_table = static_cast<const int32_t*>(block_table->data);
+  a.entries = static_cast<const int32_t*>(req_pool_entries->data);
+  a.latent_cache = latent_cache->data;
+  a.cache_scale = static_cast<float*>(cache_scale->data);
+  a.token_positions = static_cast<int32_t*>(token_positions->data);
+  a.token_weights = static_cast<float*>(token_weights->data);
+  a.move_src = static_cast<int32_t*>(move_src_slots->data);
+  a.move_dst = static_cast<int32_t*>(move_dst_slots->data);
+  a.move_counts = static_cast<int32_t*>(move_counts->data);
+  a.kept_lengths = static_cast<int32_t*>(kept_lengths->data);
+  a.batch = B;
+  a.cols = cols;
+  a.blocks = sz(latent_cache, 0);
+  a.latent_heads = G;
+  a.pool_rows = sz(token_positions, 0);
+  a.protect_first = protect_first;
+  a.protect_last = protect_last;
+  a.workspace = workspace;
+  return launch_status(nvdsa::launch_latent8_evict(a, static_cast<hipStream_t>(stream)), "latent8_evict");
 }
 
 // ------------------------------------------------------------------------

@@ -36,7 +36,13 @@ enum KernelId : int {
   kKernIdxKw = 20,
   kKernIdxKwFinish = 21,
   kKernStage = 22,
-  kKernCount = 23
+  kKernLatent8Append = 23,
+  kKernLatent8Attention = 24,
+  kKernLatent8Join = 25,
+  kKernLatent8Weights = 26,
+  kKernLatent8Select = 27,
+  kKernLatent8Move = 28,
+  kKernCount = 29
 };
 // Timing events for the next launch of `kernel_id` when instrumentation is
 // on for the calling thread (nvdsa_profile_begin); both null otherwise.
@@ -268,5 +274,66 @@ struct StageArgs {
   int32_t count;
 };
 hipError_t launch_stage_inputs(StageArgs& a, hipStream_t stream);
+
+// ---- 8-bit latent cache -----------------------------------------------------
+struct Latent8AppendArgs {
+  const void* kv;               // [rows, G, 512] 16-bit
+  const void* k_rope;           // [rows, G, 64]
+  const int32_t* positions;     // [rows] (with token_positions)
+  const int32_t* seq_q;         // [B] end of each request's rows
+  const int32_t* seq_kv;        // [B] cached tokens, the new ones among them
+  const int32_t* block_table;   // [B, cols]
+  const int32_t* entries;       // [B], or null: no token records
+  void* latent_cache;           // [blocks, 128, G, 576] e4m3
+  float* cache_scale;           // [blocks, G]
+  int32_t* token_positions;     // [pool_rows, cols * 128], or null
+  float* token_weights;         // [pool_rows, cols * 128], or null
+  int64_t rows, batch, cols, blocks, latent_heads, pool_rows;
+  Elem elem;
+};
+hipError_t launch_latent8_append(const Latent8AppendArgs& a, hipStream_t stream);
+
+struct Latent8Args {
+  const void* query;            // [rows, heads, 512] 16-bit
+  const void* query_rope;       // [rows, heads, 64]
+  const int32_t* seq_q;         // [B] end of each request's rows
+  const int32_t* seq_kv;        // [B]
+  const int32_t* block_table;   // [B, cols]
+  const void* latent_cache;     // [blocks, 128, G, 576] e4m3
+  const float* cache_scale;     // [blocks, G]
+  const int32_t* topk;          // [rows, list_len], or null: every cached token
+  const int32_t* entries;       // [B] (with token_weights)
+  float* token_weights;         // [pool_rows, cols * 128], or null
+  void* out;                    // [rows, heads, 512]
+  int64_t rows, heads, latent_heads, batch, cols, blocks, list_len, pool_rows;
+  int64_t parts;                // set by the launch
+  float scale;
+  Elem elem;
+  void* workspace;
+};
+size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights);
+hipError_t launch_latent8_attention(const Latent8Args& a, hipStream_t stream);
+
+struct Latent8EvictArgs {
+  const int32_t* seq_kv;        // [B]
+  const int32_t* budgets;       // [B]
+  const int32_t* block_table;   // [B, cols]
+  const int32_t* entries;       // [B]
+  void* latent_cache;           // [blocks, 128, G, 576] e4m3
+  float* cache_scale;           // [blocks, G]
+  int32_t* token_positions;     // [pool_rows, cols * 128]
+  float* token_weights;         // [pool_rows, cols * 128]
+  int32_t* move_src;            // [B, cols * 128]
+  int32_t* move_dst;            // [B, cols * 128]
+  int32_t* move_counts;         // [B]
+  int32_t* kept_lengths;        // [B]
+  int64_t batch, cols, blocks, latent_heads, pool_rows;
+  int64_t protect_first, protect_last;
+  void* workspace;
+  int32_t* hole_start;          // workspace, set by the launch: [B, cols + 1]
+  float* border_scale;          // [B, G]
+};
+size_t latent8_evict_workspace_bytes(int64_t batch, int64_t cols, int64_t latent_heads);
+hipError_t launch_latent8_evict(const Latent8EvictArgs& a, hipStream_t stream);
 
 }  // namespace nvdsa

@@ -20,7 +20,7 @@ import torch  # noqa: F401  -- must precede the CDLL load (shared HIP runtime)
 LIB_PATH = Path(__file__).resolve().parent / "libnvdsa.so"
 
 # nvdsa_dtype
-INT32, FLOAT16, BFLOAT16, FLOAT32 = 0, 1, 2, 3
+INT32, FLOAT16, BFLOAT16, FLOAT32, FLOAT8_E4M3 = 0, 1, 2, 3, 4
 HOST_MAPPED_DEVICE = -1
 _NOT_DEVICE = -2  # ordinary (pageable) CPU memory: rejected by every entry point
 
@@ -90,6 +90,11 @@ EXT_SIGNATURES = {
     "nvdsa_dsa_indexer_project_kw_workspace_size": ([_I64, _I64, _I64, ctypes.c_int32], _SZ),
     "nvdsa_stage_inputs": ([_VP, _I64, _VP], ctypes.c_int),
     "nvdsa_dsa_indexer_project_kw": ([_P] * 9 + [_I64, _DBL, _VP, _SZ, _VP], ctypes.c_int),
+    "nvdsa_latent8_append": ([_P] * 11 + [_VP], ctypes.c_int),
+    "nvdsa_latent8_attention_workspace_size": ([_I64, _I64, ctypes.c_int32], _SZ),
+    "nvdsa_latent8_attention": ([_P] * 10 + [_DBL, _P, _VP, _SZ, _VP], ctypes.c_int),
+    "nvdsa_latent8_evict_workspace_size": ([_I64, _I64, _I64], _SZ),
+    "nvdsa_latent8_evict": ([_P] * 8 + [_I64, _I64] + [_P] * 4 + [_VP, _SZ, _VP], ctypes.c_int),
 }
 
 
@@ -130,6 +135,7 @@ _DTYPE_CODES = {
     torch.float16: FLOAT16,
     torch.bfloat16: BFLOAT16,
     torch.float32: FLOAT32,
+    torch.float8_e4m3fn: FLOAT8_E4M3,
 }
 
 
