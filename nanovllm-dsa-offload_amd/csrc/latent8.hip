@@ -1018,112 +1018,212 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
 
 // -------------------------------------------------------- attention weights
 // token_weights[slot] += sum over the request's (row, head) pairs of p, from
-// the scores once more and the rows' known log-sums.  A unit is one page of
-// one request; a wave holds 32 keys, S^T = K Q^T has keys in registers and
-// pairs in lanes, so the sum over pairs stays in registers until the end.  One
-// workgroup owns a page's weights: no atomics, one order of summation.
-constexpr int kSumThreads = 256;
-constexpr int kQStride = kRow + 8;  // 16-bit row of Q in LDS: 1168 bytes
+// the scores once more and the rows' known log-sums.  S^T = K Q^T has keys in
+// registers and pairs in lanes, so that the sum over pairs stays in registers.
+// A wave takes slices of 32 keys, their codes in its registers; 128 pairs lie
+// in LDS, and the waves go through the slices of the workgroup's run without a
+// barrier, each next slice loaded into the registers that the last product
+// leaves.  Every slot has one owner: no atomics, one order of summation.
+//
+// Bound by the cache's bytes and the products alike: 24 requests of 8,192
+// tokens and 128 heads, 113 MB and 29 GFLOP, in 39 us, of which 13 pass before
+// the first product (the part's place 4, the pairs' rows and the first codes 9).
+// One workgroup a page, its codes and 32 pairs at a time in LDS, took 111.
+constexpr int kSumThreads = 512;
+constexpr int kSumWaves = kSumThreads / 64;
+constexpr int kSumPairs = 128;
+constexpr int kSumKeys = 32;   // keys of a slice
+constexpr int kSumRun = 96;    // slices whose sums over the blocks of pairs are held at a time
+constexpr int kSumParts = 256; // one workgroup per CU (LDS)
 template <typename T>
-__global__ __launch_bounds__(kSumThreads, 1) void latent8_weights_kernel(Latent8Args a) {
-  __shared__ __align__(16) uint8_t keys[4][32 * kRow];
-  __shared__ __align__(16) uint16_t q_tile[32 * kQStride];
-  __shared__ float sums[4][32];
-  __shared__ int64_t scratch[kSumThreads / 64];
+__global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8Args a) {
+  __shared__ __align__(16) uint8_t q_tile[kSumPairs * kRow * 2];
+  __shared__ float sums[kSumRun * kSumKeys];
+  __shared__ float pair_lse[kSumPairs];
+  __shared__ int pair_vis[kSumPairs];
+  __shared__ int64_t scratch[kSumWaves];
   __shared__ int64_t found[2];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int wave = tid >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31;
   const int hh = lane >> 5;
   const Work work = carve_work(a.workspace, a.parts);
   const int per = static_cast<int>(a.heads / a.latent_heads);
-  auto pages = [&](int64_t b) -> int64_t {
+  const int64_t row_bytes = a.latent_heads * kRow;
+  auto slices = [&](int64_t b) -> int64_t {
     const Request r = request_of(a, b);
-    return r.n > 0 ? ceil_div(r.len, kBlock) : 0;
+    return r.n > 0 ? ceil_div(r.len, kSumKeys) : 0;
   };
-  const Start start = find_start<kSumThreads>(a.batch, blockIdx.x, gridDim.x, 1, pages, scratch, found);
+  const Start start = find_start<kSumThreads>(a.batch, blockIdx.x, kSumParts, kSumWaves, slices, scratch, found);
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
   int64_t b = start.b, base = start.base;
-  for (int64_t at = part_start(start.plan, blockIdx.x); at < stop; ++at) {
-    while (at >= base + pages(b)) {
-      base += pages(b);
+
+  // A pair's row in LDS holds chunk c (16 bytes) at place c ^ ((row >> 1) & 7)
+  // within its group of eight: 16 rows of one chunk lie in 64 different banks.
+  int q_at[2][2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      q_at[odd][half] = l32 * (kRow * 2) + ((4 * odd + 2 * hh + half) ^ ((l32 >> 1) & 7)) * 16;
+  const uint32_t q_lds = lds_address(q_tile);
+  // Where a lane's share of a slice's sums ends up: see below.
+  const int e_mine = l32 >> 1;
+  const int key_mine = 8 * (e_mine >> 2) + 4 * hh + (e_mine & 3);
+
+  for (int64_t at = part_start(start.plan, blockIdx.x); at < stop;) {
+    int64_t n_slices;
+    while (at >= base + (n_slices = slices(b))) {
+      base += n_slices;
       ++b;
     }
     const Request r = request_of(a, b);
-    const int page = static_cast<int>(at - base);
+    const int s0 = static_cast<int>(at - base);
+    const int64_t end = base + n_slices < stop ? base + n_slices : stop;
+    const int s1 = static_cast<int>(end - base) < s0 + kSumRun ? static_cast<int>(end - base) : s0 + kSumRun;
+    at = base + s1;
     const int64_t entry = a.entries[b];
-    const int32_t block = a.block_table[b * a.cols + page];
-    if (entry < 0 || entry >= a.pool_rows || block < 0 || block >= a.blocks) continue;
-    float sum[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+    if (entry < 0 || entry >= a.pool_rows) continue;
+    float* const record = a.token_weights + entry * a.cols * kBlock;
+    const int32_t* const table = a.block_table + b * a.cols;
+    auto block_of = [&](int slice) { return __builtin_amdgcn_readfirstlane(table[slice >> 2]); };
     const int pairs = r.n * per;
+    auto row_of = [&](int f, int g) -> int64_t {  // of pair f in query, out and lse
+      const int64_t row = r.row0 * a.heads + g * per + f;
+      return a.latent_heads == 1 ? row : row + (f / per) * (a.heads - per);
+    };
     for (int g = 0; g < a.latent_heads; ++g) {
-      const float c = fminf(fmaxf(a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g], kMinScale), FLT_MAX);
-      const float score = a.scale * kLog2e * c;
-      const uint8_t* src = static_cast<const uint8_t*>(a.latent_cache) +
-                           ((static_cast<int64_t>(block) * kBlock + wave * 32) * a.latent_heads + g) * kRow;
-#pragma unroll
-      for (int i = 0; i < 18; ++i) {  // the wave's own 32 rows
-        const int q = i * 64 + lane;
-        const int k = q / kRowChunks, ch = q - k * kRowChunks;
-        *reinterpret_cast<uint4*>(&keys[wave][k * kRow + ((ch & ~3) | ((ch ^ (k >> 2)) & 3)) * 16]) =
-            *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(k) * a.latent_heads * kRow + ch * 16);
-      }
-      for (int f0 = 0; f0 < pairs; f0 += 32) {
-        __syncthreads();
-        for (int q = tid; q < 32 * 72; q += kSumThreads) {
-          const int m = q / 72, ch = q - m * 72;
-          const int f = f0 + m < pairs ? f0 + m : f0;
-          const int i = f / per, h = f - i * per;
-          const int64_t row = (r.row0 + i) * a.heads + g * per + h;
-          *reinterpret_cast<uint4*>(&q_tile[m * kQStride + ch * 8]) =
-              ch < 64 ? static_cast<const uint4*>(a.query)[row * 64 + ch]
-                      : static_cast<const uint4*>(a.query_rope)[row * 8 + ch - 64];
+      for (int f0 = 0; f0 < pairs; f0 += kSumPairs) {
+        const bool first = g == 0 && f0 == 0, last = g == a.latent_heads - 1 && f0 + kSumPairs >= pairs;
+        const int count = pairs - f0 < kSumPairs ? pairs - f0 : kSumPairs;
+        const int tiles = count <= 32 ? 1 : (count <= 64 ? 2 : 4);  // of 32 pairs
+        const int vis_most = visible(r, (f0 + count - 1) / per), vis_least = visible(r, f0 / per);
+        u32x4_t k[18];
+        // The codes of a slice: chunks 2 j + hh of the lane's key.
+        const uint32_t lane_at = static_cast<uint32_t>(l32 * row_bytes + hh * 16);
+        auto slice_at = [&](int slice) -> const uint8_t* {
+          const int32_t block = block_of(slice < s1 ? slice : s0);
+          const int64_t row =
+              static_cast<int64_t>(block < 0 || block >= a.blocks ? 0 : block) * kBlock + (slice & 3) * kSumKeys;
+          return static_cast<const uint8_t*>(a.latent_cache) + row * row_bytes + g * kRow;
+        };
+        __syncthreads();  // (the last block's pairs are done with)
+        // The pairs' rows, straight to LDS, 64 places a wave and load, and
+        // behind them the first slice's codes.
+        const uint8_t* const qn = static_cast<const uint8_t*>(a.query);
+        const uint8_t* const qr = static_cast<const uint8_t*>(a.query_rope);
+#pragma unroll 1
+        for (int q0 = wave * 64; q0 < tiles * 32 * (kRow / 8); q0 += kSumThreads) {
+          const int q = q0 + lane;
+          const int m = q / (kRow / 8), c = (q - m * (kRow / 8)) ^ ((m >> 1) & 7);
+          const int64_t row = row_of(f0 + (m < count ? m : 0), g);
+          load_to_lds(c < kCkvDim / 8 ? qn + row * (kCkvDim * 2) + c * 16 : qr + row * (kKpeDim * 2) + c * 16 - kCkvDim * 2,
+                      q_lds + q0 * 16);
         }
-        const int f = f0 + l32;
-        int vis = 0;
-        float lse = 0.f;
-        if (f < pairs) {
-          const int i = f / per, h = f - i * per;
-          vis = visible(r, i);
-          lse = work.lse[(r.row0 + i) * a.heads + g * per + h];
+        {
+          const uint8_t* p = slice_at(s0 + wave);
+#pragma unroll
+          for (int j = 0; j < 18; ++j) k[j] = *reinterpret_cast<const u32x4_t*>(p + lane_at + 32 * j);
         }
-        __syncthreads();
-        f32x16_t s;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 18; ++j) {
-          const int ch = 2 * j + hh;
-          const uint4 k = *reinterpret_cast<const uint4*>(
-              &keys[wave][l32 * kRow + ((ch & ~3) | ((ch ^ (l32 >> 2)) & 3)) * 16]);
-          const typename T::vec8 q0 = *reinterpret_cast<const typename T::vec8*>(&q_tile[l32 * kQStride + ch * 16]);
-          const typename T::vec8 q1 = *reinterpret_cast<const typename T::vec8*>(&q_tile[l32 * kQStride + ch * 16 + 8]);
-          s = T::mfma32(widen8<T>(k.x, k.y), q0, s);
-          s = T::mfma32(widen8<T>(k.z, k.w), q1, s);
+        if (tid < kSumPairs) {
+          const int f = f0 + (tid < count ? tid : 0);
+          pair_vis[tid] = tid < count ? visible(r, f / per) : 0;
+          pair_lse[tid] = tid < count ? work.lse[row_of(f, g)] : INFINITY;
         }
-        const int key0 = page * kBlock + wave * 32 + 4 * hh;
+        wait_loads<0>();
+        lds_barrier();
+        for (int slice = s0 + wave; slice < s1; slice += kSumWaves) {
+          const int32_t block = block_of(slice);
+          const bool known = block >= 0 && block < a.blocks;
+          const int slot = slice * kSumKeys + key_mine;
+          const bool mine = (l32 & 1) == 0;
+          float* const held = &sums[(slice - s0) * kSumKeys + key_mine];
+          const float before = !first ? *held : 0.f;
+          const float total = last && known && slot < r.len ? record[slot] : 0.f;
+          float sum[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = key0 + 8 * (e >> 2) + (e & 3);
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[e], score, -lse));
-          sum[e] += key < vis ? p : 0.f;
+          for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+          if (slice * kSumKeys < vis_most) {
+            const float c = known ? a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g] : 1.f;
+            const float score = a.scale * kLog2e * fminf(fmaxf(c, kMinScale), FLT_MAX);
+            const bool ragged = (slice + 1) * kSumKeys > vis_least;
+            const uint8_t* const next = slice_at(slice + kSumWaves);
+            // The scores of all tiles of pairs in 36 steps of 16 dims, each
+            // step's operands read a step ahead.
+            auto add_pairs = [&](auto tiles_n) {
+              constexpr int N = decltype(tiles_n)::value;
+              f32x16_t s[N];
+#pragma unroll
+              for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+              u32x4_t q[2][N];
+              auto fetch = [&](int j) {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                  q[j & 1][n] = *reinterpret_cast<const u32x4_t*>(
+                      &q_tile[n * 32 * kRow * 2 + (j >> 2) * 128 + q_at[(j >> 1) & 1][j & 1]]);
+              };
+              fetch(0);
+#pragma unroll
+              for (int j = 0; j < 36; ++j) {
+                if (j < 35) fetch(j + 1);
+                // (Widened here: the compiler would do it ahead for all forms at
+                // once, and spill.)
+                if ((j & 1) == 0) asm volatile("" : "+v"(k[j >> 1]));
+                const auto kj = widen8<T>(k[j >> 1][2 * (j & 1)], k[j >> 1][2 * (j & 1) + 1]);
+                if (j & 1) k[j >> 1] = *reinterpret_cast<const u32x4_t*>(next + lane_at + 16 * (j & ~1));
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                  s[n] = T::mfma32(kj, __builtin_bit_cast(typename T::vec8, q[j & 1][n]), s[n]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+#pragma unroll
+              for (int n = 0; n < N; ++n) {
+                const float lse = pair_lse[n * 32 + l32];
+                if (ragged) {
+                  const int vis = pair_vis[n * 32 + l32] - slice * kSumKeys - 4 * hh;
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
+                    sum[e] += 8 * (e >> 2) + (e & 3) < vis ? p : 0.f;
+                  }
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
+                }
+              }
+            };
+            if (tiles == 1)
+              add_pairs(std::integral_constant<int, 1>{});
+            else if (tiles == 2)
+              add_pairs(std::integral_constant<int, 2>{});
+            else
+              add_pairs(std::integral_constant<int, 4>{});
+            // Over the 32 pairs: a lane keeps half of its values each time and
+            // hands its neighbour the others, until it holds value e_mine.
+#pragma unroll
+            for (int x = 16; x >= 2; x >>= 1) {
+              const bool up = (l32 & x) != 0;
+#pragma unroll
+              for (int e = 0; e < x / 2; ++e) {
+                const float keep = up ? sum[e + x / 2] : sum[e], give = up ? sum[e] : sum[e + x / 2];
+                sum[e] = keep + __shfl_xor(give, x, 64);
+              }
+            }
+            sum[0] += __shfl_xor(sum[0], 1, 64);
+          }
+          const float now = before + sum[0];
+          if (!last) {
+            if (mine) *held = now;
+          } else if (mine && known && slot < r.len) {
+            record[slot] = total + now;
+          }
         }
       }
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) sum[e] += __shfl_xor(sum[e], x, 64);
-      if (l32 == e) sums[wave][8 * (e >> 2) + 4 * hh + (e & 3)] = sum[e];
-    }
-    __syncthreads();
-    if (tid < kBlock && page * kBlock + tid < r.len)
-      a.token_weights[entry * a.cols * kBlock + page * kBlock + tid] += sums[tid >> 5][tid & 31];
-    __syncthreads();
   }
 }
 
@@ -1388,7 +1488,7 @@ static void attend(const Latent8Args& a, hipStream_t stream) {
   launch_kernel(kKernLatent8Join, latent8_join_kernel<T>, dim3(kJoinBlocks, static_cast<unsigned>(a.parts)),
                 dim3(kJoinThreads), stream, a);
   if (a.token_weights != nullptr)
-    launch_kernel(kKernLatent8Weights, latent8_weights_kernel<T>, dim3(512), dim3(kSumThreads), stream, a);
+    launch_kernel(kKernLatent8Weights, latent8_weights_kernel<T>, dim3(kSumParts), dim3(kSumThreads), stream, a);
 }
 
 hipError_t launch_latent8_attention(const Latent8Args& args, hipStream_t stream) {
