@@ -1229,52 +1229,110 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
 
 // ------------------------------------------------------------------ eviction
 // Selection: one workgroup per request finds the K-th largest key by three
-// digit counts, then lists holes and sources in slot order.
+// digit counts, then lists holes and sources in slot order.  Bound by the
+// passes, of which there are seven: with the keys in registers (32,768 slots)
+// 1 x 2,176 slots take 12 us, 48 x 8,320 20 us and 16 x 32,768 36 us, against
+// 13, 32 and 97 with every pass reading them anew.  About 9 us of it are the
+// barriers and scans of the digits.
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kDigitBins = 2048;
+constexpr int kHeld = 32;  // keys of a thread in registers: 32,768 slots a request
+constexpr int kAhead = 4;  // rounds loaded and walked at a time
 
-__device__ inline uint32_t evict_key(const Latent8EvictArgs& a, float w, int32_t pos, int64_t latest) {
-  if (pos < a.protect_first || pos > latest - a.protect_last) return 0xffffffffu;
-  const uint32_t k = float_key(w + 0.f);  // (-0 counts as 0)
-  return k < 0xfffffffeu ? k : 0xfffffffeu;
+// Set bits of a ballot below the lane.
+__device__ inline int before_lane(uint64_t ballot) {
+  return static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(ballot >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(ballot), 0u)));
 }
 
-__global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8EvictArgs a) {
-  __shared__ uint32_t bins[kDigitBins];
-  __shared__ int scratch[kEvictWaves + 1];
-  __shared__ int wave_latest[kEvictWaves];
-  __shared__ int s_bin, s_above;
-  __shared__ int wave_a[kEvictWaves], wave_b[kEvictWaves];
-  const int64_t b = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Protected tokens first, then NaN, then by weight; no token has key 0.
+__device__ inline uint32_t evict_key(const Latent8EvictArgs& a, float w, int32_t pos, int64_t latest) {
+  if (pos < a.protect_first || pos > latest - a.protect_last) return 0xffffffffu;
+  return w == w ? float_key(w + 0.f) : 0xfffffffeu;  // (-0 counts as 0)
+}
+
+struct SelectLds {
+  uint4 bins[kDigitBins];  // four counts a digit, one for every fourth lane
+  int scratch[kEvictWaves + 1];
+  int wave_latest[kEvictWaves];
+  int bin, above;
+  int wave_a[kEvictWaves], wave_b[kEvictWaves];
+};
+
+__device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int64_t b, int64_t entry, int len, int keep) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t cap = a.cols * kBlock;
-  int64_t len64 = a.seq_kv[b];
-  const int len = static_cast<int>(len64 < 0 ? 0 : (len64 > cap ? cap : len64));
-  const int budget = a.budgets[b] < 0 ? 0 : a.budgets[b];
-  const int64_t entry = a.entries[b];
-  const bool known = entry >= 0 && entry < a.pool_rows;
-  const int keep = known && budget < len ? budget : len;
-  if (keep == len || keep == 0) {
-    if (tid == 0) {
-      a.move_counts[b] = 0;
-      a.kept_lengths[b] = keep;
-    }
-    return;
-  }
   const float* weights = a.token_weights + entry * cap;
   const int32_t* positions = a.token_positions + entry * cap;
   // Wave w's slots: [w seg, w seg + seg), 64 a round.
   const int seg = static_cast<int>(ceil_div(ceil_div(len, kEvictWaves), 64)) * 64;
   const int s0 = wave * seg, s1 = s0 + seg < len ? s0 + seg : len;
+  auto at = [&](int s) { return s < s1 ? s : 0; };  // (slot 0 in the place of one behind the end)
   int latest = INT32_MIN;
-  for (int s = s0 + lane; s < s1; s += 64) latest = positions[s] > latest ? positions[s] : latest;
-  latest = static_cast<int>(wave_reduce_to_lane63(static_cast<uint32_t>(latest) ^ 0x80000000u, MaxU32Op{}) ^ 0x80000000u);
-  if (lane == 63) wave_latest[wave] = latest;
-  __syncthreads();
-  latest = wave_latest[0];
-  for (int w = 1; w < kEvictWaves; ++w) latest = wave_latest[w] > latest ? wave_latest[w] : latest;
-  auto key_at = [&](int s) { return evict_key(a, weights[s], positions[s], latest); };
+  // kHeld rounds of 64 keys stay in registers; what lies beyond is read anew
+  // by every pass.
+  uint32_t held[kHeld];
+  {
+    float w[kHeld];
+    int32_t p[kHeld];
+#pragma unroll
+    for (int r = 0; r < kHeld; r += kAhead)
+      if (s0 + 64 * r < s1) {
+#pragma unroll
+        for (int i = r; i < r + kAhead; ++i) {
+          w[i] = weights[at(s0 + 64 * i + lane)];
+          p[i] = positions[at(s0 + 64 * i + lane)];
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < kHeld; r += kAhead)
+      if (s0 + 64 * r < s1) {
+#pragma unroll
+        for (int i = r; i < r + kAhead; ++i) latest = p[i] > latest ? p[i] : latest;
+      }
+    for (int r0 = s0 + 64 * kHeld; r0 < s1; r0 += 64 * kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int x = positions[at(r0 + 64 * i + lane)];
+        latest = x > latest ? x : latest;
+      }
+    }
+    latest = static_cast<int>(wave_reduce_to_lane63(static_cast<uint32_t>(latest) ^ 0x80000000u, MaxU32Op{}) ^ 0x80000000u);
+    if (lane == 63) l.wave_latest[wave] = latest;
+    __syncthreads();
+    latest = l.wave_latest[0];
+    for (int k = 1; k < kEvictWaves; ++k) latest = l.wave_latest[k] > latest ? l.wave_latest[k] : latest;
+#pragma unroll
+    for (int r = 0; r < kHeld; r += kAhead)
+      if (s0 + 64 * r < s1) {
+#pragma unroll
+        for (int i = r; i < r + kAhead; ++i) held[i] = s0 + 64 * i + lane < s1 ? evict_key(a, w[i], p[i], latest) : 0u;
+      }
+  }
+  // f(first slot, key) of every round of 64 slots that the wave owns, and of
+  // some behind them; a slot that is not the wave's has key 0.
+  auto rounds = [&](auto f) {
+#pragma unroll
+    for (int r = 0; r < kHeld; r += kAhead)
+      if (s0 + 64 * r < s1) {
+#pragma unroll
+        for (int i = r; i < r + kAhead; ++i) f(s0 + 64 * i, held[i]);
+      }
+    for (int r0 = s0 + 64 * kHeld; r0 < s1; r0 += 64 * kAhead) {
+      float w[kAhead];
+      int32_t p[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        w[i] = weights[at(r0 + 64 * i + lane)];
+        p[i] = positions[at(r0 + 64 * i + lane)];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        f(r0 + 64 * i, r0 + 64 * i + lane < s1 ? evict_key(a, w[i], p[i], latest) : 0u);
+    }
+  };
 
   // The keep-th largest key: digits of 11, 11 and 10 bits from the top.
   uint32_t prefix = 0;
@@ -1283,55 +1341,55 @@ __global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8Ev
   for (int round = 0; round < 3; ++round) {
     const int bits = round < 2 ? 11 : 10;
     shift -= bits;
-    for (int i = tid; i < kDigitBins; i += kEvictThreads) bins[i] = 0;
+    for (int i = tid; i < kDigitBins; i += kEvictThreads) l.bins[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int s = s0 + lane; s < s1; s += 64) {
-      const uint32_t k = key_at(s);
-      if (round == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << bits) - 1)], 1u);
-    }
+    rounds([&](int, uint32_t k) {
+      if (k != 0 && (round == 0 || (k >> (shift + bits)) == prefix))
+        atomicAdd(reinterpret_cast<uint32_t*>(&l.bins[(k >> shift) & ((1u << bits) - 1)]) + (lane & 3), 1u);
+    });
     __syncthreads();
     // Thread t owns bins top - 2t and top - 2t - 1 (from the largest digit down).
     const int top = (1 << bits) - 1;
     const int hi = top - 2 * tid, lo = hi - 1;
-    const int c_hi = hi >= 0 ? static_cast<int>(bins[hi]) : 0, c_lo = lo >= 0 ? static_cast<int>(bins[lo]) : 0;
+    auto count = [&](int digit) -> int {
+      const uint4 v = l.bins[digit < 0 ? 0 : digit];
+      return digit < 0 ? 0 : static_cast<int>(v.x + v.y + v.z + v.w);
+    };
+    const int c_hi = count(hi), c_lo = count(lo);
     int total;
-    const int before = block_exclusive_scan(c_hi + c_lo, scratch, &total);
+    const int before = block_exclusive_scan(c_hi + c_lo, l.scratch, &total);
     if (before < want && want <= before + c_hi) {
-      s_bin = hi;
-      s_above = before;
+      l.bin = hi;
+      l.above = before;
     } else if (before + c_hi < want && want <= before + c_hi + c_lo) {
-      s_bin = lo;
-      s_above = before + c_hi;
+      l.bin = lo;
+      l.above = before + c_hi;
     }
     __syncthreads();
-    prefix = (prefix << bits) | static_cast<uint32_t>(s_bin);
-    want -= s_above;
+    prefix = (prefix << bits) | static_cast<uint32_t>(l.bin);
+    want -= l.above;
     __syncthreads();
   }
   const uint32_t threshold = prefix;  // `want` of the keys equal to it are kept, the lower slots first
 
   int equal = 0;
-  for (int r0 = s0; r0 < s1; r0 += 64) {
-    const int s = r0 + lane;
-    equal += __popcll(__ballot(s < s1 && key_at(s) == threshold));
-  }
-  if (lane == 0) wave_a[wave] = equal;
+  rounds([&](int, uint32_t k) { equal += __popcll(__ballot(k == threshold)); });
+  if (lane == 0) l.wave_a[wave] = equal;
   __syncthreads();
   int equal_before = 0;
-  for (int w = 0; w < wave; ++w) equal_before += wave_a[w];
+  for (int w = 0; w < wave; ++w) equal_before += l.wave_a[w];
   __syncthreads();
   auto walk = [&](auto each) {
     int eq = equal_before;
-    for (int r0 = s0; r0 < s1; r0 += 64) {
+    rounds([&](int r0, uint32_t k) {
       const int s = r0 + lane;
-      const uint32_t k = s < s1 ? key_at(s) : 0u;
-      const bool tie = s < s1 && k == threshold;
-      uint64_t ties;
-      const int rank = eq + wave_flag_prefix(tie, &ties);
+      const bool tie = k == threshold;
+      const uint64_t ties = __ballot(tie);
+      const int rank = eq + before_lane(ties);
       eq += __popcll(ties);
-      const bool kept = s < s1 && (k > threshold || (tie && rank < want));
-      each(r0, s, s < s1 && !kept && s < keep, kept && s >= keep);
-    }
+      const bool kept = k > threshold || (tie && rank < want);
+      each(r0, s, k != 0 && !kept && s < keep, kept && s >= keep);
+    });
   };
   int holes = 0, sources = 0;
   walk([&](int, int, bool hole, bool source) {
@@ -1339,27 +1397,26 @@ __global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8Ev
     sources += __popcll(__ballot(source));
   });
   if (lane == 0) {
-    wave_a[wave] = holes;
-    wave_b[wave] = sources;
+    l.wave_a[wave] = holes;
+    l.wave_b[wave] = sources;
   }
   __syncthreads();
   int hole_at = 0, source_at = 0, count = 0;
   for (int w = 0; w < kEvictWaves; ++w) {
     if (w < wave) {
-      hole_at += wave_a[w];
-      source_at += wave_b[w];
+      hole_at += l.wave_a[w];
+      source_at += l.wave_b[w];
     }
-    count += wave_a[w];
+    count += l.wave_a[w];
   }
   int32_t* hole_start = a.hole_start + b * (a.cols + 1);
   int32_t* dst = a.move_dst + b * cap;
   int32_t* src = a.move_src + b * cap;
   walk([&](int r0, int s, bool hole, bool source) {
-    if ((r0 & (kBlock - 1)) == 0 && lane == 0) hole_start[r0 >> kBlockShift] = hole_at;
-    uint64_t hs, ss;
-    const int ha = hole_at + wave_flag_prefix(hole, &hs), sa = source_at + wave_flag_prefix(source, &ss);
-    if (hole) dst[ha] = s;
-    if (source) src[sa] = s;
+    if ((r0 & (kBlock - 1)) == 0 && r0 < s1 && lane == 0) hole_start[r0 >> kBlockShift] = hole_at;
+    const uint64_t hs = __ballot(hole), ss = __ballot(source);
+    if (hole) dst[hole_at + before_lane(hs)] = s;
+    if (source) src[source_at + before_lane(ss)] = s;
     hole_at += __popcll(hs);
     source_at += __popcll(ss);
   });
@@ -1376,11 +1433,38 @@ __global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8Ev
   }
 }
 
-// Moves: one workgroup per (request, page that has holes).
+__global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8EvictArgs a) {
+  __shared__ SelectLds l;
+  const int64_t b = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t cap = a.cols * kBlock;
+  int64_t len64 = a.seq_kv[b];
+  const int len = static_cast<int>(len64 < 0 ? 0 : (len64 > cap ? cap : len64));
+  const int budget = a.budgets[b] < 0 ? 0 : a.budgets[b];
+  const int64_t entry = a.entries[b];
+  const bool known = entry >= 0 && entry < a.pool_rows;
+  const int keep = known && budget < len ? budget : len;
+  if (keep == len || keep == 0) {
+    if (tid == 0) {
+      a.move_counts[b] = 0;
+      a.kept_lengths[b] = keep;
+    }
+    return;
+  }
+  select_slots(a, l, b, entry, len, keep);
+}
+
+// Moves: one workgroup per (request, page that has holes).  Bound by the bytes
+// of the moved rows: 16 x 8,200 rows of 576, read and written once, in 28 us
+// (5.4 TB/s, part of it from cache).  With a load and a store in turn it took 51.
 constexpr int kMoveThreads = 256;
+constexpr int kMovePages = 256;  // workgroups of a request at most
+constexpr int kMoveAhead = 6;  // chunks of a thread in flight
 __global__ __launch_bounds__(kMoveThreads) void latent8_move_kernel(Latent8EvictArgs a) {
-  __shared__ int32_t from[kBlock];  // slot that moves into the page's row, -1: the row stays
-  __shared__ float from_scale[kBlock];
+  __shared__ int64_t from[kBlock];  // cache row of the n-th source, -1: none
+  __shared__ int to[kBlock];        // row of the page that it moves to
+  __shared__ float factor[kBlock];
+  __shared__ uint8_t moved[kBlock];
   __shared__ float wave_top[kMoveThreads / 64];
   const int64_t b = blockIdx.y;
   const int tid = threadIdx.x;
@@ -1392,6 +1476,8 @@ __global__ __launch_bounds__(kMoveThreads) void latent8_move_kernel(Latent8Evict
   const int32_t* hole_start = a.hole_start + b * (a.cols + 1);
   const int border = (keep & (kBlock - 1)) != 0 ? keep >> kBlockShift : -1;
   const int pages = static_cast<int>(ceil_div(keep, kBlock));
+  const int64_t stride = a.latent_heads * kRow;
+  uint8_t* const cache = static_cast<uint8_t*>(a.latent_cache);
   for (int page = blockIdx.x; page < pages; page += gridDim.x) {
     const int h0 = hole_start[page], h1 = page + 1 < pages ? hole_start[page + 1] : count;
     const int n = h1 - h0;
@@ -1399,14 +1485,19 @@ __global__ __launch_bounds__(kMoveThreads) void latent8_move_kernel(Latent8Evict
     if (n <= 0) continue;
     const int rows = keep - page * kBlock < kBlock ? keep - page * kBlock : kBlock;
     __syncthreads();
-    if (tid < kBlock) from[tid] = -1;
+    if (tid < kBlock) moved[tid] = 0;
     __syncthreads();
-    int64_t src = 0;
-    int dst = 0;
+    int source_page = -1;  // that thread tid's source lies in
+    int32_t source_block = -1;
     if (tid < n) {
-      src = a.move_src[b * cap + h0 + tid];
-      dst = a.move_dst[b * cap + h0 + tid] - page * kBlock;
-      from[dst] = static_cast<int32_t>(src);
+      const int src = a.move_src[b * cap + h0 + tid];
+      const int dst = a.move_dst[b * cap + h0 + tid] - page * kBlock;
+      source_page = src >> kBlockShift;
+      const int32_t sb = table[source_page];
+      if (sb >= 0 && sb < a.blocks) source_block = sb;
+      from[tid] = source_block < 0 ? -1 : static_cast<int64_t>(source_block) * kBlock + (src & (kBlock - 1));
+      to[tid] = dst;
+      moved[dst] = 1;
       float* w = a.token_weights + entry * cap;
       int32_t* p = a.token_positions + entry * cap;
       w[page * kBlock + dst] = w[src];
@@ -1417,40 +1508,44 @@ __global__ __launch_bounds__(kMoveThreads) void latent8_move_kernel(Latent8Evict
       float* scale_at = a.cache_scale + static_cast<int64_t>(block) * a.latent_heads + g;
       const float old = *scale_at;
       float mine = 0.f;
-      if (tid < n) {
-        const int sp = static_cast<int>(src >> kBlockShift);
-        const int32_t sb = table[sp];
-        if (sp == border)
-          mine = a.border_scale[b * a.latent_heads + g];
-        else if (sb >= 0 && sb < a.blocks)
-          mine = a.cache_scale[static_cast<int64_t>(sb) * a.latent_heads + g];
-      }
-      __syncthreads();  // (every thread has read the old scale and is done with the last head's)
-      if (tid < n) from_scale[dst] = mine;
+      if (source_page == border && source_page >= 0)
+        mine = a.border_scale[b * a.latent_heads + g];
+      else if (source_block >= 0)
+        mine = a.cache_scale[static_cast<int64_t>(source_block) * a.latent_heads + g];
       const float top = wave_all_op(mine, MaxOp{});
       if ((tid & 63) == 0) wave_top[tid >> 6] = top;
-      __syncthreads();
+      __syncthreads();  // (every thread has read the old scale and is done with the last head's factors)
       float now = old;
       for (int w = 0; w < kMoveThreads / 64; ++w) now = fmaxf(now, wave_top[w]);
-      const float stay = old / now;
-      const int64_t stride = a.latent_heads * kRow;
-      uint8_t* cache = static_cast<uint8_t*>(a.latent_cache);
-      uint8_t* base = cache + (static_cast<int64_t>(block) * kBlock * a.latent_heads + g) * kRow;
-      for (int q = tid; q < rows * kRowChunks; q += kMoveThreads) {
-        const int r = q / kRowChunks, c = q - r * kRowChunks;
-        const int s = from[r];
-        if (s < 0 && now == old) continue;
-        uint4* to = reinterpret_cast<uint4*>(base + r * stride) + c;
-        if (s < 0) {
-          *to = rescale16(*to, stay);
-        } else {
-          const int32_t sb = table[s >> kBlockShift];
-          if (sb < 0 || sb >= a.blocks) continue;
-          const uint4 v = *(reinterpret_cast<const uint4*>(
-                                cache + ((static_cast<int64_t>(sb) * kBlock + (s & (kBlock - 1))) * a.latent_heads + g) *
-                                            kRow) +
-                            c);
-          *to = rescale16(v, from_scale[r] / now);
+      if (tid < n) factor[tid] = mine / now;
+      __syncthreads();
+      uint8_t* base = cache + static_cast<int64_t>(block) * kBlock * stride + g * kRow;
+      if (now != old) {
+        const float stay = old / now;
+        for (int q = tid; q < rows * kRowChunks; q += kMoveThreads) {
+          const int r = q / kRowChunks, c = q - r * kRowChunks;
+          if (moved[r]) continue;
+          uint4* at = reinterpret_cast<uint4*>(base + r * stride) + c;
+          *at = rescale16(*at, stay);
+        }
+      }
+      for (int q0 = tid; q0 < n * kRowChunks; q0 += kMoveAhead * kMoveThreads) {
+        uint4 v[kMoveAhead];
+#pragma unroll
+        for (int i = 0; i < kMoveAhead; ++i) {
+          const int q = q0 + i * kMoveThreads < n * kRowChunks ? q0 + i * kMoveThreads : q0;
+          const int m = q / kRowChunks, c = q - m * kRowChunks;
+          const int64_t row = from[m] < 0 ? 0 : from[m];
+          v[i] = *(reinterpret_cast<const uint4*>(cache + row * stride + g * kRow) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < kMoveAhead; ++i) {
+          const int q = q0 + i * kMoveThreads;
+          if (q >= n * kRowChunks) break;
+          const int m = q / kRowChunks, c = q - m * kRowChunks;
+          if (from[m] < 0) continue;
+          const float f = factor[m];
+          *(reinterpret_cast<uint4*>(base + to[m] * stride) + c) = f == 1.f ? v[i] : rescale16(v[i], f);
         }
       }
       if (tid == 0 && now != old) *scale_at = now;
@@ -1515,7 +1610,7 @@ hipError_t launch_latent8_evict(const Latent8EvictArgs& args, hipStream_t stream
   launch_kernel(kKernLatent8Select, latent8_select_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(kEvictThreads),
                 stream, a);
   launch_kernel(kKernLatent8Move, latent8_move_kernel,
-                dim3(static_cast<unsigned>(std::min<int64_t>(a.cols, 64)), static_cast<unsigned>(a.batch)),
+                dim3(static_cast<unsigned>(std::min<int64_t>(a.cols, kMovePages)), static_cast<unsigned>(a.batch)),
                 dim3(kMoveThreads), stream, a);
   return hipGetLastError();
 }

@@ -376,6 +376,25 @@ def test_evict_ties_and_odd_weights():
     _check_evict(c, [333, 200, 45], weights, positions, entries, 2, 5)
 
 
+def test_evict_nan_of_either_sign():
+    c = make_cache([500], 1, seed=25)
+    weights, positions, entries = _records(c, 7)
+    row = weights[entries.long()[0]].view(torch.int32)
+    row[100:130], row[130:150], row[480:490] = -1, -0x400000, 0x7f800001  # NaN: of all ones, negative, signalling
+    print("EVICT NaN", flush=True)
+    _check_evict(c, [70], weights, positions, entries, 2, 5)
+
+
+@pytest.mark.parametrize("lengths,budgets", [([32769, 8193], [32640, 4000]), ([40001], [17000])])
+def test_evict_long(lengths, budgets):
+    """More slots than a workgroup holds in registers."""
+    print(f"EVICT long {lengths} -> {budgets}", flush=True)
+    c = make_cache(lengths, 1, seed=26)
+    weights, positions, entries = _records(c, 8)
+    weights[:, 1000:3000] = 0.25  # more equal weights than the budget leaves room for, or none
+    _check_evict(c, budgets, weights, positions, entries, 64, 500)
+
+
 def test_evict_positions_in_any_order():
     """Protection goes by position, not by slot: what an earlier eviction left."""
     c = make_cache([900, 300], 1, seed=22)
