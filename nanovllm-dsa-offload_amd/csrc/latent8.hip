@@ -242,16 +242,57 @@ constexpr int kWindow = 512;    // resolved pages (or list entries) held at a ti
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
 constexpr float kMost = 14.f;   // scores pass the maximum by this at most (base 2): P <= 2^14 and a scale's fraction fit fp16
-constexpr int kMinUnits = 2;    // least tiles of a workgroup
+constexpr int kMinUnits = 1;    // least tiles of a workgroup
+constexpr int kBegin = 4;       // what the start of a segment costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
 constexpr int kPartFloats = kRows * kCkvDim;
 
 struct Plan {
   int64_t total;  // units
   int64_t parts;  // workgroups that share them
+  int split;      // > 0: every item (of `tiles` units) in so many parts
+  int tiles;
 };
-__host__ __device__ inline int64_t part_start(const Plan& p, int64_t w) { return p.total * w / p.parts; }
-__device__ inline int64_t part_of(const Plan& p, int64_t unit) { return ((unit + 1) * p.parts + p.total - 1) / p.total - 1; }
+// x / y for 0 <= x < 2^53, y > 0 (a 64-bit division is a microsecond of
+// instructions; units stay below 2^40, their product with a part below 2^48).
+__device__ inline int64_t divide(int64_t x, int64_t y) {
+  int64_t q = static_cast<int64_t>(static_cast<double>(x) / static_cast<double>(y));
+  const int64_t rest = x - q * y;
+  q += rest < 0 ? -1 : (rest >= y ? 1 : 0);
+  return q;
+}
+__device__ inline int64_t part_start(const Plan& p, int64_t w) {
+  if (p.split > 0) {
+    const int item = static_cast<int>(w) / p.split, piece = static_cast<int>(w) - item * p.split;
+    return static_cast<int64_t>(item) * p.tiles + static_cast<int64_t>(p.tiles) * piece / p.split;
+  }
+  return divide(p.total * w, p.parts);
+}
+// The part of an item's last unit.
+__device__ inline int64_t part_of_end(const Plan& p, int64_t end) {
+  if (p.split > 0) return divide(end, p.tiles) * p.split - 1;
+  return divide(end * p.parts + p.total - 1, p.total) - 1;
+}
+
+// Equal parts of the units; or, where all items have the same number of tiles
+// and there are few of them, equal parts of every item: a part that lies across
+// two items begins anew, which costs kBegin tiles' time (24 lists of 2,048, 48
+// items of 32 tiles: 5 parts of 7 tiles an item take 31 us, 256 parts of 6 37).
+__device__ inline Plan make_plan(int64_t total, int64_t parts, int64_t least, int tiles) {
+  Plan p{total, divide(total, least), 0, tiles};
+  if (p.parts > parts) p.parts = parts;
+  if (p.parts < 1) p.parts = 1;
+  if (tiles > 0 && total > 0) {
+    const int64_t items = divide(total, tiles);
+    int64_t split = divide(parts, items);
+    if (split * least > tiles) split = divide(tiles, least) > 0 ? divide(tiles, least) : 1;
+    if (split > 0 && (tiles - kBegin * split) * p.parts <= total * split) {
+      p.split = static_cast<int>(split);
+      p.parts = items * split;
+    }
+  }
+  return p;
+}
 
 struct Request {
   int64_t row0;   // first query row
@@ -259,24 +300,25 @@ struct Request {
   int len;        // cached tokens, clipped to the table
   int items_g;    // items of one latent head
   int64_t items;
-  int64_t tiles;  // units of an item
+  int tiles;      // units of an item
 };
+__device__ inline Request make_request(const Latent8Args& a, int64_t row0, int n, int len) {
+  Request r;
+  r.row0 = row0;
+  r.n = n;
+  r.len = len;
+  r.items_g = a.topk != nullptr ? n * ((a.per + kRows - 1) / kRows) : (n * a.per + kRows - 1) / kRows;
+  r.items = static_cast<int64_t>(r.items_g) * a.latent_heads;
+  r.tiles = ((a.topk != nullptr ? static_cast<int>(a.list_len) : len) + kKeys - 1) / kKeys;
+  if (r.tiles < 1) r.tiles = 1;
+  return r;
+}
 __device__ inline Request request_of(const Latent8Args& a, int64_t b) {
   int64_t lo = b > 0 ? a.seq_q[b - 1] : 0, hi = a.seq_q[b];
   lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
   hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
-  Request r;
-  r.row0 = lo;
-  r.n = static_cast<int>(hi - lo);
-  const int64_t cap = a.cols * kBlock;
-  int64_t len = a.seq_kv[b];
-  r.len = static_cast<int>(len < 0 ? 0 : (len > cap ? cap : len));
-  const int64_t per = a.heads / a.latent_heads;
-  r.items_g = static_cast<int>(a.topk != nullptr ? r.n * ceil_div(per, kRows) : ceil_div(r.n * per, kRows));
-  r.items = static_cast<int64_t>(r.items_g) * a.latent_heads;
-  r.tiles = a.topk != nullptr ? ceil_div(a.list_len, kKeys) : ceil_div(r.len, kKeys);
-  if (r.tiles < 1) r.tiles = 1;
-  return r;
+  const int64_t cap = a.cols * kBlock, len = a.seq_kv[b];
+  return make_request(a, lo, static_cast<int>(hi - lo), static_cast<int>(len < 0 ? 0 : (len > cap ? cap : len)));
 }
 
 // Exclusive prefix of a 64-bit count over the workgroup's threads.
@@ -310,52 +352,57 @@ struct Start {
   Plan plan;
   int64_t b;
   int64_t base;  // first unit of the request
+  Request r;
 };
-template <int THREADS, typename COST>
-__device__ inline Start find_start(int64_t batch, int64_t part, int64_t parts, int64_t least, COST cost,
-                                   int64_t* scratch, int64_t* found) {
+template <int THREADS, typename UNITS>
+__device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t parts, int64_t least, int tiles,
+                                   UNITS units) {
+  __shared__ int64_t scratch[THREADS / 64];
+  __shared__ int64_t found[5];
   Start s;
   const int tid = threadIdx.x;
-  int64_t sum = 0;
-  const int64_t first = tid < batch ? cost(static_cast<int64_t>(tid)) : 0;
-  for (int64_t b = tid + THREADS; b < batch; b += THREADS) sum += cost(b);
+  Request r{};
+  int64_t first = 0, sum = 0;
+  if (tid < a.batch) {
+    r = request_of(a, tid);
+    first = units(r);
+  }
+  for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum += units(request_of(a, b));
   int64_t total;
   if (tid == 0) found[0] = -1;
-  if (batch <= THREADS) {
-    const int64_t at = scan64<THREADS>(first, scratch, &total);
-    s.plan.total = total = uniform64(total);
-    s.plan.parts = total / least < 1 ? 1 : (total / least < parts ? total / least : parts);
-    if (part < s.plan.parts && total > 0) {
-      const int64_t u = part_start(s.plan, part);
-      if (u >= at && u < at + first) {
-        found[0] = tid;
-        found[1] = at;
-      }
-    }
-  } else {
-    scan64<THREADS>(first + sum, scratch, &total);
-    s.plan.total = total = uniform64(total);
-    s.plan.parts = total / least < 1 ? 1 : (total / least < parts ? total / least : parts);
-    if (part < s.plan.parts && total > 0) {
-      const int64_t u = part_start(s.plan, part);
-      int64_t before = 0;
-      for (int64_t b0 = 0; b0 < batch; b0 += THREADS) {
-        const int64_t b = b0 + tid;
-        const int64_t c = b < batch ? cost(b) : 0;
-        int64_t chunk;
-        const int64_t at = before + scan64<THREADS>(c, scratch, &chunk);
-        if (u >= at && u < at + c) {
-          found[0] = b;
-          found[1] = at;
+  int64_t at = scan64<THREADS>(first + sum, scratch, &total);
+  total = uniform64(total);
+  s.plan = make_plan(total, parts, least, tiles);
+  if (part < s.plan.parts && total > 0) {
+    const int64_t u = part_start(s.plan, part);
+    int64_t before = 0;
+    for (int64_t b0 = 0; b0 < a.batch; b0 += THREADS) {
+      const int64_t b = b0 + tid;
+      if (a.batch > THREADS) {  // (the first scan was over strided sums)
+        r = Request{};
+        first = 0;
+        if (b < a.batch) {
+          r = request_of(a, b);
+          first = units(r);
         }
+        int64_t chunk;
+        at = before + scan64<THREADS>(first, scratch, &chunk);
         before += chunk;
-        if (u < before) break;
       }
+      if (u >= at && u < at + first) {
+        found[0] = b;
+        found[1] = at;
+        found[2] = r.row0;
+        found[3] = r.n;
+        found[4] = r.len;
+      }
+      if (u < before) break;
     }
   }
   __syncthreads();
   s.b = uniform64(found[0]);
   s.base = uniform64(found[1]);
+  s.r = make_request(a, uniform64(found[2]), static_cast<int>(uniform64(found[3])), static_cast<int>(uniform64(found[4])));
   return s;
 }
 
@@ -369,11 +416,11 @@ struct Item {
 };
 __device__ inline Item item_of(const Latent8Args& a, const Request& r, int64_t it) {
   Item x;
-  const int per = static_cast<int>(a.heads / a.latent_heads);
-  x.g = static_cast<int>(it / r.items_g);
-  int j = static_cast<int>(it - static_cast<int64_t>(x.g) * r.items_g);
+  const int per = a.per;
+  x.g = a.latent_heads == 1 ? 0 : static_cast<int>(it) / r.items_g;
+  int j = static_cast<int>(it) - x.g * r.items_g;
   if (a.topk != nullptr) {
-    const int groups = static_cast<int>(ceil_div(per, kRows));
+    const int groups = (per + kRows - 1) / kRows;
     x.lead = j / groups;
     j -= x.lead * groups;
     x.first = x.lead * per + j * kRows;
@@ -459,19 +506,19 @@ struct Window {
   float exponent;
   float fraction;
 };
-__device__ inline Window resolve(const Latent8Args& a, int64_t b, int g, int64_t slot, bool ok) {
-  Window w{-1, 0.f, 0.f, 0.f};
-  if (!ok) return w;
+__device__ inline int32_t row_of_slot(const Latent8Args& a, int64_t b, int64_t slot, bool ok) {
+  if (!ok) return -1;
   const int32_t block = a.block_table[b * a.cols + (slot >> kBlockShift)];
-  if (block < 0 || block >= a.blocks) return w;
-  float c = a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g];
+  return block < 0 || block >= a.blocks ? -1 : block * kBlock + static_cast<int32_t>(slot & (kBlock - 1));
+}
+__device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // the fields but row
+  const int32_t block = w.row >> kBlockShift;
+  float c = w.row < 0 ? 1.f : a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g];
   c = fminf(fmaxf(c, kMinScale), FLT_MAX);
   const uint32_t u = __float_as_uint(c);
-  w.row = block * kBlock + static_cast<int32_t>(slot & (kBlock - 1));
   w.score = a.scale * kLog2e * c;
   w.exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
   w.fraction = __uint_as_float((u & 0x7fffffu) | 0x3f800000u);
-  return w;
 }
 
 // Eight waves in two groups of four: group g owns rows 32 g .. 32 g + 31 of the
@@ -505,8 +552,6 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   __shared__ int outgrown[2][2];                        // group, tile parity
   __shared__ int bad_entries[2][LIST ? kWindow / kKeys : 1];  // tiles of a window with entries that name nothing
   __shared__ Window windows[2][kWindow];
-  __shared__ int64_t scratch[kAttnThreads / 64];
-  __shared__ int64_t found[2];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -514,13 +559,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int hh = lane >> 5;
   const int grp = wave >> 2, kg = wave & 1, dh = (wave >> 1) & 1, wg = wave & 3;
   const int64_t part = blockIdx.x;
-  const Start start = find_start<kAttnThreads>(
-      a.batch, part, a.parts, kMinUnits,
-      [&](int64_t b) {
-        const Request r = request_of(a, b);
-        return r.items * r.tiles;
-      },
-      scratch, found);
+  const Start start =
+      find_start<kAttnThreads>(a, part, a.parts, kMinUnits, LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
+                               [](const Request& r) { return r.items * r.tiles; });
   const Work work = carve_work(a.workspace, a.parts);
   if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
   if (part >= start.plan.parts || start.b < 0) return;
@@ -528,7 +569,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   int64_t at = part_start(start.plan, part);
   int64_t b = start.b;
   int64_t base = start.base;
-  const int per = static_cast<int>(a.heads / a.latent_heads);
+  Request r = start.r;
+  const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
 
   // A tile's row k in LDS holds chunk c (16 bytes) at place c ^ ((k >> 2) & 3)
@@ -568,13 +610,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 
   while (at < stop) {
     // The next segment: units [u0, u1) of one item.
-    Request r = request_of(a, b);
     while (at >= base + r.items * r.tiles) {
       base += r.items * r.tiles;
       ++b;
       r = request_of(a, b);
     }
-    const int64_t it = (at - base) / r.tiles;
+    const int64_t it = divide(at - base, r.tiles);
     const int64_t item_start = base + it * r.tiles;
     const int64_t item_end = item_start + r.tiles;
     const int64_t seg_end = item_end < stop ? item_end : stop;
@@ -589,6 +630,27 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     if (t0 > t1) t0 = t1;
     const bool busy = grp == 0 || x.count > 32;  // the group has rows
 
+    const int32_t* list = LIST ? a.topk + (r.row0 + x.lead) * a.list_len : nullptr;
+    // Windows of resolved pages (list: entries), the tile's own and the next.
+    constexpr int kWindowTiles = LIST ? kWindow / kKeys : 2 * kWindow;
+    const int w0 = LIST ? t0 : t0 & ~1;
+    // This thread's entry of the window that begins with a tile: its row, and
+    // the rest, for which nobody waits before the rows themselves are on the way.
+    auto window_at = [&](int tile) -> Window& { return windows[((tile - w0) / kWindowTiles) & 1][tid]; };
+    auto window_rows = [&](int tile) {
+      if (LIST) {
+        const int e = tile * kKeys + tid;
+        const int id = e < list_len ? list[e] : -1;
+        const int32_t row = row_of_slot(a, b, id, id >= 0 && id < vis_most);
+        window_at(tile).row = row;
+        const bool bad = __any(row < 0);
+        if (lane == 0) bad_entries[((tile - w0) / kWindowTiles) & 1][LIST ? wave : 0] = bad;
+      } else {
+        const int64_t slot = (static_cast<int64_t>(tile >> 1) + tid) * kBlock;
+        window_at(tile).row = row_of_slot(a, b, slot, slot < vis_most);
+      }
+    };
+    auto window_scales = [&](int tile) { add_scale(a, x.g, window_at(tile)); };
     int vis_row;
     u32x4_t q[9][2];
     {
@@ -606,6 +668,11 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         q[j][1] = p[1];
       }
     }
+    lds_barrier();  // the previous segment is done with LDS
+    if (t0 < t1) {
+      window_rows(w0);
+      if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
+    }
     f32x16_t o[4], s;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
@@ -614,24 +681,6 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     float m_run = kNoMax, l_run = 0.f, l_tile = 0.f;
     float sc[8];
 
-    const int32_t* list = LIST ? a.topk + (r.row0 + x.lead) * a.list_len : nullptr;
-    // Windows of resolved pages (list: entries), the tile's own and the next.
-    constexpr int kWindowTiles = LIST ? kWindow / kKeys : 2 * kWindow;
-    const int w0 = LIST ? t0 : t0 & ~1;
-    auto fill_window = [&](int tile) {  // the window that begins with this tile
-      Window* w = windows[((tile - w0) / kWindowTiles) & 1];
-      if (LIST) {
-        const int e = tile * kKeys + tid;
-        const int id = e < list_len ? list[e] : -1;
-        const Window v = resolve(a, b, x.g, id, id >= 0 && id < vis_most);
-        w[tid] = v;
-        const bool bad = __any(v.row < 0);
-        if (lane == 0) bad_entries[((tile - w0) / kWindowTiles) & 1][LIST ? wave : 0] = bad;
-      } else {
-        const int64_t slot = (static_cast<int64_t>(tile >> 1) + tid) * kBlock;
-        w[tid] = resolve(a, b, x.g, slot, slot < vis_most);
-      }
-    };
     auto window_of = [&](int tile) -> const Window* {
       const unsigned i = tile - w0;
       return &windows[(i / kWindowTiles) & 1][LIST ? (i % kWindowTiles) * kKeys : (i % kWindowTiles) >> 1];
@@ -791,12 +840,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     auto again = [&](int g, int t) -> bool {
       return t > t0 && __builtin_amdgcn_readfirstlane(outgrown[g][(t - 1) & 1]) != 0;
     };
-    __syncthreads();  // the previous segment is done with LDS
     if (t0 < t1) {
-      fill_window(w0);
-      if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
-      __syncthreads();
+      lds_barrier();
       load_tile(t0, 0);
+      window_scales(w0);
       wait_loads<0>();
       lds_barrier();
       // Group 0 multiplies tile t in phase 2 (t - t0) and weighs it in the
@@ -807,7 +854,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       auto load_next = [&](int tile, int to) {
         if (tile >= t1) return;
         if ((tile - w0) % kWindowTiles == 0) {
-          fill_window(tile);
+          window_rows(tile);
+          window_scales(tile);
           __syncthreads();
         }
         load_tile(tile, to);
@@ -937,7 +985,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         j.g = x.g;
         j.w0 = static_cast<int32_t>(part - 1);
         j.slot0 = static_cast<int32_t>(2 * (part - 1) + (part_start(start.plan, part - 1) == item_start ? 0 : 1));
-        j.w1 = static_cast<int32_t>(part_of(start.plan, item_end - 1));
+        j.w1 = static_cast<int32_t>(part_of_end(start.plan, item_end));
         work.join[part] = j;
       }
     }
@@ -969,7 +1017,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
   const int grp = blockIdx.x >> 4, wg = (blockIdx.x >> 2) & 3, dt = blockIdx.x & 3;
   if (grp * 32 >= j.count) return;
   const int n = j.w1 - j.w0 + 1;
-  const int per = static_cast<int>(a.heads / a.latent_heads);
+  const int per = a.per;
   const int m = tid & 31, s = tid >> 5;  // thread (s, m): parts s, s + 8, ... of row m
   auto slot_of = [&](int w) -> int64_t { return w == 0 ? j.slot0 : 2 * static_cast<int64_t>(j.w0 + w); };
   auto ml_of = [&](int w) { return reinterpret_cast<const float2*>(work.ml)[slot_of(w) * kRows + grp * 32 + m]; };
@@ -1041,24 +1089,20 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   __shared__ float sums[kSumRun * kSumKeys];
   __shared__ float pair_lse[kSumPairs];
   __shared__ int pair_vis[kSumPairs];
-  __shared__ int64_t scratch[kSumWaves];
-  __shared__ int64_t found[2];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31;
   const int hh = lane >> 5;
   const Work work = carve_work(a.workspace, a.parts);
-  const int per = static_cast<int>(a.heads / a.latent_heads);
+  const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
-  auto slices = [&](int64_t b) -> int64_t {
-    const Request r = request_of(a, b);
-    return r.n > 0 ? ceil_div(r.len, kSumKeys) : 0;
-  };
-  const Start start = find_start<kSumThreads>(a.batch, blockIdx.x, kSumParts, kSumWaves, slices, scratch, found);
+  auto slices = [](const Request& r) -> int64_t { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
+  const Start start = find_start<kSumThreads>(a, blockIdx.x, kSumParts, kSumWaves, 0, slices);
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
   int64_t b = start.b, base = start.base;
+  Request r = start.r;
 
   // A pair's row in LDS holds chunk c (16 bytes) at place c ^ ((row >> 1) & 7)
   // within its group of eight: 16 rows of one chunk lie in 64 different banks.
@@ -1074,12 +1118,12 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int key_mine = 8 * (e_mine >> 2) + 4 * hh + (e_mine & 3);
 
   for (int64_t at = part_start(start.plan, blockIdx.x); at < stop;) {
-    int64_t n_slices;
-    while (at >= base + (n_slices = slices(b))) {
-      base += n_slices;
+    while (at >= base + slices(r)) {
+      base += slices(r);
       ++b;
+      r = request_of(a, b);
     }
-    const Request r = request_of(a, b);
+    const int64_t n_slices = slices(r);
     const int s0 = static_cast<int>(at - base);
     const int64_t end = base + n_slices < stop ? base + n_slices : stop;
     const int s1 = static_cast<int>(end - base) < s0 + kSumRun ? static_cast<int>(end - base) : s0 + kSumRun;
@@ -1590,6 +1634,7 @@ hipError_t launch_latent8_attention(const Latent8Args& args, hipStream_t stream)
   if (args.rows == 0 || args.batch == 0) return hipSuccess;
   Latent8Args a = args;
   a.parts = kParts;
+  a.per = static_cast<int32_t>(a.heads / a.latent_heads);
   if (a.elem == Elem::kBf16)
     attend<Bf16>(a, stream);
   else

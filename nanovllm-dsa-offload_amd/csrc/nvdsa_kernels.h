@@ -306,7 +306,8 @@ struct Latent8Args {
   float* token_weights;         // [pool_rows, cols * 128], or null
   void* out;                    // [rows, heads, 512]
   int64_t rows, heads, latent_heads, batch, cols, blocks, list_len, pool_rows;
-  int64_t parts;                // set by the launch
+  int64_t parts;                // set by the launch, as is
+  int32_t per;                  // heads / latent_heads
   float scale;
   Elem elem;
   void* workspace;
