@@ -243,13 +243,14 @@ constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
 constexpr float kMost = 14.f;   // scores pass the maximum by this at most (base 2): P <= 2^14 and a scale's fraction fit fp16
 constexpr int kMinUnits = 1;    // least tiles of a workgroup
-constexpr int kBegin = 4;       // what the start of a segment costs, in tiles
+constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
 constexpr int kPartFloats = kRows * kCkvDim;
 
 struct Plan {
   int64_t total;  // units
   int64_t parts;  // workgroups that share them
+  int begin;      // units of an item before its first tile
   int split;      // > 0: every item (of `tiles` units) in so many parts
   int tiles;
 };
@@ -274,22 +275,30 @@ __device__ inline int64_t part_of_end(const Plan& p, int64_t end) {
   return divide(end * p.parts + p.total - 1, p.total) - 1;
 }
 
-// Equal parts of the units; or, where all items have the same number of tiles
-// and there are few of them, equal parts of every item: a part that lies across
-// two items begins anew, which costs kBegin tiles' time (24 lists of 2,048, 48
-// items of 32 tiles: 5 parts of 7 tiles an item take 31 us, 256 parts of 6 37).
-__device__ inline Plan make_plan(int64_t total, int64_t parts, int64_t least, int tiles) {
-  Plan p{total, divide(total, least), 0, tiles};
+// Equal parts of the units.  A part that lies across two items begins anew,
+// which costs kBegin tiles' time, so an item counts that much more than its
+// tiles (at most an eighth of a part more: a part that lies in the first units
+// only has nothing to do).  Where all items have the same number of tiles and
+// there are few of them, equal parts of every item may be faster: 24 lists of
+// 2,048, 48 items of 32 tiles, take 31 us in 5 parts of 7 tiles an item, and 37
+// in 256 parts of 6.
+__device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, int64_t least, bool begins, int tiles) {
+  Plan p{tiles_all, divide(tiles_all, least), 0, 0, tiles};
   if (p.parts > parts) p.parts = parts;
   if (p.parts < 1) p.parts = 1;
-  if (tiles > 0 && total > 0) {
-    const int64_t items = divide(total, tiles);
+  if (tiles > 0 && items > 0) {
     int64_t split = divide(parts, items);
     if (split * least > tiles) split = divide(tiles, least) > 0 ? divide(tiles, least) : 1;
-    if (split > 0 && (tiles - kBegin * split) * p.parts <= total * split) {
+    if (split > 0 && (tiles - kBegin * split) * p.parts <= tiles_all * split) {
       p.split = static_cast<int>(split);
       p.parts = items * split;
+      return p;
     }
+  }
+  if (begins) {
+    const int64_t eighth = divide(tiles_all, 8 * p.parts);
+    p.begin = eighth < kBegin ? static_cast<int>(eighth) : kBegin;
+    p.total += items * p.begin;
   }
   return p;
 }
@@ -354,25 +363,34 @@ struct Start {
   int64_t base;  // first unit of the request
   Request r;
 };
-template <int THREADS, typename UNITS>
+// UNITS(request): {items, units of an item}; BEGINS: see make_plan.
+struct Units {
+  int64_t items;
+  int64_t tiles;
+};
+template <int THREADS, bool BEGINS, typename UNITS>
 __device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t parts, int64_t least, int tiles,
                                    UNITS units) {
   __shared__ int64_t scratch[THREADS / 64];
   __shared__ int64_t found[5];
   Start s;
   const int tid = threadIdx.x;
+  // Items (below 2^24 + 2^16) and tiles (below 2^39) in one scan.
+  constexpr int kItems = 39;
+  constexpr int64_t kTiles = (int64_t{1} << kItems) - 1;
+  auto both = [](const Units& u) { return (u.items << kItems) + u.items * u.tiles; };
   Request r{};
   int64_t first = 0, sum = 0;
   if (tid < a.batch) {
     r = request_of(a, tid);
-    first = units(r);
+    first = both(units(r));
   }
-  for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum += units(request_of(a, b));
+  for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum += both(units(request_of(a, b)));
   int64_t total;
   if (tid == 0) found[0] = -1;
   int64_t at = scan64<THREADS>(first + sum, scratch, &total);
   total = uniform64(total);
-  s.plan = make_plan(total, parts, least, tiles);
+  s.plan = make_plan(total >> kItems, total & kTiles, parts, least, BEGINS, tiles);
   if (part < s.plan.parts && total > 0) {
     const int64_t u = part_start(s.plan, part);
     int64_t before = 0;
@@ -383,20 +401,21 @@ __device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t p
         first = 0;
         if (b < a.batch) {
           r = request_of(a, b);
-          first = units(r);
+          first = both(units(r));
         }
         int64_t chunk;
         at = before + scan64<THREADS>(first, scratch, &chunk);
         before += chunk;
       }
-      if (u >= at && u < at + first) {
+      auto place = [&](int64_t x) { return (x & kTiles) + (x >> kItems) * s.plan.begin; };
+      if (u >= place(at) && u < place(at + first)) {
         found[0] = b;
-        found[1] = at;
+        found[1] = place(at);
         found[2] = r.row0;
         found[3] = r.n;
         found[4] = r.len;
       }
-      if (u < before) break;
+      if (u < place(before)) break;
     }
   }
   __syncthreads();
@@ -534,15 +553,14 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
 // where a tile outgrows that by more than fp16 holds (the first one does), the
 // group weighs it again against its own.
 //
-// Bound by the phases: 34 MFMAs of 32 clocks a wave (1,088) take about 1,800
+// Bound by the phases: 34 MFMAs of 32 clocks a wave (1,088) take about 2,600
 // with the widening of the codes between them and the other group's softmax on
-// the same SIMD, so a tile takes 1.75 us on a CU; 24 requests of 32,768 tokens
-// and 128 heads in 170 us (0.62 of the large product's rate), 40 ragged ones
-// with 8 heads, whose padded rows cost half the products, in 116 us at
-// 4.1 TB/s.  Before the groups ran in opposite phases these were 175 and
-// 166 us.  Weighed against it: the same products on the 8-bit MFMAs, with bf16
-// queries split into two codes and P into three, took 164 us there and 70
-// instead of 38 us for 24 lists of 2,048.
+// the same SIMD: 24 requests of 32,768 tokens and 64 heads in 168 us (110 GFLOP
+// and 453 MB, 0.51 of the large product's rate), 40 ragged ones with 8 heads in
+// 108 us (4.4 TB/s).  Before the groups ran in opposite phases these were 175
+// and 166 us.  Weighed against it: the same products on the 8-bit MFMAs, with
+// bf16 queries split into two codes and P into three, took 164 us instead of
+// 168 there and 70 instead of 38 for 24 lists of 2,048.
 template <typename T, bool LIST>
 __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Latent8Args a) {
   __shared__ __align__(16) uint8_t keys[3][kKeys * kRow];
@@ -560,8 +578,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int grp = wave >> 2, kg = wave & 1, dh = (wave >> 1) & 1, wg = wave & 3;
   const int64_t part = blockIdx.x;
   const Start start =
-      find_start<kAttnThreads>(a, part, a.parts, kMinUnits, LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
-                               [](const Request& r) { return r.items * r.tiles; });
+      find_start<kAttnThreads, true>(a, part, a.parts, kMinUnits,
+                                     LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
+                                     [](const Request& r) { return Units{r.items, r.tiles}; });
   const Work work = carve_work(a.workspace, a.parts);
   if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
   if (part >= start.plan.parts || start.b < 0) return;
@@ -610,21 +629,24 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 
   while (at < stop) {
     // The next segment: units [u0, u1) of one item.
-    while (at >= base + r.items * r.tiles) {
-      base += r.items * r.tiles;
+    const int begin = start.plan.begin;
+    while (at >= base + r.items * (r.tiles + begin)) {
+      base += r.items * (r.tiles + begin);
       ++b;
       r = request_of(a, b);
     }
-    const int64_t it = divide(at - base, r.tiles);
-    const int64_t item_start = base + it * r.tiles;
-    const int64_t item_end = item_start + r.tiles;
+    const int64_t it = divide(at - base, r.tiles + begin);
+    const int64_t item_start = base + it * (r.tiles + begin);
+    const int64_t item_end = item_start + r.tiles + begin;
     const int64_t seg_end = item_end < stop ? item_end : stop;
     const Item x = item_of(a, r, it);
     const int i_last = LIST ? x.lead : (x.first + x.count - 1) / per;
     const int i_first = LIST ? x.lead : x.first / per;
     const int vis_most = visible(r, i_last), vis_least = visible(r, i_first);
     const int list_len = LIST ? static_cast<int>(a.list_len) : vis_most;
-    int t0 = static_cast<int>(at - item_start), t1 = static_cast<int>(seg_end - item_start);
+    int t0 = static_cast<int>(at - item_start) - begin, t1 = static_cast<int>(seg_end - item_start) - begin;
+    if (t0 < 0) t0 = 0;
+    if (t1 < 0) t1 = 0;
     const int tiles_seen = (list_len + kKeys - 1) / kKeys;
     if (t1 > tiles_seen) t1 = tiles_seen;
     if (t0 > t1) t0 = t1;
@@ -1098,7 +1120,8 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
   auto slices = [](const Request& r) -> int64_t { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
-  const Start start = find_start<kSumThreads>(a, blockIdx.x, kSumParts, kSumWaves, 0, slices);
+  const Start start = find_start<kSumThreads, false>(a, blockIdx.x, kSumParts, kSumWaves, 0,
+                                                     [&](const Request& r) { return Units{1, slices(r)}; });
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
   int64_t b = start.b, base = start.base;

@@ -175,9 +175,11 @@ def pack(*tensors: torch.Tensor | None):
     per tensor, at a third of its host time (a fused step describes 27
     tensors); the buffer has to outlive the call that reads it."""
     values: list[int] = []
+    missing = False
     for t in tensors:
         if t is None:
             values += _NO_TENSOR
+            missing = True
             continue
         shape = t.shape
         n = len(shape)
@@ -190,7 +192,7 @@ def pack(*tensors: torch.Tensor | None):
     packer.pack_into(buf, 0, *values)
     base = ctypes.addressof(buf)
     at = [base + i * _ITEM_BYTES for i in range(len(tensors))]
-    if any(t is None for t in tensors):
+    if missing:
         at = [None if t is None else p for t, p in zip(tensors, at)]
     return buf, at
 

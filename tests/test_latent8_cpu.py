@@ -170,6 +170,20 @@ def test_attention_refusals(mutate, code, msg):
     assert (status, msg in text) == (code, True), (status, text)
 
 
+@pytest.mark.parametrize("rows,topk", [((1 << 20) - 1, False), ((1 << 20) - 1, True)])
+def test_attention_refuses_more_items_than_it_counts(rows, topk):
+    """1,024 latent heads of one head each: an item for every row and head."""
+    a = _attention_args(T=rows, N=1024)
+    B = 1 << 15
+    for key, i, n in (("cache", 2, 1024), ("scale", 1, 1024), ("table", 0, B), ("seq_q", 0, B), ("seq_kv", 0, B),
+                      ("entries", 0, B)):
+        a[key].shape[i] = n
+    if topk:
+        a.update(topk=_desc((rows, 16), 0), entries=None, weights_pool=None)
+    status, text = _attention(a)
+    assert (status, "too many query rows and heads" in text) == (1, True), (status, text)
+
+
 def test_attention_workspace_refusals():
     from nanovllm_amd import _lib
 
