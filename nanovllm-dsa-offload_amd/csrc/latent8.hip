@@ -239,6 +239,7 @@ constexpr int kAttnThreads = 512;
 constexpr int kRows = 64;       // (query row, head) pairs of an item
 constexpr int kKeys = 64;       // keys of a tile
 constexpr int kWindow = 512;    // resolved pages (or list entries) held at a time
+constexpr int kLoads = kKeys * kRowChunks / (kAttnThreads / 2);  // of a thread (group 1) for a tile
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
 constexpr float kMost = 14.f;   // scores pass the maximum by this at most (base 2): P <= 2^14 and a scale's fraction fit fp16
@@ -569,7 +570,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   __shared__ __align__(16) float row_max[2][2][32][4];  // group, tile parity, row, wave
   __shared__ int outgrown[2][2];                        // group, tile parity
   __shared__ int bad_entries[2][LIST ? kWindow / kKeys : 1];  // tiles of a window with entries that name nothing
-  __shared__ Window windows[2][kWindow];
+  __shared__ Window windows[LIST ? 2 : 1][kWindow];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -594,18 +595,19 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 
   // A tile's row k in LDS holds chunk c (16 bytes) at place c ^ ((k >> 2) & 3)
   // within its group of four: 16 keys of one chunk then lie in 64 different
-  // banks.  Rows go straight to LDS, 64 places a wave and load; this lane's
-  // places of a tile, the keys and the byte of the row that belong there:
-  int key_of[LIST ? 5 : 1];
-  uint32_t byte_of[5];
+  // banks.  Rows go straight to LDS, 64 places a wave (of group 1) and load;
+  // this lane's places of a tile, the keys and the byte of the row that belong
+  // there:
+  int key_of[LIST ? kLoads : 1];
+  uint32_t byte_of[kLoads];
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const int q = i * kAttnThreads + tid;
+  for (int i = 0; i < kLoads; ++i) {
+    const int q = i * (kAttnThreads / 2) + wg * 64 + lane;
     const int k = q / kRowChunks, c = q - k * kRowChunks;
     if (LIST) key_of[LIST ? i : 0] = k;
     byte_of[i] = static_cast<uint32_t>(((c & ~3) | ((c ^ (k >> 2)) & 3)) * 16 + (LIST ? 0 : k * row_bytes));
   }
-  const uint32_t lds_keys = lds_address(keys) + wave * 1024;
+  const uint32_t lds_keys = lds_address(keys) + wg * 1024;
   // LDS addresses of the score operand (chunks 18 dh + 2 j + hh) and of V.
   int k_at[2], v_at[2];
   {
@@ -653,12 +655,13 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     const bool busy = grp == 0 || x.count > 32;  // the group has rows
 
     const int32_t* list = LIST ? a.topk + (r.row0 + x.lead) * a.list_len : nullptr;
-    // Windows of resolved pages (list: entries), the tile's own and the next.
+    // Tiles [c0, c1) run together: their pages are resolved before them, or,
+    // with a list, windows of entries as the tiles pass, two at a time.
     constexpr int kWindowTiles = LIST ? kWindow / kKeys : 2 * kWindow;
-    const int w0 = LIST ? t0 : t0 & ~1;
+    int c0 = t0, c1 = t1, w0 = t0;
     // This thread's entry of the window that begins with a tile: its row, and
     // the rest, for which nobody waits before the rows themselves are on the way.
-    auto window_at = [&](int tile) -> Window& { return windows[((tile - w0) / kWindowTiles) & 1][tid]; };
+    auto window_at = [&](int tile) -> Window& { return windows[LIST ? ((tile - w0) / kWindowTiles) & 1 : 0][tid]; };
     auto window_rows = [&](int tile) {
       if (LIST) {
         const int e = tile * kKeys + tid;
@@ -690,11 +693,6 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         q[j][1] = p[1];
       }
     }
-    lds_barrier();  // the previous segment is done with LDS
-    if (t0 < t1) {
-      window_rows(w0);
-      if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
-    }
     f32x16_t o[4], s;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
@@ -705,51 +703,72 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 
     auto window_of = [&](int tile) -> const Window* {
       const unsigned i = tile - w0;
-      return &windows[(i / kWindowTiles) & 1][LIST ? (i % kWindowTiles) * kKeys : (i % kWindowTiles) >> 1];
+      if (LIST) return &windows[LIST ? (i / kWindowTiles) & 1 : 0][(i % kWindowTiles) * kKeys];
+      return &windows[0][(i >> 1) & (kWindow - 1)];
     };
-    auto load_tile = [&](int tile, int buf) {
-      const Window* w = window_of(tile);
-      const uint32_t to = lds_keys + buf * (kKeys * kRow);
+    // Without a list: the pages of the tiles in the three buffers and of the
+    // one after them, in scalar registers.
+    Window page_before{}, page_now{}, page_next{}, page_far{};
+    auto scalar = [&](const Window& v) {
+      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.exponent), first_lane(v.fraction)};
+    };
+    // A tile's loads, by the waves of group 1, issued a few at a time.
+    struct TileLoad {
+      const uint8_t* base;
+      uint32_t to;
+      int32_t row[LIST ? kLoads : 1];
+      bool on;
+    };
+    auto begin_load = [&](int tile, int buf, int32_t page_row) {
+      TileLoad l;
+      l.on = tile < c1;
+      l.to = lds_keys + buf * (kKeys * kRow);
       if (LIST) {
-        int32_t row[LIST ? 5 : 1];
+        l.base = static_cast<const uint8_t*>(a.latent_cache) + x.g * kRow;
+        if (l.on) {
+          const Window* w = window_of(tile);
 #pragma unroll
-        for (int i = 0; i < 5; ++i) row[LIST ? i : 0] = w[key_of[LIST ? i : 0] & (kKeys - 1)].row;
-#pragma unroll
-        for (int i = 0; i < 5; ++i)
-          if (i < 4 || wave < 4)
-            load_to_lds(static_cast<const uint8_t*>(a.latent_cache) +
-                            static_cast<int64_t>(row[LIST ? i : 0] < 0 ? 0 : row[LIST ? i : 0]) * row_bytes + x.g * kRow +
-                            byte_of[i],
-                        to + i * (kAttnThreads * 16));
+          for (int i = 0; i < kLoads; ++i) l.row[LIST ? i : 0] = w[key_of[LIST ? i : 0]].row;
+        }
       } else {
-        const int32_t page = __builtin_amdgcn_readfirstlane(w->row);
-        const uint8_t* p = static_cast<const uint8_t*>(a.latent_cache) +
-                           (static_cast<int64_t>(page < 0 ? 0 : page) + (tile & 1) * kKeys) * row_bytes + x.g * kRow;
+        l.base = static_cast<const uint8_t*>(a.latent_cache) +
+                 (static_cast<int64_t>(page_row < 0 ? 0 : page_row) + (tile & 1) * kKeys) * row_bytes + x.g * kRow;
+      }
+      return l;
+    };
+    auto issue_load = [&](const TileLoad& l, int i0, int i1) {
+      if (!l.on) return;
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
-          if (i < 4 || wave < 4) load_to_lds(p, byte_of[i], to + i * (kAttnThreads * 16));
+      for (int i = i0; i < i1; ++i) {
+        if (LIST) {
+          const int32_t row = l.row[LIST ? i : 0];
+          load_to_lds(l.base + static_cast<int64_t>(row < 0 ? 0 : row) * row_bytes + byte_of[i], l.to + i * 4096);
+        } else {
+          load_to_lds(l.base, byte_of[i], l.to + i * 4096);
+        }
       }
     };
-    // Scale fields of this lane's keys of a tile: one page's (uniform), or each entry's.
+    auto load_tile = [&](int tile, int buf, int32_t page_row) {
+      const TileLoad l = begin_load(tile, buf, page_row);
+      issue_load(l, 0, kLoads);
+    };
+    // Scale fields of this lane's keys of the tile before: one page's (uniform), or each entry's.
     auto fields = [&](int tile, Window(&w)[LIST ? 8 : 1]) {
-      const Window* from = window_of(tile);
       if (LIST) {
+        const Window* from = window_of(tile);
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[LIST ? e : 0] = from[key_mine + 8 * (e >> 2) + (e & 3)];
       } else {
-        w[0].row = __builtin_amdgcn_readfirstlane(from->row);
-        w[0].score = first_lane(from->score);
-        w[0].exponent = first_lane(from->exponent);
-        w[0].fraction = first_lane(from->fraction);
+        w[0] = page_before;
       }
     };
-    // Whether some row must not see some key of the tile.
+    // Whether some row must not see some key of the tile before.
     auto ragged_tile = [&](int tile) -> bool {
       if (LIST) {
         const unsigned i = tile - w0;
         return __builtin_amdgcn_readfirstlane(bad_entries[(i / kWindowTiles) & 1][LIST ? i % kWindowTiles : 0]) != 0;
       }
-      return (tile + 1) * kKeys > vis_least || __builtin_amdgcn_readfirstlane(window_of(tile)->row) < 0;
+      return (tile + 1) * kKeys > vis_least || page_before.row < 0;
     };
     // P of the tile's scores against the maximum, into LDS; l_tile: their sum.
     auto weigh = [&](const Window(&w)[LIST ? 8 : 1]) {
@@ -782,44 +801,64 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= grow;
     };
-    // S^T of tile t in nine steps of 32 dims, and O^T of tile t - 1 in
-    // eight steps of 16 keys and two of the wave's four tiles of dims
-    // (OUTPUT), step by step together: two independent streams of MFMAs, each
-    // step's operands read a step ahead.
-    auto multiply = [&](const uint8_t* k_tile, const uint8_t* v_tile, auto with_output) {
+    // A tile that outgrew the maximum, against its own.
+    auto weigh_again = [&](int tile) {
+      follow_max(tile);
+      Window w[LIST ? 8 : 1];
+      fields(tile, w);
+      weigh(w);
+    };
+    // S^T of tile t in nine steps of 32 dims, and O^T of tile t - 1 in eight
+    // steps of 16 keys and two of the wave's four tiles of dims (OUTPUT), step
+    // by step together: two independent streams of MFMAs, each step's operands
+    // read two steps ahead.
+    auto multiply = [&](int t, const uint8_t* k_tile, const uint8_t* v_tile, auto with_output) {
       constexpr bool OUTPUT = decltype(with_output)::value;
-      u32x4_t k[2];
-      uint2 v[2][2];
+      constexpr int kAhead = 2;
+      u32x4_t k[kAhead + 1];
+      uint2 v[kAhead + 1][2];
       f16x8_t p[2];
+      auto fetch_p = [&](int ks) {
+        p[ks & 1] = *reinterpret_cast<const f16x8_t*>(&p_mine[l32 * kPStride + ks * 16 + 8 * hh]);
+      };
       auto fetch = [&](int j) {
-        if (j < 9) k[j & 1] = *reinterpret_cast<const u32x4_t*>(&k_tile[k_at[j & 1] + (j >> 1) * 64]);
+        const int at = j % (kAhead + 1);
+        if (j < 9) k[at] = *reinterpret_cast<const u32x4_t*>(&k_tile[k_at[j & 1] + (j >> 1) * 64]);
         if (OUTPUT && j < 8) {
           const int ks = j >> 1;
-          if ((j & 1) == 0) p[ks & 1] = *reinterpret_cast<const f16x8_t*>(&p_mine[l32 * kPStride + ks * 16 + 8 * hh]);
+          if ((j & 1) == 0) fetch_p(ks);
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd)
-            v[j & 1][odd] = read_tr8(&v_tile[v_at[odd] + (j & 1) * 64 + ks * 16 * kRow]);
+          for (int odd = 0; odd < 2; ++odd) v[at][odd] = read_tr8(&v_tile[v_at[odd] + (j & 1) * 64 + ks * 16 * kRow]);
         }
       };
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0.f;
+      int again = 0;
+      if (OUTPUT) again = outgrown[grp][(t - 1) & 1];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) fetch(j);
       if (OUTPUT) {
+        if (__builtin_amdgcn_readfirstlane(again) != 0) {  // (every wave waits for it)
+          weigh_again(t - 1);
+          lds_barrier();
+          fetch_p(0);
+        }
         l_run += l_tile;
         // Values with one use each: the first product of a tile then adds to
         // the accumulators in place (the compiler keeps a second set otherwise).
         asm volatile("" : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]));
       }
-      fetch(0);
 #pragma unroll
       for (int j = 0; j < 9; ++j) {
-        fetch(j + 1);
-        const u32x4_t kj = k[j & 1];
+        fetch(j + kAhead);
+        const int at = j % (kAhead + 1);
+        const u32x4_t kj = k[at];
         s = T::mfma32(widen8<T>(kj[0], kj[1]), __builtin_bit_cast(typename T::vec8, q[j][0]), s);
         if (OUTPUT && j < 8)
-          o[2 * (j & 1)] = F16::mfma32(widen8<F16>(v[j & 1][0].x, v[j & 1][0].y), p[(j >> 1) & 1], o[2 * (j & 1)]);
+          o[2 * (j & 1)] = F16::mfma32(widen8<F16>(v[at][0].x, v[at][0].y), p[(j >> 1) & 1], o[2 * (j & 1)]);
         s = T::mfma32(widen8<T>(kj[2], kj[3]), __builtin_bit_cast(typename T::vec8, q[j][1]), s);
         if (OUTPUT && j < 8)
-          o[2 * (j & 1) + 1] = F16::mfma32(widen8<F16>(v[j & 1][1].x, v[j & 1][1].y), p[(j >> 1) & 1], o[2 * (j & 1) + 1]);
+          o[2 * (j & 1) + 1] = F16::mfma32(widen8<F16>(v[at][1].x, v[at][1].y), p[(j >> 1) & 1], o[2 * (j & 1) + 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
       // Keys 0-15 of a wave's 32 are finished by the first half of the
@@ -828,130 +867,153 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       for (int e = 0; e < 2; ++e)
         half_s[(wave * 2 + e) * 64 + lane] = make_float4(s[8 + 4 * e], s[9 + 4 * e], s[10 + 4 * e], s[11 + 4 * e]);
     };
-    // Phase 2: P of tile t.
-    auto softmax = [&](int t) {
-      float4 other[2];
+    // Phase 2: P of tile t, and (group 1) the loads of tile t + 2 into buffer
+    // `to`, spread over it.  Returns whether the other group weighs again in
+    // this phase.
+    auto softmax = [&](int t, int to, auto with_rows) -> bool {
+      constexpr bool ROWS = decltype(with_rows)::value;
+      const int other_tile = t + grp - 1;  // weighed last by the other group
+      int past = 0;
+      if (other_tile >= c0) past = outgrown[grp ^ 1][other_tile & 1];
+      Window far{};
+      if (!LIST) far = *window_of(t + 3);
+      if constexpr (ROWS) {
+        float4 other[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) other[e] = half_s[((wave ^ 2) * 2 + e) * 64 + lane];
-      Window w[LIST ? 8 : 1];
-      fields(t, w);
-      if (wg == 0 && lane == 0) outgrown[grp][(t + 1) & 1] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float4& x4 = other[e >> 2];
-        const float half = (e & 3) == 0 ? x4.x : (e & 3) == 1 ? x4.y : (e & 3) == 2 ? x4.z : x4.w;
-        sc[e] = fmaf(s[e] + half, w[LIST ? e : 0].score, w[LIST ? e : 0].exponent);
-      }
-      if (ragged_tile(t)) {
+        for (int e = 0; e < 2; ++e) other[e] = half_s[((wave ^ 2) * 2 + e) * 64 + lane];
+        Window w[LIST ? 8 : 1];
+        fields(t, w);
+        if (wg == 0 && lane == 0) outgrown[grp][(t + 1) & 1] = 0;
+        TileLoad load;
+        load.on = false;
+        if (grp == 1) load = begin_load(t + 2, to, page_next.row);
+        issue_load(load, 0, 3);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const bool ok = w[LIST ? e : 0].row >= 0 && (LIST || t * kKeys + key_mine + 8 * (e >> 2) + (e & 3) < vis_row);
-          sc[e] = ok ? sc[e] : -INFINITY;
+          const float4& x4 = other[e >> 2];
+          const float half = (e & 3) == 0 ? x4.x : (e & 3) == 1 ? x4.y : (e & 3) == 2 ? x4.z : x4.w;
+          sc[e] = fmaf(s[e] + half, w[LIST ? e : 0].score, w[LIST ? e : 0].exponent);
         }
-      }
-      float top = sc[0];
+        if (ragged_tile(t)) {
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
-      top = xor32_op(top, MaxOp{});
-      if (hh == 0) row_max[grp][t & 1][l32][wg] = top;
-      if (__any(top > m_run + kMost) && lane == 0) outgrown[grp][t & 1] = 1;
-      weigh(w);
+          for (int e = 0; e < 8; ++e) {
+            const bool ok = w[LIST ? e : 0].row >= 0 && (LIST || t * kKeys + key_mine + 8 * (e >> 2) + (e & 3) < vis_row);
+            sc[e] = ok ? sc[e] : -INFINITY;
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        issue_load(load, 3, 6);
+        float top = sc[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+        top = xor32_op(top, MaxOp{});
+        if (hh == 0) row_max[grp][t & 1][l32][wg] = top;
+        if (__any(top > m_run + kMost) && lane == 0) outgrown[grp][t & 1] = 1;
+        __builtin_amdgcn_sched_barrier(0);
+        issue_load(load, 6, kLoads);
+        weigh(w);
+      } else {
+        if (grp == 1) load_tile(t + 2, to, page_next.row);
+      }
+      if (!LIST) page_far = scalar(far);
+      return __builtin_amdgcn_readfirstlane(past) != 0;
     };
-    // Whether group g, about to multiply tile t, has to weigh the one before
-    // again first (then every wave waits for it).
-    auto again = [&](int g, int t) -> bool {
-      return t > t0 && __builtin_amdgcn_readfirstlane(outgrown[g][(t - 1) & 1]) != 0;
+    // Group 0 multiplies tile t in phase 2 (t - c0) and weighs it in the next,
+    // group 1 a phase later.  Tile t is in buffer (t - c0) % 3, loaded during
+    // the two phases before 2 (t - c0): the last reader of what was there,
+    // group 1's product of tile t - 3, ran in phase 2 (t - c0) - 3.
+    int buf = 0, before = 2, next = 1;
+    auto rotate = [&] {
+      page_before = page_now;
+      page_now = page_next;
+      page_next = page_far;
+      before = buf;
+      buf = next;
+      next = next == 2 ? 0 : next + 1;
     };
-    if (t0 < t1) {
+    // What every wave does at the start of the phase in which group 0
+    // multiplies tile t: with a list, the next window of entries; and, before
+    // anyone's output product of tile t - 1, zeros for its NaN codes if some
+    // row must not see some key of it (P is zero there, but zero times NaN is
+    // not; a row that does see such a key has NaN scores, hence NaN sums).
+    auto even_phase = [&](int t) {
+      if (LIST && t + 1 < c1 && (t + 1 - w0) % kWindowTiles == 0) {
+        window_rows(t + 1);
+        window_scales(t + 1);
+        __syncthreads();
+      }
+      if (t > c0 && ragged_tile(t - 1)) {
+        for (int c = tid; c < kKeys * kRowChunks; c += kAttnThreads) {
+          u32x4_t* v = reinterpret_cast<u32x4_t*>(&keys[before][c * 16]);
+          const u32x4_t u = *v;
+          *v = u32x4_t{nan_to_zero4(u[0]), nan_to_zero4(u[1]), nan_to_zero4(u[2]), nan_to_zero4(u[3])};
+        }
+        lds_barrier();
+      }
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    // The phases of a group (ROWS: it has rows; one without keeps step with
+    // the loads and barriers).
+    auto phases = [&](auto with_rows) {
+      constexpr bool ROWS = decltype(with_rows)::value;
+      even_phase(c0);
+      if (grp == 1) {
+        load_tile(c0 + 1, 1, page_next.row);
+        lds_barrier();
+      }
+      if constexpr (ROWS) multiply(c0, keys[0], keys[0], no);
+      if (grp == 1) wait_loads<0>();
       lds_barrier();
-      load_tile(t0, 0);
+      rotate();
+      for (int t = c0;; ++t) {
+        // Phase 2 of tile t.
+        if (grp == 1) even_phase(t + 1);
+        const bool past = softmax(t, next, with_rows);
+        if (past) lds_barrier();
+        lds_barrier();
+        // Phase 1 of tile t + 1.  (After the last tile its scores are those of
+        // no tile, and nobody reads them: with a second form of the product the
+        // compiler keeps a copy of the accumulators, 64 registers that spill.)
+        if (grp == 0) even_phase(t + 1);
+        if constexpr (ROWS) {
+          multiply(t + 1, keys[buf], keys[before], yes);
+        }
+        if (grp == 1) wait_loads<0>();
+        lds_barrier();
+        if (t + 1 >= c1) break;
+        rotate();
+      }
+      if (grp == 0) {
+        if (__builtin_amdgcn_readfirstlane(outgrown[1][(c1 - 1) & 1]) != 0) lds_barrier();
+        lds_barrier();
+      }
+    };
+    for (; c0 < t1; c0 = c1) {
+      lds_barrier();  // the tiles before are done with LDS
+      if (!LIST) c1 = t1 - (c0 & ~1) < kWindowTiles ? t1 : (c0 & ~1) + kWindowTiles;
+      w0 = LIST ? c0 : c0 & ~1;
+      window_rows(w0);
+      if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
+      lds_barrier();
+      buf = 0;
+      before = 2;
+      next = 1;
+      if (grp == 1) load_tile(c0, 0, LIST ? 0 : __builtin_amdgcn_readfirstlane(window_of(c0)->row));
       window_scales(w0);
       wait_loads<0>();
       lds_barrier();
-      // Group 0 multiplies tile t in phase 2 (t - t0) and weighs it in the
-      // next, group 1 a phase later.  Tile t is in buffer (t - t0) % 3, loaded
-      // during the two phases before 2 (t - t0): the last reader of what was
-      // there, group 1's product of tile t - 3, ran in phase 2 (t - t0) - 3.
-      int buf = 0, before = 2, next = 1;
-      auto load_next = [&](int tile, int to) {
-        if (tile >= t1) return;
-        if ((tile - w0) % kWindowTiles == 0) {
-          window_rows(tile);
-          window_scales(tile);
-          __syncthreads();
-        }
-        load_tile(tile, to);
-      };
-      auto rotate = [&] {
-        before = buf;
-        buf = next;
-        next = next == 2 ? 0 : next + 1;
-      };
-      // What every wave does at the start of the phase in which group 0
-      // multiplies tile t: the loads of the next tile; and, before anyone's
-      // output product of tile t - 1, zeros for its NaN codes if some row must
-      // not see some key of it (P is zero there, but zero times NaN is not; a
-      // row that does see such a key has NaN scores, hence NaN sums).
-      auto even_phase = [&](int t, int to, int buf_before) {
-        load_next(t + 1, to);
-        if (t > t0 && ragged_tile(t - 1)) {
-          for (int c = tid; c < kKeys * kRowChunks; c += kAttnThreads) {
-            u32x4_t* v = reinterpret_cast<u32x4_t*>(&keys[buf_before][c * 16]);
-            const u32x4_t u = *v;
-            *v = u32x4_t{nan_to_zero4(u[0]), nan_to_zero4(u[1]), nan_to_zero4(u[2]), nan_to_zero4(u[3])};
-          }
-          lds_barrier();
-        }
-      };
-      const std::true_type yes;
-      const std::false_type no;
-      // The phases of a group (ROWS: it has rows; one without keeps step with
-      // the loads and barriers).  Group 1 begins a phase later.
-      auto phases = [&](auto with_rows) {
-        constexpr bool ROWS = decltype(with_rows)::value;
-        even_phase(t0, 1, 2);
-        if (grp == 1) lds_barrier();
-        if (ROWS) multiply(keys[0], keys[0], no);
-        if (grp == 1) wait_loads<0>();
-        lds_barrier();
-        rotate();
-        for (int t = t0;; ++t) {
-          // Phase 2 of tile t.
-          if (grp == 1) even_phase(t + 1, next, before);
-          if (again(grp ^ 1, t + grp)) lds_barrier();
-          if (ROWS) softmax(t);
-          if (grp == 0) wait_loads<0>();
-          lds_barrier();
-          // Phase 1 of tile t + 1.
-          if (grp == 0) even_phase(t + 1, next, before);
-          if (again(grp, t + 1)) {
-            if (ROWS) {
-              follow_max(t);
-              Window w[LIST ? 8 : 1];
-              fields(t, w);
-              weigh(w);
-            }
-            lds_barrier();
-          }
-          // (After the last tile its scores are those of no tile, and nobody
-          // reads them: with a second form of the product the compiler keeps a
-          // copy of the accumulators, 64 registers that spill.)
-          if (ROWS) multiply(keys[buf], keys[before], yes);
-          if (grp == 1) wait_loads<0>();
-          lds_barrier();
-          if (t + 1 >= t1) break;
-          rotate();
-        }
-        if (grp == 0) {
-          if (again(1, t1)) lds_barrier();
-          lds_barrier();
-        }
-      };
+      if (!LIST) {
+        page_now = scalar(*window_of(c0));
+        page_next = scalar(*window_of(c0 + 1));
+        page_far = scalar(*window_of(c0 + 2));
+      }
       if (busy)
         phases(yes);
       else
         phases(no);
     }
+    lds_barrier();
 
     // Sum of p of every row: over the lane halves and the group's four waves.
     l_run = xor32_op(l_run, AddOp{});
