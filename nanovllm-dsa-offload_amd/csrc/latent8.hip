@@ -596,16 +596,14 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   // A tile's row k in LDS holds chunk c (16 bytes) at place c ^ ((k >> 2) & 3)
   // within its group of four: 16 keys of one chunk then lie in 64 different
   // banks.  Rows go straight to LDS, 64 places a wave (of group 1) and load;
-  // this lane's places of a tile, the keys and the byte of the row that belong
-  // there:
-  int key_of[LIST ? kLoads : 1];
+  // this lane's places of a tile, the byte that belongs there: of the page, or,
+  // with a list, of its row in the low 16 bits and the key above them.
   uint32_t byte_of[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int q = i * (kAttnThreads / 2) + wg * 64 + lane;
     const int k = q / kRowChunks, c = q - k * kRowChunks;
-    if (LIST) key_of[LIST ? i : 0] = k;
-    byte_of[i] = static_cast<uint32_t>(((c & ~3) | ((c ^ (k >> 2)) & 3)) * 16 + (LIST ? 0 : k * row_bytes));
+    byte_of[i] = static_cast<uint32_t>(((c & ~3) | ((c ^ (k >> 2)) & 3)) * 16 + (LIST ? k << 16 : k * row_bytes));
   }
   const uint32_t lds_keys = lds_address(keys) + wg * 1024;
   // LDS addresses of the score operand (chunks 18 dh + 2 j + hh) and of V.
@@ -728,7 +726,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         if (l.on) {
           const Window* w = window_of(tile);
 #pragma unroll
-          for (int i = 0; i < kLoads; ++i) l.row[LIST ? i : 0] = w[key_of[LIST ? i : 0]].row;
+          for (int i = 0; i < kLoads; ++i) l.row[LIST ? i : 0] = w[byte_of[i] >> 16].row;
         }
       } else {
         l.base = static_cast<const uint8_t*>(a.latent_cache) +
@@ -742,7 +740,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       for (int i = i0; i < i1; ++i) {
         if (LIST) {
           const int32_t row = l.row[LIST ? i : 0];
-          load_to_lds(l.base + static_cast<int64_t>(row < 0 ? 0 : row) * row_bytes + byte_of[i], l.to + i * 4096);
+          load_to_lds(l.base + static_cast<int64_t>(row < 0 ? 0 : row) * row_bytes + (byte_of[i] & 0xffffu), l.to + i * 4096);
         } else {
           load_to_lds(l.base, byte_of[i], l.to + i * 4096);
         }
@@ -886,7 +884,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         if (wg == 0 && lane == 0) outgrown[grp][(t + 1) & 1] = 0;
         TileLoad load;
         load.on = false;
-        if (grp == 1) load = begin_load(t + 2, to, page_next.row);
+        if (!LIST && grp == 1) load = begin_load(t + 2, to, page_next.row);
         issue_load(load, 0, 3);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -902,7 +900,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
           }
         }
         __builtin_amdgcn_sched_barrier(0);
-        issue_load(load, 3, 6);
+        // (A list's rows come when its scale fields have been used: both at
+        // once do not fit the registers.)
+        if (LIST && grp == 1) load = begin_load(t + 2, to, 0);
+        issue_load(load, LIST ? 0 : 3, 6);
         float top = sc[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
