@@ -242,7 +242,7 @@ constexpr int kWindow = 512;    // resolved pages (or list entries) held at a ti
 constexpr int kLoads = kKeys * kRowChunks / (kAttnThreads / 2);  // of a thread (group 1) for a tile
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
-constexpr float kMost = 14.f;   // scores pass the maximum by this at most (base 2): P <= 2^14 and a scale's fraction fit fp16
+constexpr float kMost = 15.f;   // scores pass a row's reference by this at most (base 2): P <= 2^15 fits fp16
 constexpr int kMinUnits = 1;    // least tiles of a workgroup
 constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
@@ -517,14 +517,15 @@ __device__ inline float first_lane(float x) {
   return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
 }
 
-// A page's (or list entry's) scale c = fraction * 2^exponent, fraction in
-// [1, 2): scores take c, P enters the product with V as p * 2^exponent *
-// fraction against the codes, and the sum of p divides 2^exponent out again.
+// What a page's (or list entry's) scale c enters: scores take it as a factor,
+// P its logarithm into the exponent (p * c multiplies V's codes; exact for a
+// power of two, else off by the logarithm's rounding), and the sum of p
+// divides it out again.
 struct Window {
   int32_t row;    // first cache row of the page, or the entry's row; -1: none
   float score;    // softmax scale * log2(e) * c
-  float exponent;
-  float fraction;
+  float log2c;
+  float inverse;
 };
 __device__ inline int32_t row_of_slot(const Latent8Args& a, int64_t b, int64_t slot, bool ok) {
   if (!ok) return -1;
@@ -537,8 +538,9 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
   c = fminf(fmaxf(c, kMinScale), FLT_MAX);
   const uint32_t u = __float_as_uint(c);
   w.score = a.scale * kLog2e * c;
-  w.exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
-  w.fraction = __uint_as_float((u & 0x7fffffu) | 0x3f800000u);
+  const float exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
+  w.log2c = exponent + __builtin_amdgcn_logf(__uint_as_float((u & 0x7fffffu) | 0x3f800000u));
+  w.inverse = 1.f / c;
 }
 
 // Eight waves in two groups of four: group g owns rows 32 g .. 32 g + 31 of the
@@ -550,18 +552,20 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
 // The groups run in opposite phases, one barrier a phase: while one multiplies
 // (the scores of tile t and the output product of tile t - 1, two independent
 // streams of MFMAs), the other takes its softmax, and each SIMD holds one wave
-// of either.  P(t) is taken against the running maximum of the tiles before t;
-// where a tile outgrows that by more than fp16 holds (the first one does), the
-// group weighs it again against its own.
+// of either.  P(t) is taken against a reference, the running maximum at some
+// tile before; where a tile outgrows that by more than fp16 holds, or is the
+// first that a row sees, the group weighs it again against its own maximum.
 //
-// Bound by the phases: 34 MFMAs of 32 clocks a wave (1,088) take about 2,600
-// with the widening of the codes between them and the other group's softmax on
-// the same SIMD: 24 requests of 32,768 tokens and 64 heads in 168 us (110 GFLOP
-// and 453 MB, 0.51 of the large product's rate), 40 ragged ones with 8 heads in
-// 108 us (4.4 TB/s).  Before the groups ran in opposite phases these were 175
-// and 166 us.  Weighed against it: the same products on the 8-bit MFMAs, with
-// bf16 queries split into two codes and P into three, took 164 us instead of
-// 168 there and 70 instead of 38 for 24 lists of 2,048.
+// Bound by the phases, of about 2,050 clocks each: a wave's 34 MFMAs of 32
+// clocks (1,088) take 1,600 alone on their SIMD and 1,900 next to the other
+// group's softmax, group 1's softmax with the loads 1,500.  In the loop that is
+// 1.0 PFLOP/s, of the 1.27 that a large product reaches.  A part's start (10
+// us) and its partial sums (3 us) come to that: 24 requests of 32,768 tokens
+// and 64 heads in 155 us (110 GFLOP, 453 MB), 40 ragged ones with 8 heads in
+// 103 us (4.6 TB/s), 2 x 515 rows over up to 8,197 tokens, 2 x 16 heads, in
+// 465 us.  One phase for all waves took 175, 166 and 565.  Weighed against it:
+// the same products on the 8-bit MFMAs, with bf16 queries split into two codes
+// and P into three, took 164 us for the first and twice as long for lists.
 template <typename T, bool LIST>
 __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Latent8Args a) {
   __shared__ __align__(16) uint8_t keys[3][kKeys * kRow];
@@ -708,7 +712,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     // one after them, in scalar registers.
     Window page_before{}, page_now{}, page_next{}, page_far{};
     auto scalar = [&](const Window& v) {
-      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.exponent), first_lane(v.fraction)};
+      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.log2c), first_lane(v.inverse)};
     };
     // A tile's loads, by the waves of group 1, issued a few at a time.
     struct TileLoad {
@@ -768,7 +772,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       }
       return (tile + 1) * kKeys > vis_least || page_before.row < 0;
     };
-    // P of the tile's scores against the maximum, into LDS; l_tile: their sum.
+    // P of the tile's scores against the row's reference, into LDS; l_tile: their sum.
     auto weigh = [&](const Window(&w)[LIST ? 8 : 1]) {
       l_tile = 0.f;
 #pragma unroll
@@ -776,24 +780,27 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         float pw[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const Window& wk = w[LIST ? 4 * e + k : 0];
-          const float v = __builtin_amdgcn_exp2f(sc[4 * e + k] - m_run);
-          l_tile += LIST ? ldexpf(v, -static_cast<int>(wk.exponent)) : v;
-          pw[k] = v * wk.fraction;
+          pw[k] = __builtin_amdgcn_exp2f(sc[4 * e + k]);
+          l_tile = LIST ? fmaf(pw[k], w[LIST ? 4 * e + k : 0].inverse, l_tile) : l_tile + pw[k];
         }
         const uint2 packed = make_uint2(F16::pack2(pw[0], pw[1]), F16::pack2(pw[2], pw[3]));
         *reinterpret_cast<uint2*>(&p_mine[l32 * kPStride + key_mine + 8 * e]) = packed;
       }
-      if (!LIST) l_tile = ldexpf(l_tile, -static_cast<int>(w[0].exponent));
+      if (!LIST) l_tile *= w[0].inverse;
     };
-    // The running maximum against that of a tile; the sums so far follow.
+    // The row's reference, which scores are relative to, follows its maximum;
+    // the sums so far follow the reference.
+    auto reference = [&] { return m_run == kNoMax ? 0.f : m_run; };
     auto follow_max = [&](int tile) {
       const float4 v = *reinterpret_cast<const float4*>(row_max[grp][tile & 1][l32]);
       const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
       const bool past = most > m_run;
       const float grow = past ? __builtin_amdgcn_exp2f(m_run - most) : 1.f;
+      const float down = past ? reference() - most : 0.f;
       m_run = past ? most : m_run;
       l_run *= grow;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sc[e] += down;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -886,11 +893,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         load.on = false;
         if (!LIST && grp == 1) load = begin_load(t + 2, to, page_next.row);
         issue_load(load, 0, 3);
+        const float ref = reference();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4& x4 = other[e >> 2];
           const float half = (e & 3) == 0 ? x4.x : (e & 3) == 1 ? x4.y : (e & 3) == 2 ? x4.z : x4.w;
-          sc[e] = fmaf(s[e] + half, w[LIST ? e : 0].score, w[LIST ? e : 0].exponent);
+          sc[e] = fmaf(s[e] + half, w[LIST ? e : 0].score, w[LIST ? e : 0].log2c - ref);
         }
         if (ragged_tile(t)) {
 #pragma unroll
@@ -908,8 +916,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 #pragma unroll
         for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
         top = xor32_op(top, MaxOp{});
-        if (hh == 0) row_max[grp][t & 1][l32][wg] = top;
-        if (__any(top > m_run + kMost) && lane == 0) outgrown[grp][t & 1] = 1;
+        if (hh == 0) row_max[grp][t & 1][l32][wg] = top + ref;
+        if (__any(top > (m_run == kNoMax ? -INFINITY : kMost)) && lane == 0) outgrown[grp][t & 1] = 1;
         __builtin_amdgcn_sched_barrier(0);
         issue_load(load, 6, kLoads);
         weigh(w);

@@ -55,11 +55,15 @@ def attention_bound(out, size, reach, dtype, keys: int, scale):
     ``keys`` terms in fp32; a score of 576 products in fp32 is off by at most
     578 * 2^-24 of |q| . |k|, which moves p (and its normaliser) by that factor
     each, and the exponential by 2^-22 of itself and 2^-23 of its argument.
+    A page's scale enters p through its logarithm, which for other scales than
+    powers of two is off by half a step of at most 126 (2^-18) and the
+    logarithm's own 2^-21: below 2^-17.8, times ln 2, 2^-18 of p, and of the
+    normaliser as much.
     Below fp16's normal range a P is off by 2^-25 next to a largest one of at
     least 1 in units of its page's scale: 2^-25 * 448 of the largest scale a
     key, twice that for a scale's fraction."""
     score = reach * (578 * 2.0 ** -24 + 2.0 ** -22)
-    per = 2.0 ** -11 + keys * 2.0 ** -23 + 2 * score + 2.0 ** -21
+    per = 2.0 ** -11 + keys * 2.0 ** -23 + 2 * score + 2.0 ** -21 + 2.0 ** -17
     tail = keys * 2.0 ** -25 * 896 * float(scale.max())
     return out.abs() * HALF_STEP[dtype] + size * per[..., None] + tail
 
@@ -68,8 +72,10 @@ def weights_bound(added, total, reach, keys: int, terms: int):
     """How far a token's accumulated weight may be from the 64-bit one: every p
     by its score's factor (its own and its normaliser's), the exponential and
     the logarithm; the normaliser's sum of ``keys`` and the sum of ``terms``
-    (rows times heads) round in fp32, and the addition to the record."""
-    off = float(reach.max()) * (2 * 578 * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -20 + keys * 2.0 ** -23 + terms * 2.0 ** -24
+    (rows times heads) round in fp32, and the addition to the record.  The
+    normaliser holds the logarithm of the pages' scales (2^-18, see above)."""
+    off = float(reach.max()) * (2 * 578 * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -20 + keys * 2.0 ** -23 + terms * 2.0 ** -24 \
+        + 2.0 ** -18
     return added.abs() * off + total.abs() * 2.0 ** -23
 
 
