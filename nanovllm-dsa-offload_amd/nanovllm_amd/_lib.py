@@ -185,8 +185,9 @@ def pack(*tensors: torch.Tensor | None):
         n = len(shape)
         if n > 4:
             n, shape = 5, shape[:4]
+        device = t.get_device()  # (-1: a host tensor's)
         values += (t.data_ptr(), _DTYPE_CODES.get(t.dtype, -1), n, *shape, *_FILL[n], t.is_contiguous(),
-                   t.get_device() if t.is_cuda else _host_device(t))
+                   device if device >= 0 else _host_device(t))
     packer, buffer_type = _PACKERS[len(tensors)]
     buf = buffer_type()
     packer.pack_into(buf, 0, *values)

@@ -248,6 +248,81 @@ def test_attention_long():
     _check_attention(c, qr, q, ends, weights=True, seed=3)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_scales_of_any_size(dtype):
+    """Scales that are no powers of two, in dense order and in a list's."""
+    c = make_cache([1500, 200], 1, seed=17)
+    c["scale"] *= 1 + torch.rand(c["scale"].shape, generator=torch.Generator().manual_seed(17))
+    qr, q, ends = queries([2, 1], 24, DTYPES[dtype], 17)
+    print(f"ATTENTION scales {dtype}", flush=True)
+    _check_attention(c, qr, q, ends, weights=True, seed=5)
+    topk = torch.randint(0, 200, (3, 333), generator=torch.Generator().manual_seed(18), dtype=torch.int32)
+    _check_attention(c, qr, q, ends, topk=topk)
+
+
+@pytest.mark.parametrize("heads,step", [(64, 40.0), (64, 12.0), (20, 300.0)])
+def test_attention_scores_that_grow(heads, step):
+    """Scores that grow from tile to tile by `step` for some rows, fall for
+    others and stay for the rest: references follow late and in either group."""
+    c = make_cache([832], 1, seed=19)
+    sign = torch.where(torch.rand(576, generator=torch.Generator().manual_seed(19)) < 0.5, -1.0, 1.0)
+    for page in range(7):
+        tile = torch.arange(page * PAGE, (page + 1) * PAGE) // 64
+        codes = torch.where(sign > 0, 1.0, -1.0) * (tile.float() * 8 + 1)[:, None]
+        c["cache"][int(c["table"][0, page]), :, 0] = codes.to(torch.float8_e4m3fn)
+    c["scale"].fill_(2.0 ** -6)
+    # 576 * 8 codes a tile at that scale and factor: q of `size` moves a score by `step` a tile.
+    size = step / (576 * 8 * 2.0 ** -6 * SCALE)
+    way = torch.tensor([1.0, -1.0, 0.0])[torch.arange(heads) % 3]
+    both = (sign * size)[None, None] * way[None, :, None]
+    q, qr = both[..., :512].contiguous().bfloat16(), both[..., 512:].contiguous().bfloat16()
+    print(f"ATTENTION growing N={heads} step={step}", flush=True)
+    _check_attention(c, qr, q, i32([1]), weights=True, seed=6)
+    topk = torch.arange(832, dtype=torch.int32)[None].contiguous()
+    _check_attention(c, qr, q, i32([1]), topk=topk)
+
+
+def test_attention_many_long_requests():
+    """22 requests of 806,000 tokens each in three pages: more tiles a part than
+    pages are resolved at a time, more slices than sums are held.  Equal scores
+    and small whole values: p is 1, and every sum is exact in fp32 (below 2^24)
+    up to the division and the store."""
+    cols, length, batch, heads = 6300, 806_000, 22, 64
+    g = torch.Generator().manual_seed(20)
+    cache = torch.randint(0, 4, (3, PAGE, 1, 576), generator=g).float()
+    cache[0, ..., 170:], cache[1, ..., :170], cache[1, ..., 340:], cache[2, ..., :340] = 0, 0, 0, 0
+    row = torch.randint(0, 3, (cols,), generator=g, dtype=torch.int32)
+    seen = torch.zeros(3, PAGE, dtype=torch.float64)
+    for page in range(3):
+        at = (row == page).nonzero().flatten() * PAGE
+        seen[page] = ((at[:, None] + torch.arange(PAGE)) < length).sum(0)
+    want = torch.einsum("pk,pkd->d", seen, cache[:, :, 0, :512].double()) / length
+    zero = torch.zeros(batch, heads, 576, dtype=torch.float16)
+    c = {"cache": cache.to(torch.float8_e4m3fn), "scale": torch.ones(3, 1), "table": row.expand(batch, cols).contiguous(),
+         "lengths": i32([length] * batch)}
+    weights = torch.zeros(batch, cols * PAGE)
+    print("ATTENTION many long", flush=True)
+    out, after = _run_attention(c, zero[..., :64].contiguous(), zero[..., :512].contiguous(),
+                                torch.arange(1, batch + 1, dtype=torch.int32), entries=torch.arange(batch, dtype=torch.int32),
+                                weights=weights)
+    # fp16's half step, and 2^-22 for 1 / l and the product with it.
+    assert ((out.double() - want).abs() <= want * (2.0 ** -11 + 2.0 ** -22)).all()
+    # p = 2^-lse with lse = log2(806,000) < 32: 2^-20 and the logarithm's and the
+    # exponential's 2^-21 each, times ln 2 and once more for the sum of 64.
+    assert ((after[:, :length].double() * length / heads - 1).abs() <= 2.0 ** -19).all()
+    assert (after[:, length:] == 0).all()
+
+
+def test_attention_list_of_many_windows():
+    """Parts of a list that are longer than the entries resolved at a time."""
+    lengths = [700 - 3 * i for i in range(60)]
+    c = make_cache(lengths, 1, seed=21)
+    qr, q, ends = queries([1] * 60, 3, torch.bfloat16, 21)
+    topk = torch.randint(-1, 720, (60, 8200), generator=torch.Generator().manual_seed(21), dtype=torch.int32)
+    print("LIST many windows", flush=True)
+    _check_attention(c, qr, q, ends, topk=topk)
+
+
 def test_attention_nan_in_unseen_places():
     """NaN codes behind the last token, and in tokens that only later rows
     see, leave the rows that do not see them alone; rows that see one are NaN."""
