@@ -1369,7 +1369,7 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
 // Selection: one workgroup per request finds the K-th largest key by three
 // digit counts, then lists holes and sources in slot order.  Bound by the
 // passes, of which there are seven: with the keys in registers (32,768 slots)
-// 1 x 2,176 slots take 12 us, 48 x 8,320 20 us and 16 x 32,768 36 us, against
+// 1 x 2,176 slots take 11 us, 48 x 8,320 20 us and 16 x 32,768 34 us, against
 // 13, 32 and 97 with every pass reading them anew.  About 9 us of it are the
 // barriers and scans of the digits.
 constexpr int kEvictThreads = 1024;
@@ -1517,22 +1517,26 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
   int equal_before = 0;
   for (int w = 0; w < wave; ++w) equal_before += l.wave_a[w];
   __syncthreads();
+  // each(first slot, its holes, its sources) of every round, as lane masks.
   auto walk = [&](auto each) {
     int eq = equal_before;
     rounds([&](int r0, uint32_t k) {
-      const int s = r0 + lane;
-      const bool tie = k == threshold;
-      const uint64_t ties = __ballot(tie);
-      const int rank = eq + before_lane(ties);
-      eq += __popcll(ties);
-      const bool kept = k > threshold || (tie && rank < want);
-      each(r0, s, k != 0 && !kept && s < keep, kept && s >= keep);
+      const uint64_t owned = __ballot(k != 0), ties = __ballot(k == threshold);
+      uint64_t kept = __ballot(k > threshold);
+      if (ties != 0) {
+        const int room = want - eq, n = __popcll(ties);
+        kept |= room >= n ? ties : __ballot(k == threshold && before_lane(ties) < room);
+        eq += n;
+      }
+      const int under = keep - r0;  // slots of the round below the budget
+      const uint64_t below = under >= 64 ? ~0ull : (under > 0 ? (1ull << under) - 1 : 0ull);
+      each(r0, owned & below & ~kept, kept & ~below);
     });
   };
   int holes = 0, sources = 0;
-  walk([&](int, int, bool hole, bool source) {
-    holes += __popcll(__ballot(hole));
-    sources += __popcll(__ballot(source));
+  walk([&](int, uint64_t hole, uint64_t source) {
+    holes += __popcll(hole);
+    sources += __popcll(source);
   });
   if (lane == 0) {
     l.wave_a[wave] = holes;
@@ -1550,13 +1554,13 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
   int32_t* hole_start = a.hole_start + b * (a.cols + 1);
   int32_t* dst = a.move_dst + b * cap;
   int32_t* src = a.move_src + b * cap;
-  walk([&](int r0, int s, bool hole, bool source) {
+  const uint64_t me = 1ull << lane;
+  walk([&](int r0, uint64_t hole, uint64_t source) {
     if ((r0 & (kBlock - 1)) == 0 && r0 < s1 && lane == 0) hole_start[r0 >> kBlockShift] = hole_at;
-    const uint64_t hs = __ballot(hole), ss = __ballot(source);
-    if (hole) dst[hole_at + before_lane(hs)] = s;
-    if (source) src[source_at + before_lane(ss)] = s;
-    hole_at += __popcll(hs);
-    source_at += __popcll(ss);
+    if (hole & me) dst[hole_at + before_lane(hole)] = r0 + lane;
+    if (source & me) src[source_at + before_lane(source)] = r0 + lane;
+    hole_at += __popcll(hole);
+    source_at += __popcll(source);
   });
   if (tid == 0) {
     a.move_counts[b] = count;
