@@ -255,6 +255,8 @@ struct Plan {
   int split;      // > 0: every item (of `tiles` units) in so many parts
   int tiles;
 };
+constexpr int64_t kMostItems = int64_t{1} << 24;  // with tiles below 2^15 an item: see divide
+
 // x / y for 0 <= x < 2^53, y > 0 (a 64-bit division is a microsecond of
 // instructions; units stay below 2^40, their product with a part below 2^48).
 __device__ inline int64_t divide(int64_t x, int64_t y) {
@@ -266,7 +268,7 @@ __device__ inline int64_t divide(int64_t x, int64_t y) {
 __device__ inline int64_t part_start(const Plan& p, int64_t w) {
   if (p.split > 0) {
     const int item = static_cast<int>(w) / p.split, piece = static_cast<int>(w) - item * p.split;
-    return static_cast<int64_t>(item) * p.tiles + static_cast<int64_t>(p.tiles) * piece / p.split;
+    return static_cast<int64_t>(item) * p.tiles + divide(static_cast<int64_t>(p.tiles) * piece, p.split);
   }
   return divide(p.total * w, p.parts);
 }
@@ -331,23 +333,31 @@ __device__ inline Request request_of(const Latent8Args& a, int64_t b) {
   return make_request(a, lo, static_cast<int>(hi - lo), static_cast<int>(len < 0 ? 0 : (len > cap ? cap : len)));
 }
 
-// Exclusive prefix of a 64-bit count over the workgroup's threads.
+// Work of a request, or of several.
+struct Units {
+  int64_t items;
+  int64_t tiles;
+};
+// Exclusive prefix over the workgroup's threads.
 template <int THREADS>
-__device__ inline int64_t scan64(int64_t v, int64_t* scratch, int64_t* total) {
+__device__ inline Units scan_units(const Units& v, Units* scratch, Units* total) {
   const int wid = threadIdx.x >> 6;
-  const int64_t x = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(v)));
+  const Units x{static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(v.items))),
+                static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(v.tiles)))};
   if ((threadIdx.x & 63) == 63) scratch[wid] = x;
   __syncthreads();
-  int64_t before = 0, tot = 0;
+  Units before{0, 0}, all{0, 0};
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) {
-    const int64_t t = scratch[w];
-    before += w < wid ? t : 0;
-    tot += t;
+    const Units t = scratch[w];
+    before.items += w < wid ? t.items : 0;
+    before.tiles += w < wid ? t.tiles : 0;
+    all.items += t.items;
+    all.tiles += t.tiles;
   }
-  *total = tot;
+  *total = all;
   __syncthreads();
-  return before + x - v;
+  return {before.items + x.items - v.items, before.tiles + x.tiles - v.tiles};
 }
 
 // A value that every lane holds, in scalar registers.
@@ -364,59 +374,59 @@ struct Start {
   int64_t base;  // first unit of the request
   Request r;
 };
-// UNITS(request): {items, units of an item}; BEGINS: see make_plan.
-struct Units {
-  int64_t items;
-  int64_t tiles;
-};
+// UNITS(request): its items and all their tiles; BEGINS: see make_plan.
 template <int THREADS, bool BEGINS, typename UNITS>
 __device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t parts, int64_t least, int tiles,
                                    UNITS units) {
-  __shared__ int64_t scratch[THREADS / 64];
+  __shared__ Units scratch[THREADS / 64];
   __shared__ int64_t found[5];
   Start s;
   const int tid = threadIdx.x;
-  // Items (below 2^24 + 2^16) and tiles (below 2^39) in one scan.
-  constexpr int kItems = 39;
-  constexpr int64_t kTiles = (int64_t{1} << kItems) - 1;
-  auto both = [](const Units& u) { return (u.items << kItems) + u.items * u.tiles; };
   Request r{};
-  int64_t first = 0, sum = 0;
+  Units mine{0, 0}, sum{0, 0};
   if (tid < a.batch) {
     r = request_of(a, tid);
-    first = both(units(r));
+    sum = mine = units(r);
   }
-  for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum += both(units(request_of(a, b)));
-  int64_t total;
+  for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) {
+    const Units u = units(request_of(a, b));
+    sum.items += u.items;
+    sum.tiles += u.tiles;
+  }
+  Units total;
   if (tid == 0) found[0] = -1;
-  int64_t at = scan64<THREADS>(first + sum, scratch, &total);
-  total = uniform64(total);
-  s.plan = make_plan(total >> kItems, total & kTiles, parts, least, BEGINS, tiles);
-  if (part < s.plan.parts && total > 0) {
+  Units at = scan_units<THREADS>(sum, scratch, &total);
+  total = {uniform64(total.items), uniform64(total.tiles)};
+  s.plan = make_plan(total.items, total.tiles, parts, least, BEGINS, tiles);
+  // (More items than the rows can have: requests whose ends decrease share
+  // rows.  Nothing is done.)
+  if (total.items > kMostItems) s.plan.parts = 0;
+  if (part < s.plan.parts && total.tiles > 0) {
     const int64_t u = part_start(s.plan, part);
-    int64_t before = 0;
+    auto place = [&](const Units& x) { return x.tiles + x.items * s.plan.begin; };
+    Units before{0, 0};
     for (int64_t b0 = 0; b0 < a.batch; b0 += THREADS) {
       const int64_t b = b0 + tid;
       if (a.batch > THREADS) {  // (the first scan was over strided sums)
         r = Request{};
-        first = 0;
+        mine = {0, 0};
         if (b < a.batch) {
           r = request_of(a, b);
-          first = both(units(r));
+          mine = units(r);
         }
-        int64_t chunk;
-        at = before + scan64<THREADS>(first, scratch, &chunk);
-        before += chunk;
+        Units chunk;
+        at = scan_units<THREADS>(mine, scratch, &chunk);
+        at = {at.items + before.items, at.tiles + before.tiles};
+        before = {before.items + chunk.items, before.tiles + chunk.tiles};
       }
-      auto place = [&](int64_t x) { return (x & kTiles) + (x >> kItems) * s.plan.begin; };
-      if (u >= place(at) && u < place(at + first)) {
+      if (u >= place(at) && u < place({at.items + mine.items, at.tiles + mine.tiles})) {
         found[0] = b;
         found[1] = place(at);
         found[2] = r.row0;
         found[3] = r.n;
         found[4] = r.len;
       }
-      if (u < place(before)) break;
+      if (a.batch > THREADS && u < place(before)) break;
     }
   }
   __syncthreads();
@@ -585,7 +595,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const Start start =
       find_start<kAttnThreads, true>(a, part, a.parts, kMinUnits,
                                      LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
-                                     [](const Request& r) { return Units{r.items, r.tiles}; });
+                                     [](const Request& r) { return Units{r.items, r.items * r.tiles}; });
   const Work work = carve_work(a.workspace, a.parts);
   if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
   if (part >= start.plan.parts || start.b < 0) return;

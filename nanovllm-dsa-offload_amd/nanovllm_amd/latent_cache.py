@@ -34,7 +34,8 @@ token_weights         [pool rows, C * 128]        float32, likewise
 ====================  ==========================  =======================================
 
 Two requests of one call must not share a page or a pool row that the call
-writes.  Packed rows behind the last request are neither read nor written.
+writes, and the ends of packed rows must not decrease.  Packed rows behind the
+last request are neither read nor written.
 """
 
 from __future__ import annotations
