@@ -1067,7 +1067,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       const int64_t slot = 2 * part + (first_seg ? 0 : 1);
       float4* p = reinterpret_cast<float4*>(work.part) + slot * (kPartFloats / 4);
       const bool empty = t0 >= t1;
-      if (!empty && busy) {
+      if (!empty && m_mine < x.count) {
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -1132,6 +1132,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
   for (int k = 0; k < 8; ++k) most = fmaxf(most, row_part[k][m]);
   float l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool mine = grp * 32 + m < j.count;  // (m == lane & 31; the parts hold no other rows)
   const u32x4_t* parts = reinterpret_cast<const u32x4_t*>(work.part) + (blockIdx.x * 4 + e) * 64 + lane;
   for (int c0 = 0; c0 < n; c0 += kJoinParts) {
     const int c1 = c0 + kJoinParts < n ? c0 + kJoinParts : n;
@@ -1145,7 +1146,8 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
     __syncthreads();
 #pragma unroll 8
     for (int w = c0; w < c1; ++w) {
-      const u32x4_t v = parts[slot_of(w) * (kPartFloats / 4)];
+      u32x4_t v{0, 0, 0, 0};
+      if (mine) v = parts[slot_of(w) * (kPartFloats / 4)];
       const float f = factor[w - c0][lane & 31];
       // (A part without tiles wrote no sums: its factor is zero, its memory anything.)
 #pragma unroll
@@ -1157,7 +1159,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
   l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) l += row_part[k][m];
-  if (grp * 32 + m >= j.count) return;  // (m == lane & 31)
+  if (!mine) return;
   const int f = j.first + grp * 32 + m, i = f / per, h = f - i * per;
   const int64_t row = (j.row0 + i) * a.heads + j.g * per + h;
   if (a.token_weights != nullptr && wg == 0 && dt == 0 && s == 0) work.lse[row] = most + __builtin_amdgcn_logf(l);
