@@ -252,8 +252,7 @@ struct Plan {
   int64_t total;  // units
   int64_t parts;  // workgroups that share them
   int begin;      // units of an item before its first tile
-  int split;      // > 0: every item (of `tiles` units) in so many parts
-  int tiles;
+  int share;      // > 0: a part is a unit, up to so many tiles of one item
 };
 constexpr int64_t kMostItems = int64_t{1} << 24;  // with tiles below 2^15 an item: see divide
 
@@ -265,44 +264,44 @@ __device__ inline int64_t divide(int64_t x, int64_t y) {
   q += rest < 0 ? -1 : (rest >= y ? 1 : 0);
   return q;
 }
-__device__ inline int64_t part_start(const Plan& p, int64_t w) {
-  if (p.split > 0) {
-    const int item = static_cast<int>(w) / p.split, piece = static_cast<int>(w) - item * p.split;
-    return static_cast<int64_t>(item) * p.tiles + divide(static_cast<int64_t>(p.tiles) * piece, p.split);
-  }
-  return divide(p.total * w, p.parts);
-}
+__device__ inline int64_t part_start(const Plan& p, int64_t w) { return p.share > 0 ? w : divide(p.total * w, p.parts); }
 // The part of an item's last unit.
 __device__ inline int64_t part_of_end(const Plan& p, int64_t end) {
-  if (p.split > 0) return divide(end, p.tiles) * p.split - 1;
-  return divide(end * p.parts + p.total - 1, p.total) - 1;
+  return p.share > 0 ? end - 1 : divide(end * p.parts + p.total - 1, p.total) - 1;
+}
+// Units of an item of so many tiles, and the tile at which unit u of it begins.
+__device__ inline int units_of(const Plan& p, int tiles) {
+  return p.share > 0 ? (tiles + p.share - 1) / p.share : tiles + p.begin;
+}
+__device__ inline int tile_of(const Plan& p, int tiles, int u) {
+  if (p.share > 0) return tiles * u / units_of(p, tiles);
+  return u > p.begin ? u - p.begin : 0;
 }
 
 // Equal parts of the units.  A part that lies across two items begins anew,
 // which costs kBegin tiles' time, so an item counts that much more than its
 // tiles (at most an eighth of a part more: a part that lies in the first units
-// only has nothing to do).  Where all items have the same number of tiles and
-// there are few of them, equal parts of every item may be faster: 24 lists of
-// 2,048, 48 items of 32 tiles, take 31 us in 5 parts of 7 tiles an item, and 37
-// in 256 parts of 6.
+// only has nothing to do).  What the eighth leaves out costs a part that many
+// tiles; where shares of single items, of up to total / (parts - items) tiles,
+// are shorter than that, they are the parts (`tiles`: what every item has, or
+// 0).  48 lists' items of 32 tiles take 31 us in 5 shares of 7 tiles each and 37
+// in 256 parts of 6; 24 items of about 129 tiles 46 in shares of 14 and 50 in
+// 256 parts of 12; 24 of 512 stay in 256 parts of 48.
 __device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, int64_t least, bool begins, int tiles) {
-  Plan p{tiles_all, divide(tiles_all, least), 0, 0, tiles};
+  Plan p{tiles_all, divide(tiles_all, least), 0, 0};
   if (p.parts > parts) p.parts = parts;
   if (p.parts < 1) p.parts = 1;
-  if (tiles > 0 && items > 0) {
-    int64_t split = divide(parts, items);
-    if (split * least > tiles) split = divide(tiles, least) > 0 ? divide(tiles, least) : 1;
-    if (split > 0 && (tiles - kBegin * split) * p.parts <= tiles_all * split) {
-      p.split = static_cast<int>(split);
-      p.parts = items * split;
-      return p;
+  if (!begins || items <= 0) return p;
+  const int64_t eighth = divide(tiles_all, 8 * p.parts);
+  p.begin = eighth < kBegin ? static_cast<int>(eighth) : kBegin;
+  if (items > 1 && items < parts) {
+    int64_t share = tiles > 0 ? divide(tiles - 1, divide(parts, items)) + 1 : divide(tiles_all - 1, parts - items) + 1;
+    if ((share + p.begin - kBegin) * p.parts < tiles_all + items * p.begin) {
+      p.share = static_cast<int>(share);
+      return p;  // (total and parts: counted over the requests next)
     }
   }
-  if (begins) {
-    const int64_t eighth = divide(tiles_all, 8 * p.parts);
-    p.begin = eighth < kBegin ? static_cast<int>(eighth) : kBegin;
-    p.total += items * p.begin;
-  }
+  p.total += items * p.begin;
   return p;
 }
 
@@ -401,18 +400,35 @@ __device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t p
   // (More items than the rows can have: requests whose ends decrease share
   // rows.  Nothing is done.)
   if (total.items > kMostItems) s.plan.parts = 0;
+  // Shares: parts are counted in the place of tiles; where all items have as
+  // many, the items say it.
+  const bool shares = BEGINS && s.plan.share > 0, alike = shares && tiles > 0;
+  auto counted = [&](const Request& q) -> Units {
+    if (shares && !alike) return {0, q.items * units_of(s.plan, q.tiles)};
+    return units(q);
+  };
+  if (alike) {
+    s.plan.total = s.plan.parts = total.items * units_of(s.plan, tiles);
+  } else if (shares) {
+    if (tid < a.batch) sum = mine = counted(r);
+    for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum.tiles += counted(request_of(a, b)).tiles;
+    at = scan_units<THREADS>(sum, scratch, &total);
+    s.plan.total = s.plan.parts = uniform64(total.tiles);
+  }
   if (part < s.plan.parts && total.tiles > 0) {
     const int64_t u = part_start(s.plan, part);
-    auto place = [&](const Units& x) { return x.tiles + x.items * s.plan.begin; };
+    auto place = [&](const Units& x) {
+      return alike ? x.items * units_of(s.plan, tiles) : x.tiles + x.items * s.plan.begin;
+    };
     Units before{0, 0};
     for (int64_t b0 = 0; b0 < a.batch; b0 += THREADS) {
       const int64_t b = b0 + tid;
-      if (a.batch > THREADS) {  // (the first scan was over strided sums)
+      if (a.batch > THREADS) {  // (the first scans were over strided sums)
         r = Request{};
         mine = {0, 0};
         if (b < a.batch) {
           r = request_of(a, b);
-          mine = units(r);
+          mine = counted(r);
         }
         Units chunk;
         at = scan_units<THREADS>(mine, scratch, &chunk);
@@ -643,24 +659,24 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 
   while (at < stop) {
     // The next segment: units [u0, u1) of one item.
-    const int begin = start.plan.begin;
-    while (at >= base + r.items * (r.tiles + begin)) {
-      base += r.items * (r.tiles + begin);
+    int units = units_of(start.plan, r.tiles);
+    while (at >= base + r.items * units) {
+      base += r.items * units;
       ++b;
       r = request_of(a, b);
+      units = units_of(start.plan, r.tiles);
     }
-    const int64_t it = divide(at - base, r.tiles + begin);
-    const int64_t item_start = base + it * (r.tiles + begin);
-    const int64_t item_end = item_start + r.tiles + begin;
+    const int64_t it = divide(at - base, units);
+    const int64_t item_start = base + it * units;
+    const int64_t item_end = item_start + units;
     const int64_t seg_end = item_end < stop ? item_end : stop;
     const Item x = item_of(a, r, it);
     const int i_last = LIST ? x.lead : (x.first + x.count - 1) / per;
     const int i_first = LIST ? x.lead : x.first / per;
     const int vis_most = visible(r, i_last), vis_least = visible(r, i_first);
     const int list_len = LIST ? static_cast<int>(a.list_len) : vis_most;
-    int t0 = static_cast<int>(at - item_start) - begin, t1 = static_cast<int>(seg_end - item_start) - begin;
-    if (t0 < 0) t0 = 0;
-    if (t1 < 0) t1 = 0;
+    int t0 = tile_of(start.plan, r.tiles, static_cast<int>(at - item_start));
+    int t1 = tile_of(start.plan, r.tiles, static_cast<int>(seg_end - item_start));
     const int tiles_seen = (list_len + kKeys - 1) / kKeys;
     if (t1 > tiles_seen) t1 = tiles_seen;
     if (t0 > t1) t0 = t1;

@@ -240,6 +240,22 @@ def test_attention_many_requests():
     _check_attention(c, qr, q, ends, weights=True, seed=2)
 
 
+@pytest.mark.parametrize("topk", [False, True])
+def test_attention_many_requests_few_rows(topk):
+    """More requests than a workgroup has threads, most of them without rows:
+    the few items are split one by one."""
+    lengths = [(i * 61) % 700 + 40 for i in range(620)]
+    rows = [i % 31 == 3 for i in range(620)]
+    lengths = [n if r else 5 for n, r in zip(lengths, rows)]
+    c = make_cache(lengths, 1, seed=27)
+    qr, q, ends = queries([int(r) for r in rows], 20, torch.bfloat16, 27)
+    lists = None
+    if topk:
+        lists = torch.randint(-1, 60, (q.shape[0], 700), generator=torch.Generator().manual_seed(27), dtype=torch.int32)
+    print(f"ATTENTION few rows topk={topk}", flush=True)
+    _check_attention(c, qr, q, ends, topk=lists, weights=not topk, seed=7)
+
+
 def test_attention_long():
     """One request across every part of the launch, window changes among them."""
     c = make_cache([70001, 40], 1, seed=8)
