@@ -324,13 +324,20 @@ __device__ inline Request make_request(const Latent8Args& a, int64_t row0, int n
   if (r.tiles < 1) r.tiles = 1;
   return r;
 }
-__device__ inline Request request_of(const Latent8Args& a, int64_t b) {
-  int64_t lo = b > 0 ? a.seq_q[b - 1] : 0, hi = a.seq_q[b];
+struct Ends {  // as they lie in memory
+  int32_t lo, hi, len;
+};
+__device__ inline Ends ends_of(const Latent8Args& a, int64_t b) {
+  return {a.seq_q[b > 0 ? b - 1 : 0], a.seq_q[b], a.seq_kv[b]};
+}
+__device__ inline Request request_of(const Latent8Args& a, int64_t b, const Ends& e) {
+  int64_t lo = b > 0 ? e.lo : 0, hi = e.hi;
   lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
   hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
-  const int64_t cap = a.cols * kBlock, len = a.seq_kv[b];
+  const int64_t cap = a.cols * kBlock, len = e.len;
   return make_request(a, lo, static_cast<int>(hi - lo), static_cast<int>(len < 0 ? 0 : (len > cap ? cap : len)));
 }
+__device__ inline Request request_of(const Latent8Args& a, int64_t b) { return request_of(a, b, ends_of(a, b)); }
 
 // Work of a request, or of several.
 struct Units {
@@ -373,10 +380,11 @@ struct Start {
   int64_t base;  // first unit of the request
   Request r;
 };
-// UNITS(request): its items and all their tiles; BEGINS: see make_plan.
+// UNITS(request): its items and all their tiles; BEGINS: see make_plan; `ends`:
+// of request threadIdx.x (of request 0 where there is none), on its way.
 template <int THREADS, bool BEGINS, typename UNITS>
-__device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t parts, int64_t least, int tiles,
-                                   UNITS units) {
+__device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64_t part, int64_t parts, int64_t least,
+                                   int tiles, UNITS units) {
   __shared__ Units scratch[THREADS / 64];
   __shared__ int64_t found[5];
   Start s;
@@ -384,7 +392,7 @@ __device__ inline Start find_start(const Latent8Args& a, int64_t part, int64_t p
   Request r{};
   Units mine{0, 0}, sum{0, 0};
   if (tid < a.batch) {
-    r = request_of(a, tid);
+    r = request_of(a, tid, ends);
     sum = mine = units(r);
   }
   for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) {
@@ -608,18 +616,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int hh = lane >> 5;
   const int grp = wave >> 2, kg = wave & 1, dh = (wave >> 1) & 1, wg = wave & 3;
   const int64_t part = blockIdx.x;
-  const Start start =
-      find_start<kAttnThreads, true>(a, part, a.parts, kMinUnits,
-                                     LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
-                                     [](const Request& r) { return Units{r.items, r.items * r.tiles}; });
-  const Work work = carve_work(a.workspace, a.parts);
-  if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
-  if (part >= start.plan.parts || start.b < 0) return;
-  const int64_t stop = part_start(start.plan, part + 1);
-  int64_t at = part_start(start.plan, part);
-  int64_t b = start.b;
-  int64_t base = start.base;
-  Request r = start.r;
+  const Ends ends = ends_of(a, tid < a.batch ? tid : 0);
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
 
@@ -656,6 +653,19 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int key_mine = kg * 32 + dh * 16 + 4 * hh;  // keys key_mine + 8 e + 0..3, e < 2, of a tile
   const int m_mine = grp * 32 + l32;
   uint16_t* const p_mine = p_tile[grp];
+
+  const Start start =
+      find_start<kAttnThreads, true>(a, ends, part, a.parts, kMinUnits,
+                                     LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
+                                     [](const Request& r) { return Units{r.items, r.items * r.tiles}; });
+  const Work work = carve_work(a.workspace, a.parts);
+  if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
+  if (part >= start.plan.parts || start.b < 0) return;
+  const int64_t stop = part_start(start.plan, part + 1);
+  int64_t at = part_start(start.plan, part);
+  int64_t b = start.b;
+  int64_t base = start.base;
+  Request r = start.r;
 
   while (at < stop) {
     // The next segment: units [u0, u1) of one item.
@@ -1219,7 +1229,7 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
   auto slices = [](const Request& r) -> int64_t { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
-  const Start start = find_start<kSumThreads, false>(a, blockIdx.x, kSumParts, kSumWaves, 0,
+  const Start start = find_start<kSumThreads, false>(a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, kSumWaves, 0,
                                                      [&](const Request& r) { return Units{1, slices(r)}; });
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
