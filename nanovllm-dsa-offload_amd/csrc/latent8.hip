@@ -1406,10 +1406,11 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
 // ------------------------------------------------------------------ eviction
 // Selection: one workgroup per request finds the K-th largest key by three
 // digit counts, then lists holes and sources in slot order.  Bound by the
-// passes, of which there are seven: with the keys in registers (32,768 slots)
-// 1 x 2,176 slots take 11 us, 48 x 8,320 20 us and 16 x 32,768 34 us, against
-// 13, 32 and 97 with every pass reading them anew.  About 9 us of it are the
-// barriers and scans of the digits.
+// passes: with the keys in registers (32,768 slots) and lanes that count for
+// themselves 1 x 2,176 slots take 10 us, 48 x 8,320 17 us and 16 x 32,768 29 us,
+// against 13, 32 and 97 with every pass reading them anew, and 10, 20 and 35
+// with lane masks in the one scalar unit of a CU.  About 6 us of it are the
+// digits' barriers and scans.
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kDigitBins = 2048;
@@ -1446,6 +1447,7 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
   const int seg = static_cast<int>(ceil_div(ceil_div(len, kEvictWaves), 64)) * 64;
   const int s0 = wave * seg, s1 = s0 + seg < len ? s0 + seg : len;
   auto at = [&](int s) { return s < s1 ? s : 0; };  // (slot 0 in the place of one behind the end)
+  for (int i = tid; i < kDigitBins; i += kEvictThreads) l.bins[i] = make_uint4(0, 0, 0, 0);
   int latest = INT32_MIN;
   // kHeld rounds of 64 keys stay in registers; what lies beyond is read anew
   // by every pass.
@@ -1517,21 +1519,22 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
   for (int round = 0; round < 3; ++round) {
     const int bits = round < 2 ? 11 : 10;
     shift -= bits;
-    for (int i = tid; i < kDigitBins; i += kEvictThreads) l.bins[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
     rounds([&](int, uint32_t k) {
       if (k != 0 && (round == 0 || (k >> (shift + bits)) == prefix))
         atomicAdd(reinterpret_cast<uint32_t*>(&l.bins[(k >> shift) & ((1u << bits) - 1)]) + (lane & 3), 1u);
     });
     __syncthreads();
-    // Thread t owns bins top - 2t and top - 2t - 1 (from the largest digit down).
+    // Thread t owns bins top - 2t and top - 2t - 1 (from the largest digit
+    // down), and leaves them empty for the next digit.
     const int top = (1 << bits) - 1;
     const int hi = top - 2 * tid, lo = hi - 1;
-    auto count = [&](int digit) -> int {
-      const uint4 v = l.bins[digit < 0 ? 0 : digit];
-      return digit < 0 ? 0 : static_cast<int>(v.x + v.y + v.z + v.w);
+    auto take = [&](int digit) -> int {
+      if (digit < 0) return 0;
+      const uint4 v = l.bins[digit];
+      l.bins[digit] = make_uint4(0, 0, 0, 0);
+      return static_cast<int>(v.x + v.y + v.z + v.w);
     };
-    const int c_hi = count(hi), c_lo = count(lo);
+    const int c_hi = take(hi), c_lo = take(lo);
     int total;
     const int before = block_exclusive_scan(c_hi + c_lo, l.scratch, &total);
     if (before < want && want <= before + c_hi) {
@@ -1544,38 +1547,52 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
     __syncthreads();
     prefix = (prefix << bits) | static_cast<uint32_t>(l.bin);
     want -= l.above;
-    __syncthreads();
   }
   const uint32_t threshold = prefix;  // `want` of the keys equal to it are kept, the lower slots first
 
-  int equal = 0;
-  rounds([&](int, uint32_t k) { equal += __popcll(__ballot(k == threshold)); });
+  // Larger keys and ties of the wave below the budget (low half) and above it,
+  // counted by lanes: one scalar unit serves all waves, and masks keep it busy.
+  uint32_t larger = 0, ties = 0;
+  rounds([&](int r0, uint32_t k) {
+    const uint32_t one = r0 + lane < keep ? 1u : 0x10000u;
+    larger += k > threshold ? one : 0u;
+    ties += k == threshold ? one : 0u;
+  });
+  auto over_wave = [](uint32_t v) { return static_cast<int>(__builtin_amdgcn_readlane(wave_inclusive_scan(v), 63)); };
+  const int larger_below = over_wave(larger & 0xffffu), larger_above = over_wave(larger >> 16);
+  const int ties_below = over_wave(ties & 0xffffu), ties_above = over_wave(ties >> 16);
+  const int equal = ties_below + ties_above;
   if (lane == 0) l.wave_a[wave] = equal;
   __syncthreads();
   int equal_before = 0;
   for (int w = 0; w < wave; ++w) equal_before += l.wave_a[w];
   __syncthreads();
-  // each(first slot, its holes, its sources) of every round, as lane masks.
-  auto walk = [&](auto each) {
-    int eq = equal_before;
+  const int room = want - equal_before;  // for the wave's ties
+  const bool partly = room > 0 && room < equal;
+  const int below_all = (s1 < keep ? s1 : keep) - s0;
+  int holes = (below_all > 0 ? below_all : 0) - larger_below, sources = larger_above;
+  if (room >= equal) {
+    holes -= ties_below;
+    sources += ties_above;
+  }
+  // A wave that keeps some of its ties (there is one at most): each(first slot,
+  // its holes, its sources) of every round, as lane masks.
+  auto walk_ties = [&](auto each) {
+    int left = room;
     rounds([&](int r0, uint32_t k) {
-      const uint64_t owned = __ballot(k != 0), ties = __ballot(k == threshold);
-      uint64_t kept = __ballot(k > threshold);
-      if (ties != 0) {
-        const int room = want - eq, n = __popcll(ties);
-        kept |= room >= n ? ties : __ballot(k == threshold && before_lane(ties) < room);
-        eq += n;
-      }
-      const int under = keep - r0;  // slots of the round below the budget
-      const uint64_t below = under >= 64 ? ~0ull : (under > 0 ? (1ull << under) - 1 : 0ull);
+      const uint64_t owned = __ballot(k != 0), same = __ballot(k == threshold), below = __ballot(r0 + lane < keep);
+      const uint64_t kept = __ballot(k > threshold || (k == threshold && before_lane(same) < left));
+      left -= __popcll(same);
       each(r0, owned & below & ~kept, kept & ~below);
     });
   };
-  int holes = 0, sources = 0;
-  walk([&](int, uint64_t hole, uint64_t source) {
-    holes += __popcll(hole);
-    sources += __popcll(source);
-  });
+  if (partly) {
+    holes = sources = 0;
+    walk_ties([&](int, uint64_t hole, uint64_t source) {
+      holes += __popcll(hole);
+      sources += __popcll(source);
+    });
+  }
   if (lane == 0) {
     l.wave_a[wave] = holes;
     l.wave_b[wave] = sources;
@@ -1592,14 +1609,29 @@ __device__ inline void select_slots(const Latent8EvictArgs& a, SelectLds& l, int
   int32_t* hole_start = a.hole_start + b * (a.cols + 1);
   int32_t* dst = a.move_dst + b * cap;
   int32_t* src = a.move_src + b * cap;
-  const uint64_t me = 1ull << lane;
-  walk([&](int r0, uint64_t hole, uint64_t source) {
+  auto page_start = [&](int r0) {
     if ((r0 & (kBlock - 1)) == 0 && r0 < s1 && lane == 0) hole_start[r0 >> kBlockShift] = hole_at;
-    if (hole & me) dst[hole_at + before_lane(hole)] = r0 + lane;
-    if (source & me) src[source_at + before_lane(source)] = r0 + lane;
-    hole_at += __popcll(hole);
-    source_at += __popcll(source);
-  });
+  };
+  auto list = [&](int32_t* to, int& at_slot, int r0, bool mine) {
+    const uint64_t all = __ballot(mine);
+    if (mine) to[at_slot + before_lane(all)] = r0 + lane;
+    at_slot += __popcll(all);
+  };
+  if (partly) {
+    const uint64_t me = 1ull << lane;
+    walk_ties([&](int r0, uint64_t hole, uint64_t source) {
+      page_start(r0);
+      list(dst, hole_at, r0, (hole & me) != 0);
+      list(src, source_at, r0, (source & me) != 0);
+    });
+  } else {
+    const uint32_t last_out = room >= equal ? threshold - 1 : threshold;  // the largest key that goes (0: no token's)
+    rounds([&](int r0, uint32_t k) {
+      page_start(r0);
+      if (r0 < keep) list(dst, hole_at, r0, k - 1u < last_out && r0 + lane < keep);
+      if (r0 + 64 > keep) list(src, source_at, r0, k > last_out && r0 + lane >= keep);
+    });
+  }
   if (tid == 0) {
     a.move_counts[b] = count;
     a.kept_lengths[b] = keep;
