@@ -517,6 +517,40 @@ def test_evict_keeps_lengths_in_place():
     assert d[0].tolist() == [200, 90]
 
 
+def test_registered_operators_are_the_same():
+    """By name, as a traced program calls them: the same outputs."""
+    c = make_cache([300, 140], 1, seed=28)
+    qr, q, ends = queries([1, 2], 8, torch.bfloat16, 28)
+    weights, positions, entries = _records(c, 9)
+    print("BY NAME", flush=True)
+    state = []
+    for by_name in (False, True):
+        ops = torch.ops.nanovllm_dsa
+        d = dict(zip(("qr", "q", "ends", "lens", "table", "cache", "scale", "entries", "pos", "w"),
+                     _gpu(qr, q, ends, c["lengths"], c["table"], c["cache"].clone(), c["scale"].clone(), entries,
+                          positions.clone(), weights.clone())))
+        out, kv = torch.zeros_like(d["q"]), d["q"][:, :1].contiguous()
+        rope = d["qr"][:, :1].contiguous()
+        lists = [torch.zeros(2, c["cols"] * PAGE, dtype=torch.int32, device="cuda") for _ in range(2)]
+        counts, kept = (torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2))
+        budgets = i32([200, 128]).cuda()
+        if by_name:
+            ops.latent8_append(kv, rope, d["ends"], d["lens"], d["table"], d["cache"], d["scale"])
+            ops.latent8_attention(d["qr"], d["q"], d["ends"], d["lens"], d["table"], d["cache"], d["scale"], SCALE, out,
+                                  None, d["entries"], d["w"])
+            ops.latent8_evict(d["lens"], budgets, d["table"], d["entries"], d["cache"], d["scale"], d["pos"], d["w"],
+                              *lists, counts, kept, 2, 9)
+        else:
+            _api().latent8_append(kv, rope, d["ends"], d["lens"], d["table"], d["cache"], d["scale"])
+            _api().latent8_attention(d["qr"], d["q"], d["ends"], d["lens"], d["table"], d["cache"], d["scale"], SCALE, out,
+                                     req_pool_entries=d["entries"], token_weights=d["w"])
+            _api().latent8_evict(d["lens"], budgets, d["table"], d["entries"], d["cache"], d["scale"], d["pos"], d["w"],
+                                 *lists, counts, kept, protect_first=2, protect_last=9)
+        state.append([out, d["cache"].view(torch.uint8), d["scale"], d["pos"], d["w"], *lists, counts, kept])
+    for mine, named in zip(*state):
+        assert torch.equal(mine, named)
+
+
 # ------------------------------------------------------- the three together
 def _chain(steps, dtype, latent_heads, heads, seed):
     """Prompts, then decode steps that append, attend with weights, and evict
