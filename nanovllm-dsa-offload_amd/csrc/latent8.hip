@@ -279,7 +279,7 @@ __device__ inline int tile_of(const Plan& p, int tiles, int u) {
 }
 
 // Equal parts of the units.  A part that lies across two items begins anew,
-// which costs kBegin tiles' time, so an item counts that much more than its
+// which costs the time of `cost` tiles, so an item counts that much more than its
 // tiles (at most an eighth of a part more: a part that lies in the first units
 // only has nothing to do).  What the eighth leaves out costs a part that many
 // tiles; where shares of single items, of up to total / (parts - items) tiles,
@@ -287,16 +287,16 @@ __device__ inline int tile_of(const Plan& p, int tiles, int u) {
 // 0).  48 lists' items of 32 tiles take 31 us in 5 shares of 7 tiles each and 37
 // in 256 parts of 6; 24 items of about 129 tiles 46 in shares of 14 and 50 in
 // 256 parts of 12; 24 of 512 stay in 256 parts of 48.
-__device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, int64_t least, bool begins, int tiles) {
+__device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, int64_t least, int cost, int tiles) {
   Plan p{tiles_all, divide(tiles_all, least), 0, 0};
   if (p.parts > parts) p.parts = parts;
   if (p.parts < 1) p.parts = 1;
-  if (!begins || items <= 0) return p;
+  if (items <= 0) return p;
   const int64_t eighth = divide(tiles_all, 8 * p.parts);
-  p.begin = eighth < kBegin ? static_cast<int>(eighth) : kBegin;
+  p.begin = eighth < cost ? static_cast<int>(eighth) : cost;
   if (items > 1 && items < parts) {
     int64_t share = tiles > 0 ? divide(tiles - 1, divide(parts, items)) + 1 : divide(tiles_all - 1, parts - items) + 1;
-    if ((share + p.begin - kBegin) * p.parts < tiles_all + items * p.begin) {
+    if ((share + p.begin - cost) * p.parts < tiles_all + items * p.begin) {
       p.share = static_cast<int>(share);
       return p;  // (total and parts: counted over the requests next)
     }
@@ -376,19 +376,23 @@ __device__ inline int64_t uniform64(int64_t x) {
 // Where a workgroup's part begins: the request, and its first unit.
 struct Start {
   Plan plan;
+  int64_t items;  // of all requests
   int64_t b;
-  int64_t base;  // first unit of the request
+  int64_t base;   // first unit of the request
+  int64_t item;   // its first item
   Request r;
 };
-// UNITS(request): its items and all their tiles; BEGINS: see make_plan; `ends`:
-// of request threadIdx.x (of request 0 where there is none), on its way.
-template <int THREADS, bool BEGINS, typename UNITS>
+// EACH(request): the tiles of each of its items, ITEMS(request): their number;
+// COST: see make_plan; `ends`: of request threadIdx.x (of request 0 where there
+// is none), on its way.
+template <int THREADS, int COST, typename ITEMS, typename EACH>
 __device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64_t part, int64_t parts, int64_t least,
-                                   int tiles, UNITS units) {
+                                   int tiles, ITEMS items, EACH each) {
   __shared__ Units scratch[THREADS / 64];
-  __shared__ int64_t found[5];
+  __shared__ int64_t found[6];
   Start s;
   const int tid = threadIdx.x;
+  auto units = [&](const Request& q) -> Units { return {items(q), items(q) * each(q)}; };
   Request r{};
   Units mine{0, 0}, sum{0, 0};
   if (tid < a.batch) {
@@ -404,29 +408,35 @@ __device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64
   if (tid == 0) found[0] = -1;
   Units at = scan_units<THREADS>(sum, scratch, &total);
   total = {uniform64(total.items), uniform64(total.tiles)};
-  s.plan = make_plan(total.items, total.tiles, parts, least, BEGINS, tiles);
+  s.plan = make_plan(total.items, total.tiles, parts, least, COST, tiles);
+  s.items = total.items;
   // (More items than the rows can have: requests whose ends decrease share
   // rows.  Nothing is done.)
   if (total.items > kMostItems) s.plan.parts = 0;
   // Shares: parts are counted in the place of tiles; where all items have as
   // many, the items say it.
-  const bool shares = BEGINS && s.plan.share > 0, alike = shares && tiles > 0;
+  const bool shares = s.plan.share > 0, alike = shares && tiles > 0;
   auto counted = [&](const Request& q) -> Units {
-    if (shares && !alike) return {0, q.items * units_of(s.plan, q.tiles)};
+    if (shares && !alike) return {items(q), items(q) * units_of(s.plan, each(q))};
     return units(q);
   };
   if (alike) {
     s.plan.total = s.plan.parts = total.items * units_of(s.plan, tiles);
   } else if (shares) {
     if (tid < a.batch) sum = mine = counted(r);
-    for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) sum.tiles += counted(request_of(a, b)).tiles;
+    for (int64_t b = tid + THREADS; b < a.batch; b += THREADS) {
+      const Units u = counted(request_of(a, b));
+      sum.items += u.items;
+      sum.tiles += u.tiles;
+    }
     at = scan_units<THREADS>(sum, scratch, &total);
     s.plan.total = s.plan.parts = uniform64(total.tiles);
   }
   if (part < s.plan.parts && total.tiles > 0) {
     const int64_t u = part_start(s.plan, part);
     auto place = [&](const Units& x) {
-      return alike ? x.items * units_of(s.plan, tiles) : x.tiles + x.items * s.plan.begin;
+      if (alike) return x.items * units_of(s.plan, tiles);
+      return shares ? x.tiles : x.tiles + x.items * s.plan.begin;
     };
     Units before{0, 0};
     for (int64_t b0 = 0; b0 < a.batch; b0 += THREADS) {
@@ -449,6 +459,7 @@ __device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64
         found[2] = r.row0;
         found[3] = r.n;
         found[4] = r.len;
+        found[5] = at.items;
       }
       if (a.batch > THREADS && u < place(before)) break;
     }
@@ -456,6 +467,7 @@ __device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64
   __syncthreads();
   s.b = uniform64(found[0]);
   s.base = uniform64(found[1]);
+  s.item = uniform64(found[5]);
   s.r = make_request(a, uniform64(found[2]), static_cast<int>(uniform64(found[3])), static_cast<int>(uniform64(found[4])));
   return s;
 }
@@ -507,7 +519,7 @@ struct JoinEntry {
 struct Work {
   float* part;      // [2 parts][64 * 512], in the accumulators' order
   float* ml;        // [2 parts][64][2]
-  JoinEntry* join;  // [parts], row0 < 0: nothing
+  JoinEntry* join;  // [parts], of an item each or named by a part; row0 < 0: nothing
   float* lse;       // [rows, heads], base 2 (with weights)
 };
 constexpr size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -654,17 +666,21 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int m_mine = grp * 32 + l32;
   uint16_t* const p_mine = p_tile[grp];
 
-  const Start start =
-      find_start<kAttnThreads, true>(a, ends, part, a.parts, kMinUnits,
-                                     LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
-                                     [](const Request& r) { return Units{r.items, r.items * r.tiles}; });
+  const Start start = find_start<kAttnThreads, kBegin>(
+      a, ends, part, a.parts, kMinUnits, LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
+      [](const Request& r) { return r.items; }, [](const Request& r) { return r.tiles; });
   const Work work = carve_work(a.workspace, a.parts);
-  if (tid == 0 && part < a.parts) work.join[part].row0 = -1;
-  if (part >= start.plan.parts || start.b < 0) return;
+  // Entries that no item writes below: all of the parts', or those behind the
+  // last item's.  (More items than entries: ends that decrease.)
+  const bool many = a.join_items && start.items > a.joins;
+  if (tid == 0)
+    for (int64_t k = a.join_items && !many ? start.items + part : part; k < a.joins; k += a.parts) work.join[k].row0 = -1;
+  if (many || part >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, part + 1);
   int64_t at = part_start(start.plan, part);
   int64_t b = start.b;
   int64_t base = start.base;
+  int64_t item_base = start.item;
   Request r = start.r;
 
   while (at < stop) {
@@ -672,6 +688,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     int units = units_of(start.plan, r.tiles);
     while (at >= base + r.items * units) {
       base += r.items * units;
+      item_base += r.items;
       ++b;
       r = request_of(a, b);
       units = units_of(start.plan, r.tiles);
@@ -1088,6 +1105,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         if (a.token_weights != nullptr && wg == 0 && hh == 0)
           work.lse[row] = m_run + __builtin_amdgcn_logf(l_all);
       }
+      if (a.join_items && tid == 0) work.join[item_base + it].row0 = -1;
     } else {
       const bool first_seg = at == part_start(start.plan, part);
       const int64_t slot = 2 * part + (first_seg ? 0 : 1);
@@ -1115,7 +1133,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         j.w0 = static_cast<int32_t>(part - 1);
         j.slot0 = static_cast<int32_t>(2 * (part - 1) + (part_start(start.plan, part - 1) == item_start ? 0 : 1));
         j.w1 = static_cast<int32_t>(part_of_end(start.plan, item_end));
-        work.join[part] = j;
+        work.join[a.join_items ? item_base + it : part] = j;
       }
     }
     at = seg_end;
@@ -1129,33 +1147,37 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 // a stride that can fall on few XCDs: y counts fastest, so that each item's
 // blocks lie on all of them (48 items over 256 parts, 34 MB: 10.7 us instead
 // of 30 with w fastest).
-constexpr int kJoinThreads = 256;
+// Four groups of waves take every fourth part each, and their sums meet in LDS.
+constexpr int kJoinGroups = 4;
+constexpr int kFewJoins = 16;
 constexpr int kJoinBlocks = 32;
-constexpr int kJoinParts = 32;  // parts whose factors are held at a time
-template <typename T>
-__global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args a) {
+constexpr int kJoinParts = 64;  // parts whose factors are held at a time
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args a) {
+  constexpr int kSlices = 8 * GROUPS;
   __shared__ float factor[kJoinParts][32];  // of a part and row
-  __shared__ float row_part[8][32];
+  __shared__ float row_part[kSlices][32];
+  __shared__ float4 sums[GROUPS > 1 ? GROUPS - 1 : 1][256];
   const Work work = carve_work(a.workspace, a.parts);
   const JoinEntry j = work.join[blockIdx.y];
   if (j.row0 < 0) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int e = tid >> 6;
+  const int e = (tid >> 6) & 3, group = tid >> 8;
   // The wave whose accumulators these are, and its tile of dims.
   const int grp = blockIdx.x >> 4, wg = (blockIdx.x >> 2) & 3, dt = blockIdx.x & 3;
   if (grp * 32 >= j.count) return;
   const int n = j.w1 - j.w0 + 1;
   const int per = a.per;
-  const int m = tid & 31, s = tid >> 5;  // thread (s, m): parts s, s + 8, ... of row m
+  const int m = tid & 31, s = tid >> 5;  // thread (s, m): parts s, s + kSlices, ... of row m
   auto slot_of = [&](int w) -> int64_t { return w == 0 ? j.slot0 : 2 * static_cast<int64_t>(j.w0 + w); };
   auto ml_of = [&](int w) { return reinterpret_cast<const float2*>(work.ml)[slot_of(w) * kRows + grp * 32 + m]; };
   float most = -INFINITY;
-  for (int w = s; w < n; w += 8) most = fmaxf(most, ml_of(w).x);
+  for (int w = s; w < n; w += kSlices) most = fmaxf(most, ml_of(w).x);
   row_part[s][m] = most;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k) most = fmaxf(most, row_part[k][m]);
+  for (int k = 0; k < kSlices; ++k) most = fmaxf(most, row_part[k][m]);
   float l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const bool mine = grp * 32 + m < j.count;  // (m == lane & 31; the parts hold no other rows)
@@ -1163,7 +1185,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
   for (int c0 = 0; c0 < n; c0 += kJoinParts) {
     const int c1 = c0 + kJoinParts < n ? c0 + kJoinParts : n;
     __syncthreads();
-    for (int w = c0 + s; w < c1; w += 8) {
+    for (int w = c0 + s; w < c1; w += kSlices) {
       const float2 v = ml_of(w);
       const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - most);
       factor[w - c0][m] = f;
@@ -1171,7 +1193,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
     }
     __syncthreads();
 #pragma unroll 8
-    for (int w = c0; w < c1; ++w) {
+    for (int w = c0 + group; w < c1; w += GROUPS) {
       u32x4_t v{0, 0, 0, 0};
       if (mine) v = parts[slot_of(w) * (kPartFloats / 4)];
       const float f = factor[w - c0][lane & 31];
@@ -1181,11 +1203,20 @@ __global__ __launch_bounds__(kJoinThreads) void latent8_join_kernel(Latent8Args 
     }
   }
   row_part[s][m] = l;
+  if (group > 0) sums[group - 1][tid & 255] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
+  if (group > 0 || !mine) return;
   l = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) l += row_part[k][m];
-  if (!mine) return;
+  for (int k = 0; k < kSlices; ++k) l += row_part[k][m];
+#pragma unroll
+  for (int k = 0; k < GROUPS - 1; ++k) {
+    const float4 v = sums[k][tid];
+    acc[0] += v.x;
+    acc[1] += v.y;
+    acc[2] += v.z;
+    acc[3] += v.w;
+  }
   const int f = j.first + grp * 32 + m, i = f / per, h = f - i * per;
   const int64_t row = (j.row0 + i) * a.heads + j.g * per + h;
   if (a.token_weights != nullptr && wg == 0 && dt == 0 && s == 0) work.lse[row] = most + __builtin_amdgcn_logf(l);
@@ -1212,6 +1243,7 @@ constexpr int kSumThreads = 512;
 constexpr int kSumWaves = kSumThreads / 64;
 constexpr int kSumPairs = 128;
 constexpr int kSumKeys = 32;   // keys of a slice
+constexpr int kSumBegin = 12;  // what the pairs of a request cost, in slices
 constexpr int kSumRun = 96;    // slices whose sums over the blocks of pairs are held at a time
 constexpr int kSumParts = 256; // one workgroup per CU (LDS)
 template <typename T>
@@ -1228,9 +1260,10 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const Work work = carve_work(a.workspace, a.parts);
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
-  auto slices = [](const Request& r) -> int64_t { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
-  const Start start = find_start<kSumThreads, false>(a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, kSumWaves, 0,
-                                                     [&](const Request& r) { return Units{1, slices(r)}; });
+  auto slices = [](const Request& r) -> int { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
+  const Start start = find_start<kSumThreads, kSumBegin>(
+      a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, 1, 0,
+      [&](const Request& r) -> int64_t { return slices(r) > 0; }, slices);
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
   int64_t b = start.b, base = start.base;
@@ -1250,152 +1283,156 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int key_mine = 8 * (e_mine >> 2) + 4 * hh + (e_mine & 3);
 
   for (int64_t at = part_start(start.plan, blockIdx.x); at < stop;) {
-    while (at >= base + slices(r)) {
-      base += slices(r);
+    int n_units = slices(r) > 0 ? units_of(start.plan, slices(r)) : 0;
+    while (at >= base + n_units) {
+      base += n_units;
       ++b;
       r = request_of(a, b);
+      n_units = slices(r) > 0 ? units_of(start.plan, slices(r)) : 0;
     }
-    const int64_t n_slices = slices(r);
-    const int s0 = static_cast<int>(at - base);
-    const int64_t end = base + n_slices < stop ? base + n_slices : stop;
-    const int s1 = static_cast<int>(end - base) < s0 + kSumRun ? static_cast<int>(end - base) : s0 + kSumRun;
-    at = base + s1;
+    const int64_t end = base + n_units < stop ? base + n_units : stop;
+    const int first_slice = tile_of(start.plan, slices(r), static_cast<int>(at - base));
+    const int stop_slice = tile_of(start.plan, slices(r), static_cast<int>(end - base));
+    at = end;
     const int64_t entry = a.entries[b];
     if (entry < 0 || entry >= a.pool_rows) continue;
     float* const record = a.token_weights + entry * a.cols * kBlock;
     const int32_t* const table = a.block_table + b * a.cols;
     auto block_of = [&](int slice) { return __builtin_amdgcn_readfirstlane(table[slice >> 2]); };
     const int pairs = r.n * per;
-    auto row_of = [&](int f, int g) -> int64_t {  // of pair f in query, out and lse
-      const int64_t row = r.row0 * a.heads + g * per + f;
-      return a.latent_heads == 1 ? row : row + (f / per) * (a.heads - per);
-    };
-    for (int g = 0; g < a.latent_heads; ++g) {
-      for (int f0 = 0; f0 < pairs; f0 += kSumPairs) {
-        const bool first = g == 0 && f0 == 0, last = g == a.latent_heads - 1 && f0 + kSumPairs >= pairs;
-        const int count = pairs - f0 < kSumPairs ? pairs - f0 : kSumPairs;
-        const int tiles = count <= 32 ? 1 : (count <= 64 ? 2 : 4);  // of 32 pairs
-        const int vis_most = visible(r, (f0 + count - 1) / per), vis_least = visible(r, f0 / per);
-        u32x4_t k[18];
-        // The codes of a slice: chunks 2 j + hh of the lane's key.
-        const uint32_t lane_at = static_cast<uint32_t>(l32 * row_bytes + hh * 16);
-        auto slice_at = [&](int slice) -> const uint8_t* {
-          const int32_t block = block_of(slice < s1 ? slice : s0);
-          const int64_t row =
-              static_cast<int64_t>(block < 0 || block >= a.blocks ? 0 : block) * kBlock + (slice & 3) * kSumKeys;
-          return static_cast<const uint8_t*>(a.latent_cache) + row * row_bytes + g * kRow;
-        };
-        __syncthreads();  // (the last block's pairs are done with)
-        // The pairs' rows, straight to LDS, 64 places a wave and load, and
-        // behind them the first slice's codes.
-        const uint8_t* const qn = static_cast<const uint8_t*>(a.query);
-        const uint8_t* const qr = static_cast<const uint8_t*>(a.query_rope);
+    for (int s0 = first_slice; s0 < stop_slice; s0 += kSumRun) {
+      const int s1 = stop_slice < s0 + kSumRun ? stop_slice : s0 + kSumRun;
+      auto row_of = [&](int f, int g) -> int64_t {  // of pair f in query, out and lse
+        const int64_t row = r.row0 * a.heads + g * per + f;
+        return a.latent_heads == 1 ? row : row + (f / per) * (a.heads - per);
+      };
+      for (int g = 0; g < a.latent_heads; ++g) {
+        for (int f0 = 0; f0 < pairs; f0 += kSumPairs) {
+          const bool first = g == 0 && f0 == 0, last = g == a.latent_heads - 1 && f0 + kSumPairs >= pairs;
+          const int count = pairs - f0 < kSumPairs ? pairs - f0 : kSumPairs;
+          const int tiles = count <= 32 ? 1 : (count <= 64 ? 2 : 4);  // of 32 pairs
+          const int vis_most = visible(r, (f0 + count - 1) / per), vis_least = visible(r, f0 / per);
+          u32x4_t k[18];
+          // The codes of a slice: chunks 2 j + hh of the lane's key.
+          const uint32_t lane_at = static_cast<uint32_t>(l32 * row_bytes + hh * 16);
+          auto slice_at = [&](int slice) -> const uint8_t* {
+            const int32_t block = block_of(slice < s1 ? slice : s0);
+            const int64_t row =
+                static_cast<int64_t>(block < 0 || block >= a.blocks ? 0 : block) * kBlock + (slice & 3) * kSumKeys;
+            return static_cast<const uint8_t*>(a.latent_cache) + row * row_bytes + g * kRow;
+          };
+          __syncthreads();  // (the last block's pairs are done with)
+          // The pairs' rows, straight to LDS, 64 places a wave and load, and
+          // behind them the first slice's codes.
+          const uint8_t* const qn = static_cast<const uint8_t*>(a.query);
+          const uint8_t* const qr = static_cast<const uint8_t*>(a.query_rope);
 #pragma unroll 1
-        for (int q0 = wave * 64; q0 < tiles * 32 * (kRow / 8); q0 += kSumThreads) {
-          const int q = q0 + lane;
-          const int m = q / (kRow / 8), c = (q - m * (kRow / 8)) ^ ((m >> 1) & 7);
-          const int64_t row = row_of(f0 + (m < count ? m : 0), g);
-          load_to_lds(c < kCkvDim / 8 ? qn + row * (kCkvDim * 2) + c * 16 : qr + row * (kKpeDim * 2) + c * 16 - kCkvDim * 2,
-                      q_lds + q0 * 16);
-        }
-        {
-          const uint8_t* p = slice_at(s0 + wave);
+          for (int q0 = wave * 64; q0 < tiles * 32 * (kRow / 8); q0 += kSumThreads) {
+            const int q = q0 + lane;
+            const int m = q / (kRow / 8), c = (q - m * (kRow / 8)) ^ ((m >> 1) & 7);
+            const int64_t row = row_of(f0 + (m < count ? m : 0), g);
+            load_to_lds(c < kCkvDim / 8 ? qn + row * (kCkvDim * 2) + c * 16 : qr + row * (kKpeDim * 2) + c * 16 - kCkvDim * 2,
+                        q_lds + q0 * 16);
+          }
+          {
+            const uint8_t* p = slice_at(s0 + wave);
 #pragma unroll
-          for (int j = 0; j < 18; ++j) k[j] = *reinterpret_cast<const u32x4_t*>(p + lane_at + 32 * j);
-        }
-        if (tid < kSumPairs) {
-          const int f = f0 + (tid < count ? tid : 0);
-          pair_vis[tid] = tid < count ? visible(r, f / per) : 0;
-          pair_lse[tid] = tid < count ? work.lse[row_of(f, g)] : INFINITY;
-        }
-        wait_loads<0>();
-        lds_barrier();
-        for (int slice = s0 + wave; slice < s1; slice += kSumWaves) {
-          const int32_t block = block_of(slice);
-          const bool known = block >= 0 && block < a.blocks;
-          const int slot = slice * kSumKeys + key_mine;
-          const bool mine = (l32 & 1) == 0;
-          float* const held = &sums[(slice - s0) * kSumKeys + key_mine];
-          const float before = !first ? *held : 0.f;
-          const float total = last && known && slot < r.len ? record[slot] : 0.f;
-          float sum[16];
+            for (int j = 0; j < 18; ++j) k[j] = *reinterpret_cast<const u32x4_t*>(p + lane_at + 32 * j);
+          }
+          if (tid < kSumPairs) {
+            const int f = f0 + (tid < count ? tid : 0);
+            pair_vis[tid] = tid < count ? visible(r, f / per) : 0;
+            pair_lse[tid] = tid < count ? work.lse[row_of(f, g)] : INFINITY;
+          }
+          wait_loads<0>();
+          lds_barrier();
+          for (int slice = s0 + wave; slice < s1; slice += kSumWaves) {
+            const int32_t block = block_of(slice);
+            const bool known = block >= 0 && block < a.blocks;
+            const int slot = slice * kSumKeys + key_mine;
+            const bool mine = (l32 & 1) == 0;
+            float* const held = &sums[(slice - s0) * kSumKeys + key_mine];
+            const float before = !first ? *held : 0.f;
+            const float total = last && known && slot < r.len ? record[slot] : 0.f;
+            float sum[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-          if (slice * kSumKeys < vis_most) {
-            const float c = known ? a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g] : 1.f;
-            const float score = a.scale * kLog2e * fminf(fmaxf(c, kMinScale), FLT_MAX);
-            const bool ragged = (slice + 1) * kSumKeys > vis_least;
-            const uint8_t* const next = slice_at(slice + kSumWaves);
-            // The scores of all tiles of pairs in 36 steps of 16 dims, each
-            // step's operands read a step ahead.
-            auto add_pairs = [&](auto tiles_n) {
-              constexpr int N = decltype(tiles_n)::value;
-              f32x16_t s[N];
-#pragma unroll
-              for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
-              u32x4_t q[2][N];
-              auto fetch = [&](int j) {
+            for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+            if (slice * kSumKeys < vis_most) {
+              const float c = known ? a.cache_scale[static_cast<int64_t>(block) * a.latent_heads + g] : 1.f;
+              const float score = a.scale * kLog2e * fminf(fmaxf(c, kMinScale), FLT_MAX);
+              const bool ragged = (slice + 1) * kSumKeys > vis_least;
+              const uint8_t* const next = slice_at(slice + kSumWaves);
+              // The scores of all tiles of pairs in 36 steps of 16 dims, each
+              // step's operands read a step ahead.
+              auto add_pairs = [&](auto tiles_n) {
+                constexpr int N = decltype(tiles_n)::value;
+                f32x16_t s[N];
 #pragma unroll
                 for (int n = 0; n < N; ++n)
-                  q[j & 1][n] = *reinterpret_cast<const u32x4_t*>(
-                      &q_tile[n * 32 * kRow * 2 + (j >> 2) * 128 + q_at[(j >> 1) & 1][j & 1]]);
-              };
-              fetch(0);
 #pragma unroll
-              for (int j = 0; j < 36; ++j) {
-                if (j < 35) fetch(j + 1);
-                // (Widened here: the compiler would do it ahead for all forms at
-                // once, and spill.)
-                if ((j & 1) == 0) asm volatile("" : "+v"(k[j >> 1]));
-                const auto kj = widen8<T>(k[j >> 1][2 * (j & 1)], k[j >> 1][2 * (j & 1) + 1]);
-                if (j & 1) k[j >> 1] = *reinterpret_cast<const u32x4_t*>(next + lane_at + 16 * (j & ~1));
+                  for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+                u32x4_t q[2][N];
+                auto fetch = [&](int j) {
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-                  s[n] = T::mfma32(kj, __builtin_bit_cast(typename T::vec8, q[j & 1][n]), s[n]);
-                __builtin_amdgcn_sched_barrier(0);
-              }
+                  for (int n = 0; n < N; ++n)
+                    q[j & 1][n] = *reinterpret_cast<const u32x4_t*>(
+                        &q_tile[n * 32 * kRow * 2 + (j >> 2) * 128 + q_at[(j >> 1) & 1][j & 1]]);
+                };
+                fetch(0);
 #pragma unroll
-              for (int n = 0; n < N; ++n) {
-                const float lse = pair_lse[n * 32 + l32];
-                if (ragged) {
-                  const int vis = pair_vis[n * 32 + l32] - slice * kSumKeys - 4 * hh;
+                for (int j = 0; j < 36; ++j) {
+                  if (j < 35) fetch(j + 1);
+                  // (Widened here: the compiler would do it ahead for all forms at
+                  // once, and spill.)
+                  if ((j & 1) == 0) asm volatile("" : "+v"(k[j >> 1]));
+                  const auto kj = widen8<T>(k[j >> 1][2 * (j & 1)], k[j >> 1][2 * (j & 1) + 1]);
+                  if (j & 1) k[j >> 1] = *reinterpret_cast<const u32x4_t*>(next + lane_at + 16 * (j & ~1));
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
-                    sum[e] += 8 * (e >> 2) + (e & 3) < vis ? p : 0.f;
+                  for (int n = 0; n < N; ++n)
+                    s[n] = T::mfma32(kj, __builtin_bit_cast(typename T::vec8, q[j & 1][n]), s[n]);
+                  __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                  const float lse = pair_lse[n * 32 + l32];
+                  if (ragged) {
+                    const int vis = pair_vis[n * 32 + l32] - slice * kSumKeys - 4 * hh;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                      const float p = __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
+                      sum[e] += 8 * (e >> 2) + (e & 3) < vis ? p : 0.f;
+                    }
+                  } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
                   }
-                } else {
+                }
+              };
+              if (tiles == 1)
+                add_pairs(std::integral_constant<int, 1>{});
+              else if (tiles == 2)
+                add_pairs(std::integral_constant<int, 2>{});
+              else
+                add_pairs(std::integral_constant<int, 4>{});
+              // Over the 32 pairs: a lane keeps half of its values each time and
+              // hands its neighbour the others, until it holds value e_mine.
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[n][e], score, -lse));
+              for (int x = 16; x >= 2; x >>= 1) {
+                const bool up = (l32 & x) != 0;
+#pragma unroll
+                for (int e = 0; e < x / 2; ++e) {
+                  const float keep = up ? sum[e + x / 2] : sum[e], give = up ? sum[e] : sum[e + x / 2];
+                  sum[e] = keep + __shfl_xor(give, x, 64);
                 }
               }
-            };
-            if (tiles == 1)
-              add_pairs(std::integral_constant<int, 1>{});
-            else if (tiles == 2)
-              add_pairs(std::integral_constant<int, 2>{});
-            else
-              add_pairs(std::integral_constant<int, 4>{});
-            // Over the 32 pairs: a lane keeps half of its values each time and
-            // hands its neighbour the others, until it holds value e_mine.
-#pragma unroll
-            for (int x = 16; x >= 2; x >>= 1) {
-              const bool up = (l32 & x) != 0;
-#pragma unroll
-              for (int e = 0; e < x / 2; ++e) {
-                const float keep = up ? sum[e + x / 2] : sum[e], give = up ? sum[e] : sum[e + x / 2];
-                sum[e] = keep + __shfl_xor(give, x, 64);
-              }
+              sum[0] += __shfl_xor(sum[0], 1, 64);
             }
-            sum[0] += __shfl_xor(sum[0], 1, 64);
-          }
-          const float now = before + sum[0];
-          if (!last) {
-            if (mine) *held = now;
-          } else if (mine && known && slot < r.len) {
-            record[slot] = total + now;
+            const float now = before + sum[0];
+            if (!last) {
+              if (mine) *held = now;
+            } else if (mine && known && slot < r.len) {
+              record[slot] = total + now;
+            }
           }
         }
       }
@@ -1780,6 +1817,12 @@ hipError_t launch_latent8_append(const Latent8AppendArgs& a, hipStream_t stream)
   return hipGetLastError();
 }
 
+int64_t latent8_items(int64_t rows, int64_t heads, int64_t latent_heads, int64_t batch, bool list) {
+  if (latent_heads <= 0) return 0;
+  if (list) return rows * ceil_div(heads / latent_heads, kRows) * latent_heads;
+  return ceil_div(rows * heads, kRows) + std::min(batch, rows) * latent_heads;
+}
+
 size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights) {
   return sizeof(float) * 2 * kParts * (kPartFloats + kRows * 2) + round256(sizeof(JoinEntry) * kParts) +
          (weights ? sizeof(float) * rows * heads : 0);
@@ -1792,8 +1835,11 @@ static void attend(const Latent8Args& a, hipStream_t stream) {
     launch_kernel(kKernLatent8Attention, latent8_attention_kernel<T, true>, grid, dim3(kAttnThreads), stream, a);
   else
     launch_kernel(kKernLatent8Attention, latent8_attention_kernel<T, false>, grid, dim3(kAttnThreads), stream, a);
-  launch_kernel(kKernLatent8Join, latent8_join_kernel<T>, dim3(kJoinBlocks, static_cast<unsigned>(a.parts)),
-                dim3(kJoinThreads), stream, a);
+  const dim3 join(kJoinBlocks, static_cast<unsigned>(a.joins));
+  if (a.join_items && a.joins <= kFewJoins)
+    launch_kernel(kKernLatent8Join, latent8_join_kernel<T, kJoinGroups>, join, dim3(256 * kJoinGroups), stream, a);
+  else
+    launch_kernel(kKernLatent8Join, latent8_join_kernel<T, 1>, join, dim3(256), stream, a);
   if (a.token_weights != nullptr)
     launch_kernel(kKernLatent8Weights, latent8_weights_kernel<T>, dim3(kSumParts), dim3(kSumThreads), stream, a);
 }
@@ -1803,6 +1849,9 @@ hipError_t launch_latent8_attention(const Latent8Args& args, hipStream_t stream)
   Latent8Args a = args;
   a.parts = kParts;
   a.per = static_cast<int32_t>(a.heads / a.latent_heads);
+  const int64_t items = latent8_items(a.rows, a.heads, a.latent_heads, a.batch, a.topk != nullptr);
+  a.join_items = items <= kParts;
+  a.joins = a.join_items ? items : kParts;
   if (a.elem == Elem::kBf16)
     attend<Bf16>(a, stream);
   else

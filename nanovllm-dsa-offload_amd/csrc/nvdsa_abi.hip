@@ -1307,14 +1307,6 @@ void check_records(Check& c, const nvdsa_tensor* t, const nvdsa_tensor* block_ta
       .need(t->dtype == dtype, NVDSA_ERR_DTYPE, "token positions must be int32, token weights float32");
 }
 
-// At most so many items (up to 64 (row, head) pairs of a request and latent
-// head; with a list, of a row): the kernels count them in 24 bits.
-int64_t latent8_items(int64_t rows, int64_t heads, int64_t latent_heads, int64_t batch, bool list) {
-  if (latent_heads <= 0) return 0;
-  if (list) return rows * nvdsa::ceil_div(heads / latent_heads, 64) * latent_heads;
-  return nvdsa::ceil_div(rows * heads, 64) + std::min(batch, rows) * latent_heads;
-}
-
 void check_optional(Check& c, const nvdsa_tensor* t, int device) {
   if (t == nullptr) return;
   const nvdsa_tensor* const one[] = {t};
@@ -1422,7 +1414,7 @@ int nvdsa_latent8_attention(const nvdsa_tensor* query_rope, const nvdsa_tensor* 
         .need(N > 0 && N <= 1024 && N % G == 0, NVDSA_ERR_SHAPE,
               "heads must be a multiple of the latent heads, at most 1024")
         .need(T < (int64_t{1} << 20), NVDSA_ERR_SHAPE, "too many query rows")
-        .need(latent8_items(T, N, G, B, topk_ids != nullptr) < (int64_t{1} << 24), NVDSA_ERR_SHAPE,
+        .need(nvdsa::latent8_items(T, N, G, B, topk_ids != nullptr) < (int64_t{1} << 24), NVDSA_ERR_SHAPE,
               "too many query rows and heads for one call")
         .need(same_shape(attention_out, query), NVDSA_ERR_SHAPE, "attention_out must match query")
         .need(is_half(query) && query->dtype == query_rope->dtype && query->dtype == attention_out->dtype,

@@ -306,12 +306,17 @@ struct Latent8Args {
   float* token_weights;         // [pool_rows, cols * 128], or null
   void* out;                    // [rows, heads, 512]
   int64_t rows, heads, latent_heads, batch, cols, blocks, list_len, pool_rows;
-  int64_t parts;                // set by the launch, as is
+  int64_t parts;                // set by the launch, as are the next three
+  int64_t joins;                // entries for the joining kernel:
+  bool join_items;              //   one an item, or one a part
   int32_t per;                  // heads / latent_heads
   float scale;
   Elem elem;
   void* workspace;
 };
+// At most so many items (up to 64 (row, head) pairs of a request and latent
+// head; with a list, of a row).
+int64_t latent8_items(int64_t rows, int64_t heads, int64_t latent_heads, int64_t batch, bool list);
 size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights);
 hipError_t launch_latent8_attention(const Latent8Args& a, hipStream_t stream);
 
