@@ -243,8 +243,8 @@ constexpr int kLoads = kKeys * kRowChunks / (kAttnThreads / 2);  // of a thread 
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
 constexpr float kMost = 15.f;   // scores pass a row's reference by this at most (base 2): P <= 2^15 fits fp16
-constexpr int kMinUnits = 1;    // least tiles of a workgroup
 constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
+constexpr float kJoinCost = 0.0375f;  // what joining one part more costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
 constexpr int kPartFloats = kRows * kCkvDim;
 
@@ -287,8 +287,16 @@ __device__ inline int tile_of(const Plan& p, int tiles, int u) {
 // 0).  48 lists' items of 32 tiles take 31 us in 5 shares of 7 tiles each and 37
 // in 256 parts of 6; 24 items of about 129 tiles 46 in shares of 14 and 50 in
 // 256 parts of 12; 24 of 512 stay in 256 parts of 48.
-__device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, int64_t least, int cost, int tiles) {
-  Plan p{tiles_all, divide(tiles_all, least), 0, 0};
+// Partial sums have to be joined, at about kJoinCost tiles' time a part of an
+// item: beyond sqrt(tiles / kJoinCost) parts of an item, more of them cost more
+// than they save (1 x 32,768 tokens, 512 tiles: 28 + 11 us in 117 parts, 25 + 20
+// in 256).
+__device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, bool joins, int cost, int tiles) {
+  Plan p{tiles_all, tiles_all, 0, 0};
+  if (joins && items > 0) {
+    const int64_t most = static_cast<int64_t>(sqrtf(static_cast<float>(tiles_all) * static_cast<float>(items) / kJoinCost));
+    if (parts > most) parts = most;
+  }
   if (p.parts > parts) p.parts = parts;
   if (p.parts < 1) p.parts = 1;
   if (items <= 0) return p;
@@ -383,11 +391,11 @@ struct Start {
   Request r;
 };
 // EACH(request): the tiles of each of its items, ITEMS(request): their number;
-// COST: see make_plan; `ends`: of request threadIdx.x (of request 0 where there
+// COST, JOINS: see make_plan; `ends`: of request threadIdx.x (of request 0 where there
 // is none), on its way.
-template <int THREADS, int COST, typename ITEMS, typename EACH>
-__device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64_t part, int64_t parts, int64_t least,
-                                   int tiles, ITEMS items, EACH each) {
+template <int THREADS, int COST, bool JOINS, typename ITEMS, typename EACH>
+__device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64_t part, int64_t parts, int tiles,
+                                   ITEMS items, EACH each) {
   __shared__ Units scratch[THREADS / 64];
   __shared__ int64_t found[6];
   Start s;
@@ -408,7 +416,7 @@ __device__ inline Start find_start(const Latent8Args& a, const Ends& ends, int64
   if (tid == 0) found[0] = -1;
   Units at = scan_units<THREADS>(sum, scratch, &total);
   total = {uniform64(total.items), uniform64(total.tiles)};
-  s.plan = make_plan(total.items, total.tiles, parts, least, COST, tiles);
+  s.plan = make_plan(total.items, total.tiles, parts, JOINS, COST, tiles);
   s.items = total.items;
   // (More items than the rows can have: requests whose ends decrease share
   // rows.  Nothing is done.)
@@ -666,8 +674,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   const int m_mine = grp * 32 + l32;
   uint16_t* const p_mine = p_tile[grp];
 
-  const Start start = find_start<kAttnThreads, kBegin>(
-      a, ends, part, a.parts, kMinUnits, LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
+  const Start start = find_start<kAttnThreads, kBegin, true>(
+      a, ends, part, a.parts, LIST ? (static_cast<int>(a.list_len) + kKeys - 1) / kKeys : 0,
       [](const Request& r) { return r.items; }, [](const Request& r) { return r.tiles; });
   const Work work = carve_work(a.workspace, a.parts);
   // Entries that no item writes below: all of the parts', or those behind the
@@ -1140,14 +1148,16 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   }
 }
 
-// Joins the partials of items that lie across parts: block (y, w) takes what
-// part w names, the y-th 4 of the 128 groups of 64 x 4 values that the
-// accumulators' order consists of.  The parts' factors go through LDS first, so
-// that the loads of the partials depend on nothing.  Few parts name an item, at
-// a stride that can fall on few XCDs: y counts fastest, so that each item's
-// blocks lie on all of them (48 items over 256 parts, 34 MB: 10.7 us instead
-// of 30 with w fastest).
-// Four groups of waves take every fourth part each, and their sums meet in LDS.
+// Joins the partials of items that lie across parts: block (y, k) takes the k-th
+// entry, the y-th 4 of the 128 groups of 64 x 4 values that the accumulators'
+// order consists of.  The parts' factors go through LDS first, so that the loads
+// of the partials depend on nothing.  Entries belong to items where these are no
+// more than the parts, so that few blocks find nothing to do; y counts fastest,
+// so that each item's blocks lie on all XCDs.  Bound by the partials' bytes and
+// the launch: 24 items over 256 parts, 34 MB, in 9.5 us (30 with the entries of
+// parts, counting fastest).  Where few items have many parts, four groups of
+// waves take every fourth part each, and their sums meet in LDS: one item's 256
+// parts in 20 us instead of 40, but 80 items' in 16 instead of 9.5.
 constexpr int kJoinGroups = 4;
 constexpr int kFewJoins = 16;
 constexpr int kJoinBlocks = 32;
@@ -1236,9 +1246,10 @@ __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args 
 // leaves.  Every slot has one owner: no atomics, one order of summation.
 //
 // Bound by the cache's bytes and the products alike: 24 requests of 8,192
-// tokens and 128 heads, 113 MB and 29 GFLOP, in 39 us, of which 13 pass before
-// the first product (the part's place 4, the pairs' rows and the first codes 9).
-// One workgroup a page, its codes and 32 pairs at a time in LDS, took 111.
+// tokens and 64 heads, 113 MB and 14 GFLOP, in 33 us, of which 13 pass before the
+// first product (the part's place 4, the pairs' rows and the first codes 9).
+// Parts that lie across requests, which bring other pairs, made it 39; one
+// workgroup a page, its codes and 32 pairs at a time in LDS, took 111.
 constexpr int kSumThreads = 512;
 constexpr int kSumWaves = kSumThreads / 64;
 constexpr int kSumPairs = 128;
@@ -1261,8 +1272,8 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
   auto slices = [](const Request& r) -> int { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
-  const Start start = find_start<kSumThreads, kSumBegin>(
-      a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, 1, 0,
+  const Start start = find_start<kSumThreads, kSumBegin, false>(
+      a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, 0,
       [&](const Request& r) -> int64_t { return slices(r) > 0; }, slices);
   if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
