@@ -615,9 +615,9 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
 // group's softmax, group 1's softmax with the loads 1,500.  In the loop that is
 // 1.0 PFLOP/s, of the 1.27 that a large product reaches.  A part's start (10
 // us) and its partial sums (3 us) come to that: 24 requests of 32,768 tokens
-// and 64 heads in 155 us (110 GFLOP, 453 MB), 40 ragged ones with 8 heads in
-// 103 us (4.6 TB/s), 2 x 515 rows over up to 8,197 tokens, 2 x 16 heads, in
-// 465 us.  One phase for all waves took 175, 166 and 565.  Weighed against it:
+// and 64 heads in 145 us (110 GFLOP, 453 MB), 40 ragged ones with 8 heads in
+// 99 us (4.8 TB/s), 2 x 515 rows over up to 8,197 tokens, 2 x 16 heads, in
+// 455 us.  One phase for all waves took 175, 166 and 565.  Weighed against it:
 // the same products on the 8-bit MFMAs, with bf16 queries split into two codes
 // and P into three, took 164 us for the first and twice as long for lists.
 template <typename T, bool LIST>
