@@ -279,14 +279,14 @@ __device__ inline int tile_of(const Plan& p, int tiles, int u) {
 }
 
 // Equal parts of the units.  A part that lies across two items begins anew,
-// which costs the time of `cost` tiles, so an item counts that much more than its
-// tiles (at most an eighth of a part more: a part that lies in the first units
-// only has nothing to do).  What the eighth leaves out costs a part that many
-// tiles; where shares of single items, of up to total / (parts - items) tiles,
-// are shorter than that, they are the parts (`tiles`: what every item has, or
-// 0).  48 lists' items of 32 tiles take 31 us in 5 shares of 7 tiles each and 37
-// in 256 parts of 6; 24 items of about 129 tiles 46 in shares of 14 and 50 in
-// 256 parts of 12; 24 of 512 stay in 256 parts of 48.
+// which costs the time of `cost` tiles, so an item counts that much more than
+// its tiles (at most an eighth of a part more: a part that lies in the first
+// units only has nothing to do).  What the eighth leaves out costs a part that
+// many tiles; where shares of single items, of up to total / (parts - items)
+// tiles, are shorter than that, they are the parts (`tiles`: what every item
+// has, or 0).  24 items of 32 tiles (lists) take 30 us in 8 shares of 4 tiles
+// each and 37 in 256 parts of 3; 24 of about 129 tiles 46 in shares of 14 and 50
+// in 256 parts of 12; 24 of 512 stay in 256 parts of 48.
 // Partial sums have to be joined, at about kJoinCost tiles' time a part of an
 // item: beyond sqrt(tiles / kJoinCost) parts of an item, more of them cost more
 // than they save (1 x 32,768 tokens, 512 tiles: 28 + 11 us in 117 parts, 25 + 20
