@@ -294,15 +294,15 @@ __device__ inline int tile_of(const Plan& p, int tiles, int u) {
 __device__ inline Plan make_plan(int64_t items, int64_t tiles_all, int64_t parts, bool joins, int cost, int tiles) {
   Plan p{tiles_all, tiles_all, 0, 0};
   if (joins && items > 0) {
-    const int64_t most = static_cast<int64_t>(sqrtf(static_cast<float>(tiles_all) * static_cast<float>(items) / kJoinCost));
-    if (parts > most) parts = most;
+    const float most = static_cast<float>(tiles_all) * static_cast<float>(items) * (1.f / kJoinCost);
+    if (most < static_cast<float>(parts * parts)) parts = static_cast<int64_t>(__builtin_amdgcn_sqrtf(most));
   }
   if (p.parts > parts) p.parts = parts;
   if (p.parts < 1) p.parts = 1;
-  if (items <= 0) return p;
+  if (items <= 1) return p;
   const int64_t eighth = divide(tiles_all, 8 * p.parts);
   p.begin = eighth < cost ? static_cast<int>(eighth) : cost;
-  if (items > 1 && items < parts) {
+  if (items < parts) {
     int64_t share = tiles > 0 ? divide(tiles - 1, divide(parts, items)) + 1 : divide(tiles_all - 1, parts - items) + 1;
     if ((share + p.begin - cost) * p.parts < tiles_all + items * p.begin) {
       p.share = static_cast<int>(share);
