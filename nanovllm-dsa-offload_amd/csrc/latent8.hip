@@ -242,7 +242,15 @@ constexpr int kWindow = 512;    // resolved pages (or list entries) held at a ti
 constexpr int kLoads = kKeys * kRowChunks / (kAttnThreads / 2);  // of a thread (group 1) for a tile
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
+constexpr float kUnseen = 1.0e30f;
 constexpr float kMost = 15.f;   // scores pass a row's reference by this at most (base 2): P <= 2^15 fits fp16
+// A tile is weighed again where its largest P passes 2^kMost, or where p, P times
+// 2^up, might leave fp32's range: with a largest P of 2^top, where top passes
+// kMostSum - 4 up.  Up to up = 20 that is kMost; p stays below 2^35 of its
+// reference, and a P below 2^-126, which becomes zero, counts only where up
+// passes 55, that is where any top from -126 on passes the limit.  (A list's p
+// are exponentials of their own and may pass their reference by 2^kMostSum.)
+constexpr float kMostSum = 95.f;
 constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
 constexpr float kJoinCost = 0.0375f;  // what joining one part more costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
@@ -526,7 +534,7 @@ struct JoinEntry {
 
 struct Work {
   float* part;      // [2 parts][64 * 512], in the accumulators' order
-  float* ml;        // [2 parts][64][2]
+  float4* refs;     // [2 parts][64]: reference of the sums, of the normaliser, the normaliser
   JoinEntry* join;  // [parts], of an item each or named by a part; row0 < 0: nothing
   float* lse;       // [rows, heads], base 2 (with weights)
 };
@@ -536,8 +544,8 @@ __host__ __device__ inline Work carve_work(void* ws, int64_t parts) {
   char* p = static_cast<char*>(ws);
   w.part = reinterpret_cast<float*>(p);
   p += sizeof(float) * 2 * parts * kPartFloats;
-  w.ml = reinterpret_cast<float*>(p);
-  p += sizeof(float) * 2 * parts * kRows * 2;
+  w.refs = reinterpret_cast<float4*>(p);
+  p += sizeof(float4) * 2 * parts * kRows;
   w.join = reinterpret_cast<JoinEntry*>(p);
   p += round256(sizeof(JoinEntry) * parts);
   w.lse = reinterpret_cast<float*>(p);
@@ -573,13 +581,11 @@ __device__ inline float first_lane(float x) {
 
 // What a page's (or list entry's) scale c enters: scores take it as a factor,
 // P its logarithm into the exponent (p * c multiplies V's codes; exact for a
-// power of two, else off by the logarithm's rounding), and the sum of p
-// divides it out again.
-struct Window {
+// power of two, else off by the logarithm's rounding).
+struct alignas(16) Window {
   int32_t row;    // first cache row of the page, or the entry's row; -1: none
   float score;    // softmax scale * log2(e) * c
   float log2c;
-  float inverse;
 };
 __device__ inline int32_t row_of_slot(const Latent8Args& a, int64_t b, int64_t slot, bool ok) {
   if (!ok) return -1;
@@ -594,8 +600,19 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
   w.score = a.scale * kLog2e * c;
   const float exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
   w.log2c = exponent + __builtin_amdgcn_logf(__uint_as_float((u & 0x7fffffu) | 0x3f800000u));
-  w.inverse = 1.f / c;
 }
+
+// base * 2^x / l where l > 0, else 0: in two factors, since 2^x alone may pass
+// fp32's range on either side.
+struct Quotient {
+  float a, b;
+  __device__ inline Quotient(float x, float l) {
+    const float root = __builtin_amdgcn_exp2f(0.5f * x);
+    a = l == 0.f ? 0.f : root / l;
+    b = l == 0.f ? 0.f : root;
+  }
+  __device__ inline float of(float base) const { return base * a * b; }
+};
 
 // Eight waves in two groups of four: group g owns rows 32 g .. 32 g + 31 of the
 // item.  For a tile, a group's wave takes S^T = K Q^T of 32 keys over half of
@@ -609,6 +626,11 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
 // of either.  P(t) is taken against a reference, the running maximum at some
 // tile before; where a tile outgrows that by more than fp16 holds, or is the
 // first that a row sees, the group weighs it again against its own maximum.
+//
+// The normaliser sums p without the scale, in fp32, against a reference of its
+// own: p * c and p have their maxima in different pages where scales differ, by
+// up to 2^246 (a page of zero rows has scale 2^-126 and weighs exp(0) a key all
+// the same), and one reference would overflow or lose one of the two.
 //
 // Bound by the phases, of about 2,050 clocks each: a wave's 34 MFMAs of 32
 // clocks (1,088) take 1,600 alone on their SIMD and 1,900 next to the other
@@ -626,6 +648,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   __shared__ __align__(16) float4 half_s[8 * 2 * 64];
   __shared__ __align__(16) uint16_t p_tile[2][32 * kPStride];
   __shared__ __align__(16) float row_max[2][2][32][4];  // group, tile parity, row, wave
+  __shared__ __align__(16) float row_top[LIST ? 2 : 1][2][32][4];  // likewise, without the scales
+  __shared__ float2 row_ref[2][32];                     // group, row: see lift and the normaliser's reference
   __shared__ int outgrown[2][2];                        // group, tile parity
   __shared__ int bad_entries[2][LIST ? kWindow / kKeys : 1];  // tiles of a window with entries that name nothing
   __shared__ Window windows[LIST ? 2 : 1][kWindow];
@@ -761,7 +785,11 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
-    float m_run = kNoMax, l_run = 0.f, l_tile = 0.f;
+    // ref: the reference of P and o.  l_run, l_tile: sums of p against the
+    // normaliser's, row_ref.y; it lies row_ref.x below ref ("lift": kUnseen, and
+    // ref is 0, before the row's first key).
+    float ref = 0.f, l_run = 0.f, l_tile = 0.f;
+    float2* const my_row_ref = &row_ref[grp][l32];
     float sc[8];
 
     auto window_of = [&](int tile) -> const Window* {
@@ -773,7 +801,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     // one after them, in scalar registers.
     Window page_before{}, page_now{}, page_next{}, page_far{};
     auto scalar = [&](const Window& v) {
-      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.log2c), first_lane(v.inverse)};
+      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.log2c)};
     };
     // A tile's loads, by the waves of group 1, issued a few at a time.
     struct TileLoad {
@@ -833,8 +861,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       }
       return (tile + 1) * kKeys > vis_least || page_before.row < 0;
     };
-    // P of the tile's scores against the row's reference, into LDS; l_tile: their sum.
-    auto weigh = [&](const Window(&w)[LIST ? 8 : 1]) {
+    // P of the tile's scores against the row's reference, into LDS; l_tile: the
+    // sum of p.  Where the tile has one scale, p is P times 2^(lift - log2c), as
+    // long as the row's limit keeps that in range (see below); ALONE: by
+    // exponents of its own.
+    auto weigh = [&](const Window(&w)[LIST ? 8 : 1], float lift, auto alone) {
+      constexpr bool ALONE = LIST || decltype(alone)::value;
       l_tile = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -842,37 +874,42 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           pw[k] = __builtin_amdgcn_exp2f(sc[4 * e + k]);
-          l_tile = LIST ? fmaf(pw[k], w[LIST ? 4 * e + k : 0].inverse, l_tile) : l_tile + pw[k];
+          l_tile += ALONE ? __builtin_amdgcn_exp2f(sc[4 * e + k] + (lift - w[LIST ? 4 * e + k : 0].log2c)) : pw[k];
         }
         const uint2 packed = make_uint2(F16::pack2(pw[0], pw[1]), F16::pack2(pw[2], pw[3]));
         *reinterpret_cast<uint2*>(&p_mine[l32 * kPStride + key_mine + 8 * e]) = packed;
       }
-      if (!LIST) l_tile *= w[0].inverse;
+      if (!ALONE) l_tile *= __builtin_amdgcn_exp2f(fminf(lift - w[0].log2c, 100.f));
     };
-    // The row's reference, which scores are relative to, follows its maximum;
-    // the sums so far follow the reference.
-    auto reference = [&] { return m_run == kNoMax ? 0.f : m_run; };
-    auto follow_max = [&](int tile) {
-      const float4 v = *reinterpret_cast<const float4*>(row_max[grp][tile & 1][l32]);
-      const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-      const bool past = most > m_run;
-      const float grow = past ? __builtin_amdgcn_exp2f(m_run - most) : 1.f;
-      const float down = past ? reference() - most : 0.f;
-      m_run = past ? most : m_run;
-      l_run *= grow;
+    auto most_of = [&](const float(&of)[4]) {
+      const float4 v = *reinterpret_cast<const float4*>(of);
+      return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    };
+    // A tile that outgrew a reference: both follow their maxima, the sums so far
+    // follow them, and the tile is weighed again.  Returns the row's new
+    // row_ref, to be stored when every wave has read the old one.
+    auto weigh_again = [&](int tile) {
+      const float2 old = *my_row_ref;
+      const bool unseen = old.x == kUnseen;
+      const float most = most_of(row_max[grp][tile & 1][l32]);
+      const float most_sum = LIST ? most_of(row_top[LIST ? grp : 0][tile & 1][l32]) : most - page_before.log2c;
+      const bool past = most > (unseen ? -INFINITY : ref), past_sum = most_sum > (unseen ? -INFINITY : old.y);
+      const float down = past ? ref - most : 0.f;
+      const float grow = unseen ? 1.f : __builtin_amdgcn_exp2f(down);
+      ref = past ? most : ref;
+      const float sum_ref = past_sum ? most_sum : old.y;
+      l_run *= unseen || !past_sum ? 1.f : __builtin_amdgcn_exp2f(old.y - most_sum);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sc[e] += down;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= grow;
-    };
-    // A tile that outgrew the maximum, against its own.
-    auto weigh_again = [&](int tile) {
-      follow_max(tile);
       Window w[LIST ? 8 : 1];
       fields(tile, w);
-      weigh(w);
+      const float lift = unseen && !past ? kUnseen : ref - sum_ref;
+      weigh(w, lift, std::true_type{});
+      return make_float2(lift, sum_ref);
     };
     // S^T of tile t in nine steps of 32 dims, and O^T of tile t - 1 in eight
     // steps of 16 keys and two of the wave's four tiles of dims (OUTPUT), step
@@ -905,8 +942,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       for (int j = 0; j < kAhead; ++j) fetch(j);
       if (OUTPUT) {
         if (__builtin_amdgcn_readfirstlane(again) != 0) {  // (every wave waits for it)
-          weigh_again(t - 1);
+          const float2 now = weigh_again(t - 1);
           lds_barrier();
+          if (wg == 0 && hh == 0) *my_row_ref = now;
           fetch_p(0);
         }
         l_run += l_tile;
@@ -954,7 +992,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         load.on = false;
         if (!LIST && grp == 1) load = begin_load(t + 2, to, page_next.row);
         issue_load(load, 0, 3);
-        const float ref = reference();
+        const float lift = my_row_ref->x;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4& x4 = other[e >> 2];
@@ -973,15 +1011,24 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         // once do not fit the registers.)
         if (LIST && grp == 1) load = begin_load(t + 2, to, 0);
         issue_load(load, LIST ? 0 : 3, 6);
-        float top = sc[0];
+        float top = sc[0], top_sum = sc[0] - w[0].log2c;
 #pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+        for (int e = 1; e < 8; ++e) {
+          top = fmaxf(top, sc[e]);
+          if (LIST) top_sum = fmaxf(top_sum, sc[e] - w[LIST ? e : 0].log2c);
+        }
         top = xor32_op(top, MaxOp{});
-        if (hh == 0) row_max[grp][t & 1][l32][wg] = top + ref;
-        if (__any(top > (m_run == kNoMax ? -INFINITY : kMost)) && lane == 0) outgrown[grp][t & 1] = 1;
+        if (LIST) top_sum = xor32_op(top_sum, MaxOp{});
+        if (hh == 0) {
+          row_max[grp][t & 1][l32][wg] = top + ref;
+          if (LIST) row_top[LIST ? grp : 0][t & 1][l32][wg] = top_sum + ref;
+        }
+        const float limit = fminf(kMost, kMostSum - 4.f * (lift - w[0].log2c));
+        const bool past_most = LIST ? top > kMost || top_sum + lift > kMostSum : top > limit;
+        if (__any(past_most) && lane == 0) outgrown[grp][t & 1] = 1;
         __builtin_amdgcn_sched_barrier(0);
         issue_load(load, 6, kLoads);
-        weigh(w);
+        weigh(w, lift, std::false_type{});
       } else {
         if (grp == 1) load_tile(t + 2, to, page_next.row);
       }
@@ -1065,6 +1112,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       w0 = LIST ? c0 : c0 & ~1;
       window_rows(w0);
       if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
+      if (tid < kRows && c0 == t0) row_ref[tid >> 5][tid & 31] = make_float2(kUnseen, kNoMax);
       lds_barrier();
       buf = 0;
       before = 2;
@@ -1100,18 +1148,18 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       if (m_mine < x.count) {
         const int f = x.first + m_mine, i = f / per, h = f - i * per;
         const int64_t row = (r.row0 + i) * a.heads + x.g * per + h;
-        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        const Quotient by(my_row_ref->x, l_all);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int d = wg * 128 + dt * 32 + 8 * e + 4 * hh;
-            const uint2 u = make_uint2(T::pack2(o[dt][4 * e] * inv, o[dt][4 * e + 1] * inv),
-                                       T::pack2(o[dt][4 * e + 2] * inv, o[dt][4 * e + 3] * inv));
+            const uint2 u = make_uint2(T::pack2(by.of(o[dt][4 * e]), by.of(o[dt][4 * e + 1])),
+                                       T::pack2(by.of(o[dt][4 * e + 2]), by.of(o[dt][4 * e + 3])));
             *reinterpret_cast<uint2*>(&out[row * kCkvDim + d]) = u;
           }
         if (a.token_weights != nullptr && wg == 0 && hh == 0)
-          work.lse[row] = m_run + __builtin_amdgcn_logf(l_all);
+          work.lse[row] = l_all == 0.f ? -INFINITY : my_row_ref->y + __builtin_amdgcn_logf(l_all);
       }
       if (a.join_items && tid == 0) work.join[item_base + it].row0 = -1;
     } else {
@@ -1128,8 +1176,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
                 make_float4(o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]);
       }
       if (wg == 0 && hh == 0) {
-        work.ml[(slot * kRows + m_mine) * 2] = empty ? -INFINITY : m_run;
-        work.ml[(slot * kRows + m_mine) * 2 + 1] = l_all;
+        const float2 mine = *my_row_ref;
+        work.refs[slot * kRows + m_mine] = make_float4(empty ? -INFINITY : (mine.x == kUnseen ? kNoMax : ref),
+                                                       empty ? -INFINITY : mine.y, l_all, 0.f);
       }
       // The first border of parts inside an item names it to the joining kernel.
       if (first_seg && at > item_start && tid == 0 && part_start(start.plan, part - 1) <= item_start) {
@@ -1166,7 +1215,7 @@ template <typename T, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args a) {
   constexpr int kSlices = 8 * GROUPS;
   __shared__ float factor[kJoinParts][32];  // of a part and row
-  __shared__ float row_part[kSlices][32];
+  __shared__ float2 row_part[kSlices][32];
   __shared__ float4 sums[GROUPS > 1 ? GROUPS - 1 : 1][256];
   const Work work = carve_work(a.workspace, a.parts);
   const JoinEntry j = work.join[blockIdx.y];
@@ -1181,13 +1230,16 @@ __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args 
   const int per = a.per;
   const int m = tid & 31, s = tid >> 5;  // thread (s, m): parts s, s + kSlices, ... of row m
   auto slot_of = [&](int w) -> int64_t { return w == 0 ? j.slot0 : 2 * static_cast<int64_t>(j.w0 + w); };
-  auto ml_of = [&](int w) { return reinterpret_cast<const float2*>(work.ml)[slot_of(w) * kRows + grp * 32 + m]; };
-  float most = -INFINITY;
-  for (int w = s; w < n; w += kSlices) most = fmaxf(most, ml_of(w).x);
+  auto refs_of = [&](int w) { return work.refs[slot_of(w) * kRows + grp * 32 + m]; };
+  float2 most = make_float2(-INFINITY, -INFINITY);  // references of the sums and of the normaliser
+  for (int w = s; w < n; w += kSlices) {
+    const float4 v = refs_of(w);
+    most = make_float2(fmaxf(most.x, v.x), fmaxf(most.y, v.y));
+  }
   row_part[s][m] = most;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSlices; ++k) most = fmaxf(most, row_part[k][m]);
+  for (int k = 0; k < kSlices; ++k) most = make_float2(fmaxf(most.x, row_part[k][m].x), fmaxf(most.y, row_part[k][m].y));
   float l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const bool mine = grp * 32 + m < j.count;  // (m == lane & 31; the parts hold no other rows)
@@ -1196,10 +1248,9 @@ __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args 
     const int c1 = c0 + kJoinParts < n ? c0 + kJoinParts : n;
     __syncthreads();
     for (int w = c0 + s; w < c1; w += kSlices) {
-      const float2 v = ml_of(w);
-      const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - most);
-      factor[w - c0][m] = f;
-      if (v.x != -INFINITY) l = fmaf(v.y, f, l);
+      const float4 v = refs_of(w);
+      factor[w - c0][m] = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - most.x);
+      if (v.x != -INFINITY) l = fmaf(v.z, __builtin_amdgcn_exp2f(v.y - most.y), l);
     }
     __syncthreads();
 #pragma unroll 8
@@ -1212,13 +1263,13 @@ __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args 
       for (int k = 0; k < 4; ++k) acc[k] = fmaf(f == 0.f ? 0.f : __uint_as_float(v[k]), f, acc[k]);
     }
   }
-  row_part[s][m] = l;
+  row_part[s][m].x = l;
   if (group > 0) sums[group - 1][tid & 255] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
   if (group > 0 || !mine) return;
   l = 0.f;
 #pragma unroll
-  for (int k = 0; k < kSlices; ++k) l += row_part[k][m];
+  for (int k = 0; k < kSlices; ++k) l += row_part[k][m].x;
 #pragma unroll
   for (int k = 0; k < GROUPS - 1; ++k) {
     const float4 v = sums[k][tid];
@@ -1229,11 +1280,11 @@ __global__ __launch_bounds__(256 * GROUPS) void latent8_join_kernel(Latent8Args 
   }
   const int f = j.first + grp * 32 + m, i = f / per, h = f - i * per;
   const int64_t row = (j.row0 + i) * a.heads + j.g * per + h;
-  if (a.token_weights != nullptr && wg == 0 && dt == 0 && s == 0) work.lse[row] = most + __builtin_amdgcn_logf(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.token_weights != nullptr && wg == 0 && dt == 0 && s == 0) work.lse[row] = most.y + __builtin_amdgcn_logf(l);
+  const Quotient by(most.x - most.y, l);
   const int d = wg * 128 + dt * 32 + 8 * e + 4 * (lane >> 5);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * kCkvDim + d) =
-      make_uint2(T::pack2(acc[0] * inv, acc[1] * inv), T::pack2(acc[2] * inv, acc[3] * inv));
+      make_uint2(T::pack2(by.of(acc[0]), by.of(acc[1])), T::pack2(by.of(acc[2]), by.of(acc[3])));
 }
 
 // -------------------------------------------------------- attention weights
@@ -1835,7 +1886,7 @@ int64_t latent8_items(int64_t rows, int64_t heads, int64_t latent_heads, int64_t
 }
 
 size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights) {
-  return sizeof(float) * 2 * kParts * (kPartFloats + kRows * 2) + round256(sizeof(JoinEntry) * kParts) +
+  return sizeof(float) * 2 * kParts * (kPartFloats + kRows * 4) + round256(sizeof(JoinEntry) * kParts) +
          (weights ? sizeof(float) * rows * heads : 0);
 }
 

@@ -81,3 +81,56 @@ def weights_bound(added, total, reach, keys: int, terms: int):
 
 def oracle_attention(qr, q, ends, c, topk=None):
     return O.attention(qr, q, ends, c["lengths"], c["table"], c["cache"], c["scale"], SCALE, topk)
+
+
+def wide_attention(qr, q, ends, c, topk=None):
+    """The operator in fp64, heads together: (out, sums, size, reach, tail);
+    ``tail`` is the part of the bound below for keys whose P may lie below
+    fp16's normal range, the others are those of the oracle."""
+    rows, heads, _ = q.shape
+    groups = c["cache"].shape[2]
+    per, cap = heads // groups, c["cols"] * PAGE
+    out, size, tail = (torch.zeros(rows, heads, 512, dtype=torch.float64) for _ in range(3))
+    reach = torch.zeros(rows, heads, dtype=torch.float64)
+    sums = torch.zeros(len(ends), cap, dtype=torch.float64)
+    queries_ = torch.cat([q, qr], -1).double()
+    start = 0
+    for b, end in enumerate(ends.tolist()):
+        n, length = end - start, int(c["lengths"][b])
+        pages = c["table"][b].long()
+        scale = c["scale"][pages].double().repeat_interleave(PAGE, 0)                 # [slots, G]
+        codes = c["cache"].view(torch.uint8)[pages].view(torch.float8_e4m3fn).double().flatten(0, 1)
+        for i in range(n):
+            sees = max(0, length - (n - 1 - i))
+            at = torch.arange(sees) if topk is None else topk[start + i].long()
+            at = at[(at >= 0) & (at < sees)]
+            if len(at) == 0:
+                continue
+            for g in range(groups):
+                mine = slice(g * per, (g + 1) * per)
+                x, y = queries_[start + i, mine], codes[at, g] * scale[at, g, None]
+                p = torch.softmax(x @ y.T * SCALE, -1)
+                out[start + i, mine], size[start + i, mine] = p @ y[:, :512], p @ y[:, :512].abs()
+                reach[start + i, mine] = (x.abs() @ y.abs().T).amax(-1) * SCALE
+                weight = p * scale[at, g]
+                top = weight.amax(-1, keepdim=True)
+                tail[start + i, mine] = torch.where(weight < top * 2.0 ** -14, top * 2.0 ** -25, 0.0) @ codes[at, g, :512].abs()
+                if topk is None:
+                    sums[b, at] += p.sum(0)
+        start = end
+    return out, sums, size, reach, tail
+
+
+def wide_bound(out, size, reach, tail, dtype, keys: int):
+    """How far an output may be from the 64-bit one, scales of any size.  As in
+    :func:`attention_bound`, but exponents hold the logarithms of the scales
+    (below 2^9 with the scores of these tests): each of the eight sums that an
+    exponent passes through rounds by 2^-16, times ln 2 below 2^-13 together.
+    A row's largest P is at least 1, so that those from 2^-14 of the largest
+    p times scale on lie in fp16's normal range (2^-14); one below is off by
+    2^-25 of the largest p times scale, times its key's code.  A
+    subnormal output rounds by half of its type's step."""
+    score = reach * (578 * 2.0 ** -24 + 2.0 ** -22)
+    per = 2.0 ** -11 + keys * 2.0 ** -23 + 2 * score + 2.0 ** -21 + 2.0 ** -13
+    step = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}[dtype]
+    return out.abs() * HALF_STEP[dtype] + size * per[..., None] + tail + step
