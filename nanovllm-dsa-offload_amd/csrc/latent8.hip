@@ -243,14 +243,24 @@ constexpr int kLoads = kKeys * kRowChunks / (kAttnThreads / 2);  // of a thread 
 constexpr int kPStride = kKeys + 8;  // fp16 row of P in LDS: 144 bytes
 constexpr float kNoMax = -3.0e38f;
 constexpr float kUnseen = 1.0e30f;
-constexpr float kMost = 15.f;   // scores pass a row's reference by this at most (base 2): P <= 2^15 fits fp16
+// P is fp16: each off by at most 2^-11 of itself, beside outputs of 8 or 11 bits;
+// the normaliser is summed in fp32 from values that are not rounded.  Where
+// scores set a row's reference anew its largest P is 2^kRise, and it may grow to
+// 2^kMost before the next time: keys down to 2^-22 of the largest p * c keep all
+// bits, and smaller ones are off by 2^-33 of it, so that a page of a large scale
+// that holds the maximum leaves the others theirs (a reference at the maximum
+// itself had them off by 2^-25).  Every bit more makes tiles be weighed again
+// more often: 24 lists of 2,048 take 31.1 us with 2^8 and 31.9 with 2^9, 24 x
+// 8,192 tokens 43.8 and 44.4; at the maximum itself 30.9 and 43.2.
+constexpr float kRise = 8.f;
+constexpr float kMost = 15.9f;
 // A tile is weighed again where its largest P passes 2^kMost, or where p, P times
 // 2^up, might leave fp32's range: with a largest P of 2^top, where top passes
-// kMostSum - 4 up.  Up to up = 20 that is kMost; p stays below 2^35 of its
+// kMostSum - 4 up.  Up to up = 20 that is kMost; p stays below 2^36 of its
 // reference, and a P below 2^-126, which becomes zero, counts only where up
 // passes 55, that is where any top from -126 on passes the limit.  (A list's p
 // are exponentials of their own and may pass their reference by 2^kMostSum.)
-constexpr float kMostSum = 95.f;
+constexpr float kMostSum = 95.9f;
 constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
 constexpr float kJoinCost = 0.0375f;  // what joining one part more costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
@@ -891,8 +901,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     auto weigh_again = [&](int tile) {
       const float2 old = *my_row_ref;
       const bool unseen = old.x == kUnseen;
-      const float most = most_of(row_max[grp][tile & 1][l32]);
-      const float most_sum = LIST ? most_of(row_top[LIST ? grp : 0][tile & 1][l32]) : most - page_before.log2c;
+      const float most = most_of(row_max[grp][tile & 1][l32]) - kRise;
+      const float most_sum = LIST ? most_of(row_top[LIST ? grp : 0][tile & 1][l32]) : most + (kRise - page_before.log2c);
       const bool past = most > (unseen ? -INFINITY : ref), past_sum = most_sum > (unseen ? -INFINITY : old.y);
       const float down = past ? ref - most : 0.f;
       const float grow = unseen ? 1.f : __builtin_amdgcn_exp2f(down);

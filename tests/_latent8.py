@@ -114,7 +114,7 @@ def wide_attention(qr, q, ends, c, topk=None):
                 reach[start + i, mine] = (x.abs() @ y.abs().T).amax(-1) * SCALE
                 weight = p * scale[at, g]
                 top = weight.amax(-1, keepdim=True)
-                tail[start + i, mine] = torch.where(weight < top * 2.0 ** -14, top * 2.0 ** -25, 0.0) @ codes[at, g, :512].abs()
+                tail[start + i, mine] = torch.where(weight < top * 2.0 ** -22, top * 2.0 ** -33, 0.0) @ codes[at, g, :512].abs()
                 if topk is None:
                     sums[b, at] += p.sum(0)
         start = end
@@ -126,9 +126,9 @@ def wide_bound(out, size, reach, tail, dtype, keys: int):
     :func:`attention_bound`, but exponents hold the logarithms of the scales
     (below 2^9 with the scores of these tests): each of the eight sums that an
     exponent passes through rounds by 2^-16, times ln 2 below 2^-13 together.
-    A row's largest P is at least 1, so that those from 2^-14 of the largest
+    A row's largest P is at least 2^8, so that those from 2^-22 of the largest
     p times scale on lie in fp16's normal range (2^-14); one below is off by
-    2^-25 of the largest p times scale, times its key's code.  A
+    2^-25, which is 2^-33 of the largest p times scale, times its key's code.  A
     subnormal output rounds by half of its type's step."""
     score = reach * (578 * 2.0 ** -24 + 2.0 ** -22)
     per = 2.0 ** -11 + keys * 2.0 ** -23 + 2 * score + 2.0 ** -21 + 2.0 ** -13

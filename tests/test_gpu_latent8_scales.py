@@ -1,5 +1,6 @@
 """The 8-bit latent cache's attention where pages' scales are far apart: pages
-of zero rows as the append writes them (scale 2^-126), tiny and huge scales."""
+of zero rows as the append writes them (scale 2^-126), tiny and huge scales,
+and a page that holds a row's maximum at a larger scale than the others."""
 
 from __future__ import annotations
 
@@ -125,6 +126,40 @@ def test_scales_of_every_magnitude(exponents):
     q.zero_()
     _attend(c, qr, q, ends)
     _attend(c, qr, q, ends, _lists(c, 4, 150, 5))
+
+
+def _sink(length, where, ratio, lead, seed):
+    """Nearly equal keys of positive values at scale 2^-6, and in page `where`,
+    whose scale is 2^ratio larger, one key with 2^lead times their weight and
+    values in the first 256 dims only."""
+    c = make_cache([length], 1, seed=seed, exponents=(-6, -5))
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.rand(c["cache"].shape, generator=g) * 6 + 1
+    codes[..., 512:] = 0
+    codes[..., 513] = torch.randn(codes.shape[:-1], generator=g) * 4
+    page = int(c["table"][0, where])
+    codes[page] = 0
+    codes[page, 60, :, :256], codes[page, 60, :, 512] = 3.0, 64.0
+    c["cache"] = codes.to(torch.float8_e4m3fn)
+    c["scale"][page] = 2.0 ** (ratio - 6)
+    heads = 4
+    q = torch.zeros(1, heads, 512, dtype=torch.float16)
+    qr = torch.zeros(1, heads, 64, dtype=torch.float16)
+    qr[..., 0] = lead * math.log(2) / (64 * 2.0 ** (ratio - 6) * SCALE)
+    qr[..., 1] = torch.tensor([0.0, 0.3, 0.01, 1.0]) / (4 * 2.0 ** -6 * SCALE)
+    return c, qr, q
+
+
+@pytest.mark.parametrize("ratio,lead", [(10, 14), (12, 14), (8, 14), (12, 6), (0, 14)])
+@pytest.mark.parametrize("where", [0, 100, 250])
+def test_maximum_in_a_page_of_a_larger_scale(ratio, lead, where):
+    print(f"SINK ratio={ratio} lead={lead} where={where}", flush=True)
+    c, qr, q = _sink(32600, where, ratio, lead, 13)
+    _attend(c, qr, q, i32([1]))
+    g = torch.Generator().manual_seed(14)
+    topk = torch.randperm(32600, generator=g)[:1500].to(torch.int32)[None].contiguous()
+    topk[0, 700] = where * PAGE + 60
+    _attend(c, qr, q, i32([1]), topk)
 
 
 def test_no_tile_is_left_out():
