@@ -135,13 +135,11 @@ def _register() -> torch.library.Library:
 _LIBRARY = _register()
 
 
-def _call(name: str, cache: torch.Tensor, *args) -> None:
-    """The operator by its implementation where nothing traces the call (a
-    third of a small call's host time is the dispatch), else by its name."""
-    if type(cache) is torch.Tensor and cache.is_cuda and not torch.compiler.is_compiling():
-        IMPLS[name](*args)
-    else:
-        getattr(torch.ops.nanovllm_dsa, name).default(*args)
+# (By the dispatcher, which resolves negated views and hands the calls to whatever
+# traces or wraps tensors.)
+_append_op = torch.ops.nanovllm_dsa.latent8_append.default
+_attention_op = torch.ops.nanovllm_dsa.latent8_attention.default
+_evict_op = torch.ops.nanovllm_dsa.latent8_evict.default
 
 
 def latent8_append(kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache, cache_scale,
@@ -156,8 +154,8 @@ def latent8_append(kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, 
     larger one.  Infinities and NaN are stored as NaN.  With token records, the
     new slots' positions are noted (``positions`` [T]) and their weights set to
     0."""
-    _call("latent8_append", latent_cache, kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
-          latent_cache, cache_scale, positions, req_pool_entries, token_positions, token_weights)
+    _append_op(kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache, cache_scale,
+               positions, req_pool_entries, token_positions, token_weights)
 
 
 def latent8_attention(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache,
@@ -173,9 +171,8 @@ def latent8_attention(query_rope, query, actual_seq_lengths_query, actual_seq_le
     With ``token_weights`` (and ``req_pool_entries``; not with a list) the
     attention weight of every slot, summed over the request's rows and heads,
     is added to its record."""
-    _call("latent8_attention", latent_cache, query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv,
-          block_table, latent_cache, cache_scale, float(scale_value), attention_out, topk_ids, req_pool_entries,
-          token_weights)
+    _attention_op(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache,
+                  cache_scale, float(scale_value), attention_out, topk_ids, req_pool_entries, token_weights)
 
 
 def latent8_evict(actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache, cache_scale,
@@ -194,9 +191,9 @@ def latent8_evict(actual_seq_lengths_kv, budgets, block_table, req_pool_entries,
     [B] list the moves, for other caches that follow the same slots, and
     ``kept_lengths`` [B] receives the new lengths (it may be
     ``actual_seq_lengths_kv`` itself)."""
-    _call("latent8_evict", latent_cache, actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache,
-          cache_scale, token_positions, token_weights, move_src_slots, move_dst_slots, move_counts, kept_lengths,
-          int(protect_first), int(protect_last))
+    _evict_op(actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache, cache_scale,
+              token_positions, token_weights, move_src_slots, move_dst_slots, move_counts, kept_lengths,
+              int(protect_first), int(protect_last))
 
 
 __all__ = ["LATENT_ROW", "empty_latent_cache", "latent8_append", "latent8_attention", "latent8_evict"]
