@@ -43,6 +43,7 @@ from __future__ import annotations
 from contextlib import nullcontext
 
 import torch
+from torch.autograd.graph import increment_version  # what torch's own in-place operators do to their outputs
 
 from . import BLOCK_SIZE, CKV_DIM, KPE_DIM, _lib
 from .ops import _C, _L, _pack, _stream_of, _workspace
@@ -83,12 +84,19 @@ def _device_of(t: torch.Tensor):
     return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _written(*outputs) -> None:
+    """Outputs count as written for autograd: a backward pass through values
+    that a call overwrote is refused."""
+    increment_version([t for t in outputs if t is not None])
+
+
 def _append(kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache, cache_scale,
             positions=None, req_pool_entries=None, token_positions=None, token_weights=None) -> None:
     buf, at = _pack(kv, k_rope, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache, cache_scale,
                     positions, req_pool_entries, token_positions, token_weights)
     with _device_of(latent_cache):
         _lib.check(_C.nvdsa_latent8_append(*at, _stream_of(latent_cache)))
+    _written(latent_cache, cache_scale, token_positions, token_weights)
 
 
 def _attention(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, latent_cache,
@@ -101,6 +109,7 @@ def _attention(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_k
     with _device_of(latent_cache):
         _lib.check(_C.nvdsa_latent8_attention(*at[:-1], float(scale_value), at[-1], ws.data_ptr(), ws.numel(),
                                               _stream_of(latent_cache)))
+    _written(attention_out, token_weights)
 
 
 def _evict(actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache, cache_scale, token_positions,
@@ -114,6 +123,8 @@ def _evict(actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent
     with _device_of(latent_cache):
         _lib.check(_C.nvdsa_latent8_evict(*at[:8], int(protect_first), int(protect_last), *at[8:], ws.data_ptr(),
                                           ws.numel(), _stream_of(latent_cache)))
+    _written(latent_cache, cache_scale, token_positions, token_weights, move_src_slots, move_dst_slots, move_counts,
+             kept_lengths)
 
 
 IMPLS = {"latent8_append": _append, "latent8_attention": _attention, "latent8_evict": _evict}

@@ -299,3 +299,49 @@ def test_oracle_evict_keeps_the_heaviest():
     best = sorted(free, key=lambda t: -float(w0[1, t]))[:188]
     assert survivors == sorted([0, 1, *best, *range(290, 300)])
     assert not same_codes(rows0, c["cache"])
+
+
+def test_outputs_count_as_written(monkeypatch):
+    """Autograd refuses a backward pass through values that a call overwrote,
+    and only outputs count as written."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+
+    from nanovllm_amd import latent_cache as L
+
+    calls = {f"nvdsa_latent8_{n}": lambda *a: 0 for n in ("append", "attention", "evict")}
+    monkeypatch.setattr(L, "_C", SimpleNamespace(**calls))
+    monkeypatch.setattr(L, "_device_of", lambda t: nullcontext())
+    monkeypatch.setattr(L, "_stream_of", lambda t: 0)
+    cache, scale = L.empty_latent_cache(3, 1, "cpu")
+    f16 = lambda *shape: torch.zeros(*shape, dtype=torch.float16)  # noqa: E731
+    t = {"kv": f16(2, 1, 512), "rope": f16(2, 1, 64), "ends": i32([2]), "lens": i32([2]), "table": i32([[0, 1]]),
+         "cache": cache, "scale": scale, "row_pos": i32([0, 1]), "entries": i32([0]),
+         "positions": torch.zeros(1, 256, dtype=torch.int32), "weights": torch.zeros(1, 256), "q": f16(2, 4, 512),
+         "qr": f16(2, 4, 64), "out": f16(2, 4, 512), "budgets": i32([1]), "src": torch.zeros(1, 256, dtype=torch.int32),
+         "dst": torch.zeros(1, 256, dtype=torch.int32), "counts": i32([0]), "kept": i32([0])}
+    factor = torch.ones_like(t["out"], requires_grad=True)
+    loss = (t["out"] * factor).sum()
+
+    def written(call):
+        before = {k: v._version for k, v in t.items()}
+        call()
+        return {k for k, v in t.items() if v._version > before[k]}
+
+    a = [t[k] for k in ("kv", "rope", "ends", "lens", "table", "cache", "scale")]
+    assert written(lambda: L._append(*a)) == {"cache", "scale"}
+    records = [t[k] for k in ("row_pos", "entries", "positions", "weights")]
+    assert written(lambda: L._append(*a, *records)) == {"cache", "scale", "positions", "weights"}
+    a = [t[k] for k in ("qr", "q", "ends", "lens", "table", "cache", "scale")]
+    assert written(lambda: L._attention(*a, 0.1, t["out"])) == {"out"}
+    assert written(lambda: L._attention(*a, 0.1, t["out"], None, t["entries"], t["weights"])) == {"out", "weights"}
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    a = [t[k] for k in ("lens", "budgets", "table", "entries", "cache", "scale", "positions", "weights", "src", "dst",
+                        "counts", "kept")]
+    assert written(lambda: L._evict(*a, 0, 0)) == {"cache", "scale", "positions", "weights", "src", "dst", "counts", "kept"}
+    with torch.inference_mode():
+        t["out"] = f16(2, 4, 512)
+        a = [t[k] for k in ("qr", "q", "ends", "lens", "table", "cache", "scale")]
+        L._attention(*a, 0.1, t["out"])  # (no counter to raise)
+    L._attention(*a, 0.1, t["out"])
