@@ -78,8 +78,10 @@ int nvdsa_stage_inputs(const nvdsa_stage_item* items, int64_t count, void* strea
  * Query / new rows are packed: request b's are
  * [actual_seq_lengths_query[b-1], actual_seq_lengths_query[b]), and
  * actual_seq_lengths_kv[b] counts its cached tokens with the new ones.  Ends
- * must not decrease (rows that two requests share hold either's result).  Rows
- * behind the last request are neither read nor written.  No counterpart in
+ * must not decrease: rows that two requests share hold either's result, their
+ * requests' token weights go by that, and where the rows' work counts more than
+ * once the call may leave rows and records as they were.  Rows behind the last
+ * request are neither read nor written.  No counterpart in
  * the reference, whose caches are 16-bit. */
 
 /* New row i of n goes to slot actual_seq_lengths_kv[b] - n + i.  A page's

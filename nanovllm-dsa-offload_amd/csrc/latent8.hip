@@ -546,6 +546,7 @@ struct Work {
   float* part;      // [2 parts][64 * 512], in the accumulators' order
   float4* refs;     // [2 parts][64]: reference of the sums, of the normaliser, the normaliser
   JoinEntry* join;  // [parts], of an item each or named by a part; row0 < 0: nothing
+  int32_t* idle;    // [1]: the attention did nothing (ends that decrease)
   float* lse;       // [rows, heads], base 2 (with weights)
 };
 constexpr size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -558,6 +559,8 @@ __host__ __device__ inline Work carve_work(void* ws, int64_t parts) {
   p += sizeof(float4) * 2 * parts * kRows;
   w.join = reinterpret_cast<JoinEntry*>(p);
   p += round256(sizeof(JoinEntry) * parts);
+  w.idle = reinterpret_cast<int32_t*>(p);
+  p += round256(sizeof(int32_t));
   w.lse = reinterpret_cast<float*>(p);
   return w;
 }
@@ -715,6 +718,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
   // Entries that no item writes below: all of the parts', or those behind the
   // last item's.  (More items than entries: ends that decrease.)
   const bool many = a.join_items && start.items > a.joins;
+  if (tid == 0 && part == 0) *work.idle = many || start.items > kMostItems;
   if (tid == 0)
     for (int64_t k = a.join_items && !many ? start.items + part : part; k < a.joins; k += a.parts) work.join[k].row0 = -1;
   if (many || part >= start.plan.parts || start.b < 0) return;
@@ -1330,13 +1334,14 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
   const int l32 = lane & 31;
   const int hh = lane >> 5;
   const Work work = carve_work(a.workspace, a.parts);
+  const int32_t idle = *work.idle;  // (then nobody wrote the log-sums)
   const int per = a.per;
   const int64_t row_bytes = a.latent_heads * kRow;
   auto slices = [](const Request& r) -> int { return r.n > 0 ? (r.len + kSumKeys - 1) / kSumKeys : 0; };
   const Start start = find_start<kSumThreads, kSumBegin, false>(
       a, ends_of(a, tid < a.batch ? tid : 0), blockIdx.x, kSumParts, 0,
       [&](const Request& r) -> int64_t { return slices(r) > 0; }, slices);
-  if (static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
+  if (idle != 0 || static_cast<int64_t>(blockIdx.x) >= start.plan.parts || start.b < 0) return;
   const int64_t stop = part_start(start.plan, blockIdx.x + 1);
   int64_t b = start.b, base = start.base;
   Request r = start.r;
@@ -1897,6 +1902,7 @@ int64_t latent8_items(int64_t rows, int64_t heads, int64_t latent_heads, int64_t
 
 size_t latent8_attention_workspace_bytes(int64_t rows, int64_t heads, bool weights) {
   return sizeof(float) * 2 * kParts * (kPartFloats + kRows * 4) + round256(sizeof(JoinEntry) * kParts) +
+         round256(sizeof(int32_t)) +
          (weights ? sizeof(float) * rows * heads : 0);
 }
 

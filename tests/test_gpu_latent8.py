@@ -329,6 +329,23 @@ def test_attention_many_long_requests():
     assert (after[:, length:] == 0).all()
 
 
+def test_attention_with_ends_that_decrease():
+    """More items than the rows can have: nothing is done, to the records
+    neither (the workspace holds what another call left there)."""
+    c = make_cache([90, 40, 130, 60, 128], 1, seed=29)
+    qr, q, _ = queries([130], 1, torch.bfloat16, 29)
+    before = torch.rand(5, c["cols"] * PAGE)
+    from nanovllm_amd import _lib
+
+    size = _lib.lib.nvdsa_latent8_attention_workspace_size(130, 1, 1)
+    torch.cuda.empty_cache()
+    torch.zeros(size, dtype=torch.uint8, device="cuda")
+    print("ATTENTION decreasing ends", flush=True)
+    out, after = _run_attention(c, qr, q, i32([130, 1, 130, 1, 130]), entries=torch.arange(5, dtype=torch.int32),
+                                weights=before)
+    assert (out == 7.0).all() and torch.equal(after, before)
+
+
 def test_attention_list_of_many_windows():
     """Parts of a list that are longer than the entries resolved at a time."""
     lengths = [700 - 3 * i for i in range(60)]
