@@ -1217,12 +1217,17 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 // of the partials depend on nothing.  Entries belong to items where these are no
 // more than the parts, so that few blocks find nothing to do; y counts fastest,
 // so that each item's blocks lie on all XCDs.  Bound by the partials' bytes and
-// the launch: 24 items over 256 parts, 34 MB, in 9.5 us (30 with the entries of
+// the launch: 24 items over 256 parts, 34 MB, in 9 us (30 with the entries of
 // parts, counting fastest).  Where few items have many parts, four groups of
-// waves take every fourth part each, and their sums meet in LDS: one item's 256
-// parts in 20 us instead of 40, but 80 items' in 16 instead of 9.5.
+// waves take every fourth part each, and their sums meet in LDS.  us with four
+// groups / one:
+//
+//     items       1          2         4         8        12        16        24        80
+//   32,768   11.8/21.6  11.1/20.5  9.2/12.0  9.6/10.4  11.1/8.7  11.9/9.1  14.2/8.7  34.5/11.9
+//    8,192    8.2/12.2   6.9/10.0  7.7/10.2   7.8/8.2  10.8/8.1  10.8/8.2  13.0/7.6  31.5/10.6
+//    2,048     6.4/8.2    5.4/4.7   5.8/5.1   6.7/6.2  10.6/7.2   9.7/6.6  12.1/6.6   31.1/8.8
 constexpr int kJoinGroups = 4;
-constexpr int kFewJoins = 16;
+constexpr int kFewJoins = 8;
 constexpr int kJoinBlocks = 32;
 constexpr int kJoinParts = 64;  // parts whose factors are held at a time
 template <typename T, int GROUPS>
