@@ -250,17 +250,24 @@ constexpr float kUnseen = 1.0e30f;
 // bits, and smaller ones are off by 2^-33 of it, so that a page of a large scale
 // that holds the maximum leaves the others theirs (a reference at the maximum
 // itself had them off by 2^-25).  Every bit more makes tiles be weighed again
-// more often: 24 lists of 2,048 take 31.1 us with 2^8 and 31.9 with 2^9, 24 x
-// 8,192 tokens 43.8 and 44.4; at the maximum itself 30.9 and 43.2.
+// more often: calls of 24 x 8,192 tokens with weights take 84.2 us with 2^8 and
+// 83.6 with the maximum itself, of 16 x 4 rows over up to 16,387 130.1 and 129.0.
+// fp16 outputs are 2.5e-4 (relative, all together) from the 64-bit ones, with a
+// P of 32 bits 2.1e-4; bf16 outputs 1.7e-3 either way.  A second fp16 for what P's
+// first leaves would add 16 products to a tile's 34.
 constexpr float kRise = 8.f;
 constexpr float kMost = 15.9f;
 // A tile is weighed again where its largest P passes 2^kMost, or where p, P times
 // 2^up, might leave fp32's range: with a largest P of 2^top, where top passes
 // kMostSum - 4 up.  Up to up = 20 that is kMost; p stays below 2^36 of its
 // reference, and a P below 2^-126, which becomes zero, counts only where up
-// passes 55, that is where any top from -126 on passes the limit.  (A list's p
-// are exponentials of their own and may pass their reference by 2^kMostSum.)
+// passes 55, that is where any top from -126 on passes the limit.  In a list,
+// where keys have scales of their own, up is that of the least one, and 1 / c and
+// 2^lift, which multiply P one after the other, have to be in range too.
 constexpr float kMostSum = 95.9f;
+constexpr float kMostUp = 55.f;
+constexpr float kLeast = -60.f;    // log2 of a list's scales
+constexpr float kMostLift = 100.f;
 constexpr int kBegin = 6;       // what the start of a segment costs, in tiles
 constexpr float kJoinCost = 0.0375f;  // what joining one part more costs, in tiles
 constexpr int64_t kParts = 256; // one workgroup per CU (LDS)
@@ -599,6 +606,7 @@ struct alignas(16) Window {
   int32_t row;    // first cache row of the page, or the entry's row; -1: none
   float score;    // softmax scale * log2(e) * c
   float log2c;
+  float inverse;  // 1 / c (of a list's entry)
 };
 __device__ inline int32_t row_of_slot(const Latent8Args& a, int64_t b, int64_t slot, bool ok) {
   if (!ok) return -1;
@@ -613,6 +621,7 @@ __device__ inline void add_scale(const Latent8Args& a, int g, Window& w) {  // t
   w.score = a.scale * kLog2e * c;
   const float exponent = static_cast<float>(static_cast<int>(u >> 23) - 127);
   w.log2c = exponent + __builtin_amdgcn_logf(__uint_as_float((u & 0x7fffffu) | 0x3f800000u));
+  w.inverse = 1.f / c;
 }
 
 // base * 2^x / l where l > 0, else 0: in two factors, since 2^x alone may pass
@@ -815,7 +824,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     // one after them, in scalar registers.
     Window page_before{}, page_now{}, page_next{}, page_far{};
     auto scalar = [&](const Window& v) {
-      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.log2c)};
+      return Window{__builtin_amdgcn_readfirstlane(v.row), first_lane(v.score), first_lane(v.log2c), 0.f};
     };
     // A tile's loads, by the waves of group 1, issued a few at a time.
     struct TileLoad {
@@ -876,11 +885,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       return (tile + 1) * kKeys > vis_least || page_before.row < 0;
     };
     // P of the tile's scores against the row's reference, into LDS; l_tile: the
-    // sum of p.  Where the tile has one scale, p is P times 2^(lift - log2c), as
-    // long as the row's limit keeps that in range (see below); ALONE: by
-    // exponents of its own.
+    // sum of p, which is P times 2^(lift - log2c) as long as the row's limit keeps
+    // that in range; ALONE: by exponents of its own.
     auto weigh = [&](const Window(&w)[LIST ? 8 : 1], float lift, auto alone) {
-      constexpr bool ALONE = LIST || decltype(alone)::value;
+      constexpr bool ALONE = decltype(alone)::value;
       l_tile = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -888,12 +896,13 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           pw[k] = __builtin_amdgcn_exp2f(sc[4 * e + k]);
-          l_tile += ALONE ? __builtin_amdgcn_exp2f(sc[4 * e + k] + (lift - w[LIST ? 4 * e + k : 0].log2c)) : pw[k];
+          l_tile += ALONE ? __builtin_amdgcn_exp2f(sc[4 * e + k] + (lift - w[LIST ? 4 * e + k : 0].log2c))
+                          : (LIST ? pw[k] * w[LIST ? 4 * e + k : 0].inverse : pw[k]);
         }
         const uint2 packed = make_uint2(F16::pack2(pw[0], pw[1]), F16::pack2(pw[2], pw[3]));
         *reinterpret_cast<uint2*>(&p_mine[l32 * kPStride + key_mine + 8 * e]) = packed;
       }
-      if (!ALONE) l_tile *= __builtin_amdgcn_exp2f(fminf(lift - w[0].log2c, 100.f));
+      if (!ALONE) l_tile *= __builtin_amdgcn_exp2f(fminf(LIST ? lift : lift - w[0].log2c, kMostLift));
     };
     auto most_of = [&](const float(&of)[4]) {
       const float4 v = *reinterpret_cast<const float4*>(of);
@@ -922,7 +931,22 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       Window w[LIST ? 8 : 1];
       fields(tile, w);
       const float lift = unseen && !past ? kUnseen : ref - sum_ref;
-      weigh(w, lift, std::true_type{});
+      // (Exponents of their own for a list only where they have to be: they are
+      // most of what 24 lists of 2,048 gain, 39.5 -> 38.4 us; without a list they
+      // cost nothing.)
+      if (LIST) {
+        weigh(w, lift, std::false_type{});
+        float low = w[0].log2c;
+#pragma unroll
+        for (int e = 1; e < 8; ++e) low = fminf(low, w[LIST ? e : 0].log2c);
+        if (__any(low < kLeast || lift > kMostLift || lift - low > kMostUp)) {
+          l_tile = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) l_tile += __builtin_amdgcn_exp2f(sc[e] + (lift - w[LIST ? e : 0].log2c));
+        }
+      } else {
+        weigh(w, lift, std::true_type{});
+      }
       return make_float2(lift, sum_ref);
     };
     // S^T of tile t in nine steps of 32 dims, and O^T of tile t - 1 in eight
@@ -1025,11 +1049,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
         // once do not fit the registers.)
         if (LIST && grp == 1) load = begin_load(t + 2, to, 0);
         issue_load(load, LIST ? 0 : 3, 6);
-        float top = sc[0], top_sum = sc[0] - w[0].log2c;
+        float top = sc[0], top_sum = sc[0] - w[0].log2c, low = w[0].log2c;
 #pragma unroll
         for (int e = 1; e < 8; ++e) {
           top = fmaxf(top, sc[e]);
           if (LIST) top_sum = fmaxf(top_sum, sc[e] - w[LIST ? e : 0].log2c);
+          if (LIST) low = fminf(low, w[LIST ? e : 0].log2c);
         }
         top = xor32_op(top, MaxOp{});
         if (LIST) top_sum = xor32_op(top_sum, MaxOp{});
@@ -1037,8 +1062,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
           row_max[grp][t & 1][l32][wg] = top + ref;
           if (LIST) row_top[LIST ? grp : 0][t & 1][l32][wg] = top_sum + ref;
         }
-        const float limit = fminf(kMost, kMostSum - 4.f * (lift - w[0].log2c));
-        const bool past_most = LIST ? top > kMost || top_sum + lift > kMostSum : top > limit;
+        float limit = fminf(kMost, kMostSum - 4.f * (lift - low));
+        if (LIST) limit = low < kLeast || lift > kMostLift ? -kUnseen : limit;
+        const bool past_most = top > limit;
         if (__any(past_most) && lane == 0) outgrown[grp][t & 1] = 1;
         __builtin_amdgcn_sched_barrier(0);
         issue_load(load, 6, kLoads);
@@ -1124,9 +1150,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       lds_barrier();  // the tiles before are done with LDS
       if (!LIST) c1 = t1 - (c0 & ~1) < kWindowTiles ? t1 : (c0 & ~1) + kWindowTiles;
       w0 = LIST ? c0 : c0 & ~1;
+      if (tid < kRows && c0 == t0) row_ref[tid >> 5][tid & 31] = make_float2(kUnseen, kNoMax);
       window_rows(w0);
       if (tid < 4) outgrown[tid >> 1][tid & 1] = 0;
-      if (tid < kRows && c0 == t0) row_ref[tid >> 5][tid & 31] = make_float2(kUnseen, kNoMax);
       lds_barrier();
       buf = 0;
       before = 2;
@@ -1152,6 +1178,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
     if (hh == 0) row_max[grp][0][l32][wg] = l_run;
     lds_barrier();
     float l_all;
+    const float2 refs = *my_row_ref;
     {
       const float4 v = *reinterpret_cast<const float4*>(row_max[grp][0][l32]);
       l_all = (v.x + v.y) + (v.z + v.w);
@@ -1162,7 +1189,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
       if (m_mine < x.count) {
         const int f = x.first + m_mine, i = f / per, h = f - i * per;
         const int64_t row = (r.row0 + i) * a.heads + x.g * per + h;
-        const Quotient by(my_row_ref->x, l_all);
+        const Quotient by(refs.x, l_all);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -1173,7 +1200,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
             *reinterpret_cast<uint2*>(&out[row * kCkvDim + d]) = u;
           }
         if (a.token_weights != nullptr && wg == 0 && hh == 0)
-          work.lse[row] = l_all == 0.f ? -INFINITY : my_row_ref->y + __builtin_amdgcn_logf(l_all);
+          work.lse[row] = l_all == 0.f ? -INFINITY : refs.y + __builtin_amdgcn_logf(l_all);
       }
       if (a.join_items && tid == 0) work.join[item_base + it].row0 = -1;
     } else {
@@ -1189,11 +1216,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void latent8_attention_kernel(Late
             p[((wave * 4 + dt) * 4 + e) * 64 + lane] =
                 make_float4(o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]);
       }
-      if (wg == 0 && hh == 0) {
-        const float2 mine = *my_row_ref;
-        work.refs[slot * kRows + m_mine] = make_float4(empty ? -INFINITY : (mine.x == kUnseen ? kNoMax : ref),
-                                                       empty ? -INFINITY : mine.y, l_all, 0.f);
-      }
+      if (wg == 0 && hh == 0)
+        work.refs[slot * kRows + m_mine] = make_float4(empty ? -INFINITY : (refs.x == kUnseen ? kNoMax : ref),
+                                                       empty ? -INFINITY : refs.y, l_all, 0.f);
       // The first border of parts inside an item names it to the joining kernel.
       if (first_seg && at > item_start && tid == 0 && part_start(start.plan, part - 1) <= item_start) {
         JoinEntry j;

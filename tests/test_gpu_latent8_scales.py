@@ -114,7 +114,7 @@ def test_parts_that_begin_in_zero_pages():
     _attend(c, qr, q, ends, _lists(c, 60, 700, 4))
 
 
-@pytest.mark.parametrize("exponents", [(-126, -119), (-110, -100), (60, 80), (-126, 40), (-60, 10)])
+@pytest.mark.parametrize("exponents", [(-126, -119), (-110, -100), (-63, -57), (60, 80), (105, 112), (-126, 40), (-60, 10)])
 def test_scales_of_every_magnitude(exponents):
     """Equal and unequal scores at scales of a caller's own.  Scores stay near
     zero, whatever the scale: the queries see rope codes that are zero at all
