@@ -132,12 +132,16 @@ int nvdsa_latent8_attention(const nvdsa_tensor* query_rope,
 /* Brings every request with more than budgets[b] cached tokens down to that
  * many.  Kept are tokens at a position below protect_first or among the
  * protect_last latest positions, then those of the largest weight (NaN above
- * all), ties to the lower slot.  The kept tokens at slots >= budget move, in
- * order, into the slots below it that were given up: their rows (to the
+ * all), ties to the lower slot; where more are protected than the budget holds,
+ * those at the lower slots stay (of a request that nothing was evicted from, the
+ * earliest: a budget below protect_first + protect_last gives up latest ones).
+ * The kept tokens at slots >= budget move, in order, into the slots below it that were given up: their rows (to the
  * larger of the pages' scales), positions and weights.  move_src_slots /
  * move_dst_slots [B, cols * 128] list the moves (entries past move_counts[b]
  * are left as they were), kept_lengths[b] is the new length.  A request whose
- * pool entry names no row is left alone. */
+ * pool entry names no row is left alone.  Of tokens whose page, or whose new
+ * slot's page, names no block the records move but no rows, so the pages of a
+ * request over its budget should all be there. */
 size_t nvdsa_latent8_evict_workspace_size(int64_t batch, int64_t table_cols, int64_t latent_heads);
 int nvdsa_latent8_evict(const nvdsa_tensor* actual_seq_lengths_kv,
                         const nvdsa_tensor* budgets,

@@ -659,9 +659,9 @@ struct Quotient {
 // group's softmax, group 1's softmax with the loads 1,500.  In the loop that is
 // 1.0 PFLOP/s, of the 1.27 that a large product reaches.  A part's start (10
 // us) and its partial sums (3 us) come to that: 24 requests of 32,768 tokens
-// and 64 heads in 145 us (110 GFLOP, 453 MB), 40 ragged ones with 8 heads in
+// and 64 heads in 138 us (110 GFLOP, 453 MB), 40 ragged ones with 8 heads in
 // 99 us (4.8 TB/s), 2 x 515 rows over up to 8,197 tokens, 2 x 16 heads, in
-// 455 us.  One phase for all waves took 175, 166 and 565.  Weighed against it:
+// 454 us.  One phase for all waves took 175, 166 and 565.  Weighed against it:
 // the same products on the 8-bit MFMAs, with bf16 queries split into two codes
 // and P into three, took 164 us for the first and twice as long for lists.
 template <typename T, bool LIST>
@@ -1554,7 +1554,8 @@ __global__ __launch_bounds__(kSumThreads, 2) void latent8_weights_kernel(Latent8
 // themselves 1 x 2,176 slots take 10 us, 48 x 8,320 17 us and 16 x 32,768 29 us,
 // against 13, 32 and 97 with every pass reading them anew, and 10, 20 and 35
 // with lane masks in the one scalar unit of a CU.  About 6 us of it are the
-// digits' barriers and scans.
+// digits' barriers and scans.  Slots beyond the registers are read anew by every
+// pass: 4 x 65,536 take 71 us, 2 x 1,048,576 1.9 ms.
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kDigitBins = 2048;
@@ -1813,6 +1814,8 @@ __global__ __launch_bounds__(kEvictThreads) void latent8_select_kernel(Latent8Ev
 // Moves: one workgroup per (request, page that has holes).  Bound by the bytes
 // of the moved rows: 16 x 8,200 rows of 576, read and written once, in 28 us
 // (5.4 TB/s, part of it from cache).  With a load and a store in turn it took 51.
+// That is without pages that grow their scales, whose other rows are rounded
+// again with a load and a store in turn: where 748 of them do, 39 us.
 constexpr int kMoveThreads = 256;
 constexpr int kMovePages = 256;  // workgroups of a request at most
 constexpr int kMoveAhead = 6;  // chunks of a thread in flight

@@ -194,14 +194,18 @@ def latent8_evict(actual_seq_lengths_kv, budgets, block_table, req_pool_entries,
 
     Kept are the tokens at a position below ``protect_first`` or among the
     ``protect_last`` latest positions, then those of the largest weight, ties
-    to the lower slot.  The kept tokens at slots >= budget move, in order, into
-    the slots below it that were given up, with their positions and weights;
+    to the lower slot.  Where more tokens are protected than the budget holds,
+    those at the lower slots stay, which are the earliest of a request that
+    nothing was evicted from: budgets of at least ``protect_first +
+    protect_last`` keep every protected token.  The kept tokens at slots >=
+    budget move, in order, into the slots below it that were given up, with their positions and weights;
     the slots of a request are then in no order, which attention does not mind
     (rope is in the rows) as long as the next rows are appended behind them.
     ``move_src_slots`` / ``move_dst_slots`` [B, C * 128] and ``move_counts``
     [B] list the moves, for other caches that follow the same slots, and
     ``kept_lengths`` [B] receives the new lengths (it may be
-    ``actual_seq_lengths_kv`` itself)."""
+    ``actual_seq_lengths_kv`` itself).  Of tokens on pages that name no block
+    the records move but no rows."""
     _evict_op(actual_seq_lengths_kv, budgets, block_table, req_pool_entries, latent_cache, cache_scale,
               token_positions, token_weights, move_src_slots, move_dst_slots, move_counts, kept_lengths,
               int(protect_first), int(protect_last))
