@@ -91,3 +91,12 @@ def test_wrapped_tensors_do_not_reach_the_kernels():
 
         latent8_append(s["kv"], s["rope"], s["ends"], s["lens"], s["table"], s["cache"], s["scale"])
         assert torch.equal(before, s["cache"].view(torch.uint8))
+
+
+def test_compiled_calls_write_the_same():
+    plain, compiled = _state(), _state()
+    _calls(plain)
+    torch.compile(_calls, backend="aot_eager", fullgraph=True)(compiled)
+    assert same_codes(plain["cache"], compiled["cache"])
+    for k in ("out", "scale", "weights", "positions", "src", "dst", "counts", "kept"):
+        assert torch.equal(plain[k], compiled[k]), k
