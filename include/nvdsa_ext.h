@@ -160,6 +160,92 @@ int nvdsa_latent8_evict(const nvdsa_tensor* actual_seq_lengths_kv,
                         void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Many continuations of one prefix on the 16-bit latent cache (kv_cache
+ * [blocks, 128, 1, 512], k_rope [blocks, 128, 1, 64]); packed rows, ends,
+ * lengths and tables as above.  No counterpart in the reference. */
+
+/* The rows between the projections and the attention.  Row i of a request's n
+ * goes to slot actual_seq_lengths_kv[b] - n + i (skipped where that names no
+ * page):
+ *   kv_cache[slot] = kv[t, :512] * rsqrt(mean(kv[t, :512]^2) + eps) * kv_norm_weight
+ *   k_rope[slot]   = R_t kv[t, 512:]
+ *   query_rope[t]  = R_t query[t, :, D - 64:]
+ * and with query_norm_weight [D] and query_nope [T, N, D - 64] (both or
+ * neither), the heads' queries, all D dims of them, are normalised in the same
+ * way first and the other dims written to query_nope.  R_t turns pairs by
+ * cos / sin [T, 64 or more] as dsa_indexer_query_rope_inplace does.  fp32
+ * throughout, one rounding at the store.  query [T, N, D], 64 <= D <= 576; all
+ * of one 16-bit dtype.  Rows behind the last request are neither read nor
+ * written.  No workspace. */
+int nvdsa_norm_rope_append(const nvdsa_tensor* query,
+                           const nvdsa_tensor* kv,
+                           const nvdsa_tensor* cos,
+                           const nvdsa_tensor* sin,
+                           const nvdsa_tensor* kv_norm_weight,
+                           const nvdsa_tensor* actual_seq_lengths_query,
+                           const nvdsa_tensor* actual_seq_lengths_kv,
+                           const nvdsa_tensor* block_table,
+                           const nvdsa_tensor* k_rope,
+                           const nvdsa_tensor* kv_cache,
+                           const nvdsa_tensor* query_rope,
+                           const nvdsa_tensor* query_norm_weight,
+                           const nvdsa_tensor* query_nope,
+                           double eps,
+                           void* stream);
+
+/* Requests that go on from others, and the pages that they write to next.
+ * block_table entries that name no page are -1; page_refs[p] counts the rows
+ * that hold page p (and whoever else does), 0: free.
+ * With parents [B], row b first takes over what row parents[b] held before the
+ * call, table and length, and page_refs follow; a parent that names no row
+ * leaves it empty.  Then every row gets the pages that its next new_tokens[b]
+ * tokens fall into (those within the table): a new one where it has none, and
+ * where others hold its page too, except that a page with older rows stays with
+ * the lowest of the rows that write on where only these hold it.  New pages are
+ * the lowest free ones, given out by row and column.  copy_src / copy_dst /
+ * copy_tokens [B] say which rows the new page of a row has to receive (-1, -1,
+ * 0: none).  All rows are served or, where too few pages are free, none:
+ * missing[0] is the number that lacks, or 0. */
+size_t nvdsa_pages_branch_workspace_size(int64_t pages);
+int nvdsa_pages_branch(const nvdsa_tensor* seq_lens,
+                       const nvdsa_tensor* new_tokens,
+                       const nvdsa_tensor* block_table,
+                       const nvdsa_tensor* page_refs,
+                       const nvdsa_tensor* copy_src,
+                       const nvdsa_tensor* copy_dst,
+                       const nvdsa_tensor* copy_tokens,
+                       const nvdsa_tensor* missing,
+                       const nvdsa_tensor* parents,
+                       void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Brings the held pages together: with L of them, those at or behind L go, in
+ * ascending order, to the free ones below L.  Tables and page_refs follow;
+ * move_src / move_dst [pages] list the moves (entries past move_count[0] are
+ * left as they were). */
+size_t nvdsa_pages_compact_workspace_size(int64_t pages);
+int nvdsa_pages_compact(const nvdsa_tensor* block_table,
+                        const nvdsa_tensor* page_refs,
+                        const nvdsa_tensor* move_src,
+                        const nvdsa_tensor* move_dst,
+                        const nvdsa_tensor* move_count,
+                        void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Pages src_ids[k] to dst_ids[k] of up to 16 caches [pages, ...] (an array of
+ * descriptors).  With tokens [pairs], the first tokens[k] rows of caches
+ * [pages, 128, ...] and, where there are any, whole pages of others; with
+ * count [1], the first count[0] pairs.  Pairs that name no page are skipped.
+ * No page of a call may be a source and a destination, or a destination twice. */
+int nvdsa_pages_copy(const nvdsa_tensor* src_ids,
+                     const nvdsa_tensor* dst_ids,
+                     const nvdsa_tensor* caches,
+                     int64_t cache_count,
+                     const nvdsa_tensor* tokens,
+                     const nvdsa_tensor* count,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

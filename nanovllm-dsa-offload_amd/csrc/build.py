@@ -21,7 +21,7 @@ REPO = PKG_ROOT.parent
 BUILD_DIR = REPO / "_build" / "nvdsa"
 OUTPUT = PKG_ROOT / "nanovllm_amd" / "libnvdsa.so"
 SOURCES = ("scatter_copy.hip", "lim.hip", "sfa.hip", "indexer.hip", "persist.hip", "stage.hip", "latent8.hip",
-           "nvdsa_abi.hip")
+           "norm_rope.hip", "pages.hip", "nvdsa_abi.hip")
 ARCH = os.environ.get("NVDSA_OFFLOAD_ARCH", "gfx950")
 
 COMMON_FLAGS = [

@@ -188,7 +188,10 @@ const char* nvdsa_kernel_name(int32_t kernel_id) {
                                 "indexer_kw_kernel",   "indexer_kw_finish_kernel",
                                 "stage_inputs_kernel",  "latent8_append_kernel",
                                 "latent8_attention_kernel", "latent8_join_kernel",
-                                "latent8_weights_kernel", "latent8_select_kernel", "latent8_move_kernel"};
+                                "latent8_weights_kernel", "latent8_select_kernel", "latent8_move_kernel",
+                                "norm_rope_kernel",      "pages_take_kernel", "pages_reserve_kernel",
+                                "pages_count_kernel",    "pages_rank_kernel", "pages_rename_kernel",
+                                "pages_copy_kernel"};
   static_assert(sizeof(names) / sizeof(names[0]) == nvdsa::kKernCount, "one name per kernel id");
   if (kernel_id < 0 || kernel_id >= nvdsa::kKernCount) return "unknown";
   return names[kernel_id];
@@ -1533,6 +1536,256 @@ int nvdsa_latent8_evict(const nvdsa_tensor* actual_seq_lengths_kv, const nvdsa_t
   a.protect_last = protect_last;
   a.workspace = workspace;
   return launch_status(nvdsa::launch_latent8_evict(a, static_cast<hipStream_t>(stream)), "latent8_evict");
+}
+
+}  // extern "C"
+
+namespace {
+
+// The 16-bit latent cache and its page tables.
+void check_paged_cache(Check& c, const nvdsa_tensor* k_rope, const nvdsa_tensor* kv_cache,
+                       const nvdsa_tensor* block_table, int64_t batch) {
+  c.need(dims_are(kv_cache, 4) && sz(kv_cache, 0) > 0 && sz(kv_cache, 1) == 128 && sz(kv_cache, 2) == 1 &&
+             sz(kv_cache, 3) == nvdsa::kCkvDim,
+         NVDSA_ERR_SHAPE, "kv_cache must be [blocks, 128, 1, 512]")
+      .need(dims_are(k_rope, 4) && sz(k_rope, 0) == sz(kv_cache, 0) && sz(k_rope, 1) == 128 && sz(k_rope, 2) == 1 &&
+                sz(k_rope, 3) == nvdsa::kKpeDim,
+            NVDSA_ERR_SHAPE, "k_rope must be [blocks, 128, 1, 64] with kv_cache's blocks")
+      .need(sz(kv_cache, 0) < (int64_t{1} << 24), NVDSA_ERR_SHAPE, "kv_cache holds too many blocks")
+      .need(is_half(kv_cache) && kv_cache->dtype == k_rope->dtype, NVDSA_ERR_DTYPE,
+            "kv_cache and k_rope must share one 16-bit dtype")
+      .need(dims_are(block_table, 2) && sz(block_table, 0) == batch && sz(block_table, 1) > 0, NVDSA_ERR_SHAPE,
+            "block_table must be [B, columns]")
+      .need(sz(block_table, 1) <= (1 << 14), NVDSA_ERR_SHAPE, "block-table capacity must be <= 16384 blocks")
+      .need(block_table->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE, "block_table must be int32");
+}
+
+bool is_vector(const nvdsa_tensor* t, int64_t n) { return dims_are(t, 1) && sz(t, 0) == n; }
+
+// Tables and counts of the page operators.
+void check_pages(Check& c, const nvdsa_tensor* block_table, const nvdsa_tensor* page_refs) {
+  c.need(dims_are(block_table, 2) && sz(block_table, 1) > 0, NVDSA_ERR_SHAPE, "block_table must be [B, columns]")
+      .need(sz(block_table, 1) <= (1 << 14), NVDSA_ERR_SHAPE, "block-table capacity must be <= 16384 blocks")
+      .need(sz(block_table, 0) <= nvdsa::kMostBranchRows, NVDSA_ERR_SHAPE, "at most 16384 requests")
+      .need(dims_are(page_refs, 1) && sz(page_refs, 0) > 0 && sz(page_refs, 0) < (int64_t{1} << 24), NVDSA_ERR_SHAPE,
+            "page_refs must be [pages], fewer than 2^24")
+      .need(block_table->dtype == NVDSA_INT32 && page_refs->dtype == NVDSA_INT32, NVDSA_ERR_DTYPE,
+            "block_table and page_refs must be int32");
+}
+
+int64_t dtype_bytes(int32_t dtype) {
+  switch (dtype) {
+    case NVDSA_INT32:
+    case NVDSA_FLOAT32:
+      return 4;
+    case NVDSA_FLOAT16:
+    case NVDSA_BFLOAT16:
+      return 2;
+    case NVDSA_FLOAT8_E4M3:
+      return 1;
+    default:
+      return 0;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int nvdsa_norm_rope_append(const nvdsa_tensor* query, const nvdsa_tensor* kv, const nvdsa_tensor* cos,
+                           const nvdsa_tensor* sin, const nvdsa_tensor* kv_norm_weight,
+                           const nvdsa_tensor* actual_seq_lengths_query, const nvdsa_tensor* actual_seq_lengths_kv,
+                           const nvdsa_tensor* block_table, const nvdsa_tensor* k_rope, const nvdsa_tensor* kv_cache,
+                           const nvdsa_tensor* query_rope, const nvdsa_tensor* query_norm_weight,
+                           const nvdsa_tensor* query_nope, double eps, void* stream) {
+  const nvdsa_tensor* const all[] = {query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_query, actual_seq_lengths_kv,
+                                     block_table, k_rope, kv_cache, query_rope};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "norm_rope_append: null tensor argument");
+  Check c("norm_rope_append");
+  c.need((query_norm_weight != nullptr) == (query_nope != nullptr), NVDSA_ERR_ARG,
+         "query_norm_weight and query_nope go together")
+      .need(eps >= 0.0 && eps <= 1.0, NVDSA_ERR_ARG, "eps must be in [0, 1]")
+      .need(dims_are(actual_seq_lengths_query, 1) && sz(actual_seq_lengths_query, 0) < (1 << 16), NVDSA_ERR_SHAPE,
+            "actual_seq_lengths_query must be rank one, fewer than 65536");
+  const int64_t B = sz(actual_seq_lengths_query, 0);
+  if (c.ok()) check_paged_cache(c, k_rope, kv_cache, block_table, B);
+  if (c.ok()) {
+    const int64_t T = sz(query, 0), N = sz(query, 1), D = sz(query, 2);
+    c.need(dims_are(query, 3) && N > 0 && N <= 1024 && D >= nvdsa::kKpeDim && D <= nvdsa::kQkDim && D % 8 == 0,
+           NVDSA_ERR_SHAPE, "query must be [T, heads, nope + 64]: at most 1024 heads, 64 to 576 dims, a multiple of 8")
+        .need(T < (int64_t{1} << 24) && T * N < (int64_t{1} << 30), NVDSA_ERR_SHAPE, "too many rows")
+        .need(dims_are(kv, 2) && sz(kv, 0) == T && sz(kv, 1) == nvdsa::kQkDim, NVDSA_ERR_SHAPE, "kv must be [T, 576]")
+        .need(dims_are(cos, 2) && sz(cos, 0) == T && sz(cos, 1) >= nvdsa::kKpeDim && sz(cos, 1) % 8 == 0 &&
+                  same_shape(cos, sin),
+              NVDSA_ERR_SHAPE, "cos and sin must be [T, 64 or more, a multiple of 8]")
+        .need(is_vector(kv_norm_weight, nvdsa::kCkvDim), NVDSA_ERR_SHAPE, "kv_norm_weight must be [512]")
+        .need(dims_are(query_rope, 3) && sz(query_rope, 0) == T && sz(query_rope, 1) == N &&
+                  sz(query_rope, 2) == nvdsa::kKpeDim,
+              NVDSA_ERR_SHAPE, "query_rope must be [T, heads, 64]");
+    if (query_norm_weight)
+      c.need(is_vector(query_norm_weight, D), NVDSA_ERR_SHAPE, "query_norm_weight must be [nope + 64]")
+          .need(dims_are(query_nope, 3) && sz(query_nope, 0) == T && sz(query_nope, 1) == N &&
+                    sz(query_nope, 2) == D - nvdsa::kKpeDim,
+                NVDSA_ERR_SHAPE, "query_nope must be [T, heads, nope]");
+    for (const auto* t : {query, kv, cos, sin, kv_norm_weight, query_rope, query_norm_weight, query_nope})
+      if (t) c.need(t->dtype == kv_cache->dtype, NVDSA_ERR_DTYPE, "rows, tables and weights must have kv_cache's dtype");
+    check_lengths(c, actual_seq_lengths_query, B, "actual_seq_lengths_query must be [B]");
+    check_lengths(c, actual_seq_lengths_kv, B, "actual_seq_lengths_kv must be [B]");
+    check_common(c, all, kv_cache->device);
+    check_optional(c, query_norm_weight, kv_cache->device);
+    check_optional(c, query_nope, kv_cache->device);
+    c.need(kv_cache->device >= 0, NVDSA_ERR_DEVICE, "kv_cache must be on a GPU");
+    for (const auto* t : {query, kv, cos, sin, kv_norm_weight, k_rope, kv_cache, query_rope, query_norm_weight, query_nope})
+      if (t) c.need(aligned16(t), NVDSA_ERR_LAYOUT, "rows, tables, weights and caches must be 16-byte aligned");
+  }
+  if (!c.ok()) return c.finish();
+  nvdsa::NormRopeArgs a{};
+  a.query = query->data;
+  a.kv = kv->data;
+  a.cos = cos->data;
+  a.sin = sin->data;
+  a.kv_weight = kv_norm_weight->data;
+  a.query_weight = query_norm_weight ? query_norm_weight->data : nullptr;
+  a.seq_q = static_cast<const int32_t*>(actual_seq_lengths_query->data);
+  a.seq_kv = static_cast<const int32_t*>(actual_seq_lengths_kv->data);
+  a.block_table = static_cast<const int32_t*>(block_table->data);
+  a.k_rope = k_rope->data;
+  a.kv_cache = kv_cache->data;
+  a.query_rope = query_rope->data;
+  a.query_nope = query_nope ? query_nope->data : nullptr;
+  a.rows = sz(query, 0);
+  a.heads = sz(query, 1);
+  a.query_dim = sz(query, 2);
+  a.cos_stride = sz(cos, 1);
+  a.batch = B;
+  a.cols = sz(block_table, 1);
+  a.blocks = sz(kv_cache, 0);
+  a.eps = static_cast<float>(eps);
+  a.elem = elem_of(kv_cache);
+  return launch_status(nvdsa::launch_norm_rope(a, static_cast<hipStream_t>(stream)), "norm_rope_append");
+}
+
+size_t nvdsa_pages_branch_workspace_size(int64_t pages) { return nvdsa::pages_branch_workspace_bytes(pages); }
+
+int nvdsa_pages_branch(const nvdsa_tensor* seq_lens, const nvdsa_tensor* new_tokens, const nvdsa_tensor* block_table,
+                       const nvdsa_tensor* page_refs, const nvdsa_tensor* copy_src, const nvdsa_tensor* copy_dst,
+                       const nvdsa_tensor* copy_tokens, const nvdsa_tensor* missing, const nvdsa_tensor* parents,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  const nvdsa_tensor* const all[] = {seq_lens, new_tokens, block_table, page_refs, copy_src, copy_dst, copy_tokens, missing};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "pages_branch: null tensor argument");
+  Check c("pages_branch");
+  check_pages(c, block_table, page_refs);
+  if (c.ok()) {
+    const int64_t B = sz(block_table, 0);
+    check_lengths(c, seq_lens, B, "seq_lens must be [B]");
+    check_lengths(c, new_tokens, B, "new_tokens must be [B]");
+    check_lengths(c, copy_src, B, "copy_src must be [B]");
+    check_lengths(c, copy_dst, B, "copy_dst must be [B]");
+    check_lengths(c, copy_tokens, B, "copy_tokens must be [B]");
+    check_lengths(c, missing, 1, "missing must be [1]");
+    if (parents) check_lengths(c, parents, B, "parents must be [B]");
+    check_common(c, all, page_refs->device);
+    check_optional(c, parents, page_refs->device);
+    c.need(page_refs->device >= 0, NVDSA_ERR_DEVICE, "page_refs must be on a GPU");
+  }
+  if (!c.ok()) return c.finish();
+  if (workspace == nullptr || workspace_bytes < nvdsa::pages_branch_workspace_bytes(sz(page_refs, 0)))
+    return fail(NVDSA_ERR_WORKSPACE, "pages_branch: workspace too small");
+  nvdsa::PagesBranchArgs a{};
+  a.seq_lens = static_cast<int32_t*>(seq_lens->data);
+  a.new_tokens = static_cast<const int32_t*>(new_tokens->data);
+  a.block_table = static_cast<int32_t*>(block_table->data);
+  a.page_refs = static_cast<int32_t*>(page_refs->data);
+  a.parents = parents ? static_cast<const int32_t*>(parents->data) : nullptr;
+  a.copy_src = static_cast<int32_t*>(copy_src->data);
+  a.copy_dst = static_cast<int32_t*>(copy_dst->data);
+  a.copy_tokens = static_cast<int32_t*>(copy_tokens->data);
+  a.missing = static_cast<int32_t*>(missing->data);
+  a.batch = sz(block_table, 0);
+  a.cols = sz(block_table, 1);
+  a.pages = sz(page_refs, 0);
+  a.workspace = workspace;
+  return launch_status(nvdsa::launch_pages_branch(a, static_cast<hipStream_t>(stream)), "pages_branch");
+}
+
+size_t nvdsa_pages_compact_workspace_size(int64_t pages) { return nvdsa::pages_compact_workspace_bytes(pages); }
+
+int nvdsa_pages_compact(const nvdsa_tensor* block_table, const nvdsa_tensor* page_refs, const nvdsa_tensor* move_src,
+                        const nvdsa_tensor* move_dst, const nvdsa_tensor* move_count, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  const nvdsa_tensor* const all[] = {block_table, page_refs, move_src, move_dst, move_count};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "pages_compact: null tensor argument");
+  Check c("pages_compact");
+  check_pages(c, block_table, page_refs);
+  if (c.ok()) {
+    check_lengths(c, move_src, sz(page_refs, 0), "move_src must be [pages]");
+    check_lengths(c, move_dst, sz(page_refs, 0), "move_dst must be [pages]");
+    check_lengths(c, move_count, 1, "move_count must be [1]");
+    check_common(c, all, page_refs->device);
+    c.need(page_refs->device >= 0, NVDSA_ERR_DEVICE, "page_refs must be on a GPU");
+  }
+  if (!c.ok()) return c.finish();
+  if (workspace == nullptr || workspace_bytes < nvdsa::pages_compact_workspace_bytes(sz(page_refs, 0)))
+    return fail(NVDSA_ERR_WORKSPACE, "pages_compact: workspace too small");
+  nvdsa::PagesCompactArgs a{};
+  a.block_table = static_cast<int32_t*>(block_table->data);
+  a.page_refs = static_cast<int32_t*>(page_refs->data);
+  a.move_src = static_cast<int32_t*>(move_src->data);
+  a.move_dst = static_cast<int32_t*>(move_dst->data);
+  a.move_count = static_cast<int32_t*>(move_count->data);
+  a.batch = sz(block_table, 0);
+  a.cols = sz(block_table, 1);
+  a.pages = sz(page_refs, 0);
+  a.workspace = workspace;
+  return launch_status(nvdsa::launch_pages_compact(a, static_cast<hipStream_t>(stream)), "pages_compact");
+}
+
+int nvdsa_pages_copy(const nvdsa_tensor* src_ids, const nvdsa_tensor* dst_ids, const nvdsa_tensor* caches,
+                     int64_t cache_count, const nvdsa_tensor* tokens, const nvdsa_tensor* count, void* stream) {
+  const nvdsa_tensor* const all[] = {src_ids, dst_ids};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "pages_copy: null tensor argument");
+  if (cache_count < 1 || cache_count > nvdsa::kMostCopyCaches || caches == nullptr)
+    return fail(NVDSA_ERR_ARG, "pages_copy: 1 to 16 caches");
+  Check c("pages_copy");
+  c.need(dims_are(src_ids, 1) && sz(src_ids, 0) < (int64_t{1} << 24), NVDSA_ERR_SHAPE, "src_ids must be [pairs], fewer than 2^24");
+  if (c.ok()) {
+    check_lengths(c, src_ids, sz(src_ids, 0), "src_ids must be [pairs]");
+    check_lengths(c, dst_ids, sz(src_ids, 0), "dst_ids must be [pairs]");
+    if (tokens) check_lengths(c, tokens, sz(src_ids, 0), "tokens must be [pairs]");
+    if (count) check_lengths(c, count, 1, "count must be [1]");
+    check_common(c, all, src_ids->device);
+    check_optional(c, tokens, src_ids->device);
+    check_optional(c, count, src_ids->device);
+    c.need(src_ids->device >= 0, NVDSA_ERR_DEVICE, "src_ids must be on a GPU");
+  }
+  nvdsa::PagesCopyArgs a{};
+  for (int i = 0; i < cache_count && c.ok(); ++i) {
+    const nvdsa_tensor* t = caches + i;
+    c.need(t->ndim >= 2 && t->ndim <= 4 && sz(t, 0) > 0 && sz(t, 0) < (int64_t{1} << 24) && sz(t, 0) == sz(caches, 0),
+           NVDSA_ERR_SHAPE, "caches must be [pages, ...], all with the same number of pages, of two to four dims")
+        .need(dtype_bytes(t->dtype) > 0, NVDSA_ERR_DTYPE, "caches must be 16-bit, float32, int32 or float8_e4m3fn");
+    const nvdsa_tensor* const one[] = {t};
+    check_common(c, one, src_ids->device);
+    if (!c.ok()) break;
+    int64_t bytes = dtype_bytes(t->dtype);
+    for (int d = 1; d < t->ndim; ++d) bytes *= t->shape[d];
+    const int64_t row = t->ndim >= 3 && t->shape[1] == nvdsa::kBlock ? bytes / nvdsa::kBlock : 0;
+    c.need(bytes > 0 && bytes < (int64_t{1} << 30) && bytes % 4 == 0 && row % 4 == 0 && aligned4(t), NVDSA_ERR_LAYOUT,
+           "a cache's pages (and their tokens' rows) must be multiples of 4 bytes, below 1 GiB, on 4-byte addresses");
+    a.cache[i] = t->data;
+    a.page_bytes[i] = bytes;
+    a.token_bytes[i] = row;
+    a.wide[i] = bytes % 16 == 0 && row % 16 == 0 && aligned16(t);
+  }
+  if (!c.ok()) return c.finish();
+  a.src = static_cast<const int32_t*>(src_ids->data);
+  a.dst = static_cast<const int32_t*>(dst_ids->data);
+  a.tokens = tokens ? static_cast<const int32_t*>(tokens->data) : nullptr;
+  a.count = count ? static_cast<const int32_t*>(count->data) : nullptr;
+  a.pairs = sz(src_ids, 0);
+  a.pages = sz(caches, 0);
+  a.caches = static_cast<int32_t>(cache_count);
+  return launch_status(nvdsa::launch_pages_copy(a, static_cast<hipStream_t>(stream)), "pages_copy");
 }
 
 // ------------------------------------------------------------------------

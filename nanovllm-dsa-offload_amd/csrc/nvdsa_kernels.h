@@ -42,7 +42,14 @@ enum KernelId : int {
   kKernLatent8Weights = 26,
   kKernLatent8Select = 27,
   kKernLatent8Move = 28,
-  kKernCount = 29
+  kKernNormRope = 29,
+  kKernPagesTake = 30,
+  kKernPagesReserve = 31,
+  kKernPagesCount = 32,
+  kKernPagesRank = 33,
+  kKernPagesRename = 34,
+  kKernPagesCopy = 35,
+  kKernCount = 36
 };
 // Timing events for the next launch of `kernel_id` when instrumentation is
 // on for the calling thread (nvdsa_profile_begin); both null otherwise.
@@ -341,5 +348,76 @@ struct Latent8EvictArgs {
 };
 size_t latent8_evict_workspace_bytes(int64_t batch, int64_t cols, int64_t latent_heads);
 hipError_t launch_latent8_evict(const Latent8EvictArgs& a, hipStream_t stream);
+
+// ---- new rows of the 16-bit latent cache ------------------------------------
+struct NormRopeArgs {
+  const void* query;            // [rows, heads, query_dim] 16-bit
+  const void* kv;               // [rows, 576]
+  const void* cos;              // [rows, cos_stride] (first 64 used)
+  const void* sin;
+  const void* kv_weight;        // [512]
+  const void* query_weight;     // [query_dim], or null: queries are only rotated
+  const int32_t* seq_q;         // [B] end of each request's rows
+  const int32_t* seq_kv;        // [B] cached tokens, the new ones among them
+  const int32_t* block_table;   // [B, cols]
+  void* k_rope;                 // [blocks, 128, 1, 64]
+  void* kv_cache;               // [blocks, 128, 1, 512]
+  void* query_rope;             // [rows, heads, 64]
+  void* query_nope;             // [rows, heads, query_dim - 64] (with query_weight)
+  int64_t rows, heads, query_dim, cos_stride, batch, cols, blocks;
+  float eps;
+  Elem elem;
+};
+hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream);
+
+// ---- pages of the caches ----------------------------------------------------
+constexpr int kMostBranchRows = 16384;
+struct PagesBranchArgs {
+  int32_t* seq_lens;            // [B]
+  const int32_t* new_tokens;    // [B]
+  int32_t* block_table;         // [B, cols]
+  int32_t* page_refs;           // [pages]
+  const int32_t* parents;       // [B], or null: every row goes on as it is
+  int32_t* copy_src;            // [B]
+  int32_t* copy_dst;            // [B]
+  int32_t* copy_tokens;         // [B]
+  int32_t* missing;             // [1]
+  int64_t batch, cols, pages;
+  void* workspace;
+  int32_t* fresh;               // workspace, set by the launch: [pages]
+  int32_t* given_up;            // [pages]
+};
+size_t pages_branch_workspace_bytes(int64_t pages);
+hipError_t launch_pages_branch(PagesBranchArgs a, hipStream_t stream);
+
+struct PagesCompactArgs {
+  int32_t* block_table;         // [B, cols]
+  int32_t* page_refs;           // [pages]
+  int32_t* move_src;            // [pages]
+  int32_t* move_dst;            // [pages]
+  int32_t* move_count;          // [1]
+  int64_t batch, cols, pages;
+  void* workspace;
+  int32_t* rank;                // workspace, set by the launch: [pages]
+  int32_t* counts;              // [chunks]
+};
+size_t pages_compact_workspace_bytes(int64_t pages);
+hipError_t launch_pages_compact(PagesCompactArgs a, hipStream_t stream);
+
+constexpr int kMostCopyCaches = 16;
+struct PagesCopyArgs {
+  const int32_t* src;           // [pairs]
+  const int32_t* dst;           // [pairs]
+  const int32_t* tokens;        // [pairs], or null: whole pages
+  const int32_t* count;         // [1], or null: every pair
+  int64_t pairs, pages;
+  int32_t caches;
+  void* cache[kMostCopyCaches];             // [pages, page_bytes]
+  int64_t page_bytes[kMostCopyCaches];
+  int64_t token_bytes[kMostCopyCaches];     // 0: a page of it has no rows of tokens
+  bool wide[kMostCopyCaches];               // everything in units of 16 bytes, else of 4
+  int32_t first_piece[kMostCopyCaches + 1]; // set by the launch
+};
+hipError_t launch_pages_copy(PagesCopyArgs a, hipStream_t stream);
 
 }  // namespace nvdsa

@@ -95,6 +95,12 @@ EXT_SIGNATURES = {
     "nvdsa_latent8_attention": ([_P] * 10 + [_DBL, _P, _VP, _SZ, _VP], ctypes.c_int),
     "nvdsa_latent8_evict_workspace_size": ([_I64, _I64, _I64], _SZ),
     "nvdsa_latent8_evict": ([_P] * 8 + [_I64, _I64] + [_P] * 4 + [_VP, _SZ, _VP], ctypes.c_int),
+    "nvdsa_norm_rope_append": ([_P] * 13 + [_DBL, _VP], ctypes.c_int),
+    "nvdsa_pages_branch_workspace_size": ([_I64], _SZ),
+    "nvdsa_pages_branch": ([_P] * 9 + [_VP, _SZ, _VP], ctypes.c_int),
+    "nvdsa_pages_compact_workspace_size": ([_I64], _SZ),
+    "nvdsa_pages_compact": ([_P] * 5 + [_VP, _SZ, _VP], ctypes.c_int),
+    "nvdsa_pages_copy": ([_P] * 3 + [_I64, _P, _P, _VP], ctypes.c_int),
 }
 
 
