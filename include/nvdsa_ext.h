@@ -194,6 +194,31 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query,
                            double eps,
                            void* stream);
 
+/* attention_out[r] = softmax(scale_value * q[r] . k) . k[:512] over the slots
+ * that row r sees: row i of a request's n sees the first
+ * actual_seq_lengths_kv - (n - 1 - i); slots whose table entry names no page are
+ * skipped, a row that sees nothing is zero.  query [T, N, 512], query_rope
+ * [T, N, 64].
+ * Groups (both tensors [S], or neither): requests [prefix_request_ends[s-1],
+ * prefix_request_ends[s]) hold the same pages for their first prefix_lengths[s]
+ * tokens (whole pages: the rest of that length counts as their own), which are
+ * read through the first request's table, once for the group.  Requests behind
+ * the last end share nothing.  The workspace holds no state. */
+size_t nvdsa_shared_prefix_attention_workspace_size(int64_t query_rows, int64_t heads, int64_t batch, int64_t groups);
+int nvdsa_shared_prefix_attention(const nvdsa_tensor* query_rope,
+                                  const nvdsa_tensor* query,
+                                  const nvdsa_tensor* actual_seq_lengths_query,
+                                  const nvdsa_tensor* actual_seq_lengths_kv,
+                                  const nvdsa_tensor* block_table,
+                                  const nvdsa_tensor* k_rope,
+                                  const nvdsa_tensor* kv_cache,
+                                  double scale_value,
+                                  const nvdsa_tensor* attention_out,
+                                  const nvdsa_tensor* prefix_request_ends,
+                                  const nvdsa_tensor* prefix_lengths,
+                                  void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 /* Requests that go on from others, and the pages that they write to next.
  * block_table entries that name no page are -1; page_refs[p] counts the rows
  * that hold page p (and whoever else does), 0: free.

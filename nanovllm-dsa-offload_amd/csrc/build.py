@@ -21,7 +21,7 @@ REPO = PKG_ROOT.parent
 BUILD_DIR = REPO / "_build" / "nvdsa"
 OUTPUT = PKG_ROOT / "nanovllm_amd" / "libnvdsa.so"
 SOURCES = ("scatter_copy.hip", "lim.hip", "sfa.hip", "indexer.hip", "persist.hip", "stage.hip", "latent8.hip",
-           "norm_rope.hip", "pages.hip", "nvdsa_abi.hip")
+           "norm_rope.hip", "pages.hip", "prefix_attention.hip", "nvdsa_abi.hip")
 ARCH = os.environ.get("NVDSA_OFFLOAD_ARCH", "gfx950")
 
 COMMON_FLAGS = [
@@ -44,7 +44,10 @@ COMMON_FLAGS = [
 
 # Per-unit additions.  lim.hip: MFMA results in VGPRs (the score epilogue reads
 # every accumulator; in AGPRs each one costs an extra v_accvgpr_read).
-EXTRA_FLAGS = {"lim.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
+# prefix_attention.hip: likewise, its scores; the output's accumulators, which fill
+# the AGPRs, say so themselves.
+EXTRA_FLAGS = {"lim.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+               "prefix_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
 
 
 def _hipcc() -> str:

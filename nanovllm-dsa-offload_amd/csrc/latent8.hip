@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cfloat>
 
+#include "lds_load.h"
 #include "nvdsa_common.h"
 #include "nvdsa_kernels.h"
 
@@ -576,23 +577,6 @@ __device__ inline uint2 read_tr8(const uint8_t* p) {
   typedef int v2i __attribute__((ext_vector_type(2)));
   typedef __attribute__((address_space(3))) v2i lds_v2i;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(const_cast<uint8_t*>(p))));
-}
-
-// 16 bytes a lane from base + offset straight to LDS at `lds` + 16 * lane (the
-// same for the wave).  Counts in vmcnt like a load; has no register to return.
-__device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base)
-               : "memory", "m0");
-}
-__device__ inline void load_to_lds(const uint8_t* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
-}
-template <int N>
-__device__ inline void wait_loads() {  // all but the wave's newest N are done
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ inline uint32_t lds_address(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
 }
 
 __device__ inline float first_lane(float x) {

@@ -191,7 +191,8 @@ const char* nvdsa_kernel_name(int32_t kernel_id) {
                                 "latent8_weights_kernel", "latent8_select_kernel", "latent8_move_kernel",
                                 "norm_rope_kernel",      "pages_take_kernel", "pages_reserve_kernel",
                                 "pages_count_kernel",    "pages_rank_kernel", "pages_rename_kernel",
-                                "pages_copy_kernel"};
+                                "pages_copy_kernel",     "prefix_plan_kernel", "prefix_attention_kernel",
+                                "prefix_join_kernel"};
   static_assert(sizeof(names) / sizeof(names[0]) == nvdsa::kKernCount, "one name per kernel id");
   if (kernel_id < 0 || kernel_id >= nvdsa::kKernCount) return "unknown";
   return names[kernel_id];
@@ -1663,6 +1664,84 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query, const nvdsa_tensor* kv, co
   a.eps = static_cast<float>(eps);
   a.elem = elem_of(kv_cache);
   return launch_status(nvdsa::launch_norm_rope(a, static_cast<hipStream_t>(stream)), "norm_rope_append");
+}
+
+size_t nvdsa_shared_prefix_attention_workspace_size(int64_t query_rows, int64_t heads, int64_t batch, int64_t groups) {
+  if (query_rows < 0 || heads < 0 || batch < 0 || groups < 0) return 0;
+  return nvdsa::prefix_attention_workspace_bytes(query_rows, heads, batch, groups);
+}
+
+int nvdsa_shared_prefix_attention(const nvdsa_tensor* query_rope, const nvdsa_tensor* query,
+                                  const nvdsa_tensor* actual_seq_lengths_query, const nvdsa_tensor* actual_seq_lengths_kv,
+                                  const nvdsa_tensor* block_table, const nvdsa_tensor* k_rope,
+                                  const nvdsa_tensor* kv_cache, double scale_value, const nvdsa_tensor* attention_out,
+                                  const nvdsa_tensor* prefix_request_ends, const nvdsa_tensor* prefix_lengths,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const nvdsa_tensor* const all[] = {query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
+                                     k_rope, kv_cache, attention_out};
+  if (!all_nonnull(all)) return fail(NVDSA_ERR_ARG, "shared_prefix_attention: null tensor argument");
+  Check c("shared_prefix_attention");
+  c.need((prefix_request_ends != nullptr) == (prefix_lengths != nullptr), NVDSA_ERR_ARG,
+         "prefix_request_ends and prefix_lengths go together")
+      .need(dims_are(actual_seq_lengths_query, 1) && sz(actual_seq_lengths_query, 0) < (1 << 16), NVDSA_ERR_SHAPE,
+            "actual_seq_lengths_query must be rank one, fewer than 65536");
+  const int64_t B = sz(actual_seq_lengths_query, 0);
+  const int64_t S = prefix_request_ends ? sz(prefix_request_ends, 0) : 0;
+  if (c.ok()) check_paged_cache(c, k_rope, kv_cache, block_table, B);
+  if (c.ok()) {
+    const int64_t T = sz(query, 0), N = sz(query, 1);
+    c.need(dims_are(query, 3) && sz(query, 2) == nvdsa::kCkvDim, NVDSA_ERR_SHAPE, "query must be [T, heads, 512]")
+        .need(dims_are(query_rope, 3) && sz(query_rope, 0) == T && sz(query_rope, 1) == N &&
+                  sz(query_rope, 2) == nvdsa::kKpeDim,
+              NVDSA_ERR_SHAPE, "query_rope must be [T, heads, 64]")
+        .need(N > 0 && N <= 1024, NVDSA_ERR_SHAPE, "at most 1024 heads")
+        .need(T < (int64_t{1} << 20) && T * N < (int64_t{1} << 26), NVDSA_ERR_SHAPE,
+              "too many query rows and heads for one call")
+        .need(same_shape(attention_out, query), NVDSA_ERR_SHAPE, "attention_out must match query");
+    if (prefix_request_ends) {
+      c.need(dims_are(prefix_request_ends, 1) && S <= 65536, NVDSA_ERR_SHAPE,
+             "prefix_request_ends must be rank one, at most 65536 groups");
+      check_lengths(c, prefix_request_ends, S, "prefix_request_ends must be [groups]");
+      check_lengths(c, prefix_lengths, S, "prefix_lengths must be [groups]");
+    }
+    for (const auto* t : {query, query_rope, attention_out})
+      c.need(t->dtype == kv_cache->dtype, NVDSA_ERR_DTYPE, "query, query_rope and attention_out must have kv_cache's dtype");
+    check_lengths(c, actual_seq_lengths_query, B, "actual_seq_lengths_query must be [B]");
+    check_lengths(c, actual_seq_lengths_kv, B, "actual_seq_lengths_kv must be [B]");
+    check_common(c, all, kv_cache->device);
+    check_optional(c, prefix_request_ends, kv_cache->device);
+    check_optional(c, prefix_lengths, kv_cache->device);
+    c.need(kv_cache->device >= 0, NVDSA_ERR_DEVICE, "kv_cache must be on a GPU")
+        .need(aligned16(query) && aligned16(query_rope) && aligned16(k_rope) && aligned16(kv_cache) &&
+                  aligned16(attention_out),
+              NVDSA_ERR_LAYOUT, "query, query_rope, k_rope, kv_cache and attention_out must be 16-byte aligned");
+  }
+  if (!c.ok()) return c.finish();
+  const int64_t T = sz(query, 0), N = sz(query, 1);
+  if (T == 0 || B == 0) return NVDSA_OK;
+  if (workspace == nullptr || workspace_bytes < nvdsa::prefix_attention_workspace_bytes(T, N, B, S))
+    return fail(NVDSA_ERR_WORKSPACE, "shared_prefix_attention: workspace too small");
+  nvdsa::PrefixAttentionArgs a{};
+  a.query = query->data;
+  a.query_rope = query_rope->data;
+  a.seq_q = static_cast<const int32_t*>(actual_seq_lengths_query->data);
+  a.seq_kv = static_cast<const int32_t*>(actual_seq_lengths_kv->data);
+  a.block_table = static_cast<const int32_t*>(block_table->data);
+  a.k_rope = k_rope->data;
+  a.kv_cache = kv_cache->data;
+  a.group_ends = S > 0 ? static_cast<const int32_t*>(prefix_request_ends->data) : nullptr;
+  a.prefix_lens = S > 0 ? static_cast<const int32_t*>(prefix_lengths->data) : nullptr;
+  a.out = attention_out->data;
+  a.rows = T;
+  a.heads = N;
+  a.batch = B;
+  a.groups = S;
+  a.cols = sz(block_table, 1);
+  a.blocks = sz(kv_cache, 0);
+  a.scale = static_cast<float>(scale_value);
+  a.elem = elem_of(kv_cache);
+  a.workspace = workspace;
+  return launch_status(nvdsa::launch_prefix_attention(a, static_cast<hipStream_t>(stream)), "shared_prefix_attention");
 }
 
 size_t nvdsa_pages_branch_workspace_size(int64_t pages) { return nvdsa::pages_branch_workspace_bytes(pages); }

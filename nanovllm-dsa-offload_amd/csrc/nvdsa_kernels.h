@@ -49,7 +49,10 @@ enum KernelId : int {
   kKernPagesRank = 33,
   kKernPagesRename = 34,
   kKernPagesCopy = 35,
-  kKernCount = 36
+  kKernPrefixPlan = 36,
+  kKernPrefixAttention = 37,
+  kKernPrefixJoin = 38,
+  kKernCount = 39
 };
 // Timing events for the next launch of `kernel_id` when instrumentation is
 // on for the calling thread (nvdsa_profile_begin); both null otherwise.
@@ -369,6 +372,26 @@ struct NormRopeArgs {
   Elem elem;
 };
 hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream);
+
+// ---- attention of requests that share a prefix ------------------------------
+struct PrefixAttentionArgs {
+  const void* query;            // [rows, heads, 512] 16-bit
+  const void* query_rope;       // [rows, heads, 64]
+  const int32_t* seq_q;         // [B] end of each request's rows
+  const int32_t* seq_kv;        // [B]
+  const int32_t* block_table;   // [B, cols]
+  const void* k_rope;           // [blocks, 128, 1, 64]
+  const void* kv_cache;         // [blocks, 128, 1, 512]
+  const int32_t* group_ends;    // [groups] end of each group's requests
+  const int32_t* prefix_lens;   // [groups]
+  void* out;                    // [rows, heads, 512]
+  int64_t rows, heads, batch, groups, cols, blocks;
+  float scale;
+  Elem elem;
+  void* workspace;
+};
+size_t prefix_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t batch, int64_t groups);
+hipError_t launch_prefix_attention(const PrefixAttentionArgs& a, hipStream_t stream);
 
 // ---- pages of the caches ----------------------------------------------------
 constexpr int kMostBranchRows = 16384;

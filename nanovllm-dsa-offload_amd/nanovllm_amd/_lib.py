@@ -96,6 +96,8 @@ EXT_SIGNATURES = {
     "nvdsa_latent8_evict_workspace_size": ([_I64, _I64, _I64], _SZ),
     "nvdsa_latent8_evict": ([_P] * 8 + [_I64, _I64] + [_P] * 4 + [_VP, _SZ, _VP], ctypes.c_int),
     "nvdsa_norm_rope_append": ([_P] * 13 + [_DBL, _VP], ctypes.c_int),
+    "nvdsa_shared_prefix_attention_workspace_size": ([_I64] * 4, _SZ),
+    "nvdsa_shared_prefix_attention": ([_P] * 7 + [_DBL] + [_P] * 3 + [_VP, _SZ, _VP], ctypes.c_int),
     "nvdsa_pages_branch_workspace_size": ([_I64], _SZ),
     "nvdsa_pages_branch": ([_P] * 9 + [_VP, _SZ, _VP], ctypes.c_int),
     "nvdsa_pages_compact_workspace_size": ([_I64], _SZ),

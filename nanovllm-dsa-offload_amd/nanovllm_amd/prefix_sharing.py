@@ -51,6 +51,11 @@ SCHEMAS = {
         " Tensor(b!) kv_cache, Tensor(c!) query_rope, Tensor? query_norm_weight=None, Tensor(d!)? query_nope=None,"
         " float eps=1e-06) -> ()"
     ),
+    "shared_prefix_attention": (
+        "shared_prefix_attention(Tensor query_rope, Tensor query, Tensor actual_seq_lengths_query,"
+        " Tensor actual_seq_lengths_kv, Tensor block_table, Tensor k_rope, Tensor kv_cache, float scale_value,"
+        " Tensor(a!) attention_out, Tensor? prefix_request_ends=None, Tensor? prefix_lengths=None) -> ()"
+    ),
     "pages_branch": (
         "pages_branch(Tensor(a!) seq_lens, Tensor new_tokens, Tensor(b!) block_table, Tensor(c!) page_refs,"
         " Tensor(d!) copy_src, Tensor(e!) copy_dst, Tensor(f!) copy_tokens, Tensor(g!) missing,"
@@ -74,6 +79,20 @@ def _norm_rope_append(query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_qu
     with _device_of(kv_cache):
         _lib.check(_C.nvdsa_norm_rope_append(*at, float(eps), _stream_of(kv_cache)))
     _written(k_rope, kv_cache, query_rope, query_nope)
+
+
+def _shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope,
+                             kv_cache, scale_value, attention_out, prefix_request_ends=None, prefix_lengths=None) -> None:
+    buf, at = _pack(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope, kv_cache,
+                    attention_out, prefix_request_ends, prefix_lengths)
+    rows, heads = query.shape[:2] if query.dim() == 3 else (0, 0)
+    groups = 0 if prefix_request_ends is None else prefix_request_ends.numel()
+    ws = _workspace(kv_cache.device, _L.nvdsa_shared_prefix_attention_workspace_size(
+        rows, heads, actual_seq_lengths_query.numel(), groups))
+    with _device_of(kv_cache):
+        _lib.check(_C.nvdsa_shared_prefix_attention(*at[:7], float(scale_value), *at[7:], ws.data_ptr(), ws.numel(),
+                                                    _stream_of(kv_cache)))
+    _written(attention_out)
 
 
 def _pages_branch(seq_lens, new_tokens, block_table, page_refs, copy_src, copy_dst, copy_tokens, missing,
@@ -106,8 +125,9 @@ def _pages_copy(src_ids, dst_ids, caches, tokens=None, count=None) -> None:
     _written(*caches)
 
 
-IMPLS = {"norm_rope_append": _norm_rope_append, "pages_branch": _pages_branch, "pages_compact": _pages_compact,
-         "pages_copy": _pages_copy}
+IMPLS = {"norm_rope_append": _norm_rope_append, "shared_prefix_attention": _shared_prefix_attention,
+         "pages_branch": _pages_branch,
+         "pages_compact": _pages_compact, "pages_copy": _pages_copy}
 
 
 def _meta(*args, **kwargs) -> None:
@@ -126,6 +146,7 @@ def _register() -> torch.library.Library:
 _LIBRARY = _register()
 
 _norm_rope_append_op = torch.ops.nanovllm_dsa.norm_rope_append.default
+_shared_prefix_attention_op = torch.ops.nanovllm_dsa.shared_prefix_attention.default
 _pages_branch_op = torch.ops.nanovllm_dsa.pages_branch.default
 _pages_compact_op = torch.ops.nanovllm_dsa.pages_compact.default
 _pages_copy_op = torch.ops.nanovllm_dsa.pages_copy.default
@@ -148,6 +169,25 @@ def norm_rope_append(query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_que
     cache's 16-bit dtype; values are computed in fp32 and rounded once."""
     _norm_rope_append_op(query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
                          k_rope, kv_cache, query_rope, query_norm_weight, query_nope, float(eps))
+
+
+def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope,
+                            kv_cache, scale_value, attention_out, *, prefix_request_ends=None,
+                            prefix_lengths=None) -> None:
+    """``attention_out[r] = softmax(scale_value * q[r] . k) . k[:512]`` over the
+    slots that row r sees: row i of a request's n sees the first
+    ``actual_seq_lengths_kv - (n - 1 - i)``.  A row that sees nothing is zero.
+    ``query`` [T, N, 512] and ``query_rope`` [T, N, 64] have the cache's dtype.
+
+    ``prefix_request_ends`` [S] and ``prefix_lengths`` [S] name the groups:
+    requests ``[prefix_request_ends[s-1], prefix_request_ends[s])`` hold the same
+    pages for their first ``prefix_lengths[s]`` tokens (the whole pages among
+    them; what is left counts as their own).  Those pages are taken from the
+    first request's table and multiplied with the queries of all of them at
+    once.  Results are those of a call without groups, up to the order of sums.
+    Requests behind the last end, and a group of one, share nothing."""
+    _shared_prefix_attention_op(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope,
+                                kv_cache, float(scale_value), attention_out, prefix_request_ends, prefix_lengths)
 
 
 def pages_branch(seq_lens, new_tokens, block_table, page_refs, copy_src, copy_dst, copy_tokens, missing, *,
@@ -194,4 +234,5 @@ def pages_copy(src_ids, dst_ids, caches, *, tokens=None, count=None) -> None:
     _pages_copy_op(src_ids, dst_ids, list(caches), tokens, count)
 
 
-__all__ = ["MOST_CACHES", "norm_rope_append", "pages_branch", "pages_compact", "pages_copy"]
+__all__ = ["MOST_CACHES", "norm_rope_append", "pages_branch", "pages_compact", "pages_copy",
+           "shared_prefix_attention"]

@@ -118,3 +118,29 @@ def copy(cache: torch.Tensor, pairs, tokens=None) -> None:
             cache[dst, :n] = cache[src, :n]
         elif n > 0:
             cache[dst] = cache[src]
+
+
+def attention(query_rope, query, ends, lengths, table, k_rope, kv_cache, scale):
+    """(out, size, reach): the operator in 64 bits, and, for bounds, the sums of
+    p |v| and the largest scale * sum |q| |k| of a row and head."""
+    rows, heads, _ = query.shape
+    pages = kv_cache.shape[0]
+    q = torch.cat([query, query_rope], -1).double()
+    out, size = (torch.zeros(rows, heads, 512, dtype=torch.float64) for _ in range(2))
+    reach = torch.zeros(rows, heads, dtype=torch.float64)
+    for b, (lo, hi) in enumerate(_spans(ends, rows)):
+        cap = table.shape[1] * PAGE
+        length = min(max(int(lengths[b]), 0), cap)
+        row = table[b, : -(-length // PAGE)].long()
+        named = ((row >= 0) & (row < pages)).repeat_interleave(PAGE)[:length]
+        at = torch.where((row >= 0) & (row < pages), row, 0)
+        keys = torch.cat([kv_cache[at].flatten(0, 2), k_rope[at].flatten(0, 2)], -1)[:length].double()
+        for t in range(lo, hi):
+            sees = max(0, length - (hi - 1 - t))
+            seen = keys[:sees][named[:sees]]
+            if len(seen) == 0:
+                continue
+            p = torch.softmax(q[t] @ seen.T * scale, -1)
+            out[t], size[t] = p @ seen[:, :512], p @ seen[:, :512].abs()
+            reach[t] = (q[t].abs() @ seen.abs().T).amax(-1) * abs(scale)
+    return out, size, reach

@@ -123,3 +123,76 @@ def make_pages(lengths, pages, cols, seed, shared=()):
             if 0 <= p < pages:
                 refs[p] += 1
     return table, refs
+
+
+def make_cache(prefixes, groups, own, seed, dtype, cols=None, spare=2, none=-1, size=1.0):
+    """Caches, table and lengths of requests in groups: ``groups[s]`` requests
+    share a prefix of ``prefixes[s]`` tokens (their whole pages), request b has
+    ``own[b]`` more; requests behind the groups share nothing."""
+    g = torch.Generator().manual_seed(seed)
+    table, at, lengths = [], 0, []
+    for n, tokens in zip(groups, prefixes):
+        shared = list(range(at, at + tokens // PAGE))
+        at += len(shared)
+        for _ in range(n):
+            lengths.append(tokens + own[len(lengths)])
+            more = -(-lengths[-1] // PAGE) - len(shared)
+            table.append(shared + list(range(at, at + max(0, more))))
+            at += max(0, more)
+    while len(lengths) < len(own):
+        lengths.append(own[len(lengths)])
+        more = -(-lengths[-1] // PAGE)
+        table.append(list(range(at, at + more)))
+        at += more
+    blocks = at + spare
+    order = torch.randperm(blocks, generator=g).tolist()
+    cols = cols or max(1, max(len(r) for r in table))
+    table = [[order[p] for p in r] + [none] * (cols - len(r)) for r in table]
+    rand = lambda *s: (size * torch.randn(*s, generator=g)).to(dtype)  # noqa: E731
+    return {"table": i32(table), "lengths": i32(lengths), "kv_cache": rand(blocks, PAGE, 1, 512),
+            "k_rope": rand(blocks, PAGE, 1, 64), "group_ends": i32(list(torch.tensor(groups).cumsum(0))) if groups else i32([]),
+            "prefix": i32(list(prefixes))}
+
+
+def make_queries(c, counts, heads, seed, pad=0, size=2.0):
+    g = torch.Generator().manual_seed(seed + 1000)
+    total, dtype = sum(counts) + pad, c["kv_cache"].dtype
+    c["query"] = (size * torch.randn(total, heads, 512, generator=g)).to(dtype)
+    c["query_rope"] = (size * torch.randn(total, heads, 64, generator=g)).to(dtype)
+    c["ends"] = torch.tensor(counts).cumsum(0).to(torch.int32)
+    c["out"] = torch.full((total, heads, 512), 7.0).to(dtype)
+    return c
+
+
+def call_attention(d, scale=SCALE, groups=True):
+    more = {"prefix_request_ends": d["group_ends"], "prefix_lengths": d["prefix"]} if groups else {}
+    api().shared_prefix_attention(d["query_rope"], d["query"], d["ends"], d["lengths"], d["table"], d["k_rope"],
+                                  d["kv_cache"], scale, d["out"], **more)
+
+
+def attention_bound(c, out, size, reach):
+    """How far an output may be from the 64-bit one.  The store rounds by half a
+    step; so does P, each by half a step of its own (16 bits); sums of n terms
+    in fp32 are off by n 2^-24 of their magnitudes, those of P and the output's
+    each, and the join adds as many parts at most; a score of 576 products in
+    fp32 is off by at most 578 2^-24 of |q| . |k|, with its factor 2^-22 of
+    itself, and moves p and its normaliser by that each; the exponential is off
+    by 2^-22 of itself.  fp16 holds P below its normal range to 2^-25, and a
+    row's largest P is at least 2^8: 2^-33 of the largest |v| a key."""
+    dtype = c["kv_cache"].dtype
+    keys = int(c["lengths"].max())
+    score = reach * (578 * 2.0 ** -24 + 2.0 ** -22)
+    per = HALF_STEP[dtype] + keys * 2.0 ** -22 + 2 * score + 2.0 ** -20
+    tail = keys * 2.0 ** -33 * float(torch.nan_to_num(c["kv_cache"].float(), 0, 0, 0).abs().max()) if dtype == torch.float16 else 0.0
+    return out.abs() * HALF_STEP[dtype] + size * per[..., None] + tail + TINY[dtype]
+
+
+def check_attention(got, c, scale=SCALE):
+    out, size, reach = O.attention(c["query_rope"], c["query"], c["ends"], c["lengths"], c["table"], c["k_rope"],
+                                   c["kv_cache"], scale)
+    last = min(max(int(c["ends"][-1]), 0), out.shape[0])
+    off = (got.double() - out).abs()[:last]
+    worst = float((off / attention_bound(c, out, size, reach)[:last]).max()) if last else 0.0
+    assert worst <= 1.0, worst
+    assert torch.equal(got[last:].view(torch.int16), c["out"][last:].view(torch.int16))
+    return worst
