@@ -15,6 +15,13 @@ __device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_
 __device__ inline void load_to_lds(const uint8_t* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
+// The same from base + offset + OFFSET to `lds` + OFFSET + 16 * lane.
+template <int OFFSET>
+__device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds), "v"(offset),
+               "s"(base), "n"(OFFSET)
+               : "memory", "m0");
+}
 template <int N>
 __device__ inline void wait_loads() {  // all but the wave's newest N are done
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -30,6 +37,11 @@ __device__ inline uint2 read_tr16(const uint8_t* p) {
   typedef short v4i16 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(const_cast<uint8_t*>(p))));
+}
+__device__ inline uint2 read_tr16(uint32_t lds) {  // (by address)
+  typedef short v4i16 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4i16*>(lds)));
 }
 
 }  // namespace nvdsa

@@ -10,7 +10,8 @@
 // lays the items' tiles of keys in a row and cuts it into equal parts, one per
 // workgroup; what lies across parts, and a pair's two items, leave fp32 partial
 // sums that a join kernel adds up.
-#include <algorithm>
+#include <cstddef>
+#include <utility>
 
 #include "lds_load.h"
 #include "nvdsa_common.h"
@@ -106,6 +107,17 @@ __device__ inline int part_of(int64_t total, int64_t parts, int64_t unit) {
   while (w + 1 < parts && part_start(total, parts, w + 1) <= unit) ++w;
   while (w > 0 && part_start(total, parts, w) > unit) --w;
   return static_cast<int>(w);
+}
+// Values that every lane holds, in scalar registers.
+__device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(x) >> 32));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ inline Span uniform(const Span& s) {
+  return {uniform(s.unit0), uniform(s.merge), uniform(s.pair0), uniform(s.pairs),
+          uniform(s.tile0), uniform(s.tiles), uniform(s.table), uniform(s.group)};
 }
 // Row of the partial sums of a segment's first pair.
 __device__ inline int64_t part_row(const Plan& w, int part, bool begins) { return (2 * static_cast<int64_t>(part) + (begins ? 1 : 0)) * w.stride; }
@@ -261,7 +273,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
 }
 
 // ------------------------------------------------------------- the attention
-struct Lds {
+struct LdsFew {   // items of up to 64 pairs
   alignas(16) uint8_t keys[kBuffers][kTileBytes];
   alignas(16) uint16_t p[kPairs * kKeys];
   float factor[kPairs];
@@ -270,7 +282,22 @@ struct Lds {
   int32_t moved[4];     // a wave's rows have new references
   int32_t least[4];     // the least that a row of a wave sees
 };
+struct LdsMany {  // more
+  alignas(16) uint8_t p[kPairs * kKeys * 2];   // (at a segment's end: references and sums)
+  uint8_t half[4][4][64][16];                  // scores of half the dims, to a wave
+  uint8_t rope[kPairs * kKpeBytes];            // the pairs' rope dims
+  uint8_t keys[3][kTileBytes];
+  float factor[kPairs];
+  int32_t moved[4];     // the tile at which a wave's rows have new references
+  int32_t moved_last;   // the last such tile of all
+  int32_t least[4];
+};
+union Lds {
+  LdsFew few;
+  LdsMany many;
+};
 static_assert(sizeof(Lds) <= 160 * 1024, "LDS");
+static_assert(offsetof(LdsMany, keys) % 4096 == 0 && offsetof(LdsMany, rope) % 8192 == 0, "exclusive ors within");
 
 struct Segment {
   int64_t pair0;      // of all pairs
@@ -283,21 +310,137 @@ struct Segment {
 };
 
 // o += a b, with o in accumulation registers: 256 of them hold four tiles of
-// pairs, and the compiler would share them with the scores.  The two wait states
-// cover an operand that a vector instruction wrote just before; who reads or
-// writes o otherwise calls settle() first and after.
+// pairs, and the compiler would share them with the scores.  Who reads or writes o
+// otherwise calls settle() first and after.  WAIT: two wait states, for an operand
+// that a vector instruction may have written just before (where one is first used:
+// operands come from LDS, but the compiler may have copied them).
+template <bool WAIT>
 __device__ inline void accumulate(Bf16, u32x4_t a, u32x4_t b, f32x16_t& o) {
-  asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+  if constexpr (WAIT)
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+  else
+    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
 }
+template <bool WAIT>
 __device__ inline void accumulate(F16, u32x4_t a, u32x4_t b, f32x16_t& o) {
-  asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+  if constexpr (WAIT)
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+  else
+    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
 }
 // Waits out a product that writes o, or a write of o before a product.
 __device__ inline void settle(f32x16_t& o) { asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o)); }
 
+// threadIdx.x, anew for every segment: places in LDS that follow from it would
+// otherwise be worked out once for all forms of the loop, and spilled.
+__device__ inline int own_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+// f(0), f(1) .. f(N - 1), each with a constant.
+template <typename F, int... J>
+__device__ __forceinline__ void steps_of(F&& f, std::integer_sequence<int, J...>) {
+  (f(std::integral_constant<int, J>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F&& f) {
+  steps_of(f, std::make_integer_sequence<int, N>{});
+}
+// A copy that stays one: the compiler would let a chain of products change its
+// registers halfway, and wait for it.
+__device__ inline float moved_here(float x) {
+  float r;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(r) : "v"(x));
+  return r;
+}
+// By address in LDS.
+__device__ inline u32x4_t lds_get(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(at);
+}
+__device__ inline void lds_put(uint32_t at, u32x4_t v) { *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(at) = v; }
+__device__ inline void lds_put(uint32_t at, uint32_t x, uint32_t y) {
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(at) = u32x2_t{x, y};
+}
+// Nothing is known of x from here on: what follows from it is worked out where it
+// is used, and holds no register across the loop.
+__device__ inline void forget(uint32_t& x) { asm volatile("" : "+v"(x)); }
+// (fmaxf() would first make its operands canonical.)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Zeros in the place of infinities and NaN.
+template <typename T>
+__device__ inline u32x4_t finite_or_zero(u32x4_t v) {
+  constexpr uint32_t kInf = std::is_same<T, Bf16>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t lo = (v[k] & 0x7fffu) >= kInf ? 0u : v[k] & 0xffffu;
+    const uint32_t hi = ((v[k] >> 16) & 0x7fffu) >= kInf ? 0u : v[k] & 0xffff0000u;
+    v[k] = lo | hi;
+  }
+  return v;
+}
+
+// A segment's outputs, or its partial sums; rows: references and sums of P.
 template <typename T, int TILES>
-__device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, Lds& lds) {
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void finish(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, bool empty,
+                                       const float2* rows, f32x16_t (&o)[4][TILES]) {
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < TILES; ++r) settle(o[d][r]);
+#pragma unroll
+  for (int r = 0; r < TILES; ++r) {
+    const int m = r * 32 + l32;
+    if (m >= s.count) continue;
+    const float2 row = rows[m];
+    if (s.direct) {
+      const float by = row.y == 0.f ? 0.f : 1.f / row.y;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.pair0 + m) * kCkvDim + wave * 128 + 4 * hh;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint2*>(out + d * 32 + 8 * i) =
+              make_uint2(T::pack2(o[d][r][4 * i] * by, o[d][r][4 * i + 1] * by),
+                         T::pack2(o[d][r][4 * i + 2] * by, o[d][r][4 * i + 3] * by));
+    } else {
+      const int64_t at = s.row + m * s.row_step;
+      if (wave == 0 && hh == 0) w.refs[at] = row;
+      if (!empty) {
+        float* out = w.sums + at * kCkvDim + wave * 128 + 4 * hh;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(out + d * 32 + 8 * i) =
+                make_float4(o[d][r][4 * i], o[d][r][4 * i + 1], o[d][r][4 * i + 2], o[d][r][4 * i + 3]);
+      }
+    }
+  }
+}
+
+// A segment without tiles.
+template <typename T>
+__device__ __forceinline__ void nothing(const PrefixAttentionArgs& a, const Plan& w, const Segment& s) {
+  if (s.direct) {
+    u32x4_t* out = static_cast<u32x4_t*>(a.out) + s.pair0 * (kCkvDim / 8);
+    for (int i = threadIdx.x; i < s.count * (kCkvDim / 8); i += kThreads) out[i] = u32x4_t{0, 0, 0, 0};
+  } else {
+    for (int m = threadIdx.x; m < s.count; m += kThreads) w.refs[s.row + m * s.row_step] = make_float2(-INFINITY, 0.f);
+  }
+}
+
+template <typename T, int TILES>
+__device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, LdsFew& lds) {
+  const int tid = own_thread();
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
@@ -443,17 +586,9 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   // infinity or NaN is not.  (A row that does see such a key has them in its scores.)
   auto scrub = [&](int tile) {
     uint8_t* v_tile = lds.keys[tile % kBuffers];
-    constexpr uint32_t kInf = std::is_same<T, Bf16>::value ? 0x7f80u : 0x7c00u;
     for (int i = tid; i < kKeys * kCkvBytes / 16; i += kThreads) {
       u32x4_t* p = reinterpret_cast<u32x4_t*>(v_tile + i * 16);
-      u32x4_t v = *p;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = (v[k] & 0x7fffu) >= kInf ? 0u : v[k] & 0xffffu;
-        const uint32_t hi = ((v[k] >> 16) & 0x7fffu) >= kInf ? 0u : v[k] & 0xffff0000u;
-        v[k] = lo | hi;
-      }
-      *p = v;
+      *p = finite_or_zero<T>(*p);
     }
   };
   auto output = [&](int tile) {
@@ -489,7 +624,7 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
         const uint2 hi = read_tr16(v_tile + (v_at[1] ^ (d * 64)) + ks * 16 * kCkvBytes);
         const u32x4_t v{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-        for (int r = 0; r < TILES; ++r) accumulate(T{}, v, p[r], o[d][r]);
+        for (int r = 0; r < TILES; ++r) accumulate<true>(T{}, v, p[r], o[d][r]);
       }
     }
   };
@@ -532,62 +667,355 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     if (hh == 0) lds.row[m_mine] = make_float2(most == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
   }
   lds_barrier();
+  finish<T, TILES>(a, w, s, t0 >= t1, lds.row, o);
+}
+
+// Items of more than 64 pairs, bound by their products.  For the scores of a tile
+// a wave takes 64 pairs and half of the dims, so that every operand from LDS has
+// two products; two waves meet in LDS, and each goes on with 32 pairs.  For the
+// outputs it takes 128 dims of all pairs.  The scores of tile t + 1 are multiplied
+// while the vector unit weighs tile t between the products, then the outputs of
+// tile t.  Two barriers a tile: at A everybody is done with tile t - 1 and its P,
+// tile t + 1 has arrived, and so have the halves of tile t's scores; at B P is
+// there.  Products go on across either: operands of the last ones are in registers
+// by then, and those behind it on the way.
+template <typename T>
+__device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, LdsMany& lds) {
+  const int tid = own_thread();
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int rg = wave & 1, dh = wave >> 1;  // 64 pairs, half of the dims
+  const int tile_mine = 2 * rg + dh;        // of 32 pairs that this wave weighs
+  const int m_mine = tile_mine * 32 + l32;
+  constexpr int kHalf = kSteps / 2, kLatentHalf = kHalf - 2;
+
+  // Addresses in LDS; a tile's places are attend()'s, but a wave loads eight
+  // neighbouring keys.  (Tiles and the rest lie at
+  // multiples of 4 KiB, so that places within one are reached by exclusive ors.)
+  const uint32_t keys_at = lds_address(lds.keys), half_at = lds_address(lds.half);
+  uint32_t lane16 = static_cast<uint32_t>(lane * 16);
+  auto swizzle = [](int k) { return ((k & 3) << 2) | ((k >> 2) & 3); };
+  uint32_t byte_of = static_cast<uint32_t>(wave * 8 * kCkvBytes + ((lane & 48) | ((lane ^ ((2 * wave) & 3)) & 15)) * 16);
+  const int rope_key = wave * 8 + (lane >> 3);
+  const uint32_t rope_byte = static_cast<uint32_t>(rope_key * kKpeBytes + ((lane ^ (rope_key >> 1)) & 7) * 16);
+  uint32_t k_at = keys_at + static_cast<uint32_t>(l32 * kCkvBytes + dh * 512 + ((hh ^ swizzle(l32)) & 15) * 16);
+  uint32_t r_at = keys_at + static_cast<uint32_t>(kKeys * kCkvBytes + l32 * kKpeBytes + (((4 * dh + hh) ^ (l32 >> 1)) & 7) * 16);
+  const int v_key = 8 * hh + ((lane & 15) >> 2);  // (and the key four behind it, whose swizzle differs by 1)
+  uint32_t v_at = keys_at + static_cast<uint32_t>(v_key * kCkvBytes + wave * 256 + (lane & 1) * 8 +
+                                              (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ swizzle(v_key)) & 15) * 16);
+  const int p_swz = (l32 >> 2) & 3;
+  uint32_t p_read = lds_address(lds.p) + static_cast<uint32_t>(l32 * 64 + ((hh ^ p_swz) & 3) * 16);
+  uint32_t p_write = lds_address(lds.p) + static_cast<uint32_t>(m_mine * 64 + p_swz * 16 + hh * 8);
+
+  // The ids of 64 pages, a lane each (-1: none), from column `first_held` on.
+  const int last_column = (s.tile1 - 1) / kPageTiles < a.cols ? (s.tile1 - 1) / kPageTiles : static_cast<int>(a.cols) - 1;
+  int first_held = s.tile0 / kPageTiles, held = -1;
+  auto hold_pages = [&] {
+    const int c = first_held + (own_thread() & 63);
+    const int32_t page = c <= last_column ? s.table[c] : -1;
+    held = page >= 0 && page < a.blocks ? page : -1;
+  };
+  auto page_of = [&](int tile) { return __builtin_amdgcn_readlane(held, tile / kPageTiles - first_held); };
+  // A tile's loads, nine of a wave: pairs of keys, and the rope dims.
+  struct Load {
+    const uint8_t* base;
+    const uint8_t* rope;
+  };
+  const uint32_t lds_tile = keys_at + wave * (8 * kCkvBytes), lds_rope = keys_at + kKeys * kCkvBytes + wave * 1024;
+  auto load_of = [&](int tile, int page) {
+    const uint32_t row = static_cast<uint32_t>(page < 0 ? 0 : page) * kBlock + (static_cast<uint32_t>(tile) % kPageTiles) * kKeys;
+    return Load{static_cast<const uint8_t*>(a.kv_cache) + static_cast<uint64_t>(row) * kCkvBytes,
+                static_cast<const uint8_t*>(a.k_rope) + static_cast<uint64_t>(row) * kKpeBytes};
+  };
+  auto issue = [&](const Load& l, uint32_t buffer, auto which) {  // 0 to 7: a key, 8: the rope dims
+    constexpr int n = decltype(which)::value;
+    if constexpr (n < 8)
+      load_to_lds<(n & 3) * 1024>(l.base + (n >> 2) * 4096, byte_of ^ ((n & 3) * 64 + (n >> 2) * 16),
+                                  lds_tile + buffer + (n >> 2) * 4096);
+    else
+      load_to_lds<0>(l.rope, rope_byte, lds_rope + buffer);
+  };
+
+  hold_pages();
+  lds_barrier();  // (the segment before is done with LDS)
+  const int t0 = s.tile0, t1 = s.tile1;
+  {
+    const Load l = load_of(t0, page_of(t0));
+    steps<kTileLoads>([&](auto n) { issue(l, 0, n); });
+  }
+
+  // Of the wave's half of the dims, in steps of 16: i = 2 x + g is chunk pair x of
+  // 256-byte group g, for two tiles of 32 pairs, first those that the wave weighs.
+  // The rope dims, the last two steps, lie in LDS, for which there is room, and not
+  // in registers, for which there is none.
+  u32x4_t q[kLatentHalf][2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int m = rg * 64 + (r ^ dh) * 32 + l32;
+    const int64_t pair = s.pair0 + (m < s.count ? m : 0);
+    const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + dh * 32 + hh;
+#pragma unroll
+    for (int i = 0; i < kLatentHalf; ++i) {
+      q[i][r] = qn[(i & 1) * 16 + (i >> 1) * 2];
+    }
+#pragma unroll
+    for (int i = 0; i < kLatentHalf; ++i) asm volatile("" : "+v"(q[i][r]));
+  }
+  for (int i = tid; i < kPairs * (kKpeDim / 8); i += kThreads) {
+    const int m = i >> 3;
+    const int64_t pair = s.pair0 + (m < s.count ? m : 0);
+    *reinterpret_cast<u32x4_t*>(&lds.rope[0] + m * kKpeBytes + ((i ^ (m >> 1)) & 7) * 16) =
+        static_cast<const u32x4_t*>(a.query_rope)[pair * (kKpeDim / 8) + (i & 7)];
+  }
+  // (Rows of pairs 64 rg + (r ^ dh) 32 + l32: the other tile is 32 rows away.)
+  uint32_t qr_at = lds_address(lds.rope) + static_cast<uint32_t>((tile_mine * 32 + l32) * kKpeBytes + (((4 * dh + hh) ^ (l32 >> 1)) & 7) * 16);
+  const int vis = m_mine < s.count ? w.visible[(s.pair0 + m_mine) / a.heads] : 0;
+  f32x16_t o[4][4];
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < TILES; ++r) settle(o[d][r]);
+    for (int r = 0; r < 4; ++r) {
 #pragma unroll
-  for (int r = 0; r < TILES; ++r) {
-    const int m = r * 32 + l32;
-    if (m >= s.count) continue;
-    const float2 row = lds.row[m];
-    if (s.direct) {
-      const float by = row.y == 0.f ? 0.f : 1.f / row.y;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.pair0 + m) * kCkvDim + wave * 128 + 4 * hh;
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint2*>(out + d * 32 + 8 * i) =
-              make_uint2(T::pack2(o[d][r][4 * i] * by, o[d][r][4 * i + 1] * by),
-                         T::pack2(o[d][r][4 * i + 2] * by, o[d][r][4 * i + 3] * by));
-    } else {
-      const int64_t at = s.row + m * s.row_step;
-      if (wave == 0 && hh == 0) w.refs[at] = row;
-      if (t0 < t1) {
-        float* out = w.sums + at * kCkvDim + wave * 128 + 4 * hh;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(out + d * 32 + 8 * i) =
-                make_float4(o[d][r][4 * i], o[d][r][4 * i + 1], o[d][r][4 * i + 2], o[d][r][4 * i + 3]);
-      }
+      for (int e = 0; e < 16; ++e) o[d][r][e] = 0.f;
+      settle(o[d][r]);
     }
+  float ref = 0.f, l_run = 0.f;
+  float room = -INFINITY;  // a score above the reference by more moves it (nothing seen yet: any does)
+  int vis_least = m_mine < s.count ? vis : 0x7fffffff;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) vis_least = min(vis_least, __shfl_xor(vis_least, d));
+  vis_least = __builtin_amdgcn_readfirstlane(vis_least);
+  if (lane == 0) lds.least[wave] = vis_least;
+  if (tid < 4) lds.moved[tid] = INT32_MIN;
+  if (tid == 0) lds.moved_last = INT32_MIN;
+  const float factor = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(a.scale * kLog2e)));
+
+  constexpr int kAhead = 3;   // operands of the scores on their way
+  constexpr int kLate = 4;    // products of the outputs that are left for behind barrier A
+  u32x4_t v[3], p[4];
+  f32x16_t mine;              // the wave's half of the scores of its 32 pairs, then their P
+#pragma unroll
+  for (int e = 0; e < 16; ++e) mine[e] = 0.f;
+  auto fetch_v = [&](uint32_t from, int i) {  // operand i = 4 ks + d
+    const uint32_t at = from ^ ((i & 3) * 64);
+    const uint2 lo = read_tr16(at + (i >> 2) * 16 * kCkvBytes);
+    const uint2 hi = read_tr16((at ^ 16) + ((i >> 2) * 16 + 4) * kCkvBytes);
+    v[i % 3] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+  };
+  auto fetch_p = [&](int ks, int r) { p[r] = lds_get((p_read ^ (ks * 32)) + r * 2048); };
+  u32x4_t k[kAhead + 1];
+  auto fetch_k = [&](uint32_t k_from, uint32_t r_from, int i) {
+    if (i < kHalf)
+      k[i % (kAhead + 1)] = lds_get(i < 16 ? (k_from ^ ((i >> 1) * 32)) + (i & 1) * 256 : r_from ^ ((i - 16) * 32));
+  };
+  // Barrier A before the scores of a tile in that buffer.
+  auto begin_scores = [&](uint32_t buffer) {
+    wait_loads<0>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch_k(k_at + buffer, r_at + buffer, i);
+  };
+
+  // Tile t, in buffer `now`, is weighed and put out; the scores of tile t + 1, in
+  // buffer `ahead`, come first, and of tile t - 1 kLate products are open.  One
+  // form for every t, the one before the first tile, of a page that names nothing,
+  // among them: the compiler does not find registers for more.
+  uint32_t now = 2 * kTileBytes, ahead = 0, beyond = kTileBytes;
+  int page_t = -1, page_1 = 0, page_2 = 0;  // of tiles t, t + 1 and t + 2
+  Load load{};                              // of tile t + 2
+  int seen_all = 0;                         // tiles that every row of the item sees whole
+  const int seen_mine = vis_least / kKeys;  // that every row of the wave's does
+  auto round = [&](int t) {
+    const uint32_t k_slot = k_at + ahead, r_slot = r_at + ahead, v_from = v_at + now;
+    forget(p_read);
+    forget(p_write);
+    forget(qr_at);
+    forget(byte_of);
+    forget(lane16);
+    forget(k_at);
+    forget(r_at);
+    forget(v_at);
+    u32x4_t qr[2][2], other[4];
+    f32x16_t next[2];
+    const int page = page_t;
+    Load next_load;
+    const int page_next = page_of(t + 3);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) other[e] = lds_get(half_at + wave * 4096 + lane16 + e * 1024);
+    float top = 0.f, more = 0.f;
+    int32_t moved_last = 0;
+    bool any = false;
+    __builtin_amdgcn_sched_barrier(0);
+    steps<kSteps>([&](auto step) __attribute__((always_inline)) {
+      constexpr int j = decltype(step)::value, i = j >> 1, r = j & 1;
+      if constexpr (r == 0) fetch_k(k_slot, r_slot, i + kAhead);
+      if constexpr (r == 0 && (i == 14 || i == 15)) {
+        qr[i & 1][0] = lds_get(qr_at ^ ((i - 14) * 32));
+        qr[i & 1][1] = lds_get(qr_at ^ ((i - 14) * 32 + 32 * kKpeBytes));
+      }
+      {
+        if constexpr (i == 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) next[r][e] = 0.f;
+        }
+        next[r] = T::mfma32(__builtin_bit_cast(typename T::vec8, k[i % (kAhead + 1)]),
+                            __builtin_bit_cast(typename T::vec8, i < kLatentHalf ? q[i % kLatentHalf][r] : qr[i & 1][r]), next[r]);
+      }
+      {
+        // (A load of all four waves takes 64 clocks of the way from the L2, two products.)
+        if constexpr (j % 2 == 0 && j < 2 * kTileLoads) issue(load, beyond, std::integral_constant<int, j / 2>{});
+        if constexpr (j >= 4 && j < 12) {
+          constexpr int e = 2 * (j - 4);
+          mine[e] = fmaf(mine[e] + __uint_as_float(other[e / 4][e % 4]), factor, -ref);
+          mine[e + 1] = fmaf(mine[e + 1] + __uint_as_float(other[e / 4][e % 4 + 1]), factor, -ref);
+        }
+        if constexpr (j == 12) if (((seen_mine - 1 - t) | page) < 0) {
+          const int left = vis - t * kKeys - 4 * (own_thread() >> 5 & 1);  // keys that the row sees, from the lane's first
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mine[e] = page >= 0 && 8 * (e >> 2) + (e & 3) < left ? mine[e] : -INFINITY;
+        }
+        if constexpr (j == 12) top = max3(max3(mine[0], mine[1], mine[2]), max3(mine[3], mine[4], mine[5]), max3(mine[6], mine[7], mine[8]));
+        if constexpr (j == 13) top = max3(top, max3(mine[9], mine[10], mine[11]), max3(mine[12], mine[13], max3(mine[14], mine[15], mine[15])));
+        if constexpr (j == 14) any = __any(top > room);
+        if constexpr (j == 15) {
+          if (any) {
+            const int th = own_thread();
+            top = xor32_op(top, MaxOp{});
+            const bool past = top > room;
+            const float up = past ? top - kRise : 0.f;
+            const bool seen = past && room != -INFINITY;
+            const float f = seen ? __builtin_amdgcn_exp2f(-up) : 1.f;
+            room = past ? kMost : room;
+            ref += up;
+            l_run *= f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mine[e] -= up;
+            if ((th & 32) == 0) lds.factor[tile_mine * 32 + (th & 31)] = f;
+            if (__any(seen) && (th & 63) == 0) lds.moved[tile_mine] = lds.moved_last = t;  // (else o is zero)
+          }
+        }
+        if constexpr (j >= 16 && j < 24) {
+          constexpr int e = 2 * (j - 16), n = e / 4;
+          mine[e] = __builtin_amdgcn_exp2f(mine[e]);
+          mine[e + 1] = __builtin_amdgcn_exp2f(mine[e + 1]);
+          l_run += mine[e];
+          more += mine[e + 1];
+          if constexpr (e % 4 == 2)
+            lds_put(p_write ^ (n * 16), T::pack2(mine[e - 2], mine[e - 1]), T::pack2(mine[e], mine[e + 1]));
+        }
+        if constexpr (j == 24) l_run += more;
+        if constexpr (j == 29) moved_last = lds.moved_last;
+        if constexpr (j >= 29 && j < 33) fetch_p(0, j - 29);
+        if constexpr (j == 33) fetch_v(v_from, 0);
+        if constexpr (j == 35) fetch_v(v_from, 1);
+        if constexpr (j == 28) {
+          // Values of keys that some row must not see: see attend().
+          if (((seen_all - 1 - t) | page) < 0) {
+            for (int c = own_thread(); c < kKeys * kCkvBytes / 16; c += kThreads) {
+              u32x4_t* at = reinterpret_cast<u32x4_t*>(&lds.keys[0][0] + now + c * 16);
+              *at = finite_or_zero<T>(*at);
+            }
+          }
+          lds_barrier();  // B
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    {
+      if (__builtin_amdgcn_readfirstlane(moved_last) == t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (__builtin_amdgcn_readfirstlane(lds.moved[r]) == t) {
+            const float f = lds.factor[r * 32 + (own_thread() & 31)];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              settle(o[d][r]);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[d][r][e] *= f;
+              settle(o[d][r]);
+              __builtin_amdgcn_sched_barrier(0);  // (sixteen values in other registers at a time)
+            }
+          }
+        }
+      }
+      steps<32>([&](auto step) __attribute__((always_inline)) {
+        constexpr int n = decltype(step)::value, i = n >> 2, r = n & 3;
+        if constexpr (n == 32 - kLate) begin_scores(beyond);
+        if constexpr (n == 10) next_load = load_of(t + 3, page_next);
+        if constexpr (r == 0 && i + 2 < 8) fetch_v(v_from, i + 2);
+        accumulate<r == 0 || i == 0 || i == 4>(T{}, v[i % 3], p[r], o[i & 3][r]);
+        if constexpr (n % 5 == 3 && n < 20) {
+          // To the wave with the other half of the dims, the pairs that it weighs.
+          // (Everybody has read the last ones since barrier A; B lies between.  One
+          // such write keeps LDS busy for two products of all waves.)
+          constexpr int e = 4 * (n / 5);
+          lds_put(half_at + (wave ^ 2) * 4096 + lane16 + (n / 5) * 1024,
+                  u32x4_t{__float_as_uint(next[1][e]), __float_as_uint(next[1][e + 1]), __float_as_uint(next[1][e + 2]),
+                          __float_as_uint(next[1][e + 3])});
+        }
+        if constexpr (n >= 8 && n < 24) mine[n - 8] = moved_here(next[0][n - 8]);
+        if constexpr (i == 3) fetch_p(1, r);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < kLatentHalf; ++i) asm volatile("" : "+v"(q[i][r]));
+    page_t = page_1;
+    page_1 = page_2;
+    page_2 = page_next;
+    load = next_load;
+    const uint32_t done = now;
+    now = ahead;
+    ahead = beyond;
+    beyond = done;
+  };
+
+  lds_barrier();
+  seen_all = __builtin_amdgcn_readfirstlane(min(min(lds.least[0], lds.least[1]), min(lds.least[2], lds.least[3]))) / kKeys;
+  begin_scores(0);
+  page_1 = page_of(t0);
+  page_2 = page_of(t0 + 1);
+  load = load_of(t0 + 1, page_2);
+  for (int t = t0 - 1; t < t1; ++t) {
+    if ((t + 3) / kPageTiles - first_held >= 64) {
+      first_held = t / kPageTiles;
+      hold_pages();
+    }
+    round(t);   // (the last one's scores are of no tile, and nobody reads them)
   }
+  wait_loads<0>();
+  l_run = xor32_op(l_run, AddOp{});
+  lds_barrier();
+  float2* const rows = reinterpret_cast<float2*>(&lds.p[0]);
+  if (hh == 0) rows[m_mine] = make_float2(room == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
+  lds_barrier();
+  finish<T, 4>(a, w, s, false, rows, o);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAttentionArgs a) {
-  __shared__ Lds lds;
+  __shared__ __align__(16384) Lds lds;
   Plan w;
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int part = blockIdx.x;
   if (part >= *w.used) return;
-  const Start start = w.parts[part];
-  int64_t at = start.unit;
-  int at_span = start.span;
-  while (at < start.stop) {
-    Span s = w.spans[at_span];
+  const int64_t stop = uniform(w.parts[part].stop);
+  int64_t at = uniform(w.parts[part].unit);
+  int at_span = uniform(w.parts[part].span);
+  while (at < stop) {
+    Span s = uniform(w.spans[at_span]);
     int64_t end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
     while (at >= end) {
-      s = w.spans[++at_span];
+      s = uniform(w.spans[++at_span]);
       end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
     }
     const int units = s.tiles + kBegin;
-    const int64_t item = (at - s.unit0) / units;
+    const int64_t item = uniform((at - s.unit0) / units);
     const int64_t item_start = s.unit0 + item * units, item_end = item_start + units;
-    const int64_t seg_end = item_end < start.stop ? item_end : start.stop;
+    const int64_t seg_end = item_end < stop ? item_end : stop;
     auto tile_of = [&](int64_t u) { return u > kBegin ? static_cast<int>(u) - kBegin : 0; };
     Segment g;
     const int first = static_cast<int>(item) * kPairs;
@@ -601,16 +1029,18 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
     g.row = whole ? merge_row(w, s.merge, first, at_span >= a.groups) : part_row(w, part, at == item_start);
     g.row_step = whole ? 2 : 1;
     if (at_span >= a.groups) {  // a request's last row of the item sees the most
-      const int seen = (w.visible[(g.pair0 + g.count - 1) / a.heads] + kKeys - 1) / kKeys;
+      const int seen = (uniform(w.visible[(g.pair0 + g.count - 1) / a.heads]) + kKeys - 1) / kKeys;
       g.tile1 = g.tile1 < seen ? g.tile1 : seen;
       g.tile0 = g.tile0 < g.tile1 ? g.tile0 : g.tile1;
     }
-    if (g.count <= 32)
-      attend<T, 1>(a, w, g, lds);
+    if (g.tile0 >= g.tile1)
+      nothing<T>(a, w, g);
+    else if (g.count <= 32)
+      attend<T, 1>(a, w, g, lds.few);
     else if (g.count <= 64)
-      attend<T, 2>(a, w, g, lds);
+      attend<T, 2>(a, w, g, lds.few);
     else
-      attend<T, 4>(a, w, g, lds);
+      attend_many<T>(a, w, g, lds.many);
     at = seg_end;
   }
 }
