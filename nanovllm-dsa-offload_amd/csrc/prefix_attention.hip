@@ -32,6 +32,7 @@ constexpr int kTileLoads = 9;         // of a wave
 constexpr int kWindow = 1024;         // pages whose ids are held at a time
 constexpr int kParts = 256;           // workgroups, one per CU (LDS)
 constexpr int kBegin = 4;             // what the start of a segment costs, in tiles
+constexpr int kJoinByWave = 4096;     // pairs from which a wave joins one
 constexpr int kLeastTiles = 4;        // of a part
 constexpr int kLeastShared = 8;       // tiles of a prefix that is read once
 constexpr float kLog2e = 1.4426950408889634f;
@@ -55,10 +56,14 @@ struct Start {       // where a part begins
   int64_t stop;
   int32_t span;      // groups first, then requests
 };
+struct Cut {         // of all units into parts: the first `longer` ones hold one more
+  int32_t parts;     // (0: no units)
+  int32_t longer;
+  int64_t units;     // of the others
+};
 struct Plan {
   Start* parts;      // [kParts]
-  int32_t* used;     // [1]: parts in use
-  int64_t* total;    // [1]
+  Cut* cut;          // [1]
   Span* spans;       // [groups + batch]
   int32_t* visible;  // [rows]
   int32_t* request;  // [rows], -1: of no request
@@ -85,8 +90,7 @@ __host__ __device__ inline size_t carve(void* ws, int64_t rows, int64_t heads, i
   };
   Plan w;
   w.parts = reinterpret_cast<Start*>(take(sizeof(Start) * kParts));
-  w.used = reinterpret_cast<int32_t*>(take(sizeof(int32_t)));
-  w.total = reinterpret_cast<int64_t*>(take(sizeof(int64_t)));
+  w.cut = reinterpret_cast<Cut*>(take(sizeof(Cut)));
   w.spans = reinterpret_cast<Span*>(take(sizeof(Span) * (groups + batch)));
   w.visible = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * rows));
   w.request = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * rows));
@@ -100,13 +104,14 @@ __host__ __device__ inline size_t carve(void* ws, int64_t rows, int64_t heads, i
 
 __device__ inline int64_t items_of(const Span& s) { return (static_cast<int64_t>(s.pairs) + kPairs - 1) / kPairs; }
 __device__ inline int64_t units_of(const Span& s) { return items_of(s) * (s.tiles + kBegin); }
-__device__ inline int64_t part_start(int64_t total, int64_t parts, int64_t w) { return total * w / parts; }
-// The part of a unit.
-__device__ inline int part_of(int64_t total, int64_t parts, int64_t unit) {
-  int64_t w = unit * parts / total;
-  while (w + 1 < parts && part_start(total, parts, w + 1) <= unit) ++w;
-  while (w > 0 && part_start(total, parts, w) > unit) --w;
-  return static_cast<int>(w);
+__device__ inline int64_t part_start(const Cut& c, int w) { return w * c.units + (w < c.longer ? w : c.longer); }
+// The part of a unit.  (At most kParts of them, so that the guess is off by one at most.)
+__device__ inline int part_of(const Cut& c, int64_t unit) {
+  int w = static_cast<int>(static_cast<float>(unit) / (static_cast<float>(c.units) + static_cast<float>(c.longer) / static_cast<float>(c.parts)));
+  w = w < c.parts ? w : c.parts - 1;
+  while (w + 1 < c.parts && part_start(c, w + 1) <= unit) ++w;
+  while (w > 0 && part_start(c, w) > unit) --w;
+  return w;
 }
 // Values that every lane holds, in scalar registers.
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -127,147 +132,183 @@ __device__ inline int64_t merge_row(const Plan& w, int64_t merged, int pair, boo
 
 constexpr int kPlanThreads = 1024;
 
-__device__ inline int64_t plan_scan(int64_t v, int64_t* scratch, int64_t* total) {
+// Sums of what the threads before hold, of two values at once; *all_..: of everybody's.
+__device__ inline void plan_scan(int64_t& x, int64_t& y, int64_t (*scratch)[2], int64_t* all_x, int64_t* all_y) {
   const int wid = threadIdx.x >> 6;
-  const int64_t x = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(v)));
-  if ((threadIdx.x & 63) == 63) scratch[wid] = x;
+  const int64_t sx = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(x)));
+  const int64_t sy = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(y)));
   __syncthreads();
-  int64_t before = 0, all = 0;
-#pragma unroll
-  for (int k = 0; k < kPlanThreads / 64; ++k) {
-    before += k < wid ? scratch[k] : 0;
-    all += scratch[k];
+  if ((threadIdx.x & 63) == 63) {
+    scratch[wid][0] = sx;
+    scratch[wid][1] = sy;
   }
-  *total = all;
   __syncthreads();
-  return before + x - v;
+  int64_t before_x = 0, before_y = 0, sum_x = 0, sum_y = 0;
+  for (int k = 0; k < kPlanThreads / 64; ++k) {
+    const int64_t u = scratch[k][0], v = scratch[k][1];
+    before_x += k < wid ? u : 0;
+    before_y += k < wid ? v : 0;
+    sum_x += u;
+    sum_y += v;
+  }
+  *all_x = sum_x;
+  *all_y = sum_y;
+  x = before_x + sx - x;
+  y = before_y + sy - y;
 }
 
+// One workgroup, and latency all the way: what it reads comes to LDS at once (of
+// the first kPlanThreads requests and groups; the others' from memory).
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttentionArgs a) {
-  __shared__ int64_t scratch[kPlanThreads / 64];
+  __shared__ int64_t scratch[kPlanThreads / 64][2];
+  __shared__ int64_t unit0_of[2 * kPlanThreads];
+  __shared__ Span group_of[kPlanThreads];
+  __shared__ int32_t q_ends[kPlanThreads], group_ends[kPlanThreads];
   Plan w;
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int tid = threadIdx.x;
   const int64_t cap = a.cols * kBlock;
-  auto row_at = [&](int64_t b) -> int64_t {  // first packed row of request b
-    const int64_t r = b > 0 ? a.seq_q[b - 1] : 0;
-    return r < 0 ? 0 : (r > a.rows ? a.rows : r);
+  const int batch = static_cast<int>(a.batch), groups = static_cast<int>(a.groups), rows = static_cast<int>(a.rows);
+  const int heads = static_cast<int>(a.heads), spans = groups + batch;
+  auto clamp = [](int64_t x, int64_t most) { return static_cast<int>(x < 0 ? 0 : (x > most ? most : x)); };
+  int64_t own_length = 0, own_prefix = 0;  // of request and group tid
+  if (tid < batch) {
+    q_ends[tid] = a.seq_q[tid];
+    own_length = a.seq_kv[tid];
+  }
+  if (tid < groups) {
+    group_ends[tid] = a.group_ends[tid];
+    own_prefix = a.prefix_lens[tid];
+  }
+  __syncthreads();
+  auto row_at = [&](int b) {  // first packed row of request b
+    return b > 0 ? clamp(b <= kPlanThreads ? q_ends[b - 1] : a.seq_q[b - 1], rows) : 0;
   };
-  auto end_at = [&](int64_t g) -> int64_t {  // first request of group g
-    const int64_t b = g > 0 ? a.group_ends[g - 1] : 0;
-    return b < 0 ? 0 : (b > a.batch ? a.batch : b);
-  };
+  auto group_end = [&](int g) { return clamp(g < kPlanThreads ? group_ends[g] : a.group_ends[g], batch); };
+  auto length_of = [&](int b) { return clamp(b == tid ? own_length : a.seq_kv[b], cap); };
   int64_t units = 0, merged = 0, items = 0;
   // Groups: one that shares has a request's pages read for several of them, and
   // fewer pairs a request than an item holds (else every item is full anyway).
-  for (int64_t g0 = 0; g0 < a.groups; g0 += kPlanThreads) {
-    const int64_t g = g0 + tid;
+  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+    const int g = g0 + tid;
     Span s{};
-    s.merge = -1;
-    if (g < a.groups) {
-      const int64_t b0 = end_at(g), b1 = end_at(g + 1);
+    s.merge = s.group = -1;
+    if (g < groups) {
+      const int b0 = g > 0 ? group_end(g - 1) : 0, b1 = group_end(g);
       if (b1 - b0 >= 2) {
-        const int64_t r0 = row_at(b0), r1 = row_at(b1);
-        int64_t tokens = a.prefix_lens[g];
-        tokens = tokens < 0 ? 0 : (tokens > cap ? cap : tokens);
-        const int64_t tiles = tokens / kBlock * kPageTiles, pairs = (r1 - r0) * a.heads;
-        if (tiles >= kLeastShared && r1 > r0 && pairs < (b1 - b0) * kPairs) {
-          s.pair0 = static_cast<int32_t>(r0 * a.heads);
+        const int r0 = row_at(b0), r1 = row_at(b1);
+        const int tokens = clamp(g == tid ? own_prefix : a.prefix_lens[g], cap);
+        const int tiles = tokens / kBlock * kPageTiles;
+        const int64_t pairs = static_cast<int64_t>(r1 - r0) * heads;
+        if (tiles >= kLeastShared && r1 > r0 && pairs < static_cast<int64_t>(b1 - b0) * kPairs) {
+          s.pair0 = r0 * heads;
           s.pairs = static_cast<int32_t>(pairs);
-          s.tiles = static_cast<int32_t>(tiles);
-          s.table = static_cast<int32_t>(b0);
+          s.tiles = tiles;
+          s.table = b0;
         }
       }
     }
-    int64_t total;
-    s.unit0 = units + plan_scan(s.pairs > 0 ? units_of(s) : 0, scratch, &total);
-    units += total;
-    const int64_t m = plan_scan(s.pairs, scratch, &total);
+    int64_t none = 0, m = s.pairs, sum, sum_m;
+    plan_scan(m, none, scratch, &sum_m, &sum);
+    // (Ends that decrease could count a request's pairs for several groups: there
+    // is room for each pair once.)
+    if (merged + m + s.pairs > merge_pairs(rows, heads, batch)) s.pairs = 0;
     if (s.pairs > 0) s.merge = merged + m;
-    merged += total;
-    plan_scan(s.pairs > 0 ? items_of(s) : 0, scratch, &total);
-    items += total;
-    s.group = -1;
-    if (g < a.groups) w.spans[g] = s;
+    merged += sum_m;
+    int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
+    plan_scan(u, n, scratch, &sum_u, &sum_n);
+    s.unit0 = units + u;
+    units += sum_u;
+    items += sum_n;
+    if (g < groups) {
+      w.spans[g] = s;
+      if (g < kPlanThreads) group_of[g] = s;
+      if (g < 2 * kPlanThreads) unit0_of[g] = s.unit0;
+    }
   }
   __syncthreads();
-  for (int64_t at = 0; at < a.batch; at += kPlanThreads) {
-    const int64_t b = at + tid;
+  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
     Span s{};
-    s.merge = -1;
-    s.group = -1;
-    if (b < a.batch) {
-      const int64_t r0 = row_at(b), r1 = row_at(b + 1);
-      int64_t len = a.seq_kv[b];
-      len = len < 0 ? 0 : (len > cap ? cap : len);
-      s.pair0 = static_cast<int32_t>(r0 * a.heads);
-      s.pairs = r1 > r0 ? static_cast<int32_t>((r1 - r0) * a.heads) : 0;
-      s.tiles = static_cast<int32_t>((len + kKeys - 1) / kKeys);
-      s.table = static_cast<int32_t>(b);
+    s.merge = s.group = -1;
+    if (b < batch) {
+      const int r0 = row_at(b), r1 = row_at(b + 1);
+      s.pair0 = r0 * heads;
+      s.pairs = r1 > r0 ? (r1 - r0) * heads : 0;
+      s.tiles = (length_of(b) + kKeys - 1) / kKeys;
+      s.table = b;
       // The group: the first whose end lies behind the request.
-      int64_t lo = 0, hi = a.groups;
+      int lo = 0, hi = groups;
       while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.group_ends[mid] <= b)
+        const int mid = (lo + hi) >> 1;
+        if (group_end(mid) <= b)
           lo = mid + 1;
         else
           hi = mid;
       }
-      if (lo < a.groups && s.pairs > 0) {
-        const Span g = w.spans[lo];
+      if (lo < groups && s.pairs > 0) {
+        const Span g = lo < kPlanThreads ? group_of[lo] : w.spans[lo];
         // (Ends that decrease: a request outside the group's rows is its own.)
         if (g.pairs > 0 && b >= g.table && s.pair0 >= g.pair0 && s.pair0 + s.pairs <= g.pair0 + g.pairs) {
-          s.group = static_cast<int32_t>(lo);
+          s.group = lo;
           s.merge = g.merge + (s.pair0 - g.pair0);
           s.tile0 = g.tiles;
           s.tiles = s.tiles > g.tiles ? s.tiles - g.tiles : 0;
         }
       }
     }
-    int64_t total;
-    s.unit0 = units + plan_scan(s.pairs > 0 ? units_of(s) : 0, scratch, &total);
-    units += total;
-    plan_scan(s.pairs > 0 ? items_of(s) : 0, scratch, &total);
-    items += total;
-    if (b < a.batch) w.spans[a.groups + b] = s;
-  }
-  // What the rows see, a wave a request.
-  for (int64_t t = tid; t < a.rows; t += kPlanThreads)
-    if (t >= row_at(a.batch)) w.request[t] = -1;
-  for (int64_t b = tid >> 6; b < a.batch; b += kPlanThreads / 64) {
-    const int64_t r0 = row_at(b), r1 = row_at(b + 1);
-    int64_t len = a.seq_kv[b];
-    len = len < 0 ? 0 : (len > cap ? cap : len);
-    for (int64_t t = r0 + (tid & 63); t < r1; t += 64) {
-      const int64_t v = len - (r1 - 1 - t);
-      w.visible[t] = static_cast<int32_t>(v > 0 ? v : 0);
-      w.request[t] = static_cast<int32_t>(b);
+    int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
+    plan_scan(u, n, scratch, &sum_u, &sum_n);
+    s.unit0 = units + u;
+    units += sum_u;
+    items += sum_n;
+    if (b < batch) {
+      w.spans[groups + b] = s;
+      if (groups + b < 2 * kPlanThreads) unit0_of[groups + b] = s.unit0;
     }
   }
-  int64_t parts = (units - items * kBegin) / kLeastTiles;
-  if (parts < items) parts = items;
-  if (parts > kParts) parts = kParts;
-  if (parts < 1) parts = 1;
-  if (tid == 0) {
-    *w.used = units > 0 ? static_cast<int32_t>(parts) : 0;
-    *w.total = units;
+  // What the rows see.
+  for (int t = tid; t < rows; t += kPlanThreads) {
+    int lo = 0, hi = batch;  // the request: an end behind the row, the end before it not
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (row_at(mid + 1) <= t)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    int seen = 0;
+    if (lo < batch) {
+      seen = clamp(a.seq_kv[lo], cap) - (row_at(lo + 1) - 1 - t);
+      seen = seen > 0 ? seen : 0;
+    }
+    w.visible[t] = seen;
+    w.request[t] = lo < batch ? lo : -1;
   }
+  int64_t most = (units - items * kBegin) / kLeastTiles;
+  if (most < items) most = items;
+  Cut cut;
+  cut.parts = static_cast<int32_t>(most > kParts ? kParts : (most < 1 ? 1 : most));
+  cut.units = units / cut.parts;
+  cut.longer = static_cast<int32_t>(units - cut.units * cut.parts);
+  if (units == 0) cut.parts = 0;
+  if (tid == 0) *w.cut = cut;
   __syncthreads();
-  if (tid < parts && units > 0) {
+  if (tid < cut.parts) {
     Start p;
-    p.unit = part_start(units, parts, tid);
-    p.stop = part_start(units, parts, tid + 1);
+    p.unit = part_start(cut, tid);
+    p.stop = part_start(cut, tid + 1);
     // The last span that begins at or before the unit (spans without pairs begin
     // where the next does).
-    int64_t lo = 0, hi = a.groups + a.batch - 1;
+    int lo = 0, hi = spans - 1;
     while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (w.spans[mid].unit0 <= p.unit)
+      const int mid = (lo + hi + 1) >> 1;
+      if ((mid < 2 * kPlanThreads ? unit0_of[mid] : w.spans[mid].unit0) <= p.unit)
         lo = mid;
       else
         hi = mid - 1;
     }
-    p.span = static_cast<int32_t>(lo);
+    p.span = lo;
     w.parts[tid] = p;
   }
 }
@@ -296,7 +337,8 @@ union Lds {
   LdsFew few;
   LdsMany many;
 };
-static_assert(sizeof(Lds) <= 160 * 1024, "LDS");
+constexpr int kStage = 16 * 1024;                // of the tiles' place, of a wave before and after them
+static_assert(sizeof(Lds) <= 160 * 1024 && 4 * kStage <= 2 * kTileBytes, "LDS");
 static_assert(offsetof(LdsMany, keys) % 4096 == 0 && offsetof(LdsMany, rope) % 8192 == 0, "exclusive ors within");
 
 struct Segment {
@@ -363,6 +405,8 @@ __device__ inline void lds_put(uint32_t at, uint32_t x, uint32_t y) {
   typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
   *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(at) = u32x2_t{x, y};
 }
+// What this wave has written to LDS is there, and what it has asked for.
+__device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // Nothing is known of x from here on: what follows from it is worked out where it
 // is used, and holds no register across the loop.
 __device__ inline void forget(uint32_t& x) { asm volatile("" : "+v"(x)); }
@@ -386,11 +430,14 @@ __device__ inline u32x4_t finite_or_zero(u32x4_t v) {
   return v;
 }
 
-// A segment's outputs, or its partial sums; rows: references and sums of P.
+// A segment's outputs, or its partial sums; rows: references and sums of P.  A
+// wave's 128 dims of 32 pairs go through 16 KiB of LDS of its own (at `stage`, of
+// its wave), so that a store writes 512 neighbouring bytes of a pair and not 32.
+// Place c ^ pair of a pair's chunks of 16 bytes: neighbouring pairs' lie in other banks.
 template <typename T, int TILES>
-__device__ __forceinline__ void finish(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, bool empty,
-                                       const float2* rows, f32x16_t (&o)[4][TILES]) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+__device__ __forceinline__ void finish(const PrefixAttentionArgs& a, const Plan& w, const Segment& s,
+                                       const float2* rows, uint32_t stage, f32x16_t (&o)[4][TILES]) {
+  const int lane = own_thread() & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int d = 0; d < 4; ++d)
@@ -398,32 +445,45 @@ __device__ __forceinline__ void finish(const PrefixAttentionArgs& a, const Plan&
     for (int r = 0; r < TILES; ++r) settle(o[d][r]);
 #pragma unroll
   for (int r = 0; r < TILES; ++r) {
-    const int m = r * 32 + l32;
-    if (m >= s.count) continue;
-    const float2 row = rows[m];
+    if (r * 32 >= s.count) break;
+    const int left = s.count - r * 32;
     if (s.direct) {
-      const float by = row.y == 0.f ? 0.f : 1.f / row.y;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.pair0 + m) * kCkvDim + wave * 128 + 4 * hh;
+      const float sum = rows[r * 32 + l32].y, by = sum == 0.f ? 0.f : 1.f / sum;
+      const uint32_t to = stage + static_cast<uint32_t>(l32 * 256 + 8 * hh);
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint2*>(out + d * 32 + 8 * i) =
-              make_uint2(T::pack2(o[d][r][4 * i] * by, o[d][r][4 * i + 1] * by),
-                         T::pack2(o[d][r][4 * i + 2] * by, o[d][r][4 * i + 3] * by));
+          lds_put(to + (((d * 4 + i) ^ l32) & 15) * 16, T::pack2(o[d][r][4 * i] * by, o[d][r][4 * i + 1] * by),
+                  T::pack2(o[d][r][4 * i + 2] * by, o[d][r][4 * i + 3] * by));
+      wait_lds();
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.pair0 + r * 32) * kCkvDim + wave * 128 + (lane & 15) * 8;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int m = 4 * n + (lane >> 4);
+        const u32x4_t v = lds_get(stage + static_cast<uint32_t>(m * 256 + ((lane ^ m) & 15) * 16));
+        if (m < left) *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(m) * kCkvDim) = v;
+      }
     } else {
-      const int64_t at = s.row + m * s.row_step;
-      if (wave == 0 && hh == 0) w.refs[at] = row;
-      if (!empty) {
-        float* out = w.sums + at * kCkvDim + wave * 128 + 4 * hh;
+      if (wave == 0 && hh == 0 && l32 < left) w.refs[s.row + (r * 32 + l32) * s.row_step] = rows[r * 32 + l32];
+      const uint32_t to = stage + static_cast<uint32_t>(l32 * 512);
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+      for (int d = 0; d < 4; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(out + d * 32 + 8 * i) =
-                make_float4(o[d][r][4 * i], o[d][r][4 * i + 1], o[d][r][4 * i + 2], o[d][r][4 * i + 3]);
+        for (int i = 0; i < 4; ++i)
+          lds_put(to + ((d * 8 + i * 2 + hh) ^ l32) * 16,
+                  u32x4_t{__float_as_uint(o[d][r][4 * i]), __float_as_uint(o[d][r][4 * i + 1]),
+                          __float_as_uint(o[d][r][4 * i + 2]), __float_as_uint(o[d][r][4 * i + 3])});
+      wait_lds();
+      float* out = w.sums + (s.row + r * 32 * s.row_step) * kCkvDim + wave * 128 + l32 * 4;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        const int m = 2 * n + hh;
+        const u32x4_t v = lds_get(stage + static_cast<uint32_t>(m * 512 + (l32 ^ m) * 16));
+        if (m < left) *reinterpret_cast<u32x4_t*>(out + m * s.row_step * kCkvDim) = v;
       }
     }
+    if (r + 1 < TILES) wait_lds();
   }
 }
 
@@ -667,7 +727,7 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     if (hh == 0) lds.row[m_mine] = make_float2(most == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
   }
   lds_barrier();
-  finish<T, TILES>(a, w, s, t0 >= t1, lds.row, o);
+  finish<T, TILES>(a, w, s, lds.row, lds_keys + wave * kStage, o);
 }
 
 // Items of more than 64 pairs, bound by their products.  For the scores of a tile
@@ -749,16 +809,23 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   // 256-byte group g, for two tiles of 32 pairs, first those that the wave weighs.
   // The rope dims, the last two steps, lie in LDS, for which there is room, and not
   // in registers, for which there is none.
+  // They come through LDS, 32 pairs at a time in the wave's own 16 KiB of tiles that
+  // are not there yet: a load takes two pairs' 512 neighbouring bytes, where loads
+  // to the registers would take 32 bytes of 32 pairs.
   u32x4_t q[kLatentHalf][2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int m = rg * 64 + (r ^ dh) * 32 + l32;
-    const int64_t pair = s.pair0 + (m < s.count ? m : 0);
-    const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + dh * 32 + hh;
+    const int first = rg * 64 + (r ^ dh) * 32;
+    const uint32_t stage = keys_at + kTileBytes + wave * kStage;
+    const uint8_t* from = static_cast<const uint8_t*>(a.query) + s.pair0 * kCkvBytes + dh * 512;
 #pragma unroll
-    for (int i = 0; i < kLatentHalf; ++i) {
-      q[i][r] = qn[(i & 1) * 16 + (i >> 1) * 2];
+    for (int n = 0; n < 16; ++n) {
+      const int in = 2 * n + hh, m = first + in < s.count ? first + in : 0;
+      load_to_lds(from, static_cast<uint32_t>(m * kCkvBytes + (l32 ^ in) * 16), stage + n * 1024);
     }
+    wait_loads<0>();
+#pragma unroll
+    for (int i = 0; i < kLatentHalf; ++i) q[i][r] = lds_get(stage + static_cast<uint32_t>(l32 * 512 + (((i & 1) * 16 + (i >> 1) * 2 + hh) ^ l32) * 16));
 #pragma unroll
     for (int i = 0; i < kLatentHalf; ++i) asm volatile("" : "+v"(q[i][r]));
   }
@@ -992,7 +1059,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   float2* const rows = reinterpret_cast<float2*>(&lds.p[0]);
   if (hh == 0) rows[m_mine] = make_float2(room == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
   lds_barrier();
-  finish<T, 4>(a, w, s, false, rows, o);
+  finish<T, 4>(a, w, s, rows, keys_at + wave * kStage, o);
 }
 
 template <typename T>
@@ -1001,7 +1068,7 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
   Plan w;
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int part = blockIdx.x;
-  if (part >= *w.used) return;
+  if (part >= w.cut->parts) return;
   const int64_t stop = uniform(w.parts[part].stop);
   int64_t at = uniform(w.parts[part].unit);
   int at_span = uniform(w.parts[part].span);
@@ -1046,22 +1113,24 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
 }
 
 // -------------------------------------------------------------------- the join
-// A wave a pair: its segments' references, then their sums.
-template <typename T>
+// WAVES waves a pair: its segments' references, then their sums, four at a time on
+// their way, every wave those of its turn.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a) {
+  __shared__ float4 others[WAVES > 1 ? 4 : 1][2][64];
   Plan w;
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int lane = threadIdx.x & 63;
-  const int pair = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), turn = wave % WAVES;
+  const int pair = static_cast<int>(blockIdx.x) * (4 / WAVES) + wave / WAVES;
   const int heads = static_cast<int>(a.heads);
   if (pair >= a.rows * a.heads) return;
   const int b = w.request[pair / heads];
   if (b < 0) return;
-  const int64_t total = *w.total, parts = *w.used;
+  const Cut cut = *w.cut;
   const Span own = w.spans[a.groups + b];
   struct Run {  // segments of one item
     int w0, n;
-    bool begins;      // the item begins in part w0
     int64_t whole;    // row of the sums where there is one segment
     int m;
   };
@@ -1069,8 +1138,8 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
     Run r;
     const int in = pair - s.pair0, item = in / kPairs;
     const int64_t units = s.tiles + kBegin, u0 = s.unit0 + item * units;
-    r.w0 = part_of(total, parts, u0);
-    r.n = part_of(total, parts, u0 + units - 1) - r.w0 + 1;
+    r.w0 = part_of(cut, u0);
+    r.n = part_of(cut, u0 + units - 1) - r.w0 + 1;
     r.m = in - item * kPairs;
     r.whole = r.n == 1 ? merge_row(w, s.merge, in, is_own) : -1;
     return r;
@@ -1079,7 +1148,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
   if (own.group < 0 && mine.n == 1) return;  // (written by the attention itself)
   Run shared{};
   if (own.group >= 0) shared = run_of(w.spans[own.group], false);
-  const int n = mine.n + shared.n;
+  const int n = mine.n + shared.n;  // (at most 2 kParts)
   auto row_of = [&](int k) -> int64_t {
     const Run& r = k < shared.n ? shared : mine;
     const int j = k < shared.n ? k : k - shared.n;
@@ -1102,20 +1171,50 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
     const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - top);
     l += wave_all_op(f == 0.f ? 0.f : v.y * f, AddOp{});
     const int count = n - k0 < 64 ? n - k0 : 64;
-    for (int k = 0; k < count; ++k) {
-      const float fk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), k));
-      if (fk == 0.f) continue;  // (a part without tiles wrote no sums)
-      const int64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(row), k));
-      const float4* p = reinterpret_cast<const float4*>(w.sums + lo * kCkvDim) + lane;
-      const float4 x = p[0], y = p[64];
-      acc[0] = fmaf(x.x, fk, acc[0]);
-      acc[1] = fmaf(x.y, fk, acc[1]);
-      acc[2] = fmaf(x.z, fk, acc[2]);
-      acc[3] = fmaf(x.w, fk, acc[3]);
-      acc[4] = fmaf(y.x, fk, acc[4]);
-      acc[5] = fmaf(y.y, fk, acc[5]);
-      acc[6] = fmaf(y.z, fk, acc[6]);
-      acc[7] = fmaf(y.w, fk, acc[7]);
+    for (int k = turn; k < count; k += 4 * WAVES) {
+      float4 x[4][2];
+      float by[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = k + u * WAVES;  // (lanes from `count` on hold row 0 and a factor of zero)
+        by[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), at & 63));
+        by[u] = at < count ? by[u] : 0.f;
+        const int64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(row), at & 63));
+        const float4* p = reinterpret_cast<const float4*>(w.sums + lo * kCkvDim) + lane;
+        x[u][0] = p[0];
+        x[u][1] = p[64];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (by[u] == 0.f) continue;  // (a part without tiles wrote no sums)
+        acc[0] = fmaf(x[u][0].x, by[u], acc[0]);
+        acc[1] = fmaf(x[u][0].y, by[u], acc[1]);
+        acc[2] = fmaf(x[u][0].z, by[u], acc[2]);
+        acc[3] = fmaf(x[u][0].w, by[u], acc[3]);
+        acc[4] = fmaf(x[u][1].x, by[u], acc[4]);
+        acc[5] = fmaf(x[u][1].y, by[u], acc[5]);
+        acc[6] = fmaf(x[u][1].z, by[u], acc[6]);
+        acc[7] = fmaf(x[u][1].w, by[u], acc[7]);
+      }
+    }
+  }
+  if constexpr (WAVES > 1) {  // (every wave of the workgroup is here, or none: they have one pair)
+    static_assert(WAVES == 4, "a workgroup a pair");
+    others[wave][0][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    others[wave][1][lane] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const float4 x = others[k][0][lane], y = others[k][1][lane];
+      acc[0] += x.x;
+      acc[1] += x.y;
+      acc[2] += x.z;
+      acc[3] += x.w;
+      acc[4] += y.x;
+      acc[5] += y.y;
+      acc[6] += y.z;
+      acc[7] += y.w;
     }
   }
   const float by = l == 0.f ? 0.f : 1.f / l;
@@ -1132,8 +1231,11 @@ hipError_t launch(const PrefixAttentionArgs& a, hipStream_t stream) {
   launch_kernel(kKernPrefixAttention, prefix_attention_kernel<T>, dim3(kParts), dim3(kThreads), stream, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  launch_kernel(kKernPrefixJoin, prefix_join_kernel<T>, dim3(static_cast<uint32_t>(ceil_div(a.rows * a.heads, 4))), dim3(256),
-                stream, a);
+  if (a.rows * a.heads < kJoinByWave)
+    launch_kernel(kKernPrefixJoin, prefix_join_kernel<T, 4>, dim3(static_cast<uint32_t>(a.rows * a.heads)), dim3(256), stream, a);
+  else
+    launch_kernel(kKernPrefixJoin, prefix_join_kernel<T, 1>, dim3(static_cast<uint32_t>(ceil_div(a.rows * a.heads, 4))), dim3(256),
+                  stream, a);
   return hipGetLastError();
 }
 
