@@ -29,7 +29,6 @@ constexpr int kCkvBytes = kCkvDim * 2, kKpeBytes = kKpeDim * 2;
 constexpr int kTileBytes = kKeys * (kCkvBytes + kKpeBytes);
 constexpr int kSteps = kQkDim / 16;   // products of 16 dims: 32 of the latent, 4 of the rope
 constexpr int kTileLoads = 9;         // of a wave
-constexpr int kWindow = 1024;         // pages whose ids are held at a time
 constexpr int kParts = 256;           // workgroups, one per CU (LDS)
 constexpr int kBegin = 4;             // what the start of a segment costs, in tiles
 constexpr int kJoinByWave = 4096;     // pairs from which a wave joins one
@@ -316,10 +315,10 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
 // ------------------------------------------------------------- the attention
 struct LdsFew {   // items of up to 64 pairs
   alignas(16) uint8_t keys[kBuffers][kTileBytes];
-  alignas(16) uint16_t p[kPairs * kKeys];
-  float factor[kPairs];
-  float2 row[kPairs];   // reference and sum of P, at a segment's end
-  int32_t pages[kWindow];
+  alignas(16) uint16_t p[64 * kKeys];
+  float factor[64];
+  float2 row[64];       // reference and sum of P, at a segment's end
+  float top[2][32];     // of 16 keys each
   int32_t moved[4];     // a wave's rows have new references
   int32_t least[4];     // the least that a row of a wave sees
 };
@@ -349,6 +348,26 @@ struct Segment {
   bool direct;        // the output itself
   int64_t row;        // of the partial sums
   int64_t row_step;   // between pairs of it
+};
+
+// The ids of 64 pages, a lane each (-1: none), from a column on.
+struct Pages {
+  const int32_t* table;
+  int32_t last, blocks;   // column
+  int32_t first, held;
+  __device__ Pages(const Segment& s, const PrefixAttentionArgs& a) : table(s.table), blocks(static_cast<int32_t>(a.blocks)) {
+    const int c = (s.tile1 - 1) / kPageTiles;
+    last = c < a.cols ? c : static_cast<int32_t>(a.cols) - 1;
+    hold(s.tile0);
+  }
+  __device__ void hold(int tile) {
+    first = tile / kPageTiles;
+    const int c = first + (threadIdx.x & 63);
+    const int32_t page = c <= last ? table[c] : -1;
+    held = page >= 0 && page < blocks ? page : -1;
+  }
+  __device__ bool holds(int tile) const { return tile / kPageTiles - first < 64; }
+  __device__ int of(int tile) const { return __builtin_amdgcn_readlane(held, tile / kPageTiles - first); }
 };
 
 // o += a b, with o in accumulation registers: 256 of them hold four tiles of
@@ -498,14 +517,21 @@ __device__ __forceinline__ void nothing(const PrefixAttentionArgs& a, const Plan
   }
 }
 
+// Items of up to 32 TILES pairs, bound by the tiles' way from memory.  For the
+// scores of a tile a wave takes 16 pairs, with their queries in registers: all 32
+// keys of it where there are 64 pairs, 16 keys where there are 32 (two waves then
+// meet in LDS for a row's largest score).  For the outputs it takes 128 dims of
+// all pairs.  At barrier A everybody is done with tile t - 1, and tile t + 1 and
+// the largest scores of tile t have arrived; then tile t + 3 is asked for and tile
+// t weighed; at B its P is there, and its outputs and the scores of tile t + 1 follow.
 template <typename T, int TILES>
 __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, LdsFew& lds) {
   const int tid = own_thread();
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, hh = lane >> 5;
-  const bool scores = wave < TILES;   // the wave has pairs of its own
-  const int m_mine = wave * 32 + l32;
+  const int l32 = lane & 31, hh = lane >> 5, l16 = lane & 15, quad = lane >> 4;
+  const int m_mine = (TILES == 2 ? wave : wave & 1) * 16 + l16;
+  const int half0 = TILES == 2 ? 0 : wave >> 1;   // first 16 keys of the wave's
   const uint32_t lds_keys = lds_address(lds.keys);
 
   // A row k of a tile holds chunk c (16 bytes) at place c ^ swizzle(k) within its
@@ -520,34 +546,27 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     const int k = wave * 8 + (lane >> 3);
     rope_byte = static_cast<uint32_t>(k * kKpeBytes + ((lane ^ (k >> 1)) & 7) * 16);
   }
-  const uint32_t k_at = static_cast<uint32_t>(l32 * kCkvBytes + ((hh ^ swizzle(l32)) & 15) * 16);
-  const uint32_t r_at = static_cast<uint32_t>(kKeys * kCkvBytes + l32 * kKpeBytes + ((hh ^ (l32 >> 1)) & 7) * 16);
+  const int k_row = half0 * 16 + l16;
+  const uint32_t k_at = lds_keys + static_cast<uint32_t>(k_row * kCkvBytes + ((quad ^ swizzle(l16)) & 15) * 16);
+  const uint32_t r_at = lds_keys + static_cast<uint32_t>(kKeys * kCkvBytes + k_row * kKpeBytes + ((quad ^ (l16 >> 1)) & 7) * 16);
   uint32_t v_at[2];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int key = 8 * hh + 4 * part + ((lane & 15) >> 2);
     const int c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);   // of four neighbours
-    v_at[part] = static_cast<uint32_t>(key * kCkvBytes + wave * 256 + ((c ^ swizzle(key)) & 15) * 16 + (lane & 1) * 8);
+    v_at[part] = lds_keys + static_cast<uint32_t>(key * kCkvBytes + wave * 256 + ((c ^ swizzle(key)) & 15) * 16 + (lane & 1) * 8);
   }
-  const uint32_t p_read = static_cast<uint32_t>(l32 * 64), p_swz = (l32 >> 2) & 3;
+  const uint32_t p_at = lds_address(lds.p);
+  const uint32_t p_read = p_at + static_cast<uint32_t>(l32 * 64), p_swz = (l32 >> 2) & 3;
+  const uint32_t p_write = p_at + static_cast<uint32_t>(m_mine * 64 + (quad & 1) * 8);
 
-  int page0 = s.tile0 / kPageTiles;   // of the window
-  auto fill_window = [&] {
-    for (int i = tid; i < kWindow; i += kThreads) {
-      const int64_t c = page0 + i;
-      int32_t page = -1;
-      if (c < a.cols && c * kPageTiles < s.tile1) page = s.table[c];
-      lds.pages[i] = page >= 0 && page < a.blocks ? page : -1;
-    }
-  };
-  auto page_of = [&](int tile) { return __builtin_amdgcn_readfirstlane(lds.pages[tile / kPageTiles - page0]); };
+  Pages pages(s, a);
   auto load_tile = [&](int tile) {
-    int page = page_of(tile);
+    int page = pages.of(tile);
     page = page < 0 ? 0 : page;
-    const uint8_t* base = static_cast<const uint8_t*>(a.kv_cache) +
-                          (static_cast<int64_t>(page) * kBlock + (tile % kPageTiles) * kKeys) * kCkvBytes;
-    const uint8_t* rope = static_cast<const uint8_t*>(a.k_rope) +
-                          (static_cast<int64_t>(page) * kBlock + (tile % kPageTiles) * kKeys) * kKpeBytes;
+    const int64_t row = static_cast<int64_t>(page) * kBlock + (tile % kPageTiles) * kKeys;
+    const uint8_t* base = static_cast<const uint8_t*>(a.kv_cache) + row * kCkvBytes;
+    const uint8_t* rope = static_cast<const uint8_t*>(a.k_rope) + row * kKpeBytes;
     const uint32_t to = lds_keys + (tile % kBuffers) * kTileBytes + wave * 1024;
 #pragma unroll
     for (int i = 0; i < 8; ++i) load_to_lds(base + i * 4096, byte_of[i & 3], to + i * 4096);
@@ -555,91 +574,101 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   };
 
   lds_barrier();  // (the segment before is done with LDS)
-  fill_window();
-  __syncthreads();
   const int t0 = s.tile0, t1 = s.tile1;
 #pragma unroll
   for (int k = 0; k < 3; ++k)
     if (t0 + k < t1) load_tile(t0 + k);
 
-  u32x4_t q[kSteps];
-  int vis = 0;
-  if (scores) {
-    const int64_t pair = s.pair0 + (m_mine < s.count ? m_mine : 0);
-    vis = m_mine < s.count ? w.visible[pair / a.heads] : 0;
-    const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + hh;
-    const u32x4_t* qr = static_cast<const u32x4_t*>(a.query_rope) + pair * (kKpeDim / 8) + hh;
+  constexpr int kWide = kQkDim / 32, kWideLatent = kCkvDim / 32;   // products of 32 dims
+  u32x4_t q[kWide];
+  const int64_t pair = s.pair0 + (m_mine < s.count ? m_mine : 0);
+  const int vis = m_mine < s.count ? w.visible[pair / a.heads] : 0;
+  {
+    const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + quad;
+    const u32x4_t* qr = static_cast<const u32x4_t*>(a.query_rope) + pair * (kKpeDim / 8) + quad;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) q[j] = j < 32 ? qn[2 * j] : qr[2 * (j - 32)];
+    for (int j = 0; j < kWide; ++j) q[j] = j < kWideLatent ? qn[4 * j] : qr[4 * (j - kWideLatent)];
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) asm volatile("" : "+v"(q[j]));
   }
-  f32x16_t o[4][TILES], sc;
+  f32x16_t o[4][TILES];
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < TILES; ++r)
+    for (int r = 0; r < TILES; ++r) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][r][e] = 0.f;
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int r = 0; r < TILES; ++r) settle(o[d][r]);
+      settle(o[d][r]);
+    }
   float ref = 0.f, most = -INFINITY, l_run = 0.f;   // most: what a score may reach before the reference moves
   // The least that a row of this wave sees; every wave's meet in LDS.
-  int vis_least = scores && m_mine < s.count ? vis : 0x7fffffff;
+  int vis_least = m_mine < s.count ? vis : 0x7fffffff;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) vis_least = min(vis_least, __shfl_xor(vis_least, d));
+  for (int d = 1; d < 16; d <<= 1) vis_least = min(vis_least, __shfl_xor(vis_least, d));
   vis_least = __builtin_amdgcn_readfirstlane(vis_least);
   if (lane == 0) lds.least[wave] = vis_least;
 
-  auto multiply = [&](int tile, f32x16_t& to) {
-    const uint8_t* k_tile = lds.keys[tile % kBuffers];
+  f32x4_t x[TILES];   // scores of key 16 (half0 + h) + 4 quad + e
+  float top;
+  auto score = [&](int tile) {
+    const uint32_t at = (tile % kBuffers) * kTileBytes;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) to[e] = 0.f;
+    for (int h = 0; h < TILES; ++h)
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const uint32_t at = j < 32 ? (k_at ^ ((j & 7) * 32)) + (j >> 3) * 256 : r_at ^ ((j - 32) * 32);
-      const u32x4_t k = *reinterpret_cast<const u32x4_t*>(k_tile + at);
-      to = T::mfma32(__builtin_bit_cast(typename T::vec8, k), __builtin_bit_cast(typename T::vec8, q[j]), to);
-    }
-  };
-  // Scores of a tile to P, against the row's reference.
-  auto weigh = [&](int tile, f32x16_t& x) {
-    const bool none = page_of(tile) < 0;
+      for (int e = 0; e < 4; ++e) x[h][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] *= a.scale * kLog2e;
-    if (none || (tile + 1) * kKeys > vis_least) {
+    for (int j = 0; j < kWide; ++j) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = tile * kKeys + 8 * (e >> 2) + 4 * hh + (e & 3);
-        x[e] = !none && key < vis ? x[e] : -INFINITY;
+      for (int h = 0; h < TILES; ++h) {
+        const u32x4_t k = j < kWideLatent ? lds_get(((k_at + at) ^ ((j & 3) * 64)) + (j >> 2) * 256 + h * 16 * kCkvBytes)
+                                          : lds_get(((r_at + at) ^ ((j - kWideLatent) * 64)) + h * 16 * kKpeBytes);
+        x[h] = T::mfma16(__builtin_bit_cast(typename T::vec8, k), __builtin_bit_cast(typename T::vec8, q[j]), x[h]);
       }
     }
-    float top = x[0];
+    const bool none = pages.of(tile) < 0;
 #pragma unroll
-    for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-    top = xor32_op(top, MaxOp{});
+    for (int h = 0; h < TILES; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[h][e] *= a.scale * kLog2e;
+    if (none || (tile + 1) * kKeys > vis_least) {
+      const int left = none ? 0 : vis - tile * kKeys - 16 * half0 - 4 * quad;   // keys that the row sees, from the lane's first
+#pragma unroll
+      for (int h = 0; h < TILES; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[h][e] = 16 * h + e < left ? x[h][e] : -INFINITY;
+    }
+    top = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+    if constexpr (TILES == 2) top = fmaxf(top, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    top = xor32_op(xor16_op(top, MaxOp{}), MaxOp{});
+    if constexpr (TILES == 1)
+      if (quad == 0) lds.top[half0][m_mine] = top;
+  };
+  // Scores to P, against the row's reference.
+  auto weigh = [&] {
+    if constexpr (TILES == 1) top = fmaxf(lds.top[0][m_mine], lds.top[1][m_mine]);
     const bool past = top > most;
-    const bool any = __any(past);
-    if (any) {
-      const float now = past ? top - kRise : ref;
-      const float f = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
-      if (past) most = now + kMost;
+    float f = 1.f;
+    if (past) {
+      const float now = top - kRise;
+      f = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
+      most = now + kMost;
       ref = now;
       l_run *= f;
-      if (hh == 0) lds.factor[m_mine] = f;
     }
-    if (lane == 0) lds.moved[wave] = any;
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[e] = __builtin_amdgcn_exp2f(x[e] - ref);
-      sum += x[e];
+    const bool any = __any(past);
+    if (half0 == 0) {
+      if (quad == 0) lds.factor[m_mine] = f;
+      if (lane == 0) lds.moved[wave] = any;
     }
-    l_run += sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint2 u = make_uint2(T::pack2(x[4 * i], x[4 * i + 1]), T::pack2(x[4 * i + 2], x[4 * i + 3]));
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(lds.p) + m_mine * 64 + ((i ^ p_swz) * 16) + hh * 8) = u;
+    for (int h = 0; h < TILES; ++h) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[h][e] = __builtin_amdgcn_exp2f(x[h][e] - ref);
+        l_run += x[h][e];
+      }
+      const int chunk = 2 * (half0 + h) + (quad >> 1);
+      lds_put(p_write + static_cast<uint32_t>(((chunk ^ (m_mine >> 2)) & 3) * 16), T::pack2(x[h][0], x[h][1]), T::pack2(x[h][2], x[h][3]));
     }
   };
   // Values of keys that some row must not see: P is zero there, but zero times an
@@ -652,22 +681,18 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     }
   };
   auto output = [&](int tile) {
-    const uint8_t* v_tile = lds.keys[tile % kBuffers];
+    const uint32_t at = (tile % kBuffers) * kTileBytes;
     const int4 moved = *reinterpret_cast<const int4*>(lds.moved);
-    const int any = moved.x | (TILES > 1 ? moved.y : 0) | (TILES > 2 ? moved.z | moved.w : 0);
-    if (__builtin_amdgcn_readfirstlane(any) != 0) {
 #pragma unroll
-      for (int r = 0; r < TILES; ++r) {
-        const int mine = r == 0 ? moved.x : (r == 1 ? moved.y : (r == 2 ? moved.z : moved.w));
-        if (__builtin_amdgcn_readfirstlane(mine) != 0) {
-          const float f = lds.factor[r * 32 + l32];
+    for (int r = 0; r < TILES; ++r) {
+      if (__builtin_amdgcn_readfirstlane(r == 0 ? moved.x | moved.y : moved.z | moved.w) != 0) {
+        const float f = lds.factor[r * 32 + l32];
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            settle(o[d][r]);
+        for (int d = 0; d < 4; ++d) {
+          settle(o[d][r]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][r][e] *= f;
-            settle(o[d][r]);
-          }
+          for (int e = 0; e < 16; ++e) o[d][r][e] *= f;
+          settle(o[d][r]);
         }
       }
     }
@@ -675,13 +700,11 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     for (int ks = 0; ks < 2; ++ks) {
       u32x4_t p[TILES];
 #pragma unroll
-      for (int r = 0; r < TILES; ++r)
-        p[r] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(lds.p) + r * 2048 + p_read +
-                                                          (((2 * ks + hh) ^ p_swz) * 16));
+      for (int r = 0; r < TILES; ++r) p[r] = lds_get(p_read + r * 2048 + static_cast<uint32_t>(((2 * ks + hh) ^ p_swz) * 16));
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const uint2 lo = read_tr16(v_tile + (v_at[0] ^ (d * 64)) + ks * 16 * kCkvBytes);
-        const uint2 hi = read_tr16(v_tile + (v_at[1] ^ (d * 64)) + ks * 16 * kCkvBytes);
+        const uint2 lo = read_tr16(((v_at[0] + at) ^ (d * 64)) + ks * 16 * kCkvBytes);
+        const uint2 hi = read_tr16(((v_at[1] + at) ^ (d * 64)) + ks * 16 * kCkvBytes);
         const u32x4_t v{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
         for (int r = 0; r < TILES; ++r) accumulate<true>(T{}, v, p[r], o[d][r]);
@@ -689,43 +712,33 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     }
   };
 
-  if (t0 < t1) {
-    if (t0 + 2 < t1)
+  wait_loads<0>();
+  lds_barrier();
+  const int vis_all = __builtin_amdgcn_readfirstlane(min(min(lds.least[0], lds.least[1]), min(lds.least[2], lds.least[3])));
+  score(t0);
+  for (int t = t0; t < t1; ++t) {
+    if (t + 2 < t1)
       wait_loads<kTileLoads>();
     else
       wait_loads<0>();
-    lds_barrier();
-    const int vis_all = __builtin_amdgcn_readfirstlane(
-        min(min(lds.least[0], lds.least[1]), min(lds.least[2], lds.least[3])));
-    if (scores) multiply(t0, sc);
-    for (int t = t0; t < t1; ++t) {
-      f32x16_t next;
-      if (scores && t + 1 < t1) multiply(t + 1, next);
-      lds_barrier();  // every wave is done with tile t - 1 and its P
-      if (t + 3 < t1) {
-        if ((t + 3) / kPageTiles >= page0 + kWindow) {
-          page0 = t / kPageTiles;
-          fill_window();
-          __syncthreads();
-        }
-        load_tile(t + 3);
-      }
-      if (scores) weigh(t, sc);
-      if ((t + 1) * kKeys > vis_all || page_of(t) < 0) scrub(t);
-      if (t + 3 < t1)
-        wait_loads<kTileLoads>();
-      else
-        wait_loads<0>();
-      lds_barrier();
-      output(t);
-      sc = next;
-    }
+    lds_barrier();  // A
+    if (!pages.holds(t + 3)) pages.hold(t);
+    if (t + 3 < t1) load_tile(t + 3);
+    weigh();
+    if ((t + 1) * kKeys > vis_all || pages.of(t) < 0) scrub(t);
+    lds_barrier();  // B
+    output(t);
+    if (t + 1 < t1) score(t + 1);
   }
   // References and sums of the rows, to every wave.
-  if (scores) {
-    l_run = xor32_op(l_run, AddOp{});
-    if (hh == 0) lds.row[m_mine] = make_float2(most == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
+  l_run = xor32_op(xor16_op(l_run, AddOp{}), AddOp{});
+  if constexpr (TILES == 1) {
+    lds_barrier();
+    if (half0 == 1 && quad == 0) lds.top[0][m_mine] = l_run;
+    lds_barrier();
+    l_run += lds.top[0][m_mine];
   }
+  if (half0 == 0 && quad == 0) lds.row[m_mine] = make_float2(most == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
   lds_barrier();
   finish<T, TILES>(a, w, s, lds.row, lds_keys + wave * kStage, o);
 }
@@ -768,15 +781,8 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   uint32_t p_read = lds_address(lds.p) + static_cast<uint32_t>(l32 * 64 + ((hh ^ p_swz) & 3) * 16);
   uint32_t p_write = lds_address(lds.p) + static_cast<uint32_t>(m_mine * 64 + p_swz * 16 + hh * 8);
 
-  // The ids of 64 pages, a lane each (-1: none), from column `first_held` on.
-  const int last_column = (s.tile1 - 1) / kPageTiles < a.cols ? (s.tile1 - 1) / kPageTiles : static_cast<int>(a.cols) - 1;
-  int first_held = s.tile0 / kPageTiles, held = -1;
-  auto hold_pages = [&] {
-    const int c = first_held + (own_thread() & 63);
-    const int32_t page = c <= last_column ? s.table[c] : -1;
-    held = page >= 0 && page < a.blocks ? page : -1;
-  };
-  auto page_of = [&](int tile) { return __builtin_amdgcn_readlane(held, tile / kPageTiles - first_held); };
+  Pages pages(s, a);
+  auto page_of = [&](int tile) { return pages.of(tile); };
   // A tile's loads, nine of a wave: pairs of keys, and the rope dims.
   struct Load {
     const uint8_t* base;
@@ -797,7 +803,6 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
       load_to_lds<0>(l.rope, rope_byte, lds_rope + buffer);
   };
 
-  hold_pages();
   lds_barrier();  // (the segment before is done with LDS)
   const int t0 = s.tile0, t1 = s.tile1;
   {
@@ -1047,10 +1052,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   page_2 = page_of(t0 + 1);
   load = load_of(t0 + 1, page_2);
   for (int t = t0 - 1; t < t1; ++t) {
-    if ((t + 3) / kPageTiles - first_held >= 64) {
-      first_held = t / kPageTiles;
-      hold_pages();
-    }
+    if (!pages.holds(t + 3)) pages.hold(t);
     round(t);   // (the last one's scores are of no tile, and nobody reads them)
   }
   wait_loads<0>();
