@@ -30,9 +30,10 @@ constexpr int kTileBytes = kKeys * (kCkvBytes + kKpeBytes);
 constexpr int kSteps = kQkDim / 16;   // products of 16 dims: 32 of the latent, 4 of the rope
 constexpr int kTileLoads = 9;         // of a wave
 constexpr int kParts = 256;           // workgroups, one per CU (LDS)
-constexpr int kBegin = 4;             // what the start of a segment costs, in tiles
+constexpr int kBegin = 8;             // what the start of a segment costs, in tiles
 constexpr int kJoinByWave = 4096;     // pairs from which a wave joins one
 constexpr int kLeastTiles = 4;        // of a part
+constexpr int kEasyParts = 8;         // parts of an item that may hold fewer: the join has them all on their way at once
 constexpr int kLeastShared = 8;       // tiles of a prefix that is read once
 constexpr float kLog2e = 1.4426950408889634f;
 // P = 2^(score - reference): a reference is set so that the largest P of its
@@ -112,6 +113,13 @@ __device__ inline int part_of(const Cut& c, int64_t unit) {
   while (w > 0 && part_start(c, w) > unit) --w;
   return w;
 }
+// x / d, of less than 2^21.
+__device__ inline int quotient(int64_t x, int32_t d) {
+  int q = static_cast<int>(static_cast<float>(x) / static_cast<float>(d));
+  while (static_cast<int64_t>(q + 1) * d <= x) ++q;
+  while (static_cast<int64_t>(q) * d > x) --q;
+  return q;
+}
 // Values that every lane holds, in scalar registers.
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline int64_t uniform(int64_t x) {
@@ -123,6 +131,8 @@ __device__ inline Span uniform(const Span& s) {
   return {uniform(s.unit0), uniform(s.merge), uniform(s.pair0), uniform(s.pairs),
           uniform(s.tile0), uniform(s.tiles), uniform(s.table), uniform(s.group)};
 }
+// (Pairs fit 26 bits.)
+__device__ inline uint32_t row_of(int64_t pair, int64_t heads) { return static_cast<uint32_t>(pair) / static_cast<uint32_t>(heads); }
 // Row of the partial sums of a segment's first pair.
 __device__ inline int64_t part_row(const Plan& w, int part, bool begins) { return (2 * static_cast<int64_t>(part) + (begins ? 1 : 0)) * w.stride; }
 __device__ inline int64_t merge_row(const Plan& w, int64_t merged, int pair, bool own) {
@@ -285,6 +295,8 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
     w.request[t] = lo < batch ? lo : -1;
   }
   int64_t most = (units - items * kBegin) / kLeastTiles;
+  const int64_t few = units - items * kBegin;
+  if (most < kEasyParts * items) most = few < kEasyParts * items ? few : kEasyParts * items;
   if (most < items) most = items;
   Cut cut;
   cut.parts = static_cast<int32_t>(most > kParts ? kParts : (most < 1 ? 1 : most));
@@ -323,9 +335,9 @@ struct LdsFew {   // items of up to 64 pairs
   int32_t least[4];     // the least that a row of a wave sees
 };
 struct LdsMany {  // more
-  alignas(16) uint8_t p[kPairs * kKeys * 2];   // (at a segment's end: references and sums)
-  uint8_t half[4][4][64][16];                  // scores of half the dims, to a wave
-  uint8_t rope[kPairs * kKpeBytes];            // the pairs' rope dims
+  alignas(16) uint8_t rope[kPairs * kKpeBytes];   // the pairs' rope dims (at a segment's end: references and sums)
+  uint8_t p[kPairs * kKeys * 2];
+  uint8_t half[4][4][64][16];                     // scores of half the dims, to a wave
   uint8_t keys[3][kTileBytes];
   float factor[kPairs];
   int32_t moved[4];     // the tile at which a wave's rows have new references
@@ -336,7 +348,7 @@ union Lds {
   LdsFew few;
   LdsMany many;
 };
-constexpr int kStage = 16 * 1024;                // of the tiles' place, of a wave before and after them
+constexpr int kStage = 16 * 1024;                // 32 pairs in LDS, of a wave before and after the tiles
 static_assert(sizeof(Lds) <= 160 * 1024 && 4 * kStage <= 2 * kTileBytes, "LDS");
 static_assert(offsetof(LdsMany, keys) % 4096 == 0 && offsetof(LdsMany, rope) % 8192 == 0, "exclusive ors within");
 
@@ -391,6 +403,19 @@ __device__ inline void accumulate(F16, u32x4_t a, u32x4_t b, f32x16_t& o) {
 }
 // Waits out a product that writes o, or a write of o before a product.
 __device__ inline void settle(f32x16_t& o) { asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o)); }
+// The same for all of them at once: what is before stays before, and so behind.
+template <int TILES>
+__device__ __forceinline__ void settle(f32x16_t (&o)[4][TILES]) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < TILES; ++r) asm volatile("" : "+a"(o[d][r]));
+  asm volatile("s_nop 15\n\ts_nop 7");
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < TILES; ++r) asm volatile("" : "+a"(o[d][r]));
+}
 
 // threadIdx.x, anew for every segment: places in LDS that follow from it would
 // otherwise be worked out once for all forms of the loop, and spilled.
@@ -458,10 +483,7 @@ __device__ __forceinline__ void finish(const PrefixAttentionArgs& a, const Plan&
                                        const float2* rows, uint32_t stage, f32x16_t (&o)[4][TILES]) {
   const int lane = own_thread() & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int r = 0; r < TILES; ++r) settle(o[d][r]);
+  settle(o);
 #pragma unroll
   for (int r = 0; r < TILES; ++r) {
     if (r * 32 >= s.count) break;
@@ -582,7 +604,7 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   constexpr int kWide = kQkDim / 32, kWideLatent = kCkvDim / 32;   // products of 32 dims
   u32x4_t q[kWide];
   const int64_t pair = s.pair0 + (m_mine < s.count ? m_mine : 0);
-  const int vis = m_mine < s.count ? w.visible[pair / a.heads] : 0;
+  const int vis = m_mine < s.count ? w.visible[row_of(pair, a.heads)] : 0;
   {
     const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + quad;
     const u32x4_t* qr = static_cast<const u32x4_t*>(a.query_rope) + pair * (kKpeDim / 8) + quad;
@@ -595,11 +617,10 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < TILES; ++r) {
+    for (int r = 0; r < TILES; ++r)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][r][e] = 0.f;
-      settle(o[d][r]);
-    }
+  settle(o);
   float ref = 0.f, most = -INFINITY, l_run = 0.f;   // most: what a score may reach before the reference moves
   // The least that a row of this wave sees; every wave's meet in LDS.
   int vis_least = m_mine < s.count ? vis : 0x7fffffff;
@@ -817,6 +838,13 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   // They come through LDS, 32 pairs at a time in the wave's own 16 KiB of tiles that
   // are not there yet: a load takes two pairs' 512 neighbouring bytes, where loads
   // to the registers would take 32 bytes of 32 pairs.
+  const int vis = m_mine < s.count ? w.visible[row_of(s.pair0 + m_mine, a.heads)] : 0;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int in = wave * 32 + n * 8 + (lane >> 3), m = in < s.count ? in : 0;
+    load_to_lds(static_cast<const uint8_t*>(a.query_rope) + s.pair0 * kKpeBytes,
+                static_cast<uint32_t>(m * kKpeBytes + ((lane ^ (in >> 1)) & 7) * 16), lds_address(lds.rope) + wave * 4096 + n * 1024);
+  }
   u32x4_t q[kLatentHalf][2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -834,35 +862,28 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
 #pragma unroll
     for (int i = 0; i < kLatentHalf; ++i) asm volatile("" : "+v"(q[i][r]));
   }
-  for (int i = tid; i < kPairs * (kKpeDim / 8); i += kThreads) {
-    const int m = i >> 3;
-    const int64_t pair = s.pair0 + (m < s.count ? m : 0);
-    *reinterpret_cast<u32x4_t*>(&lds.rope[0] + m * kKpeBytes + ((i ^ (m >> 1)) & 7) * 16) =
-        static_cast<const u32x4_t*>(a.query_rope)[pair * (kKpeDim / 8) + (i & 7)];
-  }
   // (Rows of pairs 64 rg + (r ^ dh) 32 + l32: the other tile is 32 rows away.)
   uint32_t qr_at = lds_address(lds.rope) + static_cast<uint32_t>((tile_mine * 32 + l32) * kKpeBytes + (((4 * dh + hh) ^ (l32 >> 1)) & 7) * 16);
-  const int vis = m_mine < s.count ? w.visible[(s.pair0 + m_mine) / a.heads] : 0;
   f32x16_t o[4][4];
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][r][e] = 0.f;
-      settle(o[d][r]);
-    }
+  settle(o);
   float ref = 0.f, l_run = 0.f;
   float room = -INFINITY;  // a score above the reference by more moves it (nothing seen yet: any does)
   int vis_least = m_mine < s.count ? vis : 0x7fffffff;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) vis_least = min(vis_least, __shfl_xor(vis_least, d));
+  for (int d = 1; d < 32; d <<= 1) vis_least = min(vis_least, __shfl_xor(vis_least, d));
   vis_least = __builtin_amdgcn_readfirstlane(vis_least);
   if (lane == 0) lds.least[wave] = vis_least;
   if (tid < 4) lds.moved[tid] = INT32_MIN;
   if (tid == 0) lds.moved_last = INT32_MIN;
   const float factor = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(a.scale * kLog2e)));
 
+  constexpr int kBefore = -2; // page of the tile before the first, whose values are zero
   constexpr int kAhead = 3;   // operands of the scores on their way
   constexpr int kLate = 4;    // products of the outputs that are left for behind barrier A
   u32x4_t v[3], p[4];
@@ -882,7 +903,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
       k[i % (kAhead + 1)] = lds_get(i < 16 ? (k_from ^ ((i >> 1) * 32)) + (i & 1) * 256 : r_from ^ ((i - 16) * 32));
   };
   // Barrier A before the scores of a tile in that buffer.
-  auto begin_scores = [&](uint32_t buffer) {
+  auto begin_scores = [&](uint32_t buffer) __attribute__((always_inline)) {
     wait_loads<0>();
     lds_barrier();
 #pragma unroll
@@ -891,10 +912,10 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
 
   // Tile t, in buffer `now`, is weighed and put out; the scores of tile t + 1, in
   // buffer `ahead`, come first, and of tile t - 1 kLate products are open.  One
-  // form for every t, the one before the first tile, of a page that names nothing,
-  // among them: the compiler does not find registers for more.
+  // form for every t, a tile of zeros before the first one among them: the compiler
+  // does not find registers for more.
   uint32_t now = 2 * kTileBytes, ahead = 0, beyond = kTileBytes;
-  int page_t = -1, page_1 = 0, page_2 = 0;  // of tiles t, t + 1 and t + 2
+  int page_t = kBefore, page_1 = 0, page_2 = 0;  // of tiles t, t + 1 and t + 2
   Load load{};                              // of tile t + 2
   int seen_all = 0;                         // tiles that every row of the item sees whole
   const int seen_mine = vis_least / kKeys;  // that every row of the wave's does
@@ -983,7 +1004,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
         if constexpr (j == 35) fetch_v(v_from, 1);
         if constexpr (j == 28) {
           // Values of keys that some row must not see: see attend().
-          if (((seen_all - 1 - t) | page) < 0) {
+          if (page == -1 || seen_all <= t) {
             for (int c = own_thread(); c < kKeys * kCkvBytes / 16; c += kThreads) {
               u32x4_t* at = reinterpret_cast<u32x4_t*>(&lds.keys[0][0] + now + c * 16);
               *at = finite_or_zero<T>(*at);
@@ -1047,6 +1068,8 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
 
   lds_barrier();
   seen_all = __builtin_amdgcn_readfirstlane(min(min(lds.least[0], lds.least[1]), min(lds.least[2], lds.least[3]))) / kKeys;
+#pragma unroll
+  for (int i = 0; i < kKeys * kCkvBytes / 16 / kThreads; ++i) lds_put(keys_at + now + (tid + i * kThreads) * 16, u32x4_t{0, 0, 0, 0});
   begin_scores(0);
   page_1 = page_of(t0);
   page_2 = page_of(t0 + 1);
@@ -1058,7 +1081,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   wait_loads<0>();
   l_run = xor32_op(l_run, AddOp{});
   lds_barrier();
-  float2* const rows = reinterpret_cast<float2*>(&lds.p[0]);
+  float2* const rows = reinterpret_cast<float2*>(&lds.rope[0]);
   if (hh == 0) rows[m_mine] = make_float2(room == -INFINITY && l_run == 0.f ? -INFINITY : ref, l_run);
   lds_barrier();
   finish<T, 4>(a, w, s, rows, keys_at + wave * kStage, o);
@@ -1082,12 +1105,12 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
       end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
     }
     const int units = s.tiles + kBegin;
-    const int64_t item = uniform((at - s.unit0) / units);
-    const int64_t item_start = s.unit0 + item * units, item_end = item_start + units;
+    const int item = uniform(quotient(at - s.unit0, units));
+    const int64_t item_start = s.unit0 + static_cast<int64_t>(item) * units, item_end = item_start + units;
     const int64_t seg_end = item_end < stop ? item_end : stop;
     auto tile_of = [&](int64_t u) { return u > kBegin ? static_cast<int>(u) - kBegin : 0; };
     Segment g;
-    const int first = static_cast<int>(item) * kPairs;
+    const int first = item * kPairs;
     g.pair0 = static_cast<int64_t>(s.pair0) + first;
     g.count = s.pairs - first < kPairs ? s.pairs - first : kPairs;
     g.tile0 = s.tile0 + tile_of(at - item_start);
@@ -1097,8 +1120,9 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
     g.direct = whole && s.merge < 0;
     g.row = whole ? merge_row(w, s.merge, first, at_span >= a.groups) : part_row(w, part, at == item_start);
     g.row_step = whole ? 2 : 1;
-    if (at_span >= a.groups) {  // a request's last row of the item sees the most
-      const int seen = (uniform(w.visible[(g.pair0 + g.count - 1) / a.heads]) + kKeys - 1) / kKeys;
+    // A request's last row of the item sees the most; its last row of all sees its length.
+    if (at_span >= a.groups && s.pairs - first - g.count >= a.heads) {
+      const int seen = (uniform(w.visible[row_of(g.pair0 + g.count - 1, a.heads)]) + kKeys - 1) / kKeys;
       g.tile1 = g.tile1 < seen ? g.tile1 : seen;
       g.tile0 = g.tile0 < g.tile1 ? g.tile0 : g.tile1;
     }
