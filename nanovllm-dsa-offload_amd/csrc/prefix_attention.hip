@@ -637,15 +637,21 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     for (int h = 0; h < TILES; ++h)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[h][e] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kWide; ++j) {
-#pragma unroll
-      for (int h = 0; h < TILES; ++h) {
-        const u32x4_t k = j < kWideLatent ? lds_get(((k_at + at) ^ ((j & 3) * 64)) + (j >> 2) * 256 + h * 16 * kCkvBytes)
-                                          : lds_get(((r_at + at) ^ ((j - kWideLatent) * 64)) + h * 16 * kKpeBytes);
-        x[h] = T::mfma16(__builtin_bit_cast(typename T::vec8, k), __builtin_bit_cast(typename T::vec8, q[j]), x[h]);
-      }
-    }
+    constexpr int kOperands = kWide * TILES, kOnTheWay = 6;   // (LDS answers after five products)
+    u32x4_t k[kOnTheWay + 1];
+    auto fetch = [&](auto n) __attribute__((always_inline)) {
+      constexpr int i = decltype(n)::value, j = i / TILES, h = i % TILES;
+      if constexpr (i < kOperands)
+        k[i % (kOnTheWay + 1)] = j < kWideLatent ? lds_get(((k_at + at) ^ ((j & 3) * 64)) + (j >> 2) * 256 + h * 16 * kCkvBytes)
+                                                 : lds_get(((r_at + at) ^ ((j - kWideLatent) * 64)) + h * 16 * kKpeBytes);
+    };
+    steps<kOnTheWay>(fetch);
+    steps<kOperands>([&](auto n) __attribute__((always_inline)) {
+      constexpr int i = decltype(n)::value, j = i / TILES, h = i % TILES;
+      fetch(std::integral_constant<int, i + kOnTheWay>{});
+      x[h] = T::mfma16(__builtin_bit_cast(typename T::vec8, k[i % (kOnTheWay + 1)]), __builtin_bit_cast(typename T::vec8, q[j]), x[h]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
     const bool none = pages.of(tile) < 0;
 #pragma unroll
     for (int h = 0; h < TILES; ++h)
@@ -667,16 +673,16 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   // Scores to P, against the row's reference.
   auto weigh = [&] {
     if constexpr (TILES == 1) top = fmaxf(lds.top[0][m_mine], lds.top[1][m_mine]);
-    const bool past = top > most;
+    const bool past = top > most, moved = past && most != -INFINITY;   // (the first time o is zero)
     float f = 1.f;
     if (past) {
       const float now = top - kRise;
-      f = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
+      f = moved ? __builtin_amdgcn_exp2f(ref - now) : 1.f;
       most = now + kMost;
       ref = now;
       l_run *= f;
     }
-    const bool any = __any(past);
+    const bool any = __any(moved);
     if (half0 == 0) {
       if (quad == 0) lds.factor[m_mine] = f;
       if (lane == 0) lds.moved[wave] = any;
@@ -717,20 +723,27 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
         }
       }
     }
+    u32x4_t p[2][TILES], v[3];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4_t p[TILES];
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int r = 0; r < TILES; ++r) p[r] = lds_get(p_read + r * 2048 + static_cast<uint32_t>(((2 * ks + hh) ^ p_swz) * 16));
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
+      for (int r = 0; r < TILES; ++r) p[ks][r] = lds_get(p_read + r * 2048 + static_cast<uint32_t>(((2 * ks + hh) ^ p_swz) * 16));
+    auto fetch = [&](auto n) __attribute__((always_inline)) {
+      constexpr int i = decltype(n)::value, ks = i >> 2, d = i & 3;
+      if constexpr (i < 8) {
         const uint2 lo = read_tr16(((v_at[0] + at) ^ (d * 64)) + ks * 16 * kCkvBytes);
         const uint2 hi = read_tr16(((v_at[1] + at) ^ (d * 64)) + ks * 16 * kCkvBytes);
-        const u32x4_t v{lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-        for (int r = 0; r < TILES; ++r) accumulate<true>(T{}, v, p[r], o[d][r]);
+        v[i % 3] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
       }
-    }
+    };
+    steps<2>(fetch);
+    steps<8>([&](auto n) __attribute__((always_inline)) {
+      constexpr int i = decltype(n)::value;
+      fetch(std::integral_constant<int, i + 2>{});
+#pragma unroll
+      for (int r = 0; r < TILES; ++r) accumulate<true>(T{}, v[i % 3], p[i >> 2][r], o[i & 3][r]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
   wait_loads<0>();
