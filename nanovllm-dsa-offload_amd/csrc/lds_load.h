@@ -15,12 +15,12 @@ __device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_
 __device__ inline void load_to_lds(const uint8_t* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
-// The same from base + offset + OFFSET to `lds` + OFFSET + 16 * lane.
+// The same from base + offset + OFFSET to `lds` + `more` + OFFSET + 16 * lane.
 template <int OFFSET>
-__device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds), "v"(offset),
+__device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds, uint32_t more) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3 offset:%4" ::"s"(lds), "s"(more), "v"(offset),
                "s"(base), "n"(OFFSET)
-               : "memory", "m0");
+               : "memory", "m0", "scc");
 }
 template <int N>
 __device__ inline void wait_loads() {  // all but the wave's newest N are done

@@ -368,18 +368,19 @@ struct Pages {
   int32_t last, blocks;   // column
   int32_t first, held;
   __device__ Pages(const Segment& s, const PrefixAttentionArgs& a) : table(s.table), blocks(static_cast<int32_t>(a.blocks)) {
-    const int c = (s.tile1 - 1) / kPageTiles;
+    const int c = column(s.tile1 - 1);
     last = c < a.cols ? c : static_cast<int32_t>(a.cols) - 1;
     hold(s.tile0);
   }
   __device__ void hold(int tile) {
-    first = tile / kPageTiles;
+    first = column(tile);
     const int c = first + (threadIdx.x & 63);
     const int32_t page = c <= last ? table[c] : -1;
     held = page >= 0 && page < blocks ? page : -1;
   }
-  __device__ bool holds(int tile) const { return tile / kPageTiles - first < 64; }
-  __device__ int of(int tile) const { return __builtin_amdgcn_readlane(held, tile / kPageTiles - first); }
+  __device__ static int column(int tile) { return static_cast<int>(static_cast<uint32_t>(tile) / kPageTiles); }
+  __device__ bool holds(int tile) const { return column(tile) - first < 64; }
+  __device__ int of(int tile) const { return __builtin_amdgcn_readlane(held, column(tile) - first); }
 };
 
 // o += a b, with o in accumulation registers: 256 of them hold four tiles of
@@ -831,10 +832,9 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   auto issue = [&](const Load& l, uint32_t buffer, auto which) {  // 0 to 7: a key, 8: the rope dims
     constexpr int n = decltype(which)::value;
     if constexpr (n < 8)
-      load_to_lds<(n & 3) * 1024>(l.base + (n >> 2) * 4096, byte_of ^ ((n & 3) * 64 + (n >> 2) * 16),
-                                  lds_tile + buffer + (n >> 2) * 4096);
+      load_to_lds<(n & 3) * 1024>(l.base, byte_of ^ ((n & 3) * 64 + (n >> 2) * (4096 + 16)), lds_tile + (n >> 2) * 4096, buffer);
     else
-      load_to_lds<0>(l.rope, rope_byte, lds_rope + buffer);
+      load_to_lds<0>(l.rope, rope_byte, lds_rope, buffer);
   };
 
   lds_barrier();  // (the segment before is done with LDS)
@@ -896,7 +896,6 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   if (tid == 0) lds.moved_last = INT32_MIN;
   const float factor = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(a.scale * kLog2e)));
 
-  constexpr int kBefore = -2; // page of the tile before the first, whose values are zero
   constexpr int kAhead = 3;   // operands of the scores on their way
   constexpr int kLate = 4;    // products of the outputs that are left for behind barrier A
   u32x4_t v[3], p[4];
@@ -915,12 +914,16 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
     if (i < kHalf)
       k[i % (kAhead + 1)] = lds_get(i < 16 ? (k_from ^ ((i >> 1) * 32)) + (i & 1) * 256 : r_from ^ ((i - 16) * 32));
   };
-  // Barrier A before the scores of a tile in that buffer.
+  // Barrier A before the scores of a tile in that buffer; `other`: half of the scores
+  // of the tile before it.
+  u32x4_t other[4];
   auto begin_scores = [&](uint32_t buffer) __attribute__((always_inline)) {
     wait_loads<0>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch_k(k_at + buffer, r_at + buffer, i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) other[e] = lds_get(half_at + wave * 4096 + lane16 + e * 1024);
   };
 
   // Tile t, in buffer `now`, is weighed and put out; the scores of tile t + 1, in
@@ -928,7 +931,8 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   // form for every t, a tile of zeros before the first one among them: the compiler
   // does not find registers for more.
   uint32_t now = 2 * kTileBytes, ahead = 0, beyond = kTileBytes;
-  int page_t = kBefore, page_1 = 0, page_2 = 0;  // of tiles t, t + 1 and t + 2
+  int page_t = -1, page_1 = 0, page_2 = 0;  // of tiles t, t + 1 and t + 2
+  int mask_now = -1, scrub_now = 0;         // negative: some row of the wave's, of the item, does not see all of tile t
   Load load{};                              // of tile t + 2
   int seen_all = 0;                         // tiles that every row of the item sees whole
   const int seen_mine = vis_least / kKeys;  // that every row of the wave's does
@@ -942,13 +946,11 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
     forget(k_at);
     forget(r_at);
     forget(v_at);
-    u32x4_t qr[2][2], other[4];
+    u32x4_t qr[2][2];
     f32x16_t next[2];
     const int page = page_t;
     Load next_load;
-    const int page_next = page_of(t + 3);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) other[e] = lds_get(half_at + wave * 4096 + lane16 + e * 1024);
+    int page_next = 0;
     float top = 0.f, more = 0.f;
     int32_t moved_last = 0;
     bool any = false;
@@ -976,7 +978,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
           mine[e] = fmaf(mine[e] + __uint_as_float(other[e / 4][e % 4]), factor, -ref);
           mine[e + 1] = fmaf(mine[e + 1] + __uint_as_float(other[e / 4][e % 4 + 1]), factor, -ref);
         }
-        if constexpr (j == 12) if (((seen_mine - 1 - t) | page) < 0) {
+        if constexpr (j == 12) if (mask_now < 0) {
           const int left = vis - t * kKeys - 4 * (own_thread() >> 5 & 1);  // keys that the row sees, from the lane's first
 #pragma unroll
           for (int e = 0; e < 16; ++e) mine[e] = page >= 0 && 8 * (e >> 2) + (e & 3) < left ? mine[e] : -INFINITY;
@@ -1005,19 +1007,22 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
           constexpr int e = 2 * (j - 16), n = e / 4;
           mine[e] = __builtin_amdgcn_exp2f(mine[e]);
           mine[e + 1] = __builtin_amdgcn_exp2f(mine[e + 1]);
-          l_run += mine[e];
-          more += mine[e + 1];
           if constexpr (e % 4 == 2)
             lds_put(p_write ^ (n * 16), T::pack2(mine[e - 2], mine[e - 1]), T::pack2(mine[e], mine[e + 1]));
         }
-        if constexpr (j == 24) l_run += more;
+        if constexpr (j >= 17 && j < 25) {
+          l_run += mine[2 * (j - 17)];
+          more += mine[2 * (j - 17) + 1];
+          asm volatile("" : "+v"(l_run), "+v"(more));  // (here, not all of them between the products)
+        }
+        if constexpr (j == 25) l_run += more;
         if constexpr (j == 29) moved_last = lds.moved_last;
         if constexpr (j >= 29 && j < 33) fetch_p(0, j - 29);
         if constexpr (j == 33) fetch_v(v_from, 0);
         if constexpr (j == 35) fetch_v(v_from, 1);
         if constexpr (j == 28) {
           // Values of keys that some row must not see: see attend().
-          if (page == -1 || seen_all <= t) {
+          if (scrub_now < 0) {
             for (int c = own_thread(); c < kKeys * kCkvBytes / 16; c += kThreads) {
               u32x4_t* at = reinterpret_cast<u32x4_t*>(&lds.keys[0][0] + now + c * 16);
               *at = finite_or_zero<T>(*at);
@@ -1048,7 +1053,15 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
       steps<32>([&](auto step) __attribute__((always_inline)) {
         constexpr int n = decltype(step)::value, i = n >> 2, r = n & 3;
         if constexpr (n == 32 - kLate) begin_scores(beyond);
+        if constexpr (n == 5) {
+          if (!pages.holds(t + 3)) pages.hold(t);
+          page_next = page_of(t + 3);
+        }
         if constexpr (n == 10) next_load = load_of(t + 3, page_next);
+        if constexpr (n == 14) {
+          mask_now = (seen_mine - 2 - t) | page_1;
+          scrub_now = (seen_all - 2 - t) | page_1;
+        }
         if constexpr (r == 0 && i + 2 < 8) fetch_v(v_from, i + 2);
         accumulate<r == 0 || i == 0 || i == 4>(T{}, v[i % 3], p[r], o[i & 3][r]);
         if constexpr (n % 5 == 3 && n < 20) {
@@ -1087,10 +1100,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   page_1 = page_of(t0);
   page_2 = page_of(t0 + 1);
   load = load_of(t0 + 1, page_2);
-  for (int t = t0 - 1; t < t1; ++t) {
-    if (!pages.holds(t + 3)) pages.hold(t);
-    round(t);   // (the last one's scores are of no tile, and nobody reads them)
-  }
+  for (int t = t0 - 1; t < t1; ++t) round(t);   // (the last one's scores are of no tile, and nobody reads them)
   wait_loads<0>();
   l_run = xor32_op(l_run, AddOp{});
   lds_barrier();
