@@ -192,7 +192,7 @@ const char* nvdsa_kernel_name(int32_t kernel_id) {
                                 "norm_rope_kernel",      "pages_take_kernel", "pages_reserve_kernel",
                                 "pages_count_kernel",    "pages_rank_kernel", "pages_rename_kernel",
                                 "pages_copy_kernel",     "prefix_plan_kernel", "prefix_attention_kernel",
-                                "prefix_join_kernel"};
+                                "prefix_join_kernel",    "pages_compact_kernel"};
   static_assert(sizeof(names) / sizeof(names[0]) == nvdsa::kKernCount, "one name per kernel id");
   if (kernel_id < 0 || kernel_id >= nvdsa::kKernCount) return "unknown";
   return names[kernel_id];

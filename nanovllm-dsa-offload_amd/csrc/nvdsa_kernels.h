@@ -52,7 +52,8 @@ enum KernelId : int {
   kKernPrefixPlan = 36,
   kKernPrefixAttention = 37,
   kKernPrefixJoin = 38,
-  kKernCount = 39
+  kKernPagesCompact = 39,
+  kKernCount = 40
 };
 // Timing events for the next launch of `kernel_id` when instrumentation is
 // on for the calling thread (nvdsa_profile_begin); both null otherwise.

@@ -23,43 +23,54 @@ namespace {
 // that swap within a shared prefix leave them alone.
 constexpr int kTakeThreads = 256;
 constexpr int kTakeEntries = 16384;  // of LDS
-constexpr int kTakeColumns = 16;     // at most
+// Columns of a workgroup: an entry a thread, as its two counts are what takes the
+// time (64 rows of 256 columns that all change: 8.7 us with 16 columns, 5.3 us with
+// 4), but 16 bytes of a row at least.
+constexpr int kTakeMost = 16, kTakeLeast = 4;
 
-__global__ __launch_bounds__(kTakeThreads) void pages_take_kernel(PagesBranchArgs a, int columns) {
-  __shared__ int32_t held[kTakeEntries];
+__device__ inline int parent_of(const PagesBranchArgs& a, int b) {
+  const int32_t p = a.parents[b];
+  return p < 0 || p >= a.batch ? -1 : p;
+}
+// Columns [col0, col0 + columns) of every row, at most kTakeEntries entries.
+template <int THREADS>
+__device__ inline void take_over(const PagesBranchArgs& a, int64_t col0, int columns, int32_t* held) {
   const int tid = threadIdx.x;
-  const int batch = static_cast<int>(a.batch);
-  const int64_t col0 = static_cast<int64_t>(blockIdx.x) * columns;
-  const int n = batch * columns;
-  auto parent_of = [&](int b) -> int {
-    const int32_t p = a.parents[b];
-    return p < 0 || p >= batch ? -1 : p;
-  };
-  for (int i = tid; i < n; i += kTakeThreads) {
+  const int n = static_cast<int>(a.batch) * columns;
+  for (int i = tid; i < n; i += THREADS) {
     const int b = i / columns;
     const int64_t c = col0 + (i - b * columns);
     held[i] = c < a.cols ? a.block_table[b * a.cols + c] : -1;
   }
   __syncthreads();
-  for (int i = tid; i < n; i += kTakeThreads) {
+  for (int i = tid; i < n; i += THREADS) {
     const int b = i / columns, k = i - b * columns;
     const int64_t c = col0 + k;
     if (c >= a.cols) continue;
-    const int p = parent_of(b);
+    const int p = parent_of(a, b);
     const int32_t before = held[i], after = p < 0 ? -1 : held[p * columns + k];
     if (before == after) continue;
     a.block_table[b * a.cols + c] = after;
     if (after >= 0 && after < a.pages) atomicAdd(&a.page_refs[after], 1);
     if (before >= 0 && before < a.pages) atomicAdd(&a.page_refs[before], -1);
   }
-  if (blockIdx.x != 0) return;
+}
+// And the rows' lengths.
+template <int THREADS>
+__device__ inline void take_lengths(const PagesBranchArgs& a, int32_t* held) {
   __syncthreads();
-  for (int b = tid; b < batch; b += kTakeThreads) held[b] = a.seq_lens[b];
+  for (int b = threadIdx.x; b < a.batch; b += THREADS) held[b] = a.seq_lens[b];
   __syncthreads();
-  for (int b = tid; b < batch; b += kTakeThreads) {
-    const int p = parent_of(b);
+  for (int b = threadIdx.x; b < a.batch; b += THREADS) {
+    const int p = parent_of(a, b);
     a.seq_lens[b] = p < 0 ? 0 : held[p];
   }
+}
+
+__global__ __launch_bounds__(kTakeThreads) void pages_take_kernel(PagesBranchArgs a, int columns) {
+  __shared__ int32_t held[kTakeEntries];
+  take_over<kTakeThreads>(a, static_cast<int64_t>(blockIdx.x) * columns, columns, held);
+  if (blockIdx.x == 0) take_lengths<kTakeThreads>(a, held);
 }
 
 // ------------------------------------------------------------------ reserve
@@ -67,6 +78,9 @@ __global__ __launch_bounds__(kTakeThreads) void pages_take_kernel(PagesBranchArg
 // who gets which.  Rows and columns are served in order, all or none.
 constexpr int kReserveThreads = 1024;
 constexpr int kScanPer = 8;  // counts of a thread and round
+// Entries of a table that this workgroup takes over by itself: 14 us for 256 that all
+// change, as much as two kernels, and a launch less; 21 us for 2048, where two take 15.
+constexpr int kTakeAlone = 512;
 
 struct Wanted {   // columns [first, stop) of a row receive tokens
   int first, stop;
@@ -82,8 +96,17 @@ __device__ inline Wanted wanted_of(const PagesBranchArgs& a, int b) {
           static_cast<int>(len & (kBlock - 1))};
 }
 
+// TAKES: and what the rows take over, first.
+template <bool TAKES>
 __global__ __launch_bounds__(kReserveThreads) void pages_reserve_kernel(PagesBranchArgs a) {
   __shared__ int32_t writes_on[kMostBranchRows];  // the page that a row's next token falls into, among older rows; -1
+  if constexpr (TAKES) {
+    __shared__ int32_t held[kTakeAlone];
+    take_over<kReserveThreads>(a, 0, static_cast<int>(a.cols), held);
+    take_lengths<kReserveThreads>(a, held);
+    __threadfence();  // (counts changed in the L2: no older copy is read)
+    __syncthreads();
+  }
   __shared__ int scratch[kReserveThreads / 64 + 1];
   const int tid = threadIdx.x;
   const int batch = static_cast<int>(a.batch);
@@ -261,6 +284,68 @@ __global__ __launch_bounds__(256) void pages_rename_kernel(PagesCompactArgs a, i
   }
 }
 
+// The same by one workgroup, ranks in LDS.  Up to 8192 pages: 5 us for 1024, 9 for 4096 and 14 for 8192, where three kernels
+// take 12, 15 and 16 (16384: 20 and 16).
+constexpr int kAlonePages = 8192;
+constexpr int kAloneEntries = 8192;   // of the table
+
+__global__ __launch_bounds__(kCompactThreads) void pages_compact_kernel(PagesCompactArgs a, int entries) {
+  constexpr int kChunks = kAlonePages / kCompactChunk;
+  __shared__ int32_t rank[kAlonePages];
+  __shared__ int scratch[kCompactThreads / 64 + 1];
+  const int tid = threadIdx.x;
+  const int pages = static_cast<int>(a.pages);
+  uint32_t live[kChunks];
+  int at[kChunks], border = 0;  // pages held before the thread's of a chunk, and in all
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) live[i] = i * kCompactChunk < pages ? live_of(a, i * kCompactChunk + tid * 4) : 0;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    at[i] = border;
+    if (i * kCompactChunk < pages) {
+      int total;
+      at[i] += block_exclusive_scan(__popc(live[i]), scratch, &total);
+      border += total;
+    }
+  }
+  int mine = 0, below;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int room = border - (i * kCompactChunk + tid * 4);
+    mine += __popc(live[i] & (room >= 4 ? 0xfu : (room <= 0 ? 0u : (1u << room) - 1u)));
+  }
+  block_exclusive_scan(mine, scratch, &below);
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int p = i * kCompactChunk + tid * 4 + k;
+      if (p >= pages) continue;
+      const bool held = (live[i] >> k) & 1u;
+      int32_t r = -1;
+      if (held && p >= border) {
+        r = at[i] - below;
+        a.move_src[r] = p;
+      } else if (!held && p < border) {
+        a.move_dst[p - at[i]] = p;
+      }
+      rank[p] = r;
+      at[i] += held ? 1 : 0;
+    }
+  }
+  if (tid == 0) *a.move_count = border - below;
+  __syncthreads();
+  for (int k = tid; k < border - below; k += kCompactThreads) {
+    const int32_t from = a.move_src[k];
+    a.page_refs[a.move_dst[k]] = a.page_refs[from];
+    a.page_refs[from] = 0;
+  }
+  for (int i = tid; i < entries; i += kCompactThreads) {
+    const int32_t page = a.block_table[i];
+    if (page >= 0 && page < pages && rank[page] >= 0) a.block_table[i] = a.move_dst[rank[page]];
+  }
+}
+
 // --------------------------------------------------------------------- copy
 // 16 KiB of a page a workgroup and turn, all loads before the first store.
 constexpr int kCopyThreads = 256;
@@ -324,15 +409,20 @@ size_t pages_branch_workspace_bytes(int64_t pages) { return sizeof(int32_t) * 2 
 hipError_t launch_pages_branch(PagesBranchArgs a, hipStream_t stream) {
   a.fresh = static_cast<int32_t*>(a.workspace);
   a.given_up = a.fresh + a.pages;
+  if (a.parents != nullptr && a.batch > 0 && a.batch * a.cols <= kTakeAlone) {
+    launch_kernel(kKernPagesReserve, pages_reserve_kernel<true>, dim3(1), dim3(kReserveThreads), stream, a);
+    return hipGetLastError();
+  }
   if (a.parents != nullptr && a.batch > 0) {
-    int64_t columns = kTakeEntries / a.batch;
-    columns = columns < kTakeColumns ? columns : kTakeColumns;
+    int64_t columns = kTakeThreads / a.batch;
+    columns = columns < kTakeLeast ? kTakeLeast : (columns > kTakeMost ? kTakeMost : columns);
+    if (columns * a.batch > kTakeEntries) columns = kTakeEntries / a.batch;
     launch_kernel(kKernPagesTake, pages_take_kernel, dim3(static_cast<uint32_t>(ceil_div(a.cols, columns))), dim3(kTakeThreads),
                   stream, a, static_cast<int>(columns));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  launch_kernel(kKernPagesReserve, pages_reserve_kernel, dim3(1), dim3(kReserveThreads), stream, a);
+  launch_kernel(kKernPagesReserve, pages_reserve_kernel<false>, dim3(1), dim3(kReserveThreads), stream, a);
   return hipGetLastError();
 }
 
@@ -341,6 +431,11 @@ size_t pages_compact_workspace_bytes(int64_t pages) {
 }
 
 hipError_t launch_pages_compact(PagesCompactArgs a, hipStream_t stream) {
+  const int64_t entries = a.batch * a.cols;
+  if (a.pages <= kAlonePages && entries <= kAloneEntries) {
+    launch_kernel(kKernPagesCompact, pages_compact_kernel, dim3(1), dim3(kCompactThreads), stream, a, static_cast<int>(entries));
+    return hipGetLastError();
+  }
   const uint32_t chunks = static_cast<uint32_t>(ceil_div(a.pages, kCompactChunk));
   a.rank = static_cast<int32_t*>(a.workspace);
   a.counts = a.rank + a.pages;
@@ -350,7 +445,6 @@ hipError_t launch_pages_compact(PagesCompactArgs a, hipStream_t stream) {
   launch_kernel(kKernPagesRank, pages_rank_kernel, dim3(chunks), dim3(kCompactThreads), stream, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t entries = a.batch * a.cols;
   launch_kernel(kKernPagesRename, pages_rename_kernel,
                 dim3(static_cast<uint32_t>(ceil_div(entries > a.pages ? entries : a.pages, 256))), dim3(256), stream, a, entries);
   return hipGetLastError();
