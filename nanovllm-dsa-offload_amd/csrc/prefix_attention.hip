@@ -45,11 +45,12 @@ constexpr float kMost = 15.9f;
 // ---------------------------------------------------------------- the plan
 struct Span {        // pairs against tiles of one table row's pages
   int64_t unit0;     // first unit of the first item
-  int64_t merge;     // first of the group's pairs that two items have (-1: one item only)
+  int32_t merge;     // first of the group's pairs that two items have (-1: one item only)
   int32_t pair0, pairs;
   int32_t tile0, tiles;
   int32_t table;     // row of the block table
   int32_t group;     // request: its group's span (-1: none)
+  int32_t length;    // request: of the tokens
 };
 struct Start {       // where a part begins
   int64_t unit;
@@ -129,7 +130,7 @@ __device__ inline int64_t uniform(int64_t x) {
 }
 __device__ inline Span uniform(const Span& s) {
   return {uniform(s.unit0), uniform(s.merge), uniform(s.pair0), uniform(s.pairs),
-          uniform(s.tile0), uniform(s.tiles), uniform(s.table), uniform(s.group)};
+          uniform(s.tile0), uniform(s.tiles), uniform(s.table), uniform(s.group), uniform(s.length)};
 }
 // (Pairs fit 26 bits.)
 __device__ inline uint32_t row_of(int64_t pair, int64_t heads) { return static_cast<uint32_t>(pair) / static_cast<uint32_t>(heads); }
@@ -142,6 +143,7 @@ __device__ inline int64_t merge_row(const Plan& w, int64_t merged, int pair, boo
 constexpr int kPlanThreads = 1024;
 
 // Sums of what the threads before hold, of two values at once; *all_..: of everybody's.
+template <int THREADS>
 __device__ inline void plan_scan(int64_t& x, int64_t& y, int64_t (*scratch)[2], int64_t* all_x, int64_t* all_y) {
   const int wid = threadIdx.x >> 6;
   const int64_t sx = static_cast<int64_t>(wave_inclusive_scan(static_cast<uint64_t>(x)));
@@ -153,7 +155,7 @@ __device__ inline void plan_scan(int64_t& x, int64_t& y, int64_t (*scratch)[2], 
   }
   __syncthreads();
   int64_t before_x = 0, before_y = 0, sum_x = 0, sum_y = 0;
-  for (int k = 0; k < kPlanThreads / 64; ++k) {
+  for (int k = 0; k < THREADS / 64; ++k) {
     const int64_t u = scratch[k][0], v = scratch[k][1];
     before_x += k < wid ? u : 0;
     before_y += k < wid ? v : 0;
@@ -166,15 +168,21 @@ __device__ inline void plan_scan(int64_t& x, int64_t& y, int64_t (*scratch)[2], 
   y = before_y + sy - y;
 }
 
-// One workgroup, and latency all the way: what it reads comes to LDS at once (of
-// the first kPlanThreads requests and groups; the others' from memory).
-__global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttentionArgs a) {
-  __shared__ int64_t scratch[kPlanThreads / 64][2];
-  __shared__ int64_t unit0_of[2 * kPlanThreads];
-  __shared__ Span group_of[kPlanThreads];
-  __shared__ int32_t q_ends[kPlanThreads], group_ends[kPlanThreads];
-  Plan w;
-  carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
+// What a plan of THREADS threads holds in LDS: of that many requests and groups
+// (the others' are read from memory again).
+template <int THREADS, bool HERE>
+struct LdsPlan {
+  int64_t scratch[THREADS / 64][2];
+  int64_t unit0[HERE ? 1 : 2 * THREADS];
+  Span group[HERE ? 1 : THREADS];
+  int32_t q_ends[THREADS], group_ends[THREADS];
+};
+
+// Latency all the way: what it reads comes to LDS at once.  HERE: all spans are
+// left in `here`, for which there are threads enough; WRITES: in memory.
+template <int THREADS, bool HERE>
+__device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Plan& w, LdsPlan<THREADS, HERE>& lds, Span* here,
+                                         bool writes) {
   const int tid = threadIdx.x;
   const int64_t cap = a.cols * kBlock;
   const int batch = static_cast<int>(a.batch), groups = static_cast<int>(a.groups), rows = static_cast<int>(a.rows);
@@ -182,23 +190,23 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
   auto clamp = [](int64_t x, int64_t most) { return static_cast<int>(x < 0 ? 0 : (x > most ? most : x)); };
   int64_t own_length = 0, own_prefix = 0;  // of request and group tid
   if (tid < batch) {
-    q_ends[tid] = a.seq_q[tid];
+    lds.q_ends[tid] = a.seq_q[tid];
     own_length = a.seq_kv[tid];
   }
   if (tid < groups) {
-    group_ends[tid] = a.group_ends[tid];
+    lds.group_ends[tid] = a.group_ends[tid];
     own_prefix = a.prefix_lens[tid];
   }
   __syncthreads();
   auto row_at = [&](int b) {  // first packed row of request b
-    return b > 0 ? clamp(b <= kPlanThreads ? q_ends[b - 1] : a.seq_q[b - 1], rows) : 0;
+    return b > 0 ? clamp(HERE || b <= THREADS ? lds.q_ends[b - 1] : a.seq_q[b - 1], rows) : 0;
   };
-  auto group_end = [&](int g) { return clamp(g < kPlanThreads ? group_ends[g] : a.group_ends[g], batch); };
+  auto group_end = [&](int g) { return clamp(HERE || g < THREADS ? lds.group_ends[g] : a.group_ends[g], batch); };
   auto length_of = [&](int b) { return clamp(b == tid ? own_length : a.seq_kv[b], cap); };
   int64_t units = 0, merged = 0, items = 0;
   // Groups: one that shares has a request's pages read for several of them, and
   // fewer pairs a request than an item holds (else every item is full anyway).
-  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+  for (int g0 = 0; g0 < groups; g0 += THREADS) {
     const int g = g0 + tid;
     Span s{};
     s.merge = s.group = -1;
@@ -218,25 +226,29 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
       }
     }
     int64_t none = 0, m = s.pairs, sum, sum_m;
-    plan_scan(m, none, scratch, &sum_m, &sum);
+    plan_scan<THREADS>(m, none, lds.scratch, &sum_m, &sum);
     // (Ends that decrease could count a request's pairs for several groups: there
     // is room for each pair once.)
     if (merged + m + s.pairs > merge_pairs(rows, heads, batch)) s.pairs = 0;
     if (s.pairs > 0) s.merge = merged + m;
     merged += sum_m;
     int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
-    plan_scan(u, n, scratch, &sum_u, &sum_n);
+    plan_scan<THREADS>(u, n, lds.scratch, &sum_u, &sum_n);
     s.unit0 = units + u;
     units += sum_u;
     items += sum_n;
     if (g < groups) {
-      w.spans[g] = s;
-      if (g < kPlanThreads) group_of[g] = s;
-      if (g < 2 * kPlanThreads) unit0_of[g] = s.unit0;
+      if (writes) w.spans[g] = s;
+      if constexpr (HERE) {
+        here[g] = s;
+      } else {
+        if (g < THREADS) lds.group[g] = s;
+        if (g < 2 * THREADS) lds.unit0[g] = s.unit0;
+      }
     }
   }
   __syncthreads();
-  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < batch; b0 += THREADS) {
     const int b = b0 + tid;
     Span s{};
     s.merge = s.group = -1;
@@ -244,7 +256,8 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
       const int r0 = row_at(b), r1 = row_at(b + 1);
       s.pair0 = r0 * heads;
       s.pairs = r1 > r0 ? (r1 - r0) * heads : 0;
-      s.tiles = (length_of(b) + kKeys - 1) / kKeys;
+      s.length = length_of(b);
+      s.tiles = (s.length + kKeys - 1) / kKeys;
       s.table = b;
       // The group: the first whose end lies behind the request.
       int lo = 0, hi = groups;
@@ -256,7 +269,11 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
           hi = mid;
       }
       if (lo < groups && s.pairs > 0) {
-        const Span g = lo < kPlanThreads ? group_of[lo] : w.spans[lo];
+        Span g;
+        if constexpr (HERE)
+          g = here[lo];
+        else
+          g = lo < THREADS ? lds.group[lo] : w.spans[lo];
         // (Ends that decrease: a request outside the group's rows is its own.)
         if (g.pairs > 0 && b >= g.table && s.pair0 >= g.pair0 && s.pair0 + s.pairs <= g.pair0 + g.pairs) {
           s.group = lo;
@@ -267,17 +284,20 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
       }
     }
     int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
-    plan_scan(u, n, scratch, &sum_u, &sum_n);
+    plan_scan<THREADS>(u, n, lds.scratch, &sum_u, &sum_n);
     s.unit0 = units + u;
     units += sum_u;
     items += sum_n;
     if (b < batch) {
-      w.spans[groups + b] = s;
-      if (groups + b < 2 * kPlanThreads) unit0_of[groups + b] = s.unit0;
+      if (writes) w.spans[groups + b] = s;
+      if constexpr (HERE)
+        here[groups + b] = s;
+      else if (groups + b < 2 * THREADS)
+        lds.unit0[groups + b] = s.unit0;
     }
   }
-  // What the rows see.
-  for (int t = tid; t < rows; t += kPlanThreads) {
+  // The rows' requests, and what they see.
+  for (int t = tid; writes && t < rows; t += THREADS) {
     int lo = 0, hi = batch;  // the request: an end behind the row, the end before it not
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -286,12 +306,14 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
       else
         hi = mid;
     }
-    int seen = 0;
-    if (lo < batch) {
-      seen = clamp(a.seq_kv[lo], cap) - (row_at(lo + 1) - 1 - t);
-      seen = seen > 0 ? seen : 0;
+    if constexpr (!HERE) {
+      int seen = 0;
+      if (lo < batch) {
+        seen = clamp(a.seq_kv[lo], cap) - (row_at(lo + 1) - 1 - t);
+        seen = seen > 0 ? seen : 0;
+      }
+      w.visible[t] = seen;
     }
-    w.visible[t] = seen;
     w.request[t] = lo < batch ? lo : -1;
   }
   int64_t most = (units - items * kBegin) / kLeastTiles;
@@ -303,25 +325,40 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttenti
   cut.units = units / cut.parts;
   cut.longer = static_cast<int32_t>(units - cut.units * cut.parts);
   if (units == 0) cut.parts = 0;
-  if (tid == 0) *w.cut = cut;
+  if (writes && tid == 0) *w.cut = cut;
   __syncthreads();
-  if (tid < cut.parts) {
-    Start p;
-    p.unit = part_start(cut, tid);
-    p.stop = part_start(cut, tid + 1);
-    // The last span that begins at or before the unit (spans without pairs begin
-    // where the next does).
-    int lo = 0, hi = spans - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((mid < 2 * kPlanThreads ? unit0_of[mid] : w.spans[mid].unit0) <= p.unit)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    p.span = lo;
-    w.parts[tid] = p;
+  return cut;
+}
+
+// Where a part begins; unit0_at(i): of span i.
+template <typename F>
+__device__ __forceinline__ Start start_of(const Cut& cut, int part, int spans, F&& unit0_at) {
+  Start p;
+  p.unit = part_start(cut, part);
+  p.stop = part_start(cut, part + 1);
+  // The last span that begins at or before the unit (spans without pairs begin
+  // where the next does).
+  int lo = 0, hi = spans - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (unit0_at(mid) <= p.unit)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
+  p.span = lo;
+  return p;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PrefixAttentionArgs a) {
+  __shared__ LdsPlan<kPlanThreads, false> lds;
+  Plan w;
+  carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
+  const Cut cut = make_plan<kPlanThreads, false>(a, w, lds, nullptr, true);
+  const int tid = threadIdx.x;
+  if (tid < cut.parts)
+    w.parts[tid] = start_of(cut, tid, static_cast<int>(a.groups + a.batch),
+                            [&](int i) { return i < 2 * kPlanThreads ? lds.unit0[i] : w.spans[i].unit0; });
 }
 
 // ------------------------------------------------------------- the attention
@@ -347,19 +384,49 @@ struct LdsMany {  // more
 union Lds {
   LdsFew few;
   LdsMany many;
+  LdsPlan<kThreads, true> plan;
 };
+constexpr int kHere = kThreads;   // spans, at most, of a plan that every workgroup makes
 constexpr int kStage = 16 * 1024;                // 32 pairs in LDS, of a wave before and after the tiles
-static_assert(sizeof(Lds) <= 160 * 1024 && 4 * kStage <= 2 * kTileBytes, "LDS");
+static_assert(sizeof(Lds) + kHere * sizeof(Span) <= 160 * 1024 && 4 * kStage <= 2 * kTileBytes, "LDS");
 static_assert(offsetof(LdsMany, keys) % 4096 == 0 && offsetof(LdsMany, rope) % 8192 == 0, "exclusive ors within");
 
 struct Segment {
   int64_t pair0;      // of all pairs
   int32_t count;
+  int32_t length, end;  // request: its tokens, and the row behind its last; else `end` is -1
   int32_t tile0, tile1;
   const int32_t* table;
   bool direct;        // the output itself
   int64_t row;        // of the partial sums
   int64_t row_step;   // between pairs of it
+};
+
+// What a row of a segment sees.
+template <bool HERE>
+struct Seen {
+  const int32_t* visible;   // [rows]; HERE: found among the requests' spans
+  const Span* requests;
+  int32_t batch, heads;
+  __device__ int operator()(const Segment& s, int64_t pair) const {
+    const int row = static_cast<int>(row_of(pair, heads));
+    int length = s.length, end = s.end;
+    if (end < 0) {
+      if constexpr (!HERE) return visible[row];
+      int lo = 0, hi = batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (requests[mid].pair0 + requests[mid].pairs <= pair)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      length = requests[lo].length;
+      end = static_cast<int>(row_of(requests[lo].pair0 + requests[lo].pairs, heads));
+    }
+    length -= end - 1 - row;
+    return length > 0 ? length : 0;
+  }
 };
 
 // The ids of 64 pages, a lane each (-1: none), from a column on.
@@ -547,8 +614,8 @@ __device__ __forceinline__ void nothing(const PrefixAttentionArgs& a, const Plan
 // all pairs.  At barrier A everybody is done with tile t - 1, and tile t + 1 and
 // the largest scores of tile t have arrived; then tile t + 3 is asked for and tile
 // t weighed; at B its P is there, and its outputs and the scores of tile t + 1 follow.
-template <typename T, int TILES>
-__device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, LdsFew& lds) {
+template <typename T, int TILES, typename SEEN>
+__device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, const SEEN& seen, LdsFew& lds) {
   const int tid = own_thread();
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -605,7 +672,7 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   constexpr int kWide = kQkDim / 32, kWideLatent = kCkvDim / 32;   // products of 32 dims
   u32x4_t q[kWide];
   const int64_t pair = s.pair0 + (m_mine < s.count ? m_mine : 0);
-  const int vis = m_mine < s.count ? w.visible[row_of(pair, a.heads)] : 0;
+  const int vis = m_mine < s.count ? seen(s, pair) : 0;
   {
     const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + quad;
     const u32x4_t* qr = static_cast<const u32x4_t*>(a.query_rope) + pair * (kKpeDim / 8) + quad;
@@ -787,8 +854,8 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
 // tile t + 1 has arrived, and so have the halves of tile t's scores; at B P is
 // there.  Products go on across either: operands of the last ones are in registers
 // by then, and those behind it on the way.
-template <typename T>
-__device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, LdsMany& lds) {
+template <typename T, typename SEEN>
+__device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const Plan& w, const Segment& s, const SEEN& seen, LdsMany& lds) {
   const int tid = own_thread();
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -851,7 +918,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   // They come through LDS, 32 pairs at a time in the wave's own 16 KiB of tiles that
   // are not there yet: a load takes two pairs' 512 neighbouring bytes, where loads
   // to the registers would take 32 bytes of 32 pairs.
-  const int vis = m_mine < s.count ? w.visible[row_of(s.pair0 + m_mine, a.heads)] : 0;
+  const int vis = m_mine < s.count ? seen(s, s.pair0 + m_mine) : 0;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     const int in = wave * 32 + n * 8 + (lane >> 3), m = in < s.count ? in : 0;
@@ -1110,21 +1177,41 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   finish<T, 4>(a, w, s, rows, keys_at + wave * kStage, o);
 }
 
-template <typename T>
+// HERE: every workgroup makes the plan by itself, of kHere spans at most; the last
+// one, which has no part where they are few, writes it down for the join.
+template <typename T, bool HERE>
 __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAttentionArgs a) {
+  struct None {};
   __shared__ __align__(16384) Lds lds;
+  __shared__ typename std::conditional<HERE, Span[kHere], None>::type here;
   Plan w;
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int part = blockIdx.x;
-  if (part >= w.cut->parts) return;
-  const int64_t stop = uniform(w.parts[part].stop);
-  int64_t at = uniform(w.parts[part].unit);
-  int at_span = uniform(w.parts[part].span);
+  Start start;
+  Seen<HERE> seen{w.visible, nullptr, static_cast<int32_t>(a.batch), static_cast<int32_t>(a.heads)};
+  if constexpr (HERE) {
+    const Cut cut = make_plan<kThreads, true>(a, w, lds.plan, here, part == kParts - 1);
+    if (part >= cut.parts) return;
+    start = start_of(cut, part, static_cast<int>(a.groups + a.batch), [&](int i) { return here[i].unit0; });
+    seen.requests = here + a.groups;
+  } else {
+    if (part >= w.cut->parts) return;
+    start = w.parts[part];
+  }
+  const int64_t stop = uniform(start.stop);
+  int64_t at = uniform(start.unit);
+  int at_span = uniform(start.span);
+  auto span_at = [&](int i) -> Span {
+    if constexpr (HERE)
+      return uniform(here[i]);
+    else
+      return uniform(w.spans[i]);
+  };
   while (at < stop) {
-    Span s = uniform(w.spans[at_span]);
+    Span s = span_at(at_span);
     int64_t end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
     while (at >= end) {
-      s = uniform(w.spans[++at_span]);
+      s = span_at(++at_span);
       end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
     }
     const int units = s.tiles + kBegin;
@@ -1139,24 +1226,25 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
     g.tile0 = s.tile0 + tile_of(at - item_start);
     g.tile1 = s.tile0 + tile_of(seg_end - item_start);
     g.table = a.block_table + s.table * a.cols;
+    g.length = s.length;
+    g.end = at_span >= a.groups ? static_cast<int>(row_of(s.pair0 + s.pairs, a.heads)) : -1;
     const bool whole = at == item_start && seg_end == item_end;
     g.direct = whole && s.merge < 0;
     g.row = whole ? merge_row(w, s.merge, first, at_span >= a.groups) : part_row(w, part, at == item_start);
     g.row_step = whole ? 2 : 1;
-    // A request's last row of the item sees the most; its last row of all sees its length.
-    if (at_span >= a.groups && s.pairs - first - g.count >= a.heads) {
-      const int seen = (uniform(w.visible[row_of(g.pair0 + g.count - 1, a.heads)]) + kKeys - 1) / kKeys;
-      g.tile1 = g.tile1 < seen ? g.tile1 : seen;
+    if (at_span >= a.groups) {  // a request's last row of the item sees the most
+      const int tiles = (seen(g, g.pair0 + g.count - 1) + kKeys - 1) / kKeys;
+      g.tile1 = g.tile1 < tiles ? g.tile1 : tiles;
       g.tile0 = g.tile0 < g.tile1 ? g.tile0 : g.tile1;
     }
     if (g.tile0 >= g.tile1)
       nothing<T>(a, w, g);
     else if (g.count <= 32)
-      attend<T, 1>(a, w, g, lds.few);
+      attend<T, 1>(a, w, g, seen, lds.few);
     else if (g.count <= 64)
-      attend<T, 2>(a, w, g, lds.few);
+      attend<T, 2>(a, w, g, seen, lds.few);
     else
-      attend_many<T>(a, w, g, lds.many);
+      attend_many<T>(a, w, g, seen, lds.many);
     at = seg_end;
   }
 }
@@ -1274,10 +1362,15 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
 
 template <typename T>
 hipError_t launch(const PrefixAttentionArgs& a, hipStream_t stream) {
-  launch_kernel(kKernPrefixPlan, prefix_plan_kernel, dim3(1), dim3(kPlanThreads), stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  launch_kernel(kKernPrefixAttention, prefix_attention_kernel<T>, dim3(kParts), dim3(kThreads), stream, a);
+  hipError_t e;
+  if (a.groups + a.batch <= kHere) {
+    launch_kernel(kKernPrefixAttention, prefix_attention_kernel<T, true>, dim3(kParts), dim3(kThreads), stream, a);
+  } else {
+    launch_kernel(kKernPrefixPlan, prefix_plan_kernel, dim3(1), dim3(kPlanThreads), stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    launch_kernel(kKernPrefixAttention, prefix_attention_kernel<T, false>, dim3(kParts), dim3(kThreads), stream, a);
+  }
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (a.rows * a.heads < kJoinByWave)
