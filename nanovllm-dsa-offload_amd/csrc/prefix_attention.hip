@@ -31,10 +31,13 @@ constexpr int kSteps = kQkDim / 16;   // products of 16 dims: 32 of the latent, 
 constexpr int kTileLoads = 9;         // of a wave
 constexpr int kParts = 256;           // workgroups, one per CU (LDS)
 constexpr int kBegin = 8;             // what the start of a segment costs, in tiles
-constexpr int kJoinByWave = 4096;     // pairs from which a wave joins one
+constexpr int kJoinByWave = 2048;     // pairs from which a wave joins one
 constexpr int kLeastTiles = 4;        // of a part
+// What sharing has to save in all, in half tiles of up to 32 pairs (0.4 us of a
+// part): below, more items that every workgroup has a part of end sooner than fewer
+// and their join.
+constexpr int kLeastSaved = 13 * kParts;
 constexpr int kEasyParts = 8;         // parts of an item that may hold fewer: the join has them all on their way at once
-constexpr int kLeastShared = 8;       // tiles of a prefix that is read once
 constexpr float kLog2e = 1.4426950408889634f;
 // P = 2^(score - reference): a reference is set so that the largest P of its
 // tile is 2^kRise and kept until one passes 2^kMost.  fp16 holds P from 2^-24
@@ -121,6 +124,9 @@ __device__ inline int quotient(int64_t x, int32_t d) {
   while (static_cast<int64_t>(q) * d > x) --q;
   return q;
 }
+// What a tile of a request's or a group's items takes, in half tiles of up to 32 pairs
+// (measured: 2100, 3000 and 3500 clocks for 32, 64 and 128 pairs).
+__device__ inline int32_t time_of(int32_t pairs) { return pairs <= 32 ? 2 : (pairs <= 64 ? 3 : (pairs + kPairs - 1) / kPairs * 4); }
 // Values that every lane holds, in scalar registers.
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline int64_t uniform(int64_t x) {
@@ -204,29 +210,41 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
   auto group_end = [&](int g) { return clamp(HERE || g < THREADS ? lds.group_ends[g] : a.group_ends[g], batch); };
   auto length_of = [&](int b) { return clamp(b == tid ? own_length : a.seq_kv[b], cap); };
   int64_t units = 0, merged = 0, items = 0;
-  // Groups: one that shares has a request's pages read for several of them, and
-  // fewer pairs a request than an item holds (else every item is full anyway).
-  for (int g0 = 0; g0 < groups; g0 += THREADS) {
-    const int g = g0 + tid;
+  // Groups: one that shares has its pages read for several requests, whose pairs
+  // fit fewer items, and saves more than its items' beginnings cost.
+  auto group_span = [&](int g, int64_t* saved) {
     Span s{};
     s.merge = s.group = -1;
-    if (g < groups) {
-      const int b0 = g > 0 ? group_end(g - 1) : 0, b1 = group_end(g);
-      if (b1 - b0 >= 2) {
-        const int r0 = row_at(b0), r1 = row_at(b1);
-        const int tokens = clamp(g == tid ? own_prefix : a.prefix_lens[g], cap);
-        const int tiles = tokens / kBlock * kPageTiles;
-        const int64_t pairs = static_cast<int64_t>(r1 - r0) * heads;
-        if (tiles >= kLeastShared && r1 > r0 && pairs < static_cast<int64_t>(b1 - b0) * kPairs) {
-          s.pair0 = r0 * heads;
-          s.pairs = static_cast<int32_t>(pairs);
-          s.tiles = tiles;
-          s.table = b0;
-        }
-      }
+    if (g >= groups) return s;
+    const int b0 = g > 0 ? group_end(g - 1) : 0, b1 = group_end(g);
+    const int r0 = row_at(b0), r1 = row_at(b1);
+    if (b1 - b0 < 2 || r1 <= r0) return s;
+    const int tokens = clamp(g == tid ? own_prefix : a.prefix_lens[g], cap);
+    s.tiles = tokens / kBlock * kPageTiles;
+    s.pair0 = r0 * heads;
+    s.table = b0;
+    const int pairs = (r1 - r0) * heads, n = b1 - b0;
+    const int64_t less = s.tiles * (static_cast<int64_t>(n) * time_of(static_cast<uint32_t>(pairs) / static_cast<uint32_t>(n)) - time_of(pairs));
+    if (pairs < static_cast<int64_t>(n) * kPairs && less > 2 * kBegin * time_of(pairs)) {
+      s.pairs = pairs;
+      *saved += less;
     }
-    int64_t none = 0, m = s.pairs, sum, sum_m;
-    plan_scan<THREADS>(m, none, lds.scratch, &sum_m, &sum);
+    return s;
+  };
+  int64_t saved = 0;
+  const Span own_group = group_span(tid, &saved);
+  for (int g = tid + THREADS; g < groups; g += THREADS) group_span(g, &saved);
+  bool shares = true;   // until the first sum is there
+  for (int g0 = 0; g0 < groups; g0 += THREADS) {
+    const int g = g0 + tid;
+    Span s = own_group;
+    int64_t rest = 0;
+    if (g0 > 0) s = group_span(g, &rest);
+    int64_t m = s.pairs, sum_m, all_saved;
+    if (g0 == 0) rest = saved;
+    plan_scan<THREADS>(m, rest, lds.scratch, &sum_m, &all_saved);
+    if (g0 == 0) shares = all_saved >= kLeastSaved;
+    if (!shares) s.pairs = 0;
     // (Ends that decrease could count a request's pairs for several groups: there
     // is room for each pair once.)
     if (merged + m + s.pairs > merge_pairs(rows, heads, batch)) s.pairs = 0;
@@ -1250,8 +1268,8 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
 }
 
 // -------------------------------------------------------------------- the join
-// WAVES waves a pair: its segments' references, then their sums, four at a time on
-// their way, every wave those of its turn.
+// WAVES waves a pair: its segments' references, then their sums, four or eight at a
+// time on their way, every wave those of its turn.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a) {
   __shared__ float4 others[WAVES > 1 ? 4 : 1][2][64];
@@ -1308,11 +1326,12 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
     const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - top);
     l += wave_all_op(f == 0.f ? 0.f : v.y * f, AddOp{});
     const int count = n - k0 < 64 ? n - k0 : 64;
-    for (int k = turn; k < count; k += 4 * WAVES) {
-      float4 x[4][2];
-      float by[4];
+    auto add = [&](int k, auto at_once) __attribute__((always_inline)) {
+      constexpr int kRows = decltype(at_once)::value;
+      float4 x[kRows][2];
+      float by[kRows];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         const int at = k + u * WAVES;  // (lanes from `count` on hold row 0 and a factor of zero)
         by[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), at & 63));
         by[u] = at < count ? by[u] : 0.f;
@@ -1322,7 +1341,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
         x[u][1] = p[64];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         if (by[u] == 0.f) continue;  // (a part without tiles wrote no sums)
         acc[0] = fmaf(x[u][0].x, by[u], acc[0]);
         acc[1] = fmaf(x[u][0].y, by[u], acc[1]);
@@ -1333,7 +1352,11 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
         acc[6] = fmaf(x[u][1].z, by[u], acc[6]);
         acc[7] = fmaf(x[u][1].w, by[u], acc[7]);
       }
-    }
+    };
+    int k = turn;
+    if constexpr (WAVES > 1)
+      for (; count - k > 4 * WAVES; k += 8 * WAVES) add(k, std::integral_constant<int, 8>{});
+    for (; k < count; k += 4 * WAVES) add(k, std::integral_constant<int, 4>{});
   }
   if constexpr (WAVES > 1) {  // (every wave of the workgroup is here, or none: they have one pair)
     static_assert(WAVES == 4, "a workgroup a pair");

@@ -196,3 +196,21 @@ def check_attention(got, c, scale=SCALE):
     assert worst <= 1.0, worst
     assert torch.equal(got[last:].view(torch.int16), c["out"][last:].view(torch.int16))
     return worst
+
+
+def shared_units(c, counts, heads):
+    """What the call's groups save, in the half tiles that decide whether their
+    prefixes are read once (2 for a tile of up to 32 pairs, 3 up to 64, 4 for 128)."""
+    time = lambda pairs: 2 if pairs <= 32 else 3 if pairs <= 64 else 4 * -(-pairs // 128)  # noqa: E731
+    at, saved = 0, 0
+    for end, prefix in zip(c["group_ends"].tolist(), c["prefix"].tolist()):
+        n, pairs = end - at, sum(counts[at:end]) * heads
+        tiles = prefix // PAGE * 4
+        less = tiles * (n * time(pairs // n) - time(pairs)) if n > 1 else 0
+        if n > 1 and 0 < pairs < n * 128 and less > 16 * time(pairs):
+            saved += less
+        at = end
+    return saved
+
+
+READ_ONCE = 13 * 256  # half tiles saved from which a call's prefixes are read once
