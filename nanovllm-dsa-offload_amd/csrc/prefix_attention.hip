@@ -33,6 +33,7 @@ constexpr int kParts = 256;           // workgroups, one per CU (LDS)
 constexpr int kBegin = 8;             // what the start of a segment costs, in tiles
 constexpr int kJoinByWave = 2048;     // pairs from which a wave joins one
 constexpr int kLeastTiles = 4;        // of a part
+constexpr int kNarrow = 5 * kParts;   // tiles up to which items hold 64 pairs
 // What sharing has to save in all, in half tiles of up to 32 pairs (0.4 us of a
 // part): below, more items that every workgroup has a part of end sooner than fewer
 // and their join.
@@ -64,6 +65,7 @@ struct Cut {         // of all units into parts: the first `longer` ones hold on
   int32_t parts;     // (0: no units)
   int32_t longer;
   int64_t units;     // of the others
+  int32_t width;     // pairs of an item
 };
 struct Plan {
   Start* parts;      // [kParts]
@@ -106,8 +108,8 @@ __host__ __device__ inline size_t carve(void* ws, int64_t rows, int64_t heads, i
   return static_cast<size_t>(p - start);
 }
 
-__device__ inline int64_t items_of(const Span& s) { return (static_cast<int64_t>(s.pairs) + kPairs - 1) / kPairs; }
-__device__ inline int64_t units_of(const Span& s) { return items_of(s) * (s.tiles + kBegin); }
+__device__ inline int32_t items_of(const Span& s, int width) { return (s.pairs + width - 1) / width; }
+__device__ inline int64_t units_of(const Span& s, int width) { return static_cast<int64_t>(items_of(s, width)) * (s.tiles + kBegin); }
 __device__ inline int64_t part_start(const Cut& c, int w) { return w * c.units + (w < c.longer ? w : c.longer); }
 // The part of a unit.  (At most kParts of them, so that the guess is off by one at most.)
 __device__ inline int part_of(const Cut& c, int64_t unit) {
@@ -210,6 +212,7 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
   auto group_end = [&](int g) { return clamp(HERE || g < THREADS ? lds.group_ends[g] : a.group_ends[g], batch); };
   auto length_of = [&](int b) { return clamp(b == tid ? own_length : a.seq_kv[b], cap); };
   int64_t units = 0, merged = 0, items = 0;
+  int width = kPairs;
   // Groups: one that shares has its pages read for several requests, whose pairs
   // fit fewer items, and saves more than its items' beginnings cost.
   auto group_span = [&](int g, int64_t* saved) {
@@ -250,7 +253,7 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
     if (merged + m + s.pairs > merge_pairs(rows, heads, batch)) s.pairs = 0;
     if (s.pairs > 0) s.merge = merged + m;
     merged += sum_m;
-    int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
+    int64_t u = units_of(s, kPairs), n = items_of(s, kPairs), sum_u, sum_n;
     plan_scan<THREADS>(u, n, lds.scratch, &sum_u, &sum_n);
     s.unit0 = units + u;
     units += sum_u;
@@ -301,11 +304,21 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
         }
       }
     }
-    int64_t u = s.pairs > 0 ? units_of(s) : 0, n = s.pairs > 0 ? items_of(s) : 0, sum_u, sum_n;
+    int64_t u = units_of(s, kPairs), sum_u, sum_n;
+    int64_t n = items_of(s, kPairs) | static_cast<int64_t>(items_of(s, kPairs / 2)) << 32;  // (both fit 31 bits)
     plan_scan<THREADS>(u, n, lds.scratch, &sum_u, &sum_n);
+    int sum_items = static_cast<int>(sum_n);
+    const int narrow_items = static_cast<int>(sum_n >> 32);
+    if (items == 0 && batch <= THREADS && narrow_items > sum_items && sum_u - sum_items * kBegin <= kNarrow) {
+      int64_t none = 0;
+      width = kPairs / 2;
+      u = units_of(s, width);
+      plan_scan<THREADS>(u, none, lds.scratch, &sum_u, &sum_n);
+      sum_items = narrow_items;
+    }
     s.unit0 = units + u;
     units += sum_u;
-    items += sum_n;
+    items += sum_items;
     if (b < batch) {
       if (writes) w.spans[groups + b] = s;
       if constexpr (HERE)
@@ -343,6 +356,7 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
   cut.units = units / cut.parts;
   cut.longer = static_cast<int32_t>(units - cut.units * cut.parts);
   if (units == 0) cut.parts = 0;
+  cut.width = width;
   if (writes && tid == 0) *w.cut = cut;
   __syncthreads();
   return cut;
@@ -426,21 +440,22 @@ struct Seen {
   const int32_t* visible;   // [rows]; HERE: found among the requests' spans
   const Span* requests;
   int32_t batch, heads;
+  // (No lane leaves the others' way here: the compiler has put the copy of a register
+  // before the point where all lanes are back.)
   __device__ int operator()(const Segment& s, int64_t pair) const {
     const int row = static_cast<int>(row_of(pair, heads));
     int length = s.length, end = s.end;
-    if (end < 0) {
+    if (s.end < 0) {
       if constexpr (!HERE) return visible[row];
-      int lo = 0, hi = batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (requests[mid].pair0 + requests[mid].pairs <= pair)
-          lo = mid + 1;
-        else
-          hi = mid;
+      int at = 0;   // requests that end at or before the pair
+      for (int step = kHere; step > 0; step >>= 1) {
+        const int next = at + step;
+        const Span& last = requests[(next < batch ? next : batch) - 1];
+        at = next < batch && last.pair0 + last.pairs <= pair ? next : at;
       }
-      length = requests[lo].length;
-      end = static_cast<int>(row_of(requests[lo].pair0 + requests[lo].pairs, heads));
+      const Span& mine = requests[at];
+      length = mine.length;
+      end = static_cast<int>(row_of(mine.pair0 + mine.pairs, heads));
     }
     length -= end - 1 - row;
     return length > 0 ? length : 0;
@@ -690,7 +705,8 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
   constexpr int kWide = kQkDim / 32, kWideLatent = kCkvDim / 32;   // products of 32 dims
   u32x4_t q[kWide];
   const int64_t pair = s.pair0 + (m_mine < s.count ? m_mine : 0);
-  const int vis = m_mine < s.count ? seen(s, pair) : 0;
+  int vis = seen(s, pair);
+  vis = m_mine < s.count ? vis : 0;
   {
     const u32x4_t* qn = static_cast<const u32x4_t*>(a.query) + pair * (kCkvDim / 8) + quad;
     const u32x4_t* qr = static_cast<const u32x4_t*>(a.query_rope) + pair * (kKpeDim / 8) + quad;
@@ -936,7 +952,8 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
   // They come through LDS, 32 pairs at a time in the wave's own 16 KiB of tiles that
   // are not there yet: a load takes two pairs' 512 neighbouring bytes, where loads
   // to the registers would take 32 bytes of 32 pairs.
-  const int vis = m_mine < s.count ? seen(s, s.pair0 + m_mine) : 0;
+  int vis = seen(s, s.pair0 + (m_mine < s.count ? m_mine : 0));
+  vis = m_mine < s.count ? vis : 0;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     const int in = wave * 32 + n * 8 + (lane >> 3), m = in < s.count ? in : 0;
@@ -1206,15 +1223,18 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
   carve(a.workspace, a.rows, a.heads, a.batch, a.groups, &w);
   const int part = blockIdx.x;
   Start start;
+  int width;
   Seen<HERE> seen{w.visible, nullptr, static_cast<int32_t>(a.batch), static_cast<int32_t>(a.heads)};
   if constexpr (HERE) {
     const Cut cut = make_plan<kThreads, true>(a, w, lds.plan, here, part == kParts - 1);
     if (part >= cut.parts) return;
+    width = cut.width;
     start = start_of(cut, part, static_cast<int>(a.groups + a.batch), [&](int i) { return here[i].unit0; });
     seen.requests = here + a.groups;
   } else {
     if (part >= w.cut->parts) return;
     start = w.parts[part];
+    width = uniform(w.cut->width);
   }
   const int64_t stop = uniform(start.stop);
   int64_t at = uniform(start.unit);
@@ -1227,10 +1247,10 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
   };
   while (at < stop) {
     Span s = span_at(at_span);
-    int64_t end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
+    int64_t end = s.unit0 + units_of(s, width);
     while (at >= end) {
       s = span_at(++at_span);
-      end = s.unit0 + (s.pairs > 0 ? units_of(s) : 0);
+      end = s.unit0 + units_of(s, width);
     }
     const int units = s.tiles + kBegin;
     const int item = uniform(quotient(at - s.unit0, units));
@@ -1238,9 +1258,9 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
     const int64_t seg_end = item_end < stop ? item_end : stop;
     auto tile_of = [&](int64_t u) { return u > kBegin ? static_cast<int>(u) - kBegin : 0; };
     Segment g;
-    const int first = item * kPairs;
+    const int first = item * width;
     g.pair0 = static_cast<int64_t>(s.pair0) + first;
-    g.count = s.pairs - first < kPairs ? s.pairs - first : kPairs;
+    g.count = s.pairs - first < width ? s.pairs - first : width;
     g.tile0 = s.tile0 + tile_of(at - item_start);
     g.tile1 = s.tile0 + tile_of(seg_end - item_start);
     g.table = a.block_table + s.table * a.cols;
@@ -1291,11 +1311,11 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
   };
   auto run_of = [&](const Span& s, bool is_own) {
     Run r;
-    const int in = pair - s.pair0, item = in / kPairs;
+    const int in = pair - s.pair0, item = in / cut.width;
     const int64_t units = s.tiles + kBegin, u0 = s.unit0 + item * units;
     r.w0 = part_of(cut, u0);
     r.n = part_of(cut, u0 + units - 1) - r.w0 + 1;
-    r.m = in - item * kPairs;
+    r.m = in - item * cut.width;
     r.whole = r.n == 1 ? merge_row(w, s.merge, in, is_own) : -1;
     return r;
   };
