@@ -6,10 +6,24 @@
 // A query (row, head) is a pair; the packed rows of a group's requests are
 // neighbours, so that all their pairs make one product with the pages that the
 // group shares: items of up to 128 pairs against those pages, read once, and
-// items of one request's pairs against the pages behind them.  A plan kernel
-// lays the items' tiles of keys in a row and cuts it into equal parts, one per
-// workgroup; what lies across parts, and a pair's two items, leave fp32 partial
-// sums that a join kernel adds up.
+// items of one request's pairs against the pages behind them.  A plan lays the
+// items' tiles of 32 keys in a row and cuts it into equal parts, one per workgroup
+// and CU; what lies across parts, and a pair's two items, leave fp32 partial sums
+// that a join kernel adds up.
+//
+// A softmax in one pass: P = 2^(score - reference) per row, with a reference that
+// moves only when a score outgrows it, sums of P and P V in fp32, one division at
+// the end.  P is rounded to the cache's 16 bits for the second product (half a step
+// of each term, as the stored output); everything else stays in fp32.
+//
+// Bounds.  Items of 128 pairs: their products, 68 of 32 x 32 x 16 a wave and tile,
+// 2176 clocks; a tile takes 3480 (loads 230 of them, the softmax 380, the wait for
+// LDS at either barrier about 90 each), and the clock falls to 1.8 GHz under them:
+// 64 rows of 64 heads on four prefixes of 32768 tokens run at 0.98 PFLOP/s, where the
+// library's 8192^3 product reaches 1.25.  Items of up to 64: the pages' way, 64
+// bytes a clock and CU (64 requests of 100 to 4000 own tokens, 16 heads: 33 us,
+// 4.5 TB/s, a large copy 4.8).  Small calls: latency, 12 us of launch, plan, page
+// ids, first tiles, last sums, and 5 of the join.
 #include <cstddef>
 #include <utility>
 
@@ -30,15 +44,33 @@ constexpr int kTileBytes = kKeys * (kCkvBytes + kKpeBytes);
 constexpr int kSteps = kQkDim / 16;   // products of 16 dims: 32 of the latent, 4 of the rope
 constexpr int kTileLoads = 9;         // of a wave
 constexpr int kParts = 256;           // workgroups, one per CU (LDS)
-constexpr int kBegin = 8;             // what the start of a segment costs, in tiles
-constexpr int kJoinByWave = 2048;     // pairs from which a wave joins one
-constexpr int kLeastTiles = 4;        // of a part
-constexpr int kNarrow = 5 * kParts;   // tiles up to which items hold 64 pairs
+// What the begin and end of a segment cost, in tiles (measured: 30 to 45 thousand
+// clocks).  With 4: a drafting step of 16 x 4 rows 54 us and not 45, a part that
+// begins many segments being the last.
+constexpr int kBegin = 8;
+// Pairs from which a wave joins one, and not four: 4000 pairs 11 us, and 23 by four
+// waves each; 192 pairs cut into 180 parts 12.5 and 7.5 us.
+constexpr int kJoinByWave = 2048;
+// Tiles of a part at least: half of it would double the sums that are written and
+// joined, twice takes as long as the tiles do (24 requests in three groups: 24 us, and
+// 35 with 8; with 3 the attention 1 us less, the join of one long request 3 more).
+constexpr int kLeastTiles = 4;
+// Tiles (of items of 128 pairs) up to which items hold 64, whose segments begin and
+// end in half the time.  128 heads, in all: 1000 tokens 25 us and not 29, 32 x 1000
+// (1024 tiles) 47 and 51; 32 x 2000 (2016 tiles) 59 and 57, 32 x 4000 88 and 73.
+constexpr int kNarrow = 5 * kParts;
 // What sharing has to save in all, in half tiles of up to 32 pairs (0.4 us of a
-// part): below, more items that every workgroup has a part of end sooner than fewer
-// and their join.
+// part each): below, more items that every workgroup has a part of end sooner than
+// fewer and their join.  In all, read once and by everybody: 16 requests of 64 heads
+// on 4096 tokens (8 a part) 45 us and 42, on 8192 (16) 54 and 56; 16 x 4 rows on
+// 8192 to 12301 (14) 56 and 60; 64 of 16 heads on 1024 (12) 39 and 33, on 2048 (24)
+// 41 and 42; 32 on 16384 tokens (64) 106 and 149.
 constexpr int kLeastSaved = 13 * kParts;
-constexpr int kEasyParts = 8;         // parts of an item that may hold fewer: the join has them all on their way at once
+// Parts of an item that may hold fewer than kLeastTiles: the join has them all on
+// their way at once.  One request of 16 heads and 1000 tokens 13.6 us and not 14.6, 2
+// short ones 12.8 and 19.4; with 16 parts 4 requests of 32 heads on 4096 tokens take
+// 3 us more.
+constexpr int kEasyParts = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 // P = 2^(score - reference): a reference is set so that the largest P of its
 // tile is 2^kRise and kept until one passes 2^kMost.  fp16 holds P from 2^-24
@@ -418,7 +450,10 @@ union Lds {
   LdsMany many;
   LdsPlan<kThreads, true> plan;
 };
-constexpr int kHere = kThreads;   // spans, at most, of a plan that every workgroup makes
+// Spans, at most, of a plan that every workgroup makes: LDS has room for them beside
+// the tiles.  Against a plan kernel before (in all): 2 short requests 18 us and not
+// 22, 24 requests in three groups 31 and 36, 32 on 16384 tokens 106 and 110.
+constexpr int kHere = kThreads;
 constexpr int kStage = 16 * 1024;                // 32 pairs in LDS, of a wave before and after the tiles
 static_assert(sizeof(Lds) + kHere * sizeof(Span) <= 160 * 1024 && 4 * kStage <= 2 * kTileBytes, "LDS");
 static_assert(offsetof(LdsMany, keys) % 4096 == 0 && offsetof(LdsMany, rope) % 8192 == 0, "exclusive ors within");
@@ -451,7 +486,8 @@ struct Seen {
       for (int step = kHere; step > 0; step >>= 1) {
         const int next = at + step;
         const Span& last = requests[(next < batch ? next : batch) - 1];
-        at = next < batch && last.pair0 + last.pairs <= pair ? next : at;
+        const int32_t last_end = last.pair0 + last.pairs;
+        at = (next < batch) & (last_end <= pair) ? next : at;
       }
       const Span& mine = requests[at];
       length = mine.length;
@@ -475,8 +511,8 @@ struct Pages {
   __device__ void hold(int tile) {
     first = column(tile);
     const int c = first + (threadIdx.x & 63);
-    const int32_t page = c <= last ? table[c] : -1;
-    held = page >= 0 && page < blocks ? page : -1;
+    const int32_t page = table[c <= last ? c : last];   // (no lane leaves: see Seen)
+    held = (c <= last) & (page >= 0) & (page < blocks) ? page : -1;
   }
   __device__ static int column(int tile) { return static_cast<int>(static_cast<uint32_t>(tile) / kPageTiles); }
   __device__ bool holds(int tile) const { return column(tile) - first < 64; }
@@ -1275,6 +1311,9 @@ __global__ __launch_bounds__(kThreads, 1) void prefix_attention_kernel(PrefixAtt
       g.tile1 = g.tile1 < tiles ? g.tile1 : tiles;
       g.tile0 = g.tile0 < g.tile1 ? g.tile0 : g.tile1;
     }
+    // Up to 32 pairs: 64 requests of 16 heads 42 us, and 50 as 64 pairs.  Up to 64: 32
+    // requests of 2 heads on 4096 tokens 25.5 us, and 29.4 as more; there are no
+    // registers for more in attend().
     if (g.tile0 >= g.tile1)
       nothing<T>(a, w, g);
     else if (g.count <= 32)

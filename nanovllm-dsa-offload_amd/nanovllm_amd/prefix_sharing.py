@@ -182,9 +182,10 @@ def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_
     ``prefix_request_ends`` [S] and ``prefix_lengths`` [S] name the groups:
     requests ``[prefix_request_ends[s-1], prefix_request_ends[s])`` hold the same
     pages for their first ``prefix_lengths[s]`` tokens (the whole pages among
-    them; what is left counts as their own).  Those pages are taken from the
-    first request's table and multiplied with the queries of all of them at
-    once.  Results are those of a call without groups, up to the order of sums.
+    them; what is left counts as their own).  Where that saves enough time, those
+    pages are taken from the first request's table, read once, and multiplied
+    with the queries of all of them; small calls read every request's own.
+    Results are those of a call without groups, up to the order of sums.
     Requests behind the last end, and a group of one, share nothing."""
     _shared_prefix_attention_op(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope,
                                 kv_cache, float(scale_value), attention_out, prefix_request_ends, prefix_lengths)
