@@ -9,7 +9,7 @@ together, and then need, beside the operators of the other modules:
 * :func:`norm_rope_append` makes a step's new cache rows (norm of the latent,
   rotation of the rope part) and writes them to their pages, and rotates, on
   request also normalises, the queries in the same pass;
-* :func:`shared_prefix_attention` is absorbed-MLA attention that reads a page
+* :func:`shared_prefix_attention` is absorbed-MLA attention that can read a page
   shared by a group of requests once for all of them;
 * :func:`pages_branch` lets requests go on from others (a page is held by
   several until someone writes to it) and gives every request pages of its own
