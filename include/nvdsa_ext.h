@@ -201,9 +201,10 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query,
  * [T, N, 64].
  * Groups (both tensors [S], or neither): requests [prefix_request_ends[s-1],
  * prefix_request_ends[s]) hold the same pages for their first prefix_lengths[s]
- * tokens (whole pages: the rest of that length counts as their own), which are
- * read through the first request's table, once for the group.  Requests behind
- * the last end share nothing.  The workspace holds no state. */
+ * tokens (whole pages: the rest of that length counts as their own).  Where that
+ * saves enough time they are read through the first request's table, once for the
+ * group.  Requests behind the last end share nothing.  The workspace holds no
+ * state. */
 size_t nvdsa_shared_prefix_attention_workspace_size(int64_t query_rows, int64_t heads, int64_t batch, int64_t groups);
 int nvdsa_shared_prefix_attention(const nvdsa_tensor* query_rope,
                                   const nvdsa_tensor* query,

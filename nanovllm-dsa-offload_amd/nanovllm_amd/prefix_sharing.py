@@ -33,7 +33,7 @@ page_refs             [P]                   int32 holders of each page, 0: free
 ====================  ====================  ==============================================
 
 The ends of packed rows must not decrease.  Packed rows behind the last request
-are neither read nor written.
+are neither read nor written.  A call's outputs must not overlap its inputs.
 """
 
 from __future__ import annotations
