@@ -1211,6 +1211,7 @@ __device__ __forceinline__ void attend_many(const PrefixAttentionArgs& a, const 
                   u32x4_t{__float_as_uint(next[1][e]), __float_as_uint(next[1][e + 1]), __float_as_uint(next[1][e + 2]),
                           __float_as_uint(next[1][e + 3])});
         }
+        // (Read by assembly: the products that made it lie ten or more products back.)
         if constexpr (n >= 8 && n < 24) mine[n - 8] = moved_here(next[0][n - 8]);
         if constexpr (i == 3) fetch_p(1, r);
         __builtin_amdgcn_sched_barrier(0);
