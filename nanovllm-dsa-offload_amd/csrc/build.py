@@ -20,6 +20,7 @@ PKG_ROOT = CSRC.parent
 REPO = PKG_ROOT.parent
 BUILD_DIR = REPO / "_build" / "nvdsa"
 OUTPUT = PKG_ROOT / "nanovllm_amd" / "libnvdsa.so"
+TENSOR_PACK = PKG_ROOT / "nanovllm_amd" / "_tensor_pack.so"
 SOURCES = ("scatter_copy.hip", "lim.hip", "sfa.hip", "indexer.hip", "persist.hip", "stage.hip", "latent8.hip",
            "norm_rope.hip", "pages.hip", "prefix_attention.hip", "nvdsa_abi.hip")
 ARCH = os.environ.get("NVDSA_OFFLOAD_ARCH", "gfx950")
@@ -64,6 +65,25 @@ def _compile(hipcc: str, src: Path, obj: Path) -> None:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{proc.stdout}\n{proc.stderr}")
 
 
+def _build_tensor_pack() -> None:
+    """The Python module that reads tensors' descriptors: host code, against torch's
+    headers and libraries."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).parent
+    tmp = TENSOR_PACK.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-I{REPO / 'include'}",
+           f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(CSRC / "tensor_pack.cpp"), f"-L{root / 'lib'}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"tensor_pack.cpp failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, TENSOR_PACK)
+
+
 def build(verbose: bool = False) -> Path:
     """Compile every HIP source and link libnvdsa.so; returns its path."""
     hipcc = _hipcc()
@@ -76,6 +96,7 @@ def build(verbose: bool = False) -> Path:
             obj = BUILD_DIR / (src.stem + ".o")
             objs.append(obj)
             futs.append(pool.submit(_compile, hipcc, src, obj))
+        futs.append(pool.submit(_build_tensor_pack))
         for f in futs:
             f.result()
     tmp = OUTPUT.with_suffix(".so.tmp")

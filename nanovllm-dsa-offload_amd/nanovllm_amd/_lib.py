@@ -176,13 +176,26 @@ _NO_TENSOR = (0,) * _ITEM_WORDS
 _MAX_PACKED = 24
 _PLACES = tuple(tuple(range(0, _ITEM_BYTES * k, _ITEM_BYTES)) for k in range(_MAX_PACKED + 1))
 _UNKNOWN_DTYPE = -1 & 0xFFFFFFFF
+try:
+    from ._tensor_pack import pack as _native_pack
+except ImportError:  # (not built: 6 us more for 13 tensors, the same descriptors)
+    _native_pack = None
 
 
 def pack(*tensors: torch.Tensor | None):
     """The tensors' descriptors in one buffer: (buffer, addresses), None for a
     None.  The same fields as :func:`describe`, which builds a ctypes structure
-    per tensor, at a fourth of its host time (a fused step describes 27
-    tensors); the buffer has to outlive the call that reads it."""
+    per tensor; the buffer has to outlive the call that reads it.  Read by
+    ``csrc/tensor_pack.cpp`` where that is built, else by :func:`pack_plain`."""
+    if _native_pack is not None and len(tensors) <= _MAX_PACKED:
+        packed_here = _native_pack(*tensors)
+        if packed_here is not None:
+            return packed_here
+    return pack_plain(*tensors)
+
+
+def pack_plain(*tensors: torch.Tensor | None):
+    """:func:`pack` through the tensors' Python attributes."""
     places = _PLACES[len(tensors)]
     words: list[int] = []
     add, code_of = words.extend, _DTYPE_CODES.get
