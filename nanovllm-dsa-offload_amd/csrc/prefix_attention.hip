@@ -359,8 +359,8 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
         lds.unit0[groups + b] = s.unit0;
     }
   }
-  // The rows' requests, and what they see.
-  for (int t = tid; writes && t < rows; t += THREADS) {
+  // The rows' requests, and what they see (HERE: every workgroup some of them).
+  for (int t = HERE ? blockIdx.x * THREADS + tid : tid; t < rows; t += HERE ? kParts * THREADS : THREADS) {
     int lo = 0, hi = batch;  // the request: an end behind the row, the end before it not
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
