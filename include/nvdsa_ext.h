@@ -198,7 +198,8 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query,
  * that row r sees: row i of a request's n sees the first
  * actual_seq_lengths_kv - (n - 1 - i); slots whose table entry names no page are
  * skipped, a row that sees nothing is zero.  query [T, N, 512], query_rope
- * [T, N, 64].
+ * [T, N, 64].  Scores and sums are fp32; the weights are rounded to the cache's
+ * 16 bits and divided by the sum of what they are rounded to.
  * Groups (both tensors [S], or neither): requests [prefix_request_ends[s-1],
  * prefix_request_ends[s]) hold the same pages for their first prefix_lengths[s]
  * tokens (whole pages: the rest of that length counts as their own).  Where that

@@ -178,6 +178,9 @@ def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_
     slots that row r sees: row i of a request's n sees the first
     ``actual_seq_lengths_kv - (n - 1 - i)``.  A row that sees nothing is zero.
     ``query`` [T, N, 512] and ``query_rope`` [T, N, 64] have the cache's dtype.
+    Scores, their sums and the output's are fp32; the weights are rounded to the
+    cache's 16 bits (they still sum to one), so that an output is off by half a
+    step of its values' mean distance from it beside the store's half step.
 
     ``prefix_request_ends`` [S] and ``prefix_lengths`` [S] name the groups:
     requests ``[prefix_request_ends[s-1], prefix_request_ends[s])`` hold the same
