@@ -1402,7 +1402,9 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixAttentionArgs a)
       v = w.refs[row];
     }
     const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - top);
-    l += wave_all_op(f == 0.f ? 0.f : v.y * f, AddOp{});
+    // (A part whose weight is zero counts for nothing, unless it has seen a NaN; where a
+    // score was infinite, f is NaN.)
+    l += wave_all_op(f == 0.f && v.y == v.y ? 0.f : v.y * f, AddOp{});
     const int count = n - k0 < 64 ? n - k0 : 64;
     auto add = [&](int k, auto at_once) __attribute__((always_inline)) {
       constexpr int kRows = decltype(at_once)::value;
