@@ -121,9 +121,10 @@ __host__ __device__ inline int64_t slot_pairs(int64_t rows, int64_t heads) {
   const int64_t n = (rows * heads + 31) / 32 * 32;
   return n < kPairs ? n : kPairs;
 }
-__host__ __device__ inline int64_t merge_pairs(int64_t rows, int64_t heads, int64_t batch) {
+// Pairs that two items may have: a group of n requests that shares has fewer than 128 n.
+__host__ __device__ inline int64_t merge_pairs(int64_t rows, int64_t heads, int64_t batch, int64_t groups) {
   const int64_t n = rows * heads;
-  return n < batch * kPairs ? n : batch * kPairs;
+  return groups == 0 ? 0 : (n < batch * kPairs ? n : batch * kPairs);
 }
 __host__ __device__ inline size_t carve(void* ws, int64_t rows, int64_t heads, int64_t batch, int64_t groups, Plan* plan) {
   char* p = static_cast<char*>(ws);
@@ -140,7 +141,7 @@ __host__ __device__ inline size_t carve(void* ws, int64_t rows, int64_t heads, i
   w.visible = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * rows));
   w.request = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * rows));
   w.stride = slot_pairs(rows, heads);
-  const int64_t partial = 2 * kParts * w.stride + 2 * merge_pairs(rows, heads, batch);
+  const int64_t partial = 2 * kParts * w.stride + 2 * merge_pairs(rows, heads, batch, groups);
   w.refs = reinterpret_cast<float2*>(take(sizeof(float2) * partial));
   w.sums = reinterpret_cast<float*>(take(sizeof(float) * partial * kCkvDim));
   if (plan) *plan = w;
@@ -289,7 +290,7 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
     if (!shares) s.pairs = 0;
     // (Ends that decrease could count a request's pairs for several groups: there
     // is room for each pair once.)
-    if (merged + m + s.pairs > merge_pairs(rows, heads, batch)) s.pairs = 0;
+    if (merged + m + s.pairs > merge_pairs(rows, heads, batch, groups)) s.pairs = 0;
     if (s.pairs > 0) s.merge = merged + m;
     merged += sum_m;
     int64_t u = units_of(s, kPairs), n = items_of(s, kPairs), sum_u, sum_n;
