@@ -230,10 +230,13 @@ int nvdsa_shared_prefix_attention(const nvdsa_tensor* query_rope,
  * tokens fall into (those within the table): a new one where it has none, and
  * where others hold its page too, except that a page with older rows stays with
  * the lowest of the rows that write on where only these hold it.  New pages are
- * the lowest free ones, given out by row and column.  copy_src / copy_dst /
- * copy_tokens [B] say which rows the new page of a row has to receive (-1, -1,
- * 0: none).  All rows are served or, where too few pages are free, none:
- * missing[0] is the number that lacks, or 0. */
+ * the lowest free ones, given out by row and column (those that the rows' old
+ * tables gave back among them).  copy_src / copy_dst / copy_tokens [B] say which
+ * rows the new page of a row has to receive (-1, -1, 0: none).  All rows get
+ * their pages or, where too few are free, none does: missing[0] is the number that
+ * lacks, or 0.  What the rows took over stays theirs either way: the call is
+ * repeated with parents NULL, or with parents that go by the rows as they are
+ * now. */
 size_t nvdsa_pages_branch_workspace_size(int64_t pages);
 int nvdsa_pages_branch(const nvdsa_tensor* seq_lens,
                        const nvdsa_tensor* new_tokens,

@@ -7,7 +7,8 @@
 //
 //   branch    table[b] = table[parents[b]], page_refs follow; then pages for the
 //             columns that the next new_tokens[b] tokens fall into: new ones
-//             where there is none or where others hold it too.
+//             where there is none or where others hold it too, or none at all
+//             where too few are free (what was taken over stays).
 //   compact   with L pages held, those at or behind L go, in order, to the free
 //             ones below L.
 //   copy      pages src[k] to dst[k] of several caches, or their first tokens[k].

@@ -206,12 +206,16 @@ def pages_branch(seq_lens, new_tokens, block_table, page_refs, copy_src, copy_ds
     ones where it has none, and in the place of pages that others hold too.  A
     page with older rows of several rows that all write on, held by nobody else,
     stays with the lowest of them.  New pages are the lowest free ones, given
-    out by row and column; pages given up by this call are free for the next.
+    out by row and column.  Pages that the rows' old tables give back are among
+    them; those that a row gives up for a new one are free for the next call.
 
     ``copy_src`` / ``copy_dst`` / ``copy_tokens`` [B] list what
     :func:`pages_copy` has to do before the rows are written (-1, -1, 0 for a
-    row without).  All rows are served, or, where too few pages are free, none,
-    and ``missing`` [1] holds the number that lacks (else 0)."""
+    row without).  All rows get their pages, or, where too few are free, none
+    does, and ``missing`` [1] holds the number that lacks (else 0).  The parents'
+    tables and lengths have been taken over then all the same: when pages are
+    free again, the call is to be repeated with ``parents=None``, or with parents
+    that go by the rows as they are now (-1 gives a row's pages back)."""
     _pages_branch_op(seq_lens, new_tokens, block_table, page_refs, copy_src, copy_dst, copy_tokens, missing, parents)
 
 
