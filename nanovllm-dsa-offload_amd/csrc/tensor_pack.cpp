@@ -74,7 +74,8 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
       std::memcpy(place, &item, sizeof(item));
       PyList_SET_ITEM(places, i, at);
     }
-  } catch (const std::exception&) {
+  } catch (...) {
+    PyErr_Clear();   // (a subclass whose sizes are Python's leaves its error set)
     known = false;   // (no memory of its own, symbolic sizes: pack() says so)
   }
   if (!known) {
