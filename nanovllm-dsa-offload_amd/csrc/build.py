@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -20,7 +21,8 @@ PKG_ROOT = CSRC.parent
 REPO = PKG_ROOT.parent
 BUILD_DIR = REPO / "_build" / "nvdsa"
 OUTPUT = PKG_ROOT / "nanovllm_amd" / "libnvdsa.so"
-TENSOR_PACK = PKG_ROOT / "nanovllm_amd" / "_tensor_pack.so"
+# (Python's own name for it: another interpreter does not load it.)
+TENSOR_PACK = PKG_ROOT / "nanovllm_amd" / ("_tensor_pack" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ("scatter_copy.hip", "lim.hip", "sfa.hip", "indexer.hip", "persist.hip", "stage.hip", "latent8.hip",
            "norm_rope.hip", "pages.hip", "prefix_attention.hip", "nvdsa_abi.hip")
 ARCH = os.environ.get("NVDSA_OFFLOAD_ARCH", "gfx950")
@@ -65,23 +67,33 @@ def _compile(hipcc: str, src: Path, obj: Path) -> None:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{proc.stdout}\n{proc.stderr}")
 
 
-def _build_tensor_pack() -> None:
+def _build_tensor_pack() -> bool:
     """The Python module that reads tensors' descriptors: host code, against torch's
-    headers and libraries."""
-    import sysconfig
-
-    import torch
-
-    root = Path(torch.__file__).parent
+    headers and libraries, whose version it carries.  The package works without it
+    (``_lib.pack_plain``), so where it does not compile there is a warning, and none
+    is left from before."""
     tmp = TENSOR_PACK.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-I{REPO / 'include'}",
-           f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-           f"-I{sysconfig.get_paths()['include']}", str(CSRC / "tensor_pack.cpp"), f"-L{root / 'lib'}", "-ltorch_python",
-           "-ltorch_cpu", "-lc10", "-o", str(tmp)]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"tensor_pack.cpp failed:\n{proc.stdout}\n{proc.stderr}")
-    os.replace(tmp, TENSOR_PACK)
+    try:
+        import torch
+
+        root = Path(torch.__file__).parent
+        cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-I{REPO / 'include'}",
+               f'-DNVDSA_TORCH_VERSION="{torch.__version__}"', f"-I{root / 'include'}",
+               f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+               str(CSRC / "tensor_pack.cpp"), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        error = proc.stdout + proc.stderr if proc.returncode != 0 else ""
+        built = proc.returncode == 0
+    except (ImportError, OSError) as e:
+        error, built = str(e), False
+    if built:
+        os.replace(tmp, TENSOR_PACK)
+    else:
+        print(f"warning: tensor_pack.cpp was not built (calls describe their tensors through Python):\n{error}", file=sys.stderr)
+    for old in TENSOR_PACK.parent.glob("_tensor_pack*.so"):
+        if not built or old != TENSOR_PACK:
+            old.unlink()
+    return built
 
 
 def build(verbose: bool = False) -> Path:

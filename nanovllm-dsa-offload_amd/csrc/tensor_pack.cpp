@@ -96,4 +96,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_pack", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensor_pack() { return PyModule_Create(&module); }
+// (torch_version: of the headers that `pack` was compiled against; the tensors' fields
+// lie where they say, so that the module is of use with that version alone.)
+PyMODINIT_FUNC PyInit__tensor_pack() {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", NVDSA_TORCH_VERSION) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -176,8 +176,18 @@ _NO_TENSOR = (0,) * _ITEM_WORDS
 _MAX_PACKED = 24
 _PLACES = tuple(tuple(range(0, _ITEM_BYTES * k, _ITEM_BYTES)) for k in range(_MAX_PACKED + 1))
 _UNKNOWN_DTYPE = -1 & 0xFFFFFFFF
+
+
+def _native_of(module):
+    """The extension's ``pack``, or None where it was built against another torch: it
+    reads tensors' fields where that one's headers say."""
+    return module.pack if getattr(module, "torch_version", None) == str(torch.__version__) else None
+
+
 try:
-    from ._tensor_pack import pack as _native_pack
+    from . import _tensor_pack
+
+    _native_pack = _native_of(_tensor_pack)
 except ImportError:  # (not built: 6 us more for 13 tensors, the same descriptors)
     _native_pack = None
 
