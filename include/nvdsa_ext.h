@@ -204,8 +204,10 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query,
  * prefix_request_ends[s]) hold the same pages for their first prefix_lengths[s]
  * tokens (whole pages: the rest of that length counts as their own).  Where that
  * saves enough time they are read through the first request's table, once for the
- * group.  Requests behind the last end share nothing.  The workspace holds no
- * state. */
+ * group.  Requests behind the last end share nothing.  Values that a row does not
+ * see may be anything; a NaN or a score of +inf that it sees makes it NaN; the dims
+ * of an infinite value whose score is -inf are NaN or without that key, as the work
+ * is cut.  The workspace holds no state. */
 size_t nvdsa_shared_prefix_attention_workspace_size(int64_t query_rows, int64_t heads, int64_t batch, int64_t groups);
 int nvdsa_shared_prefix_attention(const nvdsa_tensor* query_rope,
                                   const nvdsa_tensor* query,

@@ -850,7 +850,9 @@ __device__ __forceinline__ void attend(const PrefixAttentionArgs& a, const Plan&
     }
   };
   // Values of keys that some row must not see: P is zero there, but zero times an
-  // infinity or NaN is not.  (A row that does see such a key has them in its scores.)
+  // infinity or NaN is not.  (A row that does see such a key has them in its scores:
+  // NaN, or +inf, which makes its P NaN.  Under a score of -inf P is zero, and the row
+  // loses the NaN that an infinite value makes in its dims elsewhere.)
   auto scrub = [&](int tile) {
     uint8_t* v_tile = lds.keys[tile % kBuffers];
     for (int i = tid; i < kKeys * kCkvBytes / 16; i += kThreads) {

@@ -189,7 +189,11 @@ def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_
     pages are taken from the first request's table, read once, and multiplied
     with the queries of all of them; small calls read every request's own.
     Results are those of a call without groups, up to the order of sums.
-    Requests behind the last end, and a group of one, share nothing."""
+    Requests behind the last end, and a group of one, share nothing.
+
+    What a row does not see may hold anything.  A row that sees a NaN, or a score
+    of +inf, is NaN.  An infinite value under a score of -inf has no weight: its
+    dims are NaN, or what the row's other keys make of them, as the work is cut."""
     _shared_prefix_attention_op(query_rope, query, actual_seq_lengths_query, actual_seq_lengths_kv, block_table, k_rope,
                                 kv_cache, float(scale_value), attention_out, prefix_request_ends, prefix_lengths)
 
