@@ -102,7 +102,8 @@ __device__ inline void cache_row(const NormRopeArgs& a, int64_t t) {
   }
   const int64_t b = request_of_row(a, t);
   if (b >= a.batch) return;
-  const int64_t slot = static_cast<int64_t>(a.seq_kv[b]) - (a.seq_q[b] - t);
+  const int64_t end = a.seq_q[b] < a.rows ? a.seq_q[b] : a.rows;   // (as the attention counts a request's rows)
+  const int64_t slot = a.seq_kv[b] - (end - t);
   if (slot < 0 || slot >= a.cols * kBlock) return;
   const int32_t page = a.block_table[b * a.cols + (slot >> kBlockShift)];
   if (page < 0 || page >= a.blocks) return;

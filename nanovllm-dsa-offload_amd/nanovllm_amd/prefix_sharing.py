@@ -32,8 +32,9 @@ block_table           [B, C]                int32 pages of each request, -1: non
 page_refs             [P]                   int32 holders of each page, 0: free
 ====================  ====================  ==============================================
 
-The ends of packed rows must not decrease.  Packed rows behind the last request
-are neither read nor written.  A call's outputs must not overlap its inputs.
+The ends of packed rows must not decrease, and count as the number of rows where
+they lie past it.  Packed rows behind the last request are neither read nor
+written.  A call's outputs must not overlap its inputs.
 """
 
 from __future__ import annotations
