@@ -93,7 +93,7 @@ struct Span {        // pairs against tiles of one table row's pages
   int32_t tile0, tiles;
   int32_t table;     // row of the block table
   int32_t group;     // request: its group's span (-1: none)
-  int32_t length;    // request: of the tokens
+  int32_t length;    // request: of the tokens (more than the table holds by its rows at most)
 };
 struct Start {       // where a part begins
   int64_t unit;
@@ -250,7 +250,6 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
     return b > 0 ? clamp(HERE || b <= THREADS ? lds.q_ends[b - 1] : a.seq_q[b - 1], rows) : 0;
   };
   auto group_end = [&](int g) { return clamp(HERE || g < THREADS ? lds.group_ends[g] : a.group_ends[g], batch); };
-  auto length_of = [&](int b) { return clamp(b == tid ? own_length : a.seq_kv[b], cap); };
   int64_t units = 0, merged = 0, items = 0;
   int width = kPairs;
   // Groups: one that shares has its pages read for several requests, whose pairs
@@ -317,8 +316,9 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
       const int r0 = row_at(b), r1 = row_at(b + 1);
       s.pair0 = r0 * heads;
       s.pairs = r1 > r0 ? (r1 - r0) * heads : 0;
-      s.length = length_of(b);
-      s.tiles = (s.length + kKeys - 1) / kKeys;
+      // (Tokens past the table have no slots; the rows before the last see so many less.)
+      s.length = clamp(b == tid ? own_length : a.seq_kv[b], cap + (r1 > r0 ? r1 - r0 : 0));
+      s.tiles = static_cast<int>(((s.length < cap ? s.length : cap) + kKeys - 1) / kKeys);
       s.table = b;
       // The group: the first whose end lies behind the request.
       int lo = 0, hi = groups;
@@ -378,12 +378,7 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
         hi = mid;
     }
     if constexpr (!HERE) {
-      int seen = 0;
-      if (lo < batch) {
-        seen = clamp(a.seq_kv[lo], cap) - (row_at(lo + 1) - 1 - t);
-        seen = seen > 0 ? seen : 0;
-      }
-      w.visible[t] = seen;
+      w.visible[t] = lo < batch ? clamp(static_cast<int64_t>(a.seq_kv[lo]) - (row_at(lo + 1) - 1 - t), cap) : 0;
     }
     w.request[t] = lo < batch ? lo : -1;
   }

@@ -129,14 +129,14 @@ def attention(query_rope, query, ends, lengths, table, k_rope, kv_cache, scale):
     out, size = (torch.zeros(rows, heads, 512, dtype=torch.float64) for _ in range(2))
     reach = torch.zeros(rows, heads, dtype=torch.float64)
     for b, (lo, hi) in enumerate(_spans(ends, rows)):
-        cap = table.shape[1] * PAGE
-        length = min(max(int(lengths[b]), 0), cap)
+        cap, tokens = table.shape[1] * PAGE, int(lengths[b])
+        length = min(max(tokens, 0), cap)
         row = table[b, : -(-length // PAGE)].long()
         named = ((row >= 0) & (row < pages)).repeat_interleave(PAGE)[:length]
         at = torch.where((row >= 0) & (row < pages), row, 0)
         keys = torch.cat([kv_cache[at].flatten(0, 2), k_rope[at].flatten(0, 2)], -1)[:length].double()
         for t in range(lo, hi):
-            sees = max(0, length - (hi - 1 - t))
+            sees = min(max(0, tokens - (hi - 1 - t)), length)
             seen = keys[:sees][named[:sees]]
             if len(seen) == 0:
                 continue
