@@ -203,8 +203,9 @@ int nvdsa_norm_rope_append(const nvdsa_tensor* query,
  * Groups (both tensors [S], or neither): requests [prefix_request_ends[s-1],
  * prefix_request_ends[s]) hold the same pages for their first prefix_lengths[s]
  * tokens (whole pages: the rest of that length counts as their own).  Where that
- * saves enough time they are read through the first request's table, once for the
- * group.  Requests behind the last end share nothing.  Values that a row does not
+ * saves enough time they are read through the table of the first request that has
+ * rows, once for the group; requests without rows may hold anything.  Requests behind
+ * the last end share nothing.  Values that a row does not
  * see may be anything; a NaN or a score of +inf that it sees makes it NaN; the dims
  * of an infinite value whose score is -inf are NaN or without that key, as the work
  * is cut.  The workspace holds no state. */

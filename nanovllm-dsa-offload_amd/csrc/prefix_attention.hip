@@ -290,7 +290,21 @@ __device__ __forceinline__ Cut make_plan(const PrefixAttentionArgs& a, const Pla
     // (Ends that decrease could count a request's pairs for several groups: there
     // is room for each pair once.)
     if (merged + m + s.pairs > merge_pairs(rows, heads, batch, groups)) s.pairs = 0;
-    if (s.pairs > 0) s.merge = merged + m;
+    if (s.pairs > 0) {
+      s.merge = merged + m;
+      // The table of the first request with rows: one that has ended need not hold the
+      // pages any more.
+      const int r0 = row_at(s.table);
+      int last = group_end(g) - 1;
+      if (row_at(s.table + 1) > r0) last = s.table;
+      while (s.table < last) {
+        const int mid = (s.table + last) >> 1;
+        if (row_at(mid + 1) <= r0)
+          s.table = mid + 1;
+        else
+          last = mid;
+      }
+    }
     merged += sum_m;
     int64_t u = units_of(s, kPairs), n = items_of(s, kPairs), sum_u, sum_n;
     plan_scan<THREADS>(u, n, lds.scratch, &sum_u, &sum_n);

@@ -187,8 +187,9 @@ def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_
     requests ``[prefix_request_ends[s-1], prefix_request_ends[s])`` hold the same
     pages for their first ``prefix_lengths[s]`` tokens (the whole pages among
     them; what is left counts as their own).  Where that saves enough time, those
-    pages are taken from the first request's table, read once, and multiplied
-    with the queries of all of them; small calls read every request's own.
+    pages are taken from the table of the first request that has rows, read once,
+    and multiplied with the queries of all of them; small calls read every
+    request's own.  A group's requests without rows may hold anything.
     Results are those of a call without groups, up to the order of sums.
     Requests behind the last end, and a group of one, share nothing.
 
