@@ -167,7 +167,8 @@ def norm_rope_append(query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_que
     normalised over all its dims first, and the others written to
     ``query_nope``.  ``cos`` and ``sin`` [T, 64 or more] turn neighbouring
     pairs, as in ``dsa_indexer_query_rope_inplace``.  All tensors share the
-    cache's 16-bit dtype; values are computed in fp32 and rounded once."""
+    cache's 16-bit dtype; values are computed in fp32 and rounded once.  nope is
+    a multiple of 8, up to 512."""
     _norm_rope_append_op(query, kv, cos, sin, kv_norm_weight, actual_seq_lengths_query, actual_seq_lengths_kv, block_table,
                          k_rope, kv_cache, query_rope, query_norm_weight, query_nope, float(eps))
 
@@ -244,7 +245,8 @@ def pages_copy(src_ids, dst_ids, caches, *, tokens=None, count=None) -> None:
     [P, 128, ...] (of others whole pages, where there are any rows).  ``count``
     [1]: only the first ``count[0]`` pairs.  Pairs that name no page are
     skipped.  A page must not be a source and a destination of one call, nor a
-    destination twice."""
+    destination twice.  Pages, and the rows of caches [P, 128, ...], are whole
+    multiples of 4 bytes."""
     _pages_copy_op(src_ids, dst_ids, list(caches), tokens, count)
 
 
