@@ -191,7 +191,8 @@ def shared_prefix_attention(query_rope, query, actual_seq_lengths_query, actual_
     pages are taken from the table of the first request that has rows, read once,
     and multiplied with the queries of all of them; small calls read every
     request's own.  A group's requests without rows may hold anything.
-    Results are those of a call without groups, up to the order of sums.
+    Results are those of a call without groups, up to the order of sums and the
+    rounding of the weights.
     Requests behind the last end, and a group of one, share nothing.
 
     What a row does not see may hold anything.  A row that sees a NaN, or a score
